@@ -533,6 +533,75 @@ int pia_prefill_hit_compact(const int32_t* slot_row, int32_t* dst, int32_t* src,
                             void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Rotary positions. Pair i of a head turns by 2 pi * position * turns[i] (turns f64[pairs]:
+ * frequency / 2 pi); pairs are (i, i + pairs) or, interleaved, (2 i, 2 i + 1); elements behind
+ * 2 * pairs are copied:
+ *     (a, b) -> (a c - b s, b c + a s),  c = factor cos, s = factor sin
+ * transposed != 0: s negated (the gradient of the map above). c and s are computed in
+ * fp64 and rounded to fp32, the rest is fp32, with one rounding of the result.
+ * q / k: [num_tokens, heads, head_dim] with the given strides (elements), innermost contiguous;
+ * q_out / k_out: contiguous, not overlapping the inputs. num_heads or num_kv_heads may be 0.
+ * positions: i64[num_tokens] or, positions_i64 = 0, i32. 2 * pairs <= min(head_dim, 4096).
+ * ------------------------------------------------------------------------------------------- */
+int pia_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t q_token_stride,
+               int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+               const void* positions, int positions_i64, const double* turns, int pairs,
+               double factor, int interleaved, int transposed, int64_t num_tokens, int num_heads,
+               int num_kv_heads, int head_dim, int dtype, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
+ * Append with the rotary positions applied. Rows cu_new[b] .. cu_new[b + 1] of q / k / v (cu_new
+ * NULL: row b) are the last tokens of sequence b, whose context_lens[b] counts them; a row's
+ * position is its place in the context. k is rotated into its slot of block_tables[b], v copied
+ * into its slot, q (NULL: none) rotated into q_out (contiguous). pairs 0: nothing is rotated.
+ * Tokens without a slot (a page id outside the pool, a position outside the table or below 0) are
+ * not written; q_out is. The pages that take new tokens belong to one sequence each.
+ * k_scales / v_scales NULL: pools [num_pages, num_kv_heads, head_dim, page_size] of dtype.
+ * Else 8-bit pools (float8 e4m3 codes; head_dim and page_size multiples of 16, up to 256 and 4096):
+ *     k_pages [num_pages, num_kv_heads, head_dim / 16, page_size, 16]
+ *     v_pages [num_pages, num_kv_heads, page_size / 4, head_dim, 4]
+ *     scales f32 [num_pages, num_kv_heads, page_size / 16], one per block of 16 tokens and head.
+ * A block's scale is the smallest power of two (at least 2^-100) that holds, in 448 steps of it,
+ * the largest finite element of its new tokens (rotated k: times sqrt(2) * factor, a bound of what
+ * the rotation makes of it), or the scale it had if that is larger and the block holds earlier
+ * tokens, whose codes are rounded to the scale when it grows. Codes round to nearest even; NaN and
+ * infinities become the NaN code.
+ * ------------------------------------------------------------------------------------------- */
+int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride, int64_t q_head_stride,
+                  const void* k, int64_t k_token_stride, int64_t k_head_stride, const void* v,
+                  int64_t v_token_stride, int64_t v_head_stride, void* k_pages, void* v_pages,
+                  float* k_scales, float* v_scales, const int32_t* block_tables,
+                  int64_t bt_stride, const int32_t* context_lens, const int32_t* cu_new,
+                  int64_t num_tokens, int num_seqs, const double* turns, int pairs, double factor,
+                  int interleaved, int num_heads, int num_kv_heads, int head_dim, int page_size,
+                  int64_t num_pages, int dtype, void* stream);
+
+/* Contexts of the 8-bit pool in logical order: rows cu_seqlens[b] .. cu_seqlens[b + 1] of k_out /
+ * v_out [total_tokens, num_kv_heads, head_dim] (dtype) are sequence b's tokens, read through
+ * block_tables[b]. Tokens of a page outside the pool are zeros; rows past the table are left. */
+int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, const void* v_pages,
+                   const float* k_scales, const float* v_scales, const int32_t* block_tables,
+                   int64_t bt_stride, const int64_t* cu_seqlens, int num_seqs,
+                   int64_t total_tokens, int num_kv_heads, int head_dim, int page_size,
+                   int64_t num_pages, int dtype, void* stream);
+
+/* Attention over the 8-bit pool: q / out [total_q_rows, num_heads, head_dim], rows of sequence b =
+ * cu_q[b] .. cu_q[b + 1] (NULL: row b). Row s of b attends keys j < kv_lens[b] and, with
+ * q_pos_offsets, j <= q_pos_offsets[b] + s; q head h reads kv head h / (num_heads / num_kv_heads).
+ * A row without a key is zeros; a page id outside the pool holds no keys. q rows are q_stride
+ * elements apart (whole 16-byte vectors), out is contiguous. workspace: 16-byte aligned, of
+ * pia_kv8_attention_workspace_bytes(head_dim) bytes, any content; calls that share one are ordered on one
+ * stream. */
+int64_t pia_kv8_attention_workspace_bytes(int head_dim);
+int pia_kv8_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
+                      const void* v_pages, const float* k_scales, const float* v_scales,
+                      const int32_t* block_tables, int64_t bt_stride, const int32_t* kv_lens,
+                      const int32_t* cu_q, const int32_t* q_pos_offsets, int num_seqs,
+                      int64_t total_q_rows, int num_heads, int num_kv_heads, int head_dim,
+                      int page_size, int64_t num_pages, float scale, int dtype, void* workspace,
+                      int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * HBM streaming-read probe. No counterpart in the reference: a measurement aid for the
  * rooflines of the kernels above (bench.py --workload hbm-read times it over fresh regions and
  * fits fixed cost + rate). src: 16-byte aligned device memory of `bytes` bytes (a positive

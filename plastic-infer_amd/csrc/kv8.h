@@ -1,0 +1,67 @@
+// The 8-bit KV pool: e4m3 codes and one power-of-two scale for every block of 16 tokens of a head.
+//
+//   K codes [num_pages, Hkv, D / 16, P, 16]   a token's 16 elements together, tokens next to each
+//                                             other: the operand of K . q^T, whose lanes are tokens
+//   V codes [num_pages, Hkv, P / 4, D, 4]     an element's 4 tokens together: the operand of P . V,
+//                                             whose lanes hold 4 tokens of each block
+//   scales  fp32 [num_pages, Hkv, P / 16]
+//
+// A block of either pool is 16 D bytes; a wave loads it in whole 256-byte runs straight into matrix
+// operands, with no transposing and no LDS. With scales that are powers of two a code times its
+// scale is exact in bf16, and a block whose scale grows keeps its codes' digits: only the exponent
+// moves (but for codes that fall below 2^-6 of the new scale, which keep 2^-9 of it).
+#pragma once
+
+#include "pia_internal.h"
+
+namespace pia {
+namespace kv8 {
+
+constexpr int BLOCK = 16;
+constexpr float LARGEST = 448.f;
+
+// The smallest power of two whose multiple by 448 = 1.75 * 2^8 is at least bound (finite, >= 0),
+// within 2^-100 .. 2^119.
+__device__ __forceinline__ float scale_of(float bound) {
+  const uint32_t u = __float_as_uint(bound);
+  // exponent field of bound / 2^8, one more where its mantissa is over 1.75 (denormals: the least)
+  const int e = int(u >> 23) - 8 + ((u & 0x7fffffu) > 0x600000u ? 1 : 0);
+  return __uint_as_float(uint32_t(min(max(e, 27), 246)) << 23);
+}
+
+// Four values times inv (the inverse of a scale) as the e4m3 codes of a word: nearest
+// even, beyond the largest code the largest one, NaN and infinities the NaN code.
+__device__ __forceinline__ float clip(float x) {
+  const float c = fminf(fmaxf(x, -LARGEST), LARGEST);
+  return fabsf(x) < INFINITY ? c : __builtin_nanf("");
+}
+__device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clip(a * inv), clip(b * inv), 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(clip(c * inv), clip(d * inv), lo, true));
+}
+__device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
+  const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false);
+  const auto hi = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), true);
+  x[0] = lo[0];
+  x[1] = lo[1];
+  x[2] = hi[0];
+  x[3] = hi[1];
+}
+// a word's codes times ratio (a power of two, at most 1), rounded to codes again
+__device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
+  float x[4];
+  decode4(w, x);
+  return encode4(x[0], x[1], x[2], x[3], ratio);
+}
+
+// 1 / a scale that scale_of gave (a power of two within 2^-100 .. 2^119): exact
+__device__ __forceinline__ float inverse(float scale) {
+  return __uint_as_float((254u << 23) - __float_as_uint(scale));
+}
+
+inline bool pool_shape(int D, int P) {
+  return D > 0 && D % 16 == 0 && D <= 256 && P > 0 && P % BLOCK == 0 && P <= 4096;
+}
+
+}  // namespace kv8
+}  // namespace pia

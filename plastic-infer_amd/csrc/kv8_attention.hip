@@ -1,0 +1,726 @@
+// Attention over the 8-bit paged KV pool: one query row per sequence (decode) or several with a
+// causal limit for each, any q type, head_dim to 256.
+//
+// Bound by HBM for decode: a context token of a kv head is 2 D bytes and a few scales, against
+// 4 G D operations. What the vector ALU does for a byte has to stay small, so both products run on
+// the matrix cores, with operands that come from memory in place:
+//
+//   S^T = K . q^T  A is K: lane l holds token l % 16's elements of chunk l / 16 (kv8.h), widened to
+//                  16 bits, where an e4m3 code is exact; B is q. Lane l then has the scores of row
+//                  l % 16 for tokens 4 (l / 16) + j of each block.
+//   O += P . V     those scores' exponentials are the A operand as they are; B is V, whose words
+//                  hold an element's tokens 4 (l / 16) .. + 3. Two blocks make 32 tokens.
+//
+// Precision: the codes are exact in bf16 (and fp16), their scales are applied to scores and
+// probabilities in fp32. q is exact: one bf16 or fp16 term, or three bf16 terms of an fp32 value.
+// The probabilities times V's scale are the sum of two bf16 terms (2^-17 of each; three for fp32
+// results: 2^-25), so a result is as good as its type. Scores, sums and outputs are fp32.
+//
+// Work: an item is 16 (position, head) rows of a sequence and kv head; its keys go by steps of
+// 16 MB tokens. All steps of all items, in order, are cut into one contiguous range for every
+// resident wave, whatever the batch looks like. The next step's K and V are on their way while a
+// step is computed, across items too. An item that lies in one range is finished there; pieces of
+// the others (at most two a wave) go to the workspace, and a second kernel joins them in order, so
+// results do not depend on timing.
+#include <algorithm>
+
+#include "attn_tiles.h"
+#include "attn_tiles_f32.h"
+#include "kv8.h"
+
+namespace pia {
+namespace {
+
+using tile::f32x4_t;
+
+constexpr int KA_MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
+constexpr int KA_WG_WAVES = 4;
+constexpr int KA_WGS_PER_CU = 2;   // two waves per SIMD
+constexpr int KA_RSRC_WORD3 = 0x00020000;
+constexpr float KA_RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
+constexpr int KA_MERGE_THREADS = 256;
+
+struct AttnArgs {
+  void* out;
+  const void* q;
+  int64_t q_stride;
+  const uint8_t *kp, *vp;
+  const float *ks, *vs;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t *lens, *cu, *offs;
+  int64_t rows, num_pages;
+  float* parts;
+  int64_t* pref;
+  float scale_log2;
+  int B, Hq, Hkv, G, D, P;
+};
+
+// A sequence's part of a call: its rows, the keys that some row of it may see and their steps.
+struct Seq {
+  int64_t row0;
+  int n, kv_len, off, items, steps;
+};
+__device__ __forceinline__ Seq sequence(const AttnArgs& a, int b, int tokens) {
+  Seq s;
+  s.row0 = a.cu ? a.cu[b] : b;
+  const int64_t n = a.cu ? int64_t(a.cu[b + 1]) - s.row0 : 1;
+  s.n = s.row0 < 0 ? 0 : int(max(int64_t(0), min(n, a.rows - s.row0)));
+  s.kv_len = int(min(int64_t(max(a.lens[b], 0)), min(a.bt_stride * a.P, int64_t(0x7ffffff0))));
+  s.off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
+  const int64_t seen = a.offs ? min(int64_t(s.kv_len), int64_t(s.off) + s.n) : s.kv_len;
+  s.items = int((int64_t(s.n) * a.G + 15) >> 4);
+  s.steps = seen > 0 ? int((seen + tokens - 1) / tokens) : 0;
+  return s;
+}
+
+// ranges of the waves: wave w of n takes steps first_of(w) .. first_of(w + 1) - 1 of total
+__device__ __forceinline__ int64_t first_of(int64_t w, int64_t n, int64_t total) {
+  return total * w / n;
+}
+
+template <int DP>
+constexpr int64_t part_floats = 16 * (DP + 2);  // 16 rows' outputs, maxima and sums
+
+template <int QT>
+struct Q;  // terms of q and of the probabilities, and the 16-bit type of K and q
+template <> struct Q<PIA_DTYPE_BF16> { static constexpr int NQ = 1, NP = 2, KT = PIA_DTYPE_BF16; };
+template <> struct Q<PIA_DTYPE_F16> { static constexpr int NQ = 1, NP = 2, KT = PIA_DTYPE_F16; };
+template <> struct Q<PIA_DTYPE_F32> { static constexpr int NQ = 3, NP = 3, KT = PIA_DTYPE_BF16; };
+
+// two codes (the low or high half of a word) as two 16-bit values
+template <int T, bool HI>
+__device__ __forceinline__ uint32_t widen(uint32_t w) {
+  if constexpr (T == PIA_DTYPE_F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
+}
+template <int T>
+__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b) {
+  return make_uint4(widen<T, false>(a), widen<T, true>(a), widen<T, false>(b), widen<T, true>(b));
+}
+
+// eight consecutive q elements as NQ operands
+template <int QT>
+__device__ __forceinline__ void load_q(const typename Elem<QT>::T* p, bool ok,
+                                       uint4 (&t)[Q<QT>::NQ]) {
+  if constexpr (QT == PIA_DTYPE_F32) {
+    float x[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = ok ? p[i] : 0.f;
+#pragma unroll
+    for (int k = 0; k < 3; ++k) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        w[i] = tile::pack_bf16x2(x[2 * i], x[2 * i + 1]);
+        x[2 * i] -= bf16_lo(w[i]);
+        x[2 * i + 1] -= bf16_hi(w[i]);
+      }
+      t[k] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+  } else {
+    t[0] = ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+  }
+}
+
+__device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirstlane(x); }
+__device__ __forceinline__ float lane_value(float x, int lane) {
+  return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
+}
+// the bytes of a word that hold the NaN code, as 0x80 each
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// NT: K and V are read once by the call.
+template <int QT, int DP, bool NT>
+__global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention_kernel(AttnArgs a) {
+  using T = typename Elem<QT>::T;
+  constexpr int NQ = Q<QT>::NQ, NP = Q<QT>::NP, KT16 = Q<QT>::KT;
+  constexpr int MB = DP > 128 ? 2 : 4;  // blocks of a step (registers)
+  constexpr int STEP = 16 * MB, ND = DP / 64, AUX = NT ? 2 : 0;
+  __shared__ int64_t pref[KA_MAX_SEQS + 1];
+  __shared__ int steps_of[KA_MAX_SEQS];
+  __shared__ int64_t wsum[KA_WG_WAVES];
+  const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
+  constexpr int NTH = 64 * KA_WG_WAVES;
+
+  // steps of the sequences before each
+  if (threadIdx.x == 0) pref[0] = 0;
+  int64_t carry = 0;
+  for (int c0 = 0; c0 < a.B; c0 += NTH) {
+    const int b = c0 + threadIdx.x;
+    int64_t incl = 0;
+    if (b < a.B) {
+      const Seq s = sequence(a, b, STEP);
+      steps_of[b] = s.steps;
+      incl = int64_t(s.items) * a.Hkv * s.steps;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int64_t y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int64_t base = carry;
+    for (int w = 0; w < wave; ++w) base += wsum[w];
+    if (b < a.B) pref[b + 1] = base + incl;
+#pragma unroll
+    for (int w = 0; w < KA_WG_WAVES; ++w) carry += wsum[w];
+    __syncthreads();
+  }
+  if (blockIdx.x == 0)  // for the kernel that joins the pieces
+    for (int b = threadIdx.x; b <= a.B; b += NTH) a.pref[b] = pref[b];
+  const int64_t total = carry;
+  const int64_t nw = min(int64_t(gridDim.x) * KA_WG_WAVES, total);
+  const int64_t w = int64_t(wave) * gridDim.x + blockIdx.x;  // few steps: over all compute units
+  if (w >= nw) return;
+  const int64_t x0 = first_of(w, nw, total), x1 = first_of(w + 1, nw, total);
+  const int count = uniform(int(min(x1 - x0, int64_t(0x7fffffff))));
+
+  // where a wave is: step t of item i of kv head h of sequence b
+  struct Cursor {
+    int b, h, i, t, items, steps, kv_len;
+  };
+  auto enter = [&](Cursor& c) {
+    const int64_t per = pref[c.b + 1] - pref[c.b];
+    c.steps = uniform(steps_of[c.b]);
+    c.items = uniform(int(per / (int64_t(c.steps) * a.Hkv)));
+    c.kv_len = uniform(sequence(a, c.b, STEP).kv_len);
+  };
+  auto advance = [&](Cursor& c) {
+    if (++c.t < c.steps) return;
+    c.t = 0;
+    if (++c.i < c.items) return;
+    c.i = 0;
+    if (++c.h < a.Hkv) return;
+    c.h = 0;
+    do ++c.b;
+    while (c.b < a.B && uniform(int(pref[c.b + 1] == pref[c.b])));
+    if (c.b < a.B) enter(c);
+  };
+  Cursor cur;
+  {
+    int lo = 0, hi = a.B - 1;  // the last sequence that starts at or before x0 (and is not empty)
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid] <= x0) lo = mid; else hi = mid - 1;
+    }
+    cur.b = uniform(lo);
+    enter(cur);
+    const int64_t at = x0 - pref[cur.b], seg = at / cur.steps;
+    cur.t = uniform(int(at - seg * cur.steps));
+    cur.i = uniform(int(seg % cur.items));
+    cur.h = uniform(int(seg / cur.items));
+  }
+
+  // pages: lane m < MB has block m of a step: its (page, head) and its place in the page, or -1
+  const int PB = a.P / 16, g = lane >> 4, n16 = lane & 15;
+  struct Where {
+    int head, sub;
+  };
+  auto where = [&](const Cursor& c, bool real) {
+    Where r{-1, 0};
+    const int kb = c.t * MB + lane;
+    if (real && lane < MB && kb * 16 < c.kv_len) {
+      const int slot = kb / PB;
+      const int32_t id = a.bt[int64_t(c.b) * a.bt_stride + slot];
+      r.sub = kb - slot * PB;
+      r.head = uint32_t(id) < uint64_t(a.num_pages) ? id * a.Hkv + c.h : -1;
+    }
+    return r;
+  };
+  const int64_t tile_bytes = int64_t(a.D) * a.P;
+  uint32_t k_off[ND], v_off[ND];
+#pragma unroll
+  for (int i = 0; i < ND; ++i) {
+    k_off[i] = uint32_t(((g + 4 * i) * a.P + n16) * 16);
+    v_off[i] = uint32_t(g * 4 * a.D + 256 * i + 16 * n16);
+  }
+  // Buffer descriptors: a block that is not there gets an empty one, whose loads return zeros
+  // without reading, so loading has no branch; chunks of K past head_dim lie past its end.
+  uint4 kr[MB][ND], vr[MB][ND];
+  auto load_k = [&](const Where& r) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int head = __builtin_amdgcn_readlane(r.head, m), sub = __builtin_amdgcn_readlane(r.sub, m);
+      const bool ok = head >= 0;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a.kp + (ok ? head : 0) * tile_bytes + sub * 256), 0,
+          ok ? int(tile_bytes) - sub * 256 : 0, KA_RSRC_WORD3);
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        kr[m][i] = __builtin_bit_cast(uint4,
+                                      __builtin_amdgcn_raw_buffer_load_b128(rs, k_off[i], 0, AUX));
+    }
+  };
+  auto load_v = [&](const Where& r) {
+#pragma unroll
+    for (int m = 0; m < MB; ++m) {
+      const int head = __builtin_amdgcn_readlane(r.head, m), sub = __builtin_amdgcn_readlane(r.sub, m);
+      const bool ok = head >= 0;
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a.vp + (ok ? head : 0) * tile_bytes + int64_t(sub) * 16 * a.D), 0,
+          ok ? 16 * a.D : 0, KA_RSRC_WORD3);
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+        vr[m][i] = __builtin_bit_cast(uint4,
+                                      __builtin_amdgcn_raw_buffer_load_b128(rs, v_off[i], 0, AUX));
+    }
+  };
+  float sk = 1.f, sv = 1.f;  // lane m < MB: block m's scales
+  auto load_scales = [&](const Where& r) {
+    const bool ok = r.head >= 0;
+    const int64_t at = ok ? int64_t(r.head) * PB + r.sub : 0;
+    sk = ok ? a.ks[at] : 1.f;
+    sv = ok ? a.vs[at] : 1.f;
+  };
+
+  Cursor nxt = cur;
+  if (count > 1) advance(nxt);
+  Cursor far = nxt;
+  Where w_cur = where(cur, true), w_nxt = where(nxt, count > 1);
+  load_k(w_cur);
+  load_scales(w_cur);
+  load_v(w_cur);
+
+  // the item's rows: lane l's q operands and limit are those of row l % 16
+  uint4 qr[ND][2][NQ];
+  int lim = 0, lim_min = 0, rows_left = 0;
+  int64_t row0 = 0;
+  float m = -INFINITY, l = 0.f;
+  f32x4_t acc[4 * ND];
+  bool opened = false;
+  int begun = 0;  // step of the range at which the item began
+
+  for (int x = 0; x < count; ++x) {
+    if (x + 2 < count) advance(far);
+    const Where w_far = where(far, x + 2 < count);
+    if (!opened) {
+      opened = true;
+      begun = x;
+      const Seq s = sequence(a, cur.b, STEP);
+      row0 = s.row0;
+      rows_left = s.n * a.G - 16 * cur.i;
+      const int r = 16 * cur.i + n16, pos = r / a.G;
+      const bool ok = n16 < rows_left;
+      const T* qp = static_cast<const T*>(a.q) + (row0 + (ok ? pos : 0)) * a.q_stride +
+                    int64_t(cur.h * a.G + (ok ? r - pos * a.G : 0)) * a.D;
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const int d = 16 * (g + 4 * i) + 8 * e;
+          load_q<QT>(qp + (d < a.D ? d : 0), ok && d < a.D, qr[i][e]);
+        }
+      lim = a.offs ? min(s.kv_len, s.off + pos + 1) : s.kv_len;
+      lim_min = a.offs ? min(s.kv_len, s.off + (16 * cur.i) / a.G + 1) : s.kv_len;
+      m = -INFINITY;
+      l = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < 4 * ND; ++nb) acc[nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+    }
+
+    // scores
+    f32x4_t s[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      s[b] = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int i = 0; i < ND; ++i) {
+        const uint4 k = kr[b][i];
+        const uint4 lo = widen8<KT16>(k.x, k.y), hi = widen8<KT16>(k.z, k.w);
+#pragma unroll
+        for (int n = NQ - 1; n >= 0; --n) {
+          s[b] = tile::mfma16<KT16>(lo, qr[i][0][n], s[b]);
+          s[b] = tile::mfma16<KT16>(hi, qr[i][1][n], s[b]);
+        }
+      }
+    }
+    const float sk_cur = sk, sv_cur = sv;
+    load_k(w_nxt);
+    load_scales(w_nxt);
+
+    // softmax, base 2
+    const int there = int(__ballot(lane < MB && w_cur.head >= 0)) & ((1 << MB) - 1);
+    const int base = cur.t * STEP;
+    const bool full = there == (1 << MB) - 1 && base + STEP <= lim_min;
+    float mx = -INFINITY;
+#pragma unroll
+    for (int b = 0; b < MB; ++b) {
+      const float f = a.scale_log2 * lane_value(sk_cur, b);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s[b][j] *= f;
+    }
+    if (!full) {
+      const int rel = lim - (base + 4 * g);
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (!(16 * b + j < rel && ((there >> b) & 1))) s[b][j] = -INFINITY;
+    }
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) mx = __builtin_elementwise_maximum(mx, s[b][j]);
+    mx = tile::maximum_col4(mx);
+    const float mref = mx - m > KA_RESCALE || mx != mx ? mx : m;
+    const float alpha = m == mref ? 1.f : __builtin_amdgcn_exp2f(m - mref);
+    const bool moved = m != mref;
+    m = mref;
+    const float nm = mref == -INFINITY ? 0.f : -mref;
+    float ls = 0.f;
+    f32x4_t p[MB];
+#pragma unroll
+    for (int b = 0; b < MB; ++b)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        p[b][j] = __builtin_amdgcn_exp2f(s[b][j] + nm);
+        ls += p[b][j];
+      }
+    l = l * alpha + ls;
+    if (__ballot(moved)) {
+      float aj[4];
+#pragma unroll
+      for (int j = 0; j < 4; ++j) aj[j] = __shfl(alpha, 4 * g + j, 64);
+#pragma unroll
+      for (int nb = 0; nb < 4 * ND; ++nb)
+#pragma unroll
+        for (int j = 0; j < 4; ++j) acc[nb][j] *= aj[j];
+    }
+    // probabilities times V's scales, as the sum of NP bf16 terms: operand c is blocks 2 c, 2 c + 1
+    uint4 pt[MB / 2][NP];
+#pragma unroll
+    for (int c = 0; c < MB / 2; ++c) {
+      uint32_t t[NP][4];
+#pragma unroll
+      for (int b2 = 0; b2 < 2; ++b2) {
+        const float f = lane_value(sv_cur, 2 * c + b2);
+#pragma unroll
+        for (int j2 = 0; j2 < 2; ++j2) {
+          float u = p[2 * c + b2][2 * j2] * f, v = p[2 * c + b2][2 * j2 + 1] * f;
+#pragma unroll
+          for (int k = 0; k < NP; ++k) {
+            const uint32_t wd = tile::pack_bf16x2(u, v);
+            t[k][2 * b2 + j2] = wd;
+            u -= bf16_lo(wd);
+            v -= bf16_hi(wd);
+          }
+        }
+      }
+#pragma unroll
+      for (int k = 0; k < NP; ++k) pt[c][k] = make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
+    }
+    // V of tokens past the context is whatever the page held: zeros
+    if (base + STEP > cur.kv_len) {
+#pragma unroll
+      for (int b = 0; b < MB; ++b) {
+        const int nv = cur.kv_len - (base + 16 * b + 4 * g);
+        const uint32_t keep = nv >= 4 ? 0xffffffffu : nv <= 0 ? 0u : (1u << (8 * nv)) - 1u;
+#pragma unroll
+        for (int i = 0; i < ND; ++i) {
+          vr[b][i].x &= keep;
+          vr[b][i].y &= keep;
+          vr[b][i].z &= keep;
+          vr[b][i].w &= keep;
+        }
+      }
+    }
+    // Zero times NaN is NaN, so a NaN of V would reach rows that may not see its token. Where rows
+    // differ in what they see, NaN codes are taken out, and put into the rows that see them by a
+    // product of their places.
+    if (a.offs && !full) {
+      uint32_t any = 0;
+#pragma unroll
+      for (int b = 0; b < MB; ++b)
+#pragma unroll
+        for (int i = 0; i < ND; ++i)
+          any |= nan_bytes(vr[b][i].x) | nan_bytes(vr[b][i].y) | nan_bytes(vr[b][i].z) |
+                 nan_bytes(vr[b][i].w);
+      if (__ballot(any != 0)) {
+        const int rel = lim - (base + 4 * g);
+#pragma unroll 1
+        for (int nb = 0; nb < 4 * ND; ++nb) {
+          f32x4_t hit = f32x4_t{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+          for (int c = 0; c < MB / 2; ++c) {
+            uint32_t see[4], at[2];
+#pragma unroll
+            for (int b2 = 0; b2 < 2; ++b2) {
+              const int b = 2 * c + b2;
+              const bool here = (there >> b) & 1;
+#pragma unroll
+              for (int j2 = 0; j2 < 2; ++j2)
+                see[2 * b2 + j2] = (here && 16 * b + 2 * j2 < rel ? 0x3f80u : 0u) |
+                                   (here && 16 * b + 2 * j2 + 1 < rel ? 0x3f800000u : 0u);
+              uint32_t wd = 0;
+#pragma unroll
+              for (int i = 0; i < ND; ++i)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if (nb == 4 * i + e) {
+                    uint32_t* q4 = reinterpret_cast<uint32_t*>(&vr[b][i]);
+                    wd = nan_bytes(q4[e]);
+                    q4[e] &= ~((wd >> 7) * 0xffu);
+                  }
+              at[b2] = (wd >> 7) * 0x38u;  // the code of 1
+            }
+            hit = tile::mfma16<PIA_DTYPE_BF16>(make_uint4(see[0], see[1], see[2], see[3]),
+                                               widen8<PIA_DTYPE_BF16>(at[0], at[1]), hit);
+          }
+#pragma unroll
+          for (int k = 0; k < 4 * ND; ++k)
+            if (nb == k)
+#pragma unroll
+              for (int j = 0; j < 4; ++j)
+                if (hit[j] > 0.f) acc[k][j] = __builtin_nanf("");
+        }
+      }
+    }
+#pragma unroll
+    for (int c = 0; c < MB / 2; ++c)
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint4 v = widen8<PIA_DTYPE_BF16>(tile32::word(vr[2 * c][i], e),
+                                                 tile32::word(vr[2 * c + 1][i], e));
+#pragma unroll
+          for (int k = NP - 1; k >= 0; --k)
+            acc[4 * i + e] = tile::mfma16<PIA_DTYPE_BF16>(pt[c][k], v, acc[4 * i + e]);
+        }
+    load_v(w_nxt);
+
+    // end of the item or of the range
+    if (cur.t + 1 == cur.steps || x + 1 == count) {
+      const float lsum = tile32::sum_col4(l);
+      const bool whole = cur.t + 1 == cur.steps && cur.t == x - begun;
+      if (whole) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+          const float lj = __shfl(lsum, 4 * g + j, 64);
+          const int r = 16 * cur.i + 4 * g + j, pos = r / a.G;
+          if (4 * g + j >= rows_left) continue;
+          T* o = static_cast<T*>(a.out) +
+                 ((row0 + pos) * a.Hq + cur.h * a.G + r - pos * a.G) * a.D;
+          const float inv = lj == 0.f ? 0.f : 1.f / lj;
+#pragma unroll
+          for (int i = 0; i < ND; ++i) {
+            const int d = 64 * i + 4 * n16;
+            if (d < a.D) {
+              struct alignas(4 * sizeof(T)) Pack {
+                T v[4];
+              } pk;
+#pragma unroll
+              for (int e = 0; e < 4; ++e)
+                Elem<QT>::store(pk.v, e, lj == 0.f ? 0.f : acc[4 * i + e][j] * inv);
+              *reinterpret_cast<Pack*>(o + d) = pk;
+            }
+          }
+        }
+      } else {
+        float* part = a.parts + (w * 2 + (begun == 0 ? 0 : 1)) * part_floats<DP>;
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (4 * g + j < rows_left)
+#pragma unroll
+            for (int i = 0; i < ND; ++i)
+              *reinterpret_cast<float4*>(part + (4 * g + j) * DP + 64 * i + 4 * n16) =
+                  make_float4(acc[4 * i][j], acc[4 * i + 1][j], acc[4 * i + 2][j],
+                              acc[4 * i + 3][j]);
+        if (g == 0) {
+          part[16 * DP + n16] = m;
+          part[16 * DP + 16 + n16] = lsum;
+        }
+      }
+      opened = false;
+    }
+    cur = nxt;
+    nxt = far;
+    w_cur = w_nxt;
+    w_nxt = w_far;
+  }
+}
+
+// The items that were cut: their pieces joined in the order of the waves. One workgroup per item;
+// threads are (row, four elements). Items without keys are zeros.
+template <int QT, int DP>
+__global__ __launch_bounds__(KA_MERGE_THREADS) void kv8_attention_join_kernel(AttnArgs a,
+                                                                              int64_t waves) {
+  using T = typename Elem<QT>::T;
+  constexpr int STEP = 16 * (DP > 128 ? 2 : 4);
+  int64_t id = blockIdx.x;
+  const int h = int(id % a.Hkv);
+  id /= a.Hkv;
+  int b, i;
+  if (a.cu) {
+    int lo = 0, hi = a.B - 1;  // items of sequence b are numbered from cu[b] G / 16 + b on
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if ((int64_t(a.cu[mid]) * a.G >> 4) + mid <= id) lo = mid; else hi = mid - 1;
+    }
+    b = lo;
+    i = int(id - ((int64_t(a.cu[b]) * a.G >> 4) + b));
+  } else {
+    const int items = (a.G + 15) >> 4;
+    b = int(id / items);
+    i = int(id - int64_t(b) * items);
+  }
+  const Seq s = sequence(a, b, STEP);
+  if (i < 0 || i >= s.items) return;
+  const int rows = min(16, s.n * a.G - 16 * i);
+  const int64_t total = a.pref[a.B], nw = min(waves, total);
+  const int64_t from = a.pref[b] + (int64_t(h) * s.items + i) * s.steps, to = from + s.steps;
+  int64_t w0 = 0, w1 = 0;
+  if (s.steps > 0) {
+    w0 = ((from + 1) * nw - 1) / total;
+    w1 = (to * nw - 1) / total;
+    if (w0 == w1) return;  // finished by its wave
+  }
+  const float* first = a.parts + (w0 * 2 + (s.steps > 0 && first_of(w0, nw, total) >= from ? 0 : 1)) *
+                                     part_floats<DP>;
+  auto piece = [&](int64_t w) {
+    return w == w0 ? first : a.parts + w * 2 * part_floats<DP>;
+  };
+  for (int u = threadIdx.x; u < rows * (a.D / 4); u += KA_MERGE_THREADS) {
+    const int r = u / (a.D / 4), d = 4 * (u - r * (a.D / 4));
+    float M = -INFINITY, L = 0.f;
+    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+    if (s.steps > 0) {
+      for (int64_t w = w0; w <= w1; ++w)
+        M = __builtin_elementwise_maximum(M, piece(w)[16 * DP + r]);
+      for (int64_t w = w0; w <= w1; ++w) {
+        const float* p = piece(w);
+        const float mw = p[16 * DP + r], f = mw == M ? (M == -INFINITY ? 0.f : 1.f)
+                                                     : __builtin_amdgcn_exp2f(mw - M);
+        const float4 x = *reinterpret_cast<const float4*>(p + r * DP + d);
+        L += p[16 * DP + 16 + r] * f;
+        o.x += x.x * f;
+        o.y += x.y * f;
+        o.z += x.z * f;
+        o.w += x.w * f;
+      }
+    }
+    const float inv = L == 0.f ? 0.f : 1.f / L;
+    const int rr = 16 * i + r, pos = rr / a.G;
+    T* out = static_cast<T*>(a.out) + ((s.row0 + pos) * a.Hq + h * a.G + rr - pos * a.G) * a.D + d;
+    struct alignas(4 * sizeof(T)) Pack {
+      T v[4];
+    } pk;
+    Elem<QT>::store(pk.v, 0, L == 0.f ? 0.f : o.x * inv);
+    Elem<QT>::store(pk.v, 1, L == 0.f ? 0.f : o.y * inv);
+    Elem<QT>::store(pk.v, 2, L == 0.f ? 0.f : o.z * inv);
+    Elem<QT>::store(pk.v, 3, L == 0.f ? 0.f : o.w * inv);
+    *reinterpret_cast<Pack*>(out) = pk;
+  }
+}
+
+int padded(int D) { return D <= 64 ? 64 : D <= 128 ? 128 : 256; }
+int64_t resident_waves() { return int64_t(device_cus()) * KA_WGS_PER_CU * KA_WG_WAVES; }
+constexpr int64_t KA_PREF_BYTES = (KA_MAX_SEQS + 1) * 8 + 248;  // whole 256 bytes
+
+template <int QT, int DP>
+void launch(const AttnArgs& a, int64_t items, bool once, hipStream_t s) {
+  const unsigned wgs = unsigned(device_cus() * KA_WGS_PER_CU);
+  if (once)
+    hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, true>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
+  else
+    hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, false>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
+  hipLaunchKernelGGL((kv8_attention_join_kernel<QT, DP>), dim3(unsigned(items)),
+                     dim3(KA_MERGE_THREADS), 0, s, a, resident_waves());
+}
+
+}  // namespace
+}  // namespace pia
+
+using namespace pia;
+
+extern "C" int64_t pia_kv8_attention_workspace_bytes(int head_dim) {
+  if (head_dim <= 0 || head_dim > 256) return 0;
+  const int DP = padded(head_dim);
+  return KA_PREF_BYTES + resident_waves() * 2 * 16 * (DP + 2) * int64_t(sizeof(float));
+}
+
+extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
+                                 const void* v_pages, const float* k_scales, const float* v_scales,
+                                 const int32_t* block_tables, int64_t bt_stride,
+                                 const int32_t* kv_lens, const int32_t* cu_q,
+                                 const int32_t* q_pos_offsets, int num_seqs, int64_t total_q_rows,
+                                 int num_heads, int num_kv_heads, int head_dim, int page_size,
+                                 int64_t num_pages, float scale, int dtype, void* workspace,
+                                 int64_t workspace_bytes, void* stream) {
+  if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
+    return fail(PIA_EUNSUPPORTED, "kv8_attention: dtype must be bf16, fp16 or fp32");
+  if (num_seqs < 0 || total_q_rows < 0 || num_heads <= 0 || num_kv_heads <= 0 || num_pages <= 0 ||
+      bt_stride < 0)
+    return fail(PIA_EINVAL, "kv8_attention: invalid size");
+  if (num_heads % num_kv_heads)
+    return fail(PIA_EINVAL, "kv8_attention: num_heads % num_kv_heads != 0");
+  if (!kv8::pool_shape(head_dim, page_size))
+    return fail(PIA_EUNSUPPORTED,
+                "kv8_attention: head_dim and page_size in multiples of 16, up to 256 and 4096");
+  if (!cu_q && total_q_rows != num_seqs)
+    return fail(PIA_EINVAL, "kv8_attention: without cu_q one row per sequence");
+  if (num_seqs == 0 || total_q_rows == 0) return 0;
+  if (num_pages * num_kv_heads > 0x7fffffff || total_q_rows * num_heads > 0x7fffffff)
+    return fail(PIA_EINVAL, "kv8_attention: pool or rows too large");
+  if (!out || !q || !k_pages || !v_pages || !k_scales || !v_scales || !kv_lens ||
+      (bt_stride && !block_tables) || !workspace)
+    return fail(PIA_EINVAL, "kv8_attention: null pointer");
+  const int elem = dtype == PIA_DTYPE_F32 ? 4 : 2;
+  if (!aligned(q, 16) || !aligned(out, 16) || (q_stride * elem) % 16 || !aligned(k_pages, 16) ||
+      !aligned(v_pages, 16) || !aligned(workspace, 16))
+    return fail(PIA_EINVAL, "kv8_attention: q rows, out, pools and workspace must be 16-byte aligned");
+  if (workspace_bytes < pia_kv8_attention_workspace_bytes(head_dim))
+    return fail(PIA_EINVAL, "kv8_attention: workspace too small");
+  const int G = num_heads / num_kv_heads, DP = padded(head_dim);
+  hipStream_t s = as_stream(stream);
+  AttnArgs a{out, q, q_stride, static_cast<const uint8_t*>(k_pages),
+             static_cast<const uint8_t*>(v_pages), k_scales, v_scales, block_tables, bt_stride,
+             kv_lens, cu_q, q_pos_offsets, total_q_rows, num_pages,
+             reinterpret_cast<float*>(static_cast<char*>(workspace) + KA_PREF_BYTES),
+             static_cast<int64_t*>(workspace), scale * 1.4426950408889634f, num_seqs, num_heads,
+             num_kv_heads, G, head_dim, page_size};
+  const bool once = !cu_q && G <= 16;
+  // more sequences than a launch's tables hold: by parts, one after the other on the stream
+  for (int b0 = 0; b0 < num_seqs; b0 += KA_MAX_SEQS) {
+    AttnArgs c = a;
+    c.B = std::min(num_seqs - b0, KA_MAX_SEQS);
+    c.bt += int64_t(b0) * bt_stride;
+    c.lens += b0;
+    if (c.offs) c.offs += b0;
+    int64_t items;
+    if (cu_q) {
+      c.cu += b0;
+      items = (total_q_rows * G >> 4) + c.B;
+    } else {
+      c.q = static_cast<const char*>(q) + int64_t(b0) * q_stride * elem;
+      c.out = static_cast<char*>(out) + int64_t(b0) * num_heads * head_dim * elem;
+      c.rows = c.B;
+      items = int64_t(c.B) * ((G + 15) / 16);
+    }
+    items *= num_kv_heads;
+    if (items > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many rows");
+#define PIA_K8(QT)                                        \
+  switch (DP) {                                           \
+    case 64: launch<QT, 64>(c, items, once, s); break;    \
+    case 128: launch<QT, 128>(c, items, once, s); break;  \
+    default: launch<QT, 256>(c, items, once, s); break;   \
+  }
+    if (dtype == PIA_DTYPE_F32) {
+      PIA_K8(PIA_DTYPE_F32)
+    } else if (dtype == PIA_DTYPE_F16) {
+      PIA_K8(PIA_DTYPE_F16)
+    } else {
+      PIA_K8(PIA_DTYPE_BF16)
+    }
+#undef PIA_K8
+    const int rc = check_launch("kv8_attention");
+    if (rc) return rc;
+  }
+  return 0;
+}

@@ -1,0 +1,531 @@
+// Appending a batch's new tokens to a paged cache with the rotary positions applied on the way, into
+// pools of the model's type or 8-bit ones, and reading contexts back from the 8-bit pool.
+//
+// Rows cu_new[b] .. cu_new[b + 1] of q, k and v are the last tokens of sequence b, whose context_lens
+// counts them; a token's position is its place in the context. q is rotated into q_out, k rotated
+// into its slot, v copied into its slot.
+//
+// A workgroup owns an aligned block of 16 positions of one sequence (and a share of the heads), so
+// that one wave sees all the new tokens that share an 8-bit scale, and the (cos, sin) of its tokens
+// are computed once for all its heads. Blocks are numbered without a scan: sequence b's start at
+// cu_new[b] / 16 + 2 b, which leaves room for every block that its rows can touch. Bound by HBM for
+// prompts (each element once) and by latency for single tokens.
+#include <algorithm>
+
+#include "kv8.h"
+#include "rope.h"
+
+namespace pia {
+namespace {
+
+constexpr int KA_THREADS = 256;
+constexpr int KA_WAVES = KA_THREADS / 64;
+
+struct AppendArgs {
+  void* q_out;
+  const void *q, *k, *v;
+  int64_t q_tok, q_head, k_tok, k_head, v_tok, v_head;
+  void *k_pages, *v_pages;
+  float *k_scale, *v_scale;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t *lens, *cu;
+  int64_t num_tokens;
+  const double* turns;
+  int64_t num_pages;
+  int num_seqs, pairs, inter, Hq, Hkv, D, P;
+  double factor;
+  float k_bound;
+  int k_vec, v_vec, whole;
+};
+
+// sequence whose numbers start last at or before id: base(b) = cu[b] / 16 + step b
+__device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int64_t id, int step) {
+  int lo = 0, hi = n - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((cu[mid] >> 4) + int64_t(step) * mid <= id) lo = mid; else hi = mid - 1;
+  }
+  return lo;
+}
+
+__device__ __forceinline__ float finite_abs(float x) {
+  const float a = fabsf(x);
+  return a < INFINITY ? a : 0.f;
+}
+
+// 16 consecutive elements from p
+template <int DT>
+__device__ __forceinline__ void load16f(const typename Elem<DT>::T* p, bool vec, float (&x)[16]) {
+  if (vec) rope::load<DT, 16, true>(p, x);
+  else rope::load<DT, 16, false>(p, x);
+}
+
+// One (block, kv head) of the 8-bit pool by one wave. o0: the block's offset of its first new token,
+// n: how many; r0: their first row.
+template <int DT>
+__device__ void append8(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
+                        int o0, int n, int64_t page, int sub) {
+  using T = typename Elem<DT>::T;
+  const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = 2 * a.pairs;
+  const int64_t head = page * a.Hkv + h;
+  // K: lane (t, g) has token t's elements 16 c .. 16 c + 15 for c = g, g + 4, ...
+  {
+    const int t = lane & 15, g = lane >> 4;
+    const bool fresh = t >= o0 && t < o0 + n, old = t < o0;
+    const T* x = static_cast<const T*>(a.k) + (r0 + (fresh ? t - o0 : 0)) * a.k_tok + h * a.k_head;
+    uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.k_pages) +
+                                            head * D * P) + sub * 16 + t;
+    float* scale = a.k_scale + head * (P / 16) + sub;
+    const float was = o0 > 0 ? *scale : 0.f;
+    float most = 0.f;
+    for (int c = g; fresh && 16 * c < D; c += 4) {
+      float v[16];
+      load16f<DT>(x + 16 * c, a.k_vec, v);
+#pragma unroll
+      for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_abs(v[e]));
+    }
+    const float now = fmaxf(was, kv8::scale_of(wave_max(most) * a.k_bound));
+    const float inv = kv8::inverse(now), ratio = was * inv;
+#pragma unroll 1
+    for (int c = g; 16 * c < D; c += 4) {  // loaded again, from the cache: in registers, D 256 spills
+      uint4 w;
+      if (fresh) {
+        float v[16];
+        load16f<DT>(x + 16 * c, a.k_vec, v);
+        if (16 * c < rd) {
+          const float2* cs = tab + (t - o0) * tab_row;
+          float r[16];
+          if (a.inter) {
+#pragma unroll
+            for (int e = 0; e < 16; e += 2) {
+              const bool in = 16 * c + e < rd;
+              const float2 f = in ? cs[8 * c + e / 2] : make_float2(1.f, 0.f);
+              r[e] = in ? rope::turn(v[e], -v[e + 1], f.x, f.y) : v[e];
+              r[e + 1] = in ? rope::turn(v[e + 1], v[e], f.x, f.y) : v[e + 1];
+            }
+          } else if (a.pairs % 16 == 0) {
+            const bool first = 16 * c < a.pairs;
+            const int other = first ? 16 * c + a.pairs : 16 * c - a.pairs;
+            const float sign = first ? -1.f : 1.f;
+            float p[16];
+            load16f<DT>(x + other, a.k_vec, p);
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const float2 f = cs[(first ? 16 * c : other) + e];
+              r[e] = rope::turn(v[e], sign * p[e], f.x, f.y);
+            }
+          } else {
+#pragma unroll
+            for (int e = 0; e < 16; ++e) {
+              const int d = 16 * c + e;
+              if (d < rd) {
+                const bool first = d < a.pairs;
+                const float2 f = cs[first ? d : d - a.pairs];
+                const float p = Elem<DT>::load(x, first ? d + a.pairs : d - a.pairs);
+                r[e] = rope::turn(v[e], first ? -p : p, f.x, f.y);
+              } else {
+                r[e] = v[e];
+              }
+            }
+          }
+#pragma unroll
+          for (int e = 0; e < 16; ++e) v[e] = r[e];
+        }
+        w = make_uint4(kv8::encode4(v[0], v[1], v[2], v[3], inv),
+                       kv8::encode4(v[4], v[5], v[6], v[7], inv),
+                       kv8::encode4(v[8], v[9], v[10], v[11], inv),
+                       kv8::encode4(v[12], v[13], v[14], v[15], inv));
+        codes[c * P] = w;
+      } else if (old && now != was) {
+        w = codes[c * P];
+        w.x = kv8::rescale4(w.x, ratio);
+        w.y = kv8::rescale4(w.y, ratio);
+        w.z = kv8::rescale4(w.z, ratio);
+        w.w = kv8::rescale4(w.w, ratio);
+        codes[c * P] = w;
+      }
+    }
+    if (lane == 0) *scale = now;
+  }
+  // V: lane (x, tg) has elements 64 i + 4 x .. + 3 of tokens 4 tg .. 4 tg + 3, one word of codes for
+  // each element; a word that also holds earlier or stale tokens keeps theirs
+  {
+    const int x4 = (lane & 15) * 4, t0 = (lane >> 4) * 4;
+    uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.v_pages) + head * D * P +
+                                            (sub * 4 + (lane >> 4)) * 4 * D);
+    float* scale = a.v_scale + head * (P / 16) + sub;
+    const float was = o0 > 0 ? *scale : 0.f;
+    // the 4 tokens' elements d .. d + 3, zeros where they are not new
+    auto load_v = [&](int d, float (&v)[4][4]) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int t = t0 + j;
+        if (t >= o0 && t < o0 + n) {
+          const T* x = static_cast<const T*>(a.v) + (r0 + t - o0) * a.v_tok + h * a.v_head + d;
+          if (a.v_vec) rope::load<DT, 4, true>(x, v[j]);
+          else rope::load<DT, 4, false>(x, v[j]);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
+        }
+      }
+    };
+    float most = 0.f;
+    for (int d = x4; d < D; d += 64) {
+      float v[4][4];
+      load_v(d, v);
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = fmaxf(most, finite_abs(v[j][e]));
+    }
+    const float now = fmaxf(was, kv8::scale_of(wave_max(most)));
+    const float inv = kv8::inverse(now), ratio = was * inv;
+    // bytes of a word: new tokens, and earlier ones that the scale moves
+    uint32_t fresh = 0, old = 0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int t = t0 + j;
+      fresh |= t >= o0 && t < o0 + n ? 0xffu << (8 * j) : 0u;
+      old |= t < o0 ? 0xffu << (8 * j) : 0u;
+    }
+    const bool moved = old != 0 && now != was;
+#pragma unroll 1
+    for (int d = x4; d < D && (fresh != 0 || moved); d += 64) {
+      float v[4][4];
+      load_v(d, v);
+      uint32_t w[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) w[e] = kv8::encode4(v[0][e], v[1][e], v[2][e], v[3][e], inv);
+      uint4* at = codes + d / 4;
+      if (fresh != 0xffffffffu) {
+        const uint4 c = *at;
+        const uint32_t before[4] = {c.x, c.y, c.z, c.w};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          uint32_t b = before[e];
+          if (moved) b = (kv8::rescale4(b, ratio) & old) | (b & ~old);
+          w[e] = (w[e] & fresh) | (b & ~fresh);
+        }
+      }
+      *at = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    if (lane == 0) *scale = now;
+  }
+}
+
+// One (block, kv head) of a pool of the model's type by one wave: lanes are elements, each with the
+// block's tokens, so that a full block goes out in 16-byte stores.
+template <int DT>
+__device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
+                             int64_t p0, int n, const int32_t* row) {
+  using T = typename Elem<DT>::T;
+  constexpr int TV = 16 / int(sizeof(T));
+  const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = 2 * a.pairs;
+  const T* k = static_cast<const T*>(a.k) + r0 * a.k_tok + h * a.k_head;
+  const T* v = static_cast<const T*>(a.v) + r0 * a.v_tok + h * a.v_head;
+  T* kp = static_cast<T*>(a.k_pages);
+  T* vp = static_cast<T*>(a.v_pages);
+  auto turned = [&](int t, int d) -> float {
+    const T* x = k + t * a.k_tok;
+    const float own = Elem<DT>::load(x, d);
+    if (d >= rd) return own;
+    const bool first = a.inter ? !(d & 1) : d < a.pairs;
+    const int other = a.inter ? d ^ 1 : first ? d + a.pairs : d - a.pairs;
+    const float p = Elem<DT>::load(x, other);
+    const float2 f = tab[t * tab_row + (a.inter ? d >> 1 : first ? d : other)];
+    return rope::turn(own, first ? -p : p, f.x, f.y);
+  };
+  // a whole block in whole 16-byte vectors of one page
+  if (n == 16 && a.whole) {
+    const int32_t page = row[p0 / P];
+    if (uint32_t(page) >= uint64_t(a.num_pages)) return;
+    const int64_t at = (int64_t(page) * a.Hkv + h) * D * P + p0 % P;
+    for (int d = lane; d < D; d += 64) {
+      struct alignas(16) Pack {
+        T x[TV];
+      };
+      Pack ko[16 / TV], vo[16 / TV];
+#pragma unroll
+      for (int t = 0; t < 16; ++t) {
+        Elem<DT>::store(ko[t / TV].x, t % TV, turned(t, d));
+        vo[t / TV].x[t % TV] = v[t * a.v_tok + d];
+      }
+#pragma unroll
+      for (int i = 0; i < 16 / TV; ++i) {
+        reinterpret_cast<Pack*>(kp + at + int64_t(d) * P)[i] = ko[i];
+        reinterpret_cast<Pack*>(vp + at + int64_t(d) * P)[i] = vo[i];
+      }
+    }
+    return;
+  }
+  for (int t = 0; t < n; ++t) {
+    const int64_t pos = p0 + t;
+    const int32_t page = row[pos / P];
+    if (uint32_t(page) >= uint64_t(a.num_pages)) continue;
+    const int64_t at = (int64_t(page) * a.Hkv + h) * D * P + pos % P;
+    for (int d = lane; d < D; d += 64) {
+      Elem<DT>::store(kp, at + int64_t(d) * P, turned(t, d));
+      vp[at + int64_t(d) * P] = v[t * a.v_tok + d];
+    }
+  }
+}
+
+template <int DT, bool INTER, bool VEC>
+__device__ __forceinline__ void turn_q(const AppendArgs& a, const float2* tab, int tab_row,
+                                       int64_t r0, int n, int h0, int h1) {
+  using T = typename Elem<DT>::T;
+  using U = rope::Units<DT, INTER, VEC>;
+  const unsigned per_head = U::count(a.pairs, a.D), per_tok = per_head * (h1 - h0);
+  for (unsigned i = threadIdx.x; i < per_tok * n; i += KA_THREADS) {
+    const unsigned t = i / per_tok, r = i - t * per_tok, hh = r / per_head;
+    const int h = h0 + int(hh);
+    const T* x = static_cast<const T*>(a.q) + (r0 + t) * a.q_tok + h * a.q_head;
+    T* o = static_cast<T*>(a.q_out) + ((r0 + t) * a.Hq + h) * a.D;
+    U::run(o, x, int(r - hh * per_head), tab + t * tab_row, a.pairs, a.D, 1.f);
+  }
+}
+
+template <int DT, bool KV8, bool QVEC>
+__global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
+  extern __shared__ float2 tab[];
+  int64_t id = blockIdx.x;
+  int b = int(id), row_lo = int(id), n_b = 1;
+  if (a.cu) {
+    b = sequence_of(a.cu, a.num_seqs, id, 2);
+    row_lo = a.cu[b];
+    n_b = a.cu[b + 1] - row_lo;
+    id -= (row_lo >> 4) + int64_t(2) * b;
+  } else {
+    id = 0;
+  }
+  // the block's new tokens: positions p0 .. p0 + n - 1, rows r0 ..
+  const int64_t end = a.lens[b], start = end - n_b;
+  const int64_t blk = (start >> 4) + id;
+  const int64_t p0 = max(start, blk * 16);
+  const int64_t r0 = row_lo + (p0 - start);
+  const int n = int(min(min(end, blk * 16 + 16) - p0, a.num_tokens - r0));
+  if (n <= 0 || row_lo < 0 || id < 0) return;
+  // a row of the table more than the pairs: 16 tokens' entries of one pair then sit in 16 banks
+  const int tab_row = a.pairs + 1;
+  for (int i = threadIdx.x; i < n * a.pairs; i += KA_THREADS) {
+    const int t = i / a.pairs, p = i - t * a.pairs;
+    tab[t * tab_row + p] = rope::cos_sin(a.turns[p], p0 + t, a.factor);
+  }
+  __syncthreads();
+  const int S = gridDim.y, y = blockIdx.y;
+  if (a.q) {
+    const int h0 = int(int64_t(a.Hq) * y / S), h1 = int(int64_t(a.Hq) * (y + 1) / S);
+    if (h1 > h0) {
+      if (a.inter) turn_q<DT, true, QVEC>(a, tab, tab_row, r0, n, h0, h1);
+      else turn_q<DT, false, QVEC>(a, tab, tab_row, r0, n, h0, h1);
+    }
+  }
+  // positions outside the table (or before the context) have no slot
+  if (p0 < 0 || p0 / a.P >= a.bt_stride) return;
+  const int m = int(min(int64_t(n), a.bt_stride * a.P - p0));
+  const int32_t* row = a.bt + b * a.bt_stride;
+  const int wave = threadIdx.x >> 6;
+  for (int h = y + S * wave; h < a.Hkv; h += S * KA_WAVES) {
+    if constexpr (KV8) {
+      const int32_t page = row[p0 / a.P];
+      if (uint32_t(page) < uint64_t(a.num_pages))
+        append8<DT>(a, tab, tab_row, h, r0, int(p0 & 15), m, page, int(p0 % a.P) >> 4);
+    } else {
+      append_plain<DT>(a, tab, tab_row, h, r0, p0, m, row);
+    }
+  }
+}
+
+// Contexts of the 8-bit pool in logical order: one wave for each (block of 16 tokens, kv head).
+template <int DT>
+__global__ __launch_bounds__(256) void kv8_gather_kernel(
+    typename Elem<DT>::T* __restrict__ k_out, typename Elem<DT>::T* __restrict__ v_out,
+    const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
+    const float* __restrict__ k_scale, const float* __restrict__ v_scale,
+    const int32_t* __restrict__ bt, int64_t bt_stride, const int64_t* __restrict__ cu, int num_seqs,
+    int64_t total, int Hkv, int D, int P, int64_t num_pages) {
+  const int lane = threadIdx.x & 63;
+  const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  const int64_t id = w / Hkv;
+  const int h = int(w - id * Hkv);
+  int lo = 0, hi = num_seqs - 1;
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if ((cu[mid] >> 4) + mid <= id) lo = mid; else hi = mid - 1;
+  }
+  const int b = lo;
+  const int64_t first = cu[b], blk = id - ((first >> 4) + b);
+  const int64_t len = min(cu[b + 1], total) - first;
+  const int64_t n64 = min(len, bt_stride * P) - blk * 16;
+  if (n64 <= 0 || first < 0 || blk < 0) return;
+  const int n = int(min(n64, int64_t(16)));
+  const int32_t page = bt[b * bt_stride + blk * 16 / P];
+  const bool ok = uint32_t(page) < uint64_t(num_pages);
+  const int sub = int(blk % (P / 16));
+  const int64_t head = int64_t(ok ? page : 0) * Hkv + h;
+  const int64_t row0 = first + blk * 16;
+  const float ks = ok ? k_scale[head * (P / 16) + sub] : 0.f;
+  const float vs = ok ? v_scale[head * (P / 16) + sub] : 0.f;
+  const int t = lane & 15, g = lane >> 4;
+  const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int c = g + 4 * i;
+    if (16 * c < D && t < n) {
+      const uint4 x = ok ? reinterpret_cast<const uint4*>(k_pages + head * D * P)[c * P + sub * 16 + t]
+                         : zero;
+      const uint32_t q[4] = {x.x, x.y, x.z, x.w};
+      float r[16];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        float f[4];
+        kv8::decode4(q[e], f);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) r[4 * e + j] = f[j] * ks;
+      }
+      rope::store<DT, 16, true>(k_out + ((row0 + t) * Hkv + h) * D + 16 * c, r);
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const int d = 64 * i + 4 * t;
+    if (d < D) {
+      const uint4 x = ok ? reinterpret_cast<const uint4*>(v_pages + head * D * P +
+                                                          (sub * 4 + g) * 4 * D)[d / 4]
+                         : zero;
+      float f[4][4];
+      kv8::decode4(x.x, f[0]);
+      kv8::decode4(x.y, f[1]);
+      kv8::decode4(x.z, f[2]);
+      kv8::decode4(x.w, f[3]);
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        if (4 * g + j < n) {
+          const float r[4] = {f[0][j] * vs, f[1][j] * vs, f[2][j] * vs, f[3][j] * vs};
+          rope::store<DT, 4, true>(v_out + ((row0 + 4 * g + j) * Hkv + h) * D + d, r);
+        }
+      }
+    }
+  }
+}
+
+}  // namespace
+}  // namespace pia
+
+using namespace pia;
+
+extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
+                             int64_t q_head_stride, const void* k, int64_t k_token_stride,
+                             int64_t k_head_stride, const void* v, int64_t v_token_stride,
+                             int64_t v_head_stride, void* k_pages, void* v_pages, float* k_scales,
+                             float* v_scales, const int32_t* block_tables, int64_t bt_stride,
+                             const int32_t* context_lens, const int32_t* cu_new,
+                             int64_t num_tokens, int num_seqs, const double* turns, int pairs,
+                             double factor, int interleaved, int num_heads, int num_kv_heads,
+                             int head_dim, int page_size, int64_t num_pages, int dtype,
+                             void* stream) {
+  if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
+    return fail(PIA_EUNSUPPORTED, "kv_append: dtype must be bf16, fp16 or fp32");
+  if (num_tokens < 0 || num_seqs < 0 || num_heads < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
+      page_size <= 0 || num_pages < 0 || bt_stride < 0 || pairs < 0 ||
+      2 * int64_t(pairs) > head_dim)
+    return fail(PIA_EINVAL, "kv_append: invalid size");
+  if (head_dim > 512) return fail(PIA_EUNSUPPORTED, "kv_append: head_dim over 512");
+  const bool kv8 = k_scales != nullptr;
+  if (kv8 != (v_scales != nullptr)) return fail(PIA_EINVAL, "kv_append: one scale array of two");
+  if (kv8 && !kv8::pool_shape(head_dim, page_size))
+    return fail(PIA_EUNSUPPORTED,
+                "kv_append: 8-bit pools take head_dim and page_size in multiples of 16, up to 256 "
+                "and 4096");
+  if (num_tokens > 0x7fffffff || int64_t(num_heads) * head_dim > (1 << 24))
+    return fail(PIA_EINVAL, "kv_append: too many tokens or heads");
+  if (!cu_new && num_tokens != num_seqs)
+    return fail(PIA_EINVAL, "kv_append: without cu_new one token per sequence");
+  if (num_tokens == 0 || num_seqs == 0) return 0;
+  if (!k || !v || !k_pages || !v_pages || !context_lens || (bt_stride && !block_tables) ||
+      (pairs && !turns) || !q != !q_out)
+    return fail(PIA_EINVAL, "kv_append: null pointer");
+  const int elem = dtype == PIA_DTYPE_F32 ? 4 : 2;
+  const bool inter = interleaved != 0;
+  if (kv8 && (!aligned(k_pages, 16) || !aligned(v_pages, 16) || !aligned(k_scales, 4) ||
+              !aligned(v_scales, 4)))
+    return fail(PIA_EINVAL, "kv_append: pools must be 16-byte aligned");
+  const int64_t v16 = 16 / elem;
+  // c: a rotated element is at most sqrt(2) times the factor times the head's largest element
+  const float bound = pairs ? float(1.4142135623730951 * factor) : 1.f;
+  AppendArgs a{q_out, q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+               v_token_stride, v_head_stride, k_pages, v_pages, k_scales, v_scales, block_tables,
+               bt_stride, context_lens, cu_new, num_tokens, turns, num_pages, num_seqs, pairs,
+               interleaved != 0, q ? num_heads : 0, num_kv_heads, head_dim, page_size, factor,
+               bound, 0, 0, 0};
+  a.k_vec = aligned(k, 16) && k_token_stride % v16 == 0 && k_head_stride % v16 == 0;
+  a.whole = page_size % 16 == 0 && aligned(k_pages, 16) && aligned(v_pages, 16);
+  a.v_vec = aligned(v, 4 * elem) && v_token_stride % 4 == 0 && v_head_stride % 4 == 0;
+  const bool qvec = q && rope::vectors(elem, inter, pairs, head_dim, q, q_out, q_token_stride,
+                                       q_head_stride);
+  const int64_t blocks = cu_new ? num_tokens / 16 + 2 * int64_t(num_seqs) : num_seqs;
+  if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv_append: too many sequences");
+  // shares of the heads, until there are two workgroups for every compute unit; each computes the
+  // table of its tokens
+  const int split = int(std::max<int64_t>(
+      1, std::min<int64_t>(ceil_div(num_kv_heads, KA_WAVES), 2 * device_cus() / blocks)));
+  const dim3 grid{unsigned(blocks), unsigned(split), 1u};
+  const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1);
+  hipStream_t s = as_stream(stream);
+#define PIA_KA(DT, KV8, QV) \
+  hipLaunchKernelGGL((kv_append_kernel<DT, KV8, QV>), grid, dim3(KA_THREADS), lds, s, a)
+#define PIA_KA_D(DT)                                                   \
+  if (kv8) {                                                           \
+    if (qvec) PIA_KA(DT, true, true); else PIA_KA(DT, true, false);    \
+  } else {                                                             \
+    if (qvec) PIA_KA(DT, false, true); else PIA_KA(DT, false, false);  \
+  }
+  if (dtype == PIA_DTYPE_F32) {
+    PIA_KA_D(PIA_DTYPE_F32)
+  } else if (dtype == PIA_DTYPE_F16) {
+    PIA_KA_D(PIA_DTYPE_F16)
+  } else {
+    PIA_KA_D(PIA_DTYPE_BF16)
+  }
+#undef PIA_KA_D
+#undef PIA_KA
+  return check_launch("kv_append");
+}
+
+extern "C" int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, const void* v_pages,
+                              const float* k_scales, const float* v_scales,
+                              const int32_t* block_tables, int64_t bt_stride,
+                              const int64_t* cu_seqlens, int num_seqs, int64_t total_tokens,
+                              int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                              int dtype, void* stream) {
+  if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
+    return fail(PIA_EUNSUPPORTED, "kv8_gather: dtype must be bf16, fp16 or fp32");
+  if (num_seqs < 0 || total_tokens < 0 || num_kv_heads <= 0 || num_pages <= 0 || bt_stride < 0)
+    return fail(PIA_EINVAL, "kv8_gather: invalid size");
+  if (!kv8::pool_shape(head_dim, page_size))
+    return fail(PIA_EUNSUPPORTED,
+                "kv8_gather: head_dim and page_size in multiples of 16, up to 256 and 4096");
+  if (num_seqs == 0 || total_tokens == 0 || bt_stride == 0) return 0;
+  if (!k_out || !v_out || !k_pages || !v_pages || !k_scales || !v_scales || !block_tables ||
+      !cu_seqlens)
+    return fail(PIA_EINVAL, "kv8_gather: null pointer");
+  if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
+    return fail(PIA_EINVAL, "kv8_gather: pools and outputs must be 16-byte aligned");
+  const int64_t waves = (total_tokens / 16 + num_seqs) * int64_t(num_kv_heads);
+  const int64_t wgs = ceil_div(waves, 4);
+  if (wgs > 0x7fffffff) return fail(PIA_EINVAL, "kv8_gather: too many tokens");
+  hipStream_t s = as_stream(stream);
+#define PIA_KG(DT)                                                                              \
+  hipLaunchKernelGGL((kv8_gather_kernel<DT>), dim3(unsigned(wgs)), dim3(256), 0, s,             \
+                     static_cast<Elem<DT>::T*>(k_out), static_cast<Elem<DT>::T*>(v_out),        \
+                     static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages), \
+                     k_scales, v_scales, block_tables, bt_stride, cu_seqlens, num_seqs,         \
+                     total_tokens, num_kv_heads, head_dim, page_size, num_pages)
+  if (dtype == PIA_DTYPE_F32) PIA_KG(PIA_DTYPE_F32);
+  else if (dtype == PIA_DTYPE_F16) PIA_KG(PIA_DTYPE_F16);
+  else PIA_KG(PIA_DTYPE_BF16);
+#undef PIA_KG
+  return check_launch("kv8_gather");
+}

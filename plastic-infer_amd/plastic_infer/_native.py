@@ -22,6 +22,7 @@ _P = ctypes.c_void_p
 _I = ctypes.c_int
 _L = ctypes.c_int64
 _F = ctypes.c_float
+_D = ctypes.c_double
 
 # name -> (restype, argtypes)
 _SIGNATURES: dict[str, tuple[object, list[object]]] = {
@@ -76,6 +77,14 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pia_slot_cache_materialize": (_I, [_P, _L, _P, _P, _L, _P, _P, _P, _P, _I, _I, _P]),
     "pia_slot_cache_invalidate": (_I, [_P, _L, _P, _P, _L, _L, _L, _P]),
     "pia_prefill_hit_compact": (_I, [_P, _P, _P, _P, _L, _L, _I, _P]),
+    "pia_rotary": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _P, _I, _P, _I, _D, _I, _I, _L, _I, _I, _I,
+                        _I, _P]),
+    "pia_kv_append": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _L, _P, _P,
+                           _L, _I, _P, _I, _D, _I, _I, _I, _I, _I, _L, _I, _P]),
+    "pia_kv8_gather": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _L, _I, _I, _I, _L, _I, _P]),
+    "pia_kv8_attention_workspace_bytes": (_L, [_I]),
+    "pia_kv8_attention": (_I, [_P, _P, _L, _P, _P, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I,
+                               _I, _L, _F, _I, _P, _L, _P]),
     "pia_hbm_read_probe": (_I, [_P, _L, _P, _L, _P, _P]),
     "pia_hbm_read_rows_probe": (_I, [_P, _L, _I, _I, _P, _P]),
 }
@@ -121,6 +130,15 @@ def call(name: str, *args) -> int:
         msg = lib.pia_last_error().decode(errors="replace")
         raise NativeError(f"{name} failed ({rc}): {msg}")
     return rc
+
+
+def call_on(device: torch.device, name: str, *args) -> int:
+    """call() with `device` as the current device: launches and size rules are those of the device
+    that holds the tensors, whichever one the caller has current."""
+    if torch.cuda.current_device() == device.index:
+        return call(name, *args)
+    with torch.cuda.device(device):
+        return call(name, *args)
 
 
 def query(name: str, *args) -> int:
