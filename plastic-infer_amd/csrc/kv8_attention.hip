@@ -38,7 +38,7 @@ constexpr int KA_WG_WAVES = 4;
 constexpr int KA_WGS_PER_CU = 2;   // two waves per SIMD
 constexpr int KA_RSRC_WORD3 = 0x00020000;
 constexpr float KA_RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
-constexpr int KA_MERGE_THREADS = 256;
+constexpr int KA_JOIN_MIN = 128, KA_JOIN_MAX = 1024;  // threads of the joining workgroups
 
 struct AttnArgs {
   void* out;
@@ -546,10 +546,15 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   }
 }
 
-// The items that were cut: their pieces joined in the order of the waves. One workgroup per item;
-// threads are (row, four elements). Items without keys are zeros.
+// The items that were cut: their pieces joined, in the order of the waves. One workgroup per item.
+// Items without keys are zeros.
+// the weight of a piece whose maximum is m against the joined one
+__device__ __forceinline__ float weight(float m, float joined) {
+  return m == joined ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - joined);
+}
+
 template <int QT, int DP>
-__global__ __launch_bounds__(KA_MERGE_THREADS) void kv8_attention_join_kernel(AttnArgs a,
+__global__ __launch_bounds__(KA_JOIN_MAX) void kv8_attention_join_kernel(AttnArgs a,
                                                                               int64_t waves) {
   using T = typename Elem<QT>::T;
   constexpr int STEP = 16 * (DP > 128 ? 2 : 4);
@@ -583,28 +588,69 @@ __global__ __launch_bounds__(KA_MERGE_THREADS) void kv8_attention_join_kernel(At
   }
   const float* first = a.parts + (w0 * 2 + (s.steps > 0 && first_of(w0, nw, total) >= from ? 0 : 1)) *
                                      part_floats<DP>;
-  auto piece = [&](int64_t w) {
-    return w == w0 ? first : a.parts + w * 2 * part_floats<DP>;
-  };
-  for (int u = threadIdx.x; u < rows * (a.D / 4); u += KA_MERGE_THREADS) {
-    const int r = u / (a.D / 4), d = 4 * (u - r * (a.D / 4));
+  // A thread has four elements u of the item (row r, elements d .. d + 3) and every S-th piece, eight
+  // of them on their way at once; threads of one u meet in LDS, in order.
+  const int per_row = a.D / 4, U = rows * per_row, np = int(w1 - w0) + 1;
+  const int threads = blockDim.x;
+  const int S = s.steps > 0 ? max(1, min(threads / U, np)) : 1;
+  __shared__ float4 o_s[KA_JOIN_MAX];
+  __shared__ float2 ml_s[KA_JOIN_MAX];
+  for (int u0 = 0; u0 < U; u0 += threads) {  // more than one turn: then S is 1
+    const int u = u0 + threadIdx.x % min(U, threads), sp = threadIdx.x / min(U, threads);
+    const int r = u / per_row, d = 4 * (u - r * per_row);
+    const bool ok = u < U && sp < S;
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-    if (s.steps > 0) {
-      for (int64_t w = w0; w <= w1; ++w)
-        M = __builtin_elementwise_maximum(M, piece(w)[16 * DP + r]);
-      for (int64_t w = w0; w <= w1; ++w) {
-        const float* p = piece(w);
-        const float mw = p[16 * DP + r], f = mw == M ? (M == -INFINITY ? 0.f : 1.f)
-                                                     : __builtin_amdgcn_exp2f(mw - M);
-        const float4 x = *reinterpret_cast<const float4*>(p + r * DP + d);
-        L += p[16 * DP + 16 + r] * f;
-        o.x += x.x * f;
-        o.y += x.y * f;
-        o.z += x.z * f;
-        o.w += x.w * f;
+    if (ok && s.steps > 0) {
+      constexpr int N = 8;
+      for (int p0 = sp; p0 < np; p0 += N * S) {
+        float pm[N], pl[N];
+        float4 po[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int pi = min(p0 + j * S, np - 1);  // past the end: the last one again, without weight
+          const float* p = pi == 0 ? first : a.parts + (w0 + pi) * 2 * part_floats<DP>;
+          pm[j] = p0 + j * S < np ? p[16 * DP + r] : -INFINITY;
+          pl[j] = p[16 * DP + 16 + r];
+          po[j] = *reinterpret_cast<const float4*>(p + r * DP + d);
+        }
+        float m = M;
+#pragma unroll
+        for (int j = 0; j < N; ++j) m = __builtin_elementwise_maximum(m, pm[j]);
+        const float f0 = weight(M, m);
+        L *= f0;
+        o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          if (p0 + j * S >= np) continue;
+          const float f = weight(pm[j], m);
+          L += pl[j] * f;
+          o = make_float4(fmaf(po[j].x, f, o.x), fmaf(po[j].y, f, o.y), fmaf(po[j].z, f, o.z),
+                          fmaf(po[j].w, f, o.w));
+        }
+        M = m;
       }
     }
+    if (S > 1) {
+      o_s[threadIdx.x] = o;
+      ml_s[threadIdx.x] = make_float2(M, L);
+      __syncthreads();
+      if (sp > 0) return;  // S > 1: the only turn
+      float m = M;
+      for (int k = 1; k < S; ++k) m = __builtin_elementwise_maximum(m, ml_s[threadIdx.x + k * U].x);
+      const float f0 = weight(M, m);
+      L *= f0;
+      o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+      for (int k = 1; k < S; ++k) {
+        const float4 x = o_s[threadIdx.x + k * U];
+        const float2 ml = ml_s[threadIdx.x + k * U];
+        const float f = weight(ml.x, m);
+        L += ml.y * f;
+        o = make_float4(fmaf(x.x, f, o.x), fmaf(x.y, f, o.y), fmaf(x.z, f, o.z),
+                        fmaf(x.w, f, o.w));
+      }
+    }
+    if (!ok) continue;
     const float inv = L == 0.f ? 0.f : 1.f / L;
     const int rr = 16 * i + r, pos = rr / a.G;
     T* out = static_cast<T*>(a.out) + ((s.row0 + pos) * a.Hq + h * a.G + rr - pos * a.G) * a.D + d;
@@ -630,8 +676,10 @@ void launch(const AttnArgs& a, int64_t items, bool once, hipStream_t s) {
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, true>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, false>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
-  hipLaunchKernelGGL((kv8_attention_join_kernel<QT, DP>), dim3(unsigned(items)),
-                     dim3(KA_MERGE_THREADS), 0, s, a, resident_waves());
+  // few items: many pieces each, which the threads share; many: two or three
+  const int threads = items * 4 <= resident_waves() ? KA_JOIN_MAX : KA_JOIN_MIN;
+  hipLaunchKernelGGL((kv8_attention_join_kernel<QT, DP>), dim3(unsigned(items)), dim3(threads), 0, s,
+                     a, resident_waves());
 }
 
 }  // namespace

@@ -5,9 +5,10 @@
 // counts them; a token's position is its place in the context. q is rotated into q_out, k rotated
 // into its slot, v copied into its slot.
 //
-// A workgroup owns an aligned block of 16 positions of one sequence (and a share of the heads), so
-// that one wave sees all the new tokens that share an 8-bit scale, and the (cos, sin) of its tokens
-// are computed once for all its heads. Blocks are numbered without a scan: sequence b's start at
+// The unit of work is an aligned block of 16 positions of one sequence: one wave then sees all the new
+// tokens that share an 8-bit scale. Some workgroups rotate a block's q heads, others take four of its
+// K and V heads, one a wave, so that a single token's chain of loads is as short as it can be; each
+// computes the (cos, sin) of its tokens once. Blocks are numbered without a scan: sequence b's start at
 // cu_new[b] / 16 + 2 b, which leaves room for every block that its rows can touch. Bound by HBM for
 // prompts (each element once) and by latency for single tokens.
 #include <algorithm>
@@ -36,7 +37,7 @@ struct AppendArgs {
   int num_seqs, pairs, inter, Hq, Hkv, D, P;
   double factor;
   float k_bound;
-  int k_vec, v_vec, whole;
+  int k_vec, v_vec, k_pair, v_pair, whole, q_shares;
 };
 
 // sequence whose numbers start last at or before id: base(b) = cu[b] / 16 + step b
@@ -61,15 +62,14 @@ __device__ __forceinline__ void load16f(const typename Elem<DT>::T* p, bool vec,
   else rope::load<DT, 16, false>(p, x);
 }
 
-// One (block, kv head) of the 8-bit pool by one wave. o0: the block's offset of its first new token,
-// n: how many; r0: their first row.
+// The K codes of one (block, kv head) of the 8-bit pool by one wave: lane (t, g) has token t's
+// elements 16 c .. 16 c + 15 for c = g, g + 4, ... o0: the block's offset of its first new token, n:
+// how many; r0: their first row; was: the block's scale, 0 where it holds no earlier tokens.
 template <int DT>
-__device__ void append8(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
-                        int o0, int n, int64_t page, int sub) {
+__device__ void append8_k(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
+                          int o0, int n, int64_t head, int sub, float was) {
   using T = typename Elem<DT>::T;
   const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = 2 * a.pairs;
-  const int64_t head = page * a.Hkv + h;
-  // K: lane (t, g) has token t's elements 16 c .. 16 c + 15 for c = g, g + 4, ...
   {
     const int t = lane & 15, g = lane >> 4;
     const bool fresh = t >= o0 && t < o0 + n, old = t < o0;
@@ -77,7 +77,6 @@ __device__ void append8(const AppendArgs& a, const float2* tab, int tab_row, int
     uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.k_pages) +
                                             head * D * P) + sub * 16 + t;
     float* scale = a.k_scale + head * (P / 16) + sub;
-    const float was = o0 > 0 ? *scale : 0.f;
     float most = 0.f;
     for (int c = g; fresh && 16 * c < D; c += 4) {
       float v[16];
@@ -148,14 +147,20 @@ __device__ void append8(const AppendArgs& a, const float2* tab, int tab_row, int
     }
     if (lane == 0) *scale = now;
   }
-  // V: lane (x, tg) has elements 64 i + 4 x .. + 3 of tokens 4 tg .. 4 tg + 3, one word of codes for
-  // each element; a word that also holds earlier or stale tokens keeps theirs
+}
+
+// Its V codes: lane (x, tg) has elements 64 i + 4 x .. + 3 of tokens 4 tg .. 4 tg + 3, one word of codes
+// for each element; a word that also holds earlier or stale tokens keeps theirs.
+template <int DT>
+__device__ void append8_v(const AppendArgs& a, int h, int64_t r0, int o0, int n, int64_t head,
+                          int sub, float was) {
+  using T = typename Elem<DT>::T;
+  const int lane = threadIdx.x & 63, D = a.D, P = a.P;
   {
     const int x4 = (lane & 15) * 4, t0 = (lane >> 4) * 4;
     uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.v_pages) + head * D * P +
                                             (sub * 4 + (lane >> 4)) * 4 * D);
     float* scale = a.v_scale + head * (P / 16) + sub;
-    const float was = o0 > 0 ? *scale : 0.f;
     // the 4 tokens' elements d .. d + 3, zeros where they are not new
     auto load_v = [&](int d, float (&v)[4][4]) {
 #pragma unroll
@@ -215,48 +220,64 @@ __device__ void append8(const AppendArgs& a, const float2* tab, int tab_row, int
   }
 }
 
-// One (block, kv head) of a pool of the model's type by one wave: lanes are elements, each with the
-// block's tokens, so that a full block goes out in 16-byte stores.
+// K (which = 0) or V of one (block, kv head) of a pool of the model's type by one wave: a lane has
+// two elements of all the block's tokens, so that a full block goes out in 16-byte stores.
 template <int DT>
-__device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
-                             int64_t p0, int n, const int32_t* row) {
+__device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row, int which, int h,
+                             int64_t r0, int64_t p0, int n, const int32_t* row) {
   using T = typename Elem<DT>::T;
   constexpr int TV = 16 / int(sizeof(T));
-  const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = 2 * a.pairs;
-  const T* k = static_cast<const T*>(a.k) + r0 * a.k_tok + h * a.k_head;
-  const T* v = static_cast<const T*>(a.v) + r0 * a.v_tok + h * a.v_head;
-  T* kp = static_cast<T*>(a.k_pages);
-  T* vp = static_cast<T*>(a.v_pages);
-  auto turned = [&](int t, int d) -> float {
-    const T* x = k + t * a.k_tok;
-    const float own = Elem<DT>::load(x, d);
-    if (d >= rd) return own;
-    const bool first = a.inter ? !(d & 1) : d < a.pairs;
-    const int other = a.inter ? d ^ 1 : first ? d + a.pairs : d - a.pairs;
-    const float p = Elem<DT>::load(x, other);
-    const float2 f = tab[t * tab_row + (a.inter ? d >> 1 : first ? d : other)];
-    return rope::turn(own, first ? -p : p, f.x, f.y);
-  };
+  const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = which ? 0 : 2 * a.pairs;
+  const int64_t tok = which ? a.v_tok : a.k_tok;
+  const T* x = static_cast<const T*>(which ? a.v : a.k) + r0 * tok + h * (which ? a.v_head : a.k_head);
+  T* pool = static_cast<T*>(which ? a.v_pages : a.k_pages);
   // a whole block in whole 16-byte vectors of one page
-  if (n == 16 && a.whole) {
+  if (n == 16 && a.whole && (which ? a.v_pair : a.k_pair)) {
     const int32_t page = row[p0 / P];
     if (uint32_t(page) >= uint64_t(a.num_pages)) return;
-    const int64_t at = (int64_t(page) * a.Hkv + h) * D * P + p0 % P;
-    for (int d = lane; d < D; d += 64) {
-      struct alignas(16) Pack {
-        T x[TV];
-      };
-      Pack ko[16 / TV], vo[16 / TV];
+    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + p0 % P;
+    struct alignas(2 * sizeof(T)) Two {
+      T v[2];
+    };
+    struct alignas(16) Pack {
+      T x[TV];
+    };
+    for (int d = 2 * lane; d < D; d += 128) {
+      Two own[16], other[16];
+      const bool turned = d < rd, first = d < a.pairs;
+      const int od = first ? d + a.pairs : d - a.pairs;
+#pragma unroll
+      for (int t = 0; t < 16; ++t) own[t] = *reinterpret_cast<const Two*>(x + t * tok + d);
+      if (turned && !a.inter) {
+#pragma unroll
+        for (int t = 0; t < 16; ++t) other[t] = *reinterpret_cast<const Two*>(x + t * tok + od);
+      }
+      Pack o[2][16 / TV];
 #pragma unroll
       for (int t = 0; t < 16; ++t) {
-        Elem<DT>::store(ko[t / TV].x, t % TV, turned(t, d));
-        vo[t / TV].x[t % TV] = v[t * a.v_tok + d];
+        T e0 = own[t].v[0], e1 = own[t].v[1];
+        if (turned) {
+          const float2* cs = tab + t * tab_row;
+          const float v0 = Elem<DT>::load(own[t].v, 0), v1 = Elem<DT>::load(own[t].v, 1);
+          if (a.inter) {
+            const float2 f = cs[d / 2];
+            Elem<DT>::store(&e0, 0, rope::turn(v0, -v1, f.x, f.y));
+            Elem<DT>::store(&e1, 0, rope::turn(v1, v0, f.x, f.y));
+          } else {
+            const float2 f0 = cs[first ? d : od], f1 = cs[(first ? d : od) + 1];
+            const float w0 = Elem<DT>::load(other[t].v, 0), w1 = Elem<DT>::load(other[t].v, 1);
+            Elem<DT>::store(&e0, 0, rope::turn(v0, first ? -w0 : w0, f0.x, f0.y));
+            Elem<DT>::store(&e1, 0, rope::turn(v1, first ? -w1 : w1, f1.x, f1.y));
+          }
+        }
+        o[0][t / TV].x[t % TV] = e0;
+        o[1][t / TV].x[t % TV] = e1;
       }
 #pragma unroll
-      for (int i = 0; i < 16 / TV; ++i) {
-        reinterpret_cast<Pack*>(kp + at + int64_t(d) * P)[i] = ko[i];
-        reinterpret_cast<Pack*>(vp + at + int64_t(d) * P)[i] = vo[i];
-      }
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 16 / TV; ++i)
+          reinterpret_cast<Pack*>(to + int64_t(d + e) * P)[i] = o[e][i];
     }
     return;
   }
@@ -264,10 +285,18 @@ __device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row
     const int64_t pos = p0 + t;
     const int32_t page = row[pos / P];
     if (uint32_t(page) >= uint64_t(a.num_pages)) continue;
-    const int64_t at = (int64_t(page) * a.Hkv + h) * D * P + pos % P;
+    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + pos % P;
     for (int d = lane; d < D; d += 64) {
-      Elem<DT>::store(kp, at + int64_t(d) * P, turned(t, d));
-      vp[at + int64_t(d) * P] = v[t * a.v_tok + d];
+      const T* xt = x + t * tok;
+      T e = xt[d];
+      if (d < rd) {
+        const bool first = a.inter ? !(d & 1) : d < a.pairs;
+        const int od = a.inter ? d ^ 1 : first ? d + a.pairs : d - a.pairs;
+        const float p = Elem<DT>::load(xt, od);
+        const float2 f = tab[t * tab_row + (a.inter ? d >> 1 : first ? d : od)];
+        Elem<DT>::store(&e, 0, rope::turn(Elem<DT>::load(xt, d), first ? -p : p, f.x, f.y));
+      }
+      to[int64_t(d) * P] = e;
     }
   }
 }
@@ -307,6 +336,24 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   const int64_t r0 = row_lo + (p0 - start);
   const int n = int(min(min(end, blk * 16 + 16) - p0, a.num_tokens - r0));
   if (n <= 0 || row_lo < 0 || id < 0) return;
+  const int y = blockIdx.y, wave = threadIdx.x >> 6;
+  const bool for_q = y < a.q_shares;
+  // keys and values: what a wave needs of tables and scales is on its way before the angles
+  const bool slots = !for_q && p0 >= 0 && p0 / a.P < a.bt_stride;  // else no position has one
+  const int32_t* row = a.bt + b * a.bt_stride;
+  const int unit = (y - a.q_shares) * KA_WAVES + wave, which = unit & 1, h = unit >> 1;
+  int64_t head = -1;
+  float was = 0.f;
+  const int sub = int(p0 % a.P) >> 4, o0 = int(p0 & 15);
+  if constexpr (KV8) {
+    if (slots && h < a.Hkv) {
+      const int32_t page = row[p0 / a.P];
+      if (uint32_t(page) < uint64_t(a.num_pages)) {
+        head = int64_t(page) * a.Hkv + h;
+        if (o0 > 0) was = (which ? a.v_scale : a.k_scale)[head * (a.P / 16) + sub];
+      }
+    }
+  }
   // a row of the table more than the pairs: 16 tokens' entries of one pair then sit in 16 banks
   const int tab_row = a.pairs + 1;
   for (int i = threadIdx.x; i < n * a.pairs; i += KA_THREADS) {
@@ -314,27 +361,21 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
     tab[t * tab_row + p] = rope::cos_sin(a.turns[p], p0 + t, a.factor);
   }
   __syncthreads();
-  const int S = gridDim.y, y = blockIdx.y;
-  if (a.q) {
-    const int h0 = int(int64_t(a.Hq) * y / S), h1 = int(int64_t(a.Hq) * (y + 1) / S);
-    if (h1 > h0) {
-      if (a.inter) turn_q<DT, true, QVEC>(a, tab, tab_row, r0, n, h0, h1);
-      else turn_q<DT, false, QVEC>(a, tab, tab_row, r0, n, h0, h1);
-    }
+  if (for_q) {
+    const int h0 = int(int64_t(a.Hq) * y / a.q_shares);
+    const int h1 = int(int64_t(a.Hq) * (y + 1) / a.q_shares);
+    if (a.inter) turn_q<DT, true, QVEC>(a, tab, tab_row, r0, n, h0, h1);
+    else turn_q<DT, false, QVEC>(a, tab, tab_row, r0, n, h0, h1);
+    return;
   }
-  // positions outside the table (or before the context) have no slot
-  if (p0 < 0 || p0 / a.P >= a.bt_stride) return;
+  if (!slots || h >= a.Hkv) return;
   const int m = int(min(int64_t(n), a.bt_stride * a.P - p0));
-  const int32_t* row = a.bt + b * a.bt_stride;
-  const int wave = threadIdx.x >> 6;
-  for (int h = y + S * wave; h < a.Hkv; h += S * KA_WAVES) {
-    if constexpr (KV8) {
-      const int32_t page = row[p0 / a.P];
-      if (uint32_t(page) < uint64_t(a.num_pages))
-        append8<DT>(a, tab, tab_row, h, r0, int(p0 & 15), m, page, int(p0 % a.P) >> 4);
-    } else {
-      append_plain<DT>(a, tab, tab_row, h, r0, p0, m, row);
-    }
+  if constexpr (KV8) {
+    if (head < 0) return;
+    if (which) append8_v<DT>(a, h, r0, o0, m, head, sub, was);
+    else append8_k<DT>(a, tab, tab_row, h, r0, o0, m, head, sub, was);
+  } else {
+    append_plain<DT>(a, tab, tab_row, which, h, r0, p0, m, row);
   }
 }
 
@@ -459,19 +500,26 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
                v_token_stride, v_head_stride, k_pages, v_pages, k_scales, v_scales, block_tables,
                bt_stride, context_lens, cu_new, num_tokens, turns, num_pages, num_seqs, pairs,
                interleaved != 0, q ? num_heads : 0, num_kv_heads, head_dim, page_size, factor,
-               bound, 0, 0, 0};
+               bound};
   a.k_vec = aligned(k, 16) && k_token_stride % v16 == 0 && k_head_stride % v16 == 0;
   a.whole = page_size % 16 == 0 && aligned(k_pages, 16) && aligned(v_pages, 16);
   a.v_vec = aligned(v, 4 * elem) && v_token_stride % 4 == 0 && v_head_stride % 4 == 0;
+  a.k_pair = pairs % 2 == 0 && head_dim % 2 == 0 && aligned(k, 2 * elem) &&
+             k_token_stride % 2 == 0 && k_head_stride % 2 == 0;
+  a.v_pair = head_dim % 2 == 0 && aligned(v, 2 * elem) && v_token_stride % 2 == 0 &&
+             v_head_stride % 2 == 0;
   const bool qvec = q && rope::vectors(elem, inter, pairs, head_dim, q, q_out, q_token_stride,
                                        q_head_stride);
   const int64_t blocks = cu_new ? num_tokens / 16 + 2 * int64_t(num_seqs) : num_seqs;
   if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv_append: too many sequences");
-  // shares of the heads, until there are two workgroups for every compute unit; each computes the
-  // table of its tokens
-  const int split = int(std::max<int64_t>(
-      1, std::min<int64_t>(ceil_div(num_kv_heads, KA_WAVES), 2 * device_cus() / blocks)));
-  const dim3 grid{unsigned(blocks), unsigned(split), 1u};
+  // Workgroups of a block: some for q, about four vectors for each thread, and one for every four of
+  // the K and V heads, a wave each. Each computes the table of its tokens.
+  const int per_wg = KA_THREADS * 4 * (qvec ? int(v16) : 1) * (inter ? 1 : 2);
+  a.q_shares = a.Hq ? int(std::min<int64_t>(
+      a.Hq, ceil_div(int64_t(cu_new ? 16 : 1) * a.Hq * head_dim, per_wg))) : 0;
+  const int64_t shares = a.q_shares + ceil_div(2 * int64_t(num_kv_heads), KA_WAVES);
+  if (shares > 65535) return fail(PIA_EINVAL, "kv_append: too many heads");
+  const dim3 grid{unsigned(blocks), unsigned(shares), 1u};
   const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1);
   hipStream_t s = as_stream(stream);
 #define PIA_KA(DT, KV8, QV) \

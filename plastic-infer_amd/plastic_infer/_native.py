@@ -91,6 +91,8 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
 
 EXPECTED_ABI = 10
 
+_HIP = torch.version.hip is not None
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 _lock = threading.Lock()
 _lib: ctypes.CDLL | None = None
 
@@ -102,6 +104,8 @@ class NativeError(RuntimeError):
 def load(path: pathlib.Path | None = None) -> ctypes.CDLL:
     """dlopen the library once and declare every exported signature."""
     global _lib
+    if _lib is not None:
+        return _lib
     with _lock:
         if _lib is not None:
             return _lib
@@ -153,6 +157,12 @@ def query(name: str, *args) -> int:
 def require_device(*tensors: torch.Tensor, names: tuple[str, ...] | None = None) -> torch.device:
     """All tensors must live on the same HIP device; returns it. CPU tensors are rejected:
     this package keeps KV pages and expert slots in HBM and has no host execution path."""
+    try:   # the usual case at a quarter of the cost: nothing to report
+        index = tensors[0].get_device()
+        if _HIP and index >= 0 and all(t.is_cuda and t.get_device() == index for t in tensors):
+            return tensors[0].device
+    except (AttributeError, IndexError):
+        pass
     dev = None
     for i, t in enumerate(tensors):
         label = names[i] if names else f"argument {i}"
@@ -183,4 +193,6 @@ def ptr(t: torch.Tensor | None) -> int | None:
 
 def stream_of(device: torch.device) -> int:
     """Raw hipStream_t of torch's current stream on `device`."""
+    if _raw_stream is not None and device.index is not None:
+        return _raw_stream(device.index)   # the handle without a Stream object: 0.1 us for 1.9
     return torch.cuda.current_stream(device).cuda_stream

@@ -10,7 +10,7 @@ import torch
 
 from .. import _native as N
 from .paged_kv import _check_pool
-from .rotary import RopeParams, check_rope, heads_view
+from .rotary import RopeParams, check_rope, fresh_like, heads_view
 
 
 def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -20,13 +20,12 @@ def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
                 cu_new: torch.Tensor | None, rope: RopeParams | None) -> torch.Tensor | None:
     """Checks and launch shared by both pool types; shape: (num_pages, Hkv, D, P)."""
     num_pages, Hkv, D, P = shape
-    named = [("k", k), ("v", v), ("k_pages", pools[0]), ("v_pages", pools[1]),
-             ("block_tables", block_tables), ("context_lens", context_lens)]
-    named += [("q", q)] if q is not None else []
-    named += [("cu_new", cu_new)] if cu_new is not None else []
-    named += [("k_scale", scales[0]), ("v_scale", scales[1])] if scales is not None else []
-    dev = N.require_device(*(t for _, t in named), names=tuple(n for n, _ in named))
-    if torch.is_grad_enabled() and any(t.requires_grad for t in (k, v) + (() if q is None else (q,))):
+    dev = N.require_device(k, v, *pools, block_tables, context_lens,
+                           *(() if q is None else (q,)), *(() if cu_new is None else (cu_new,)),
+                           names=("k", "v", "k_pages", "v_pages", "block_tables", "context_lens",
+                                  "cu_new" if q is None else "q", "cu_new"))
+    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad
+                                    or (q is not None and q.requires_grad)):
         raise ValueError("an append has no gradient: call it under torch.no_grad()")
     k, v = heads_view("k", k), heads_view("v", v)
     n = k.shape[0]
@@ -46,14 +45,14 @@ def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
             raise ValueError("without cu_new there must be exactly one token per sequence")
     elif cu_new.dtype != torch.int32 or cu_new.shape != (B + 1,):
         raise ValueError("cu_new must be int32 [B + 1]")
-    if rope is not None and check_rope(rope, D) != dev:
-        raise ValueError(f"rope.turns is on {rope.turns.device}, expected {dev}")
+    if rope is not None:
+        check_rope(rope, D, dev)
     out = None
     if q is not None:
         q = heads_view("q", q)
         if q.shape[0] != n or q.shape[2] != D:
             raise ValueError(f"q must be [{n}, heads, {D}], got {tuple(q.shape)}")
-        out = torch.empty(q.shape, dtype=q.dtype, device=dev)
+        out = fresh_like(q)
     if n == 0 or B == 0:
         return out
     has_q = q is not None and q.shape[1] > 0

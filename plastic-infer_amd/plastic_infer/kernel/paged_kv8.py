@@ -16,7 +16,7 @@ import torch
 
 from .. import _native as N
 from .kv_append import append_call
-from .rotary import RopeParams
+from .rotary import RopeParams, fresh_like
 
 BLOCK = 16   # tokens that share a scale
 
@@ -64,6 +64,16 @@ def _check_shape(head_dim: int, page_size: int) -> None:
 
 
 def _check_pools(p: KV8Pools) -> tuple[int, int, int, int]:
+    """(num_pages, Hkv, D, P) of valid pools, checked once for each KV8Pools."""
+    shape = p.__dict__.get("_shape")
+    if shape is None:
+        shape = p.__dict__["_shape"] = _checked_shape(p)
+    return shape
+
+
+def _checked_shape(p: KV8Pools) -> tuple[int, int, int, int]:
+    N.require_device(p.k, p.v, p.k_scale, p.v_scale,
+                     names=("pools.k", "pools.v", "pools.k_scale", "pools.v_scale"))
     if p.k.dim() != 5 or p.k.shape[4] != 16:
         raise ValueError(f"pools.k must be [num_pages, H, D / 16, P, 16], got {tuple(p.k.shape)}")
     n, h, d, page = p.shape
@@ -72,10 +82,12 @@ def _check_pools(p: KV8Pools) -> tuple[int, int, int, int]:
         raise ValueError(f"pools.v must be {(n, h, page // 4, d, 4)}, got {tuple(p.v.shape)}")
     if p.k.dtype != torch.float8_e4m3fn or p.v.dtype != torch.float8_e4m3fn:
         raise ValueError("pools.k and pools.v must be float8_e4m3fn")
-    for name, s in (("k_scale", p.k_scale), ("v_scale", p.v_scale)):
-        if s.dtype != torch.float32 or s.shape != (n, h, page // BLOCK):
-            raise ValueError(f"pools.{name} must be float32 {(n, h, page // BLOCK)}")
-    if not all(t.is_contiguous() for t in (p.k, p.v, p.k_scale, p.v_scale)):
+    want = (n, h, page // BLOCK)
+    if p.k_scale.dtype != torch.float32 or p.v_scale.dtype != torch.float32 \
+            or p.k_scale.shape != want or p.v_scale.shape != want:
+        raise ValueError(f"pools.k_scale and pools.v_scale must be float32 {want}")
+    if not (p.k.is_contiguous() and p.v.is_contiguous() and p.k_scale.is_contiguous()
+            and p.v_scale.is_contiguous()):
         raise ValueError("KV pools must be contiguous")
     return n, h, d, page
 
@@ -100,15 +112,13 @@ def kv8_gather(pools: KV8Pools, block_tables: torch.Tensor, cu_seqlens: torch.Te
     b's tokens in logical order, [total_tokens, Hkv, D] in dtype (or that of the `out` buffers,
     whose first dimension is then the total). bf16 and fp32 hold the pool's values exactly.
     max_seq_len: a bound of every length; 0 gathers nothing."""
-    N.require_device(pools.k, pools.v, pools.k_scale, pools.v_scale, block_tables, cu_seqlens,
-                     names=("pools.k", "pools.v", "pools.k_scale", "pools.v_scale",
-                            "block_tables", "cu_seqlens"))
-    dev = pools.k.device
     num_pages, H, D, P = _check_pools(pools)
+    dev = N.require_device(pools.k, block_tables, cu_seqlens,
+                           names=("pools.k", "block_tables", "cu_seqlens"))
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
         raise ValueError("block_tables must be int32 [B, max_pages]")
     bt = block_tables.contiguous()
-    cu = cu_seqlens.to(torch.int64).contiguous()
+    cu = (cu_seqlens if cu_seqlens.dtype == torch.int64 else cu_seqlens.to(torch.int64)).contiguous()
     B = bt.shape[0]
     if cu.shape != (B + 1,):
         raise ValueError("cu_seqlens must have B + 1 entries")
@@ -119,7 +129,7 @@ def kv8_gather(pools: KV8Pools, block_tables: torch.Tensor, cu_seqlens: torch.Te
         v_out = torch.empty_like(k_out)
     else:
         k_out, v_out = out
-        N.require_device(k_out, v_out, pools.k, names=("out[0]", "out[1]", "pools.k"))
+        N.require_device(pools.k, k_out, v_out, names=("pools.k", "out[0]", "out[1]"))
         if k_out.dim() != 3 or k_out.shape[1:] != (H, D) or v_out.shape != k_out.shape \
                 or v_out.dtype != k_out.dtype \
                 or not (k_out.is_contiguous() and v_out.is_contiguous()):
@@ -148,13 +158,13 @@ def kv8_attention_workspace_bytes(head_dim: int, device: torch.device | None = N
 
 
 def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out, workspace):
-    named = [("q", q), ("pools.k", pools.k), ("pools.v", pools.v), ("pools.k_scale", pools.k_scale),
-             ("pools.v_scale", pools.v_scale), ("block_tables", block_tables),
-             ("kv_lens", kv_lens)]
-    named += [(n, t) for n, t in (("cu_q", cu_q), ("q_pos_offsets", q_pos_offsets), ("out", out),
-                                  ("workspace", workspace)) if t is not None]
-    dev = N.require_device(*(t for _, t in named), names=tuple(n for n, _ in named))
     num_pages, Hkv, D, P = _check_pools(pools)
+    dev = N.require_device(pools.k, q, block_tables, kv_lens,
+                           names=("pools.k", "q", "block_tables", "kv_lens"))
+    for name, t in (("cu_q", cu_q), ("q_pos_offsets", q_pos_offsets), ("out", out),
+                    ("workspace", workspace)):
+        if t is not None:
+            N.require_device(pools.k, t, names=("pools.k", name))
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
         raise ValueError(f"q must be [rows, Hq, {D}] with Hq a multiple of {Hkv}, got "
                          f"{tuple(q.shape)}")
@@ -163,8 +173,8 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
         raise ValueError("attention over the 8-bit cache has no gradient: call it under "
                          "torch.no_grad()")
     rows, Hq, _ = q.shape
-    vec = 16 // q.element_size()
-    if q.stride(2) != 1 or q.stride(1) != D or q.stride(0) % vec or q.data_ptr() % 16:
+    token, head, elem = q.stride()
+    if elem != 1 or head != D or token * q.element_size() % 16 or q.data_ptr() % 16:
         q = q.contiguous()
         if q.data_ptr() % 16:   # a contiguous view that starts between vectors
             q = q.clone()
@@ -182,7 +192,7 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
                                       or q_pos_offsets.shape != (B,)):
         raise ValueError("q_pos_offsets must be int32 [B]")
     if out is None:
-        out = torch.empty(rows, Hq, D, dtype=q.dtype, device=dev)
+        out = fresh_like(q)
     elif out.shape != (rows, Hq, D) or out.dtype != q.dtype or not out.is_contiguous() \
             or out.data_ptr() % 16:
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")

@@ -84,14 +84,21 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
     return RopeParams((freq / (2 * math.pi)).to(device), factor, bool(interleaved))
 
 
-def check_rope(rope: RopeParams, head_dim: int) -> torch.device:
-    dev = N.require_device(rope.turns, names=("rope.turns",))
+def check_rope(rope: RopeParams, head_dim: int, dev: torch.device) -> None:
     t = rope.turns
+    if not t.is_cuda or t.get_device() != dev.index:
+        raise ValueError(f"rope.turns is on {t.device}, expected {dev}")
     if t.dtype != torch.float64 or t.dim() != 1 or not t.is_contiguous():
         raise ValueError("rope.turns must be a contiguous float64 [pairs] tensor")
     if 2 * t.numel() > head_dim:
         raise ValueError(f"rope rotates {2 * t.numel()} elements of a head of {head_dim}")
-    return dev
+
+
+def fresh_like(t: torch.Tensor) -> torch.Tensor:
+    """A contiguous tensor of t's shape and type (empty_like takes half the time of empty)."""
+    if t.is_contiguous():
+        return torch.empty_like(t)
+    return torch.empty(t.shape, dtype=t.dtype, device=t.device)
 
 
 def heads_view(name: str, t: torch.Tensor) -> torch.Tensor:
@@ -103,21 +110,28 @@ def heads_view(name: str, t: torch.Tensor) -> torch.Tensor:
 
 def _launch(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor,
             rope: RopeParams, transposed: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
-    any_ = q if q is not None else k
-    n, _, D = any_.shape
-    views = [None if t is None else heads_view("q", t) for t in (q, k)]
-    outs = [None if t is None else torch.empty(t.shape, dtype=t.dtype, device=t.device)
-            for t in (q, k)]
-    heads = [0 if t is None else t.shape[1] for t in (q, k)]
-    strides = [s for t in views for s in ((0, 0) if t is None else (t.stride(0), t.stride(1)))]
-    if n and sum(heads):
-        N.call_on(any_.device, "pia_rotary", N.ptr(outs[0]), N.ptr(outs[1]), N.ptr(views[0]),
-                  N.ptr(views[1]), *strides, positions.data_ptr(),
-                  1 if positions.dtype == torch.int64 else 0, rope.turns.data_ptr(),
-                  rope.turns.numel(), rope.factor, 1 if rope.interleaved else 0,
-                  1 if transposed else 0, n, *heads, D, N.dtype_code(any_.dtype),
-                  N.stream_of(any_.device))
-    return outs[0], outs[1]
+    qo = ko = qp = kp = None
+    hq = hkv = qt = qh = kt = kh = 0
+    if q is not None:
+        q = heads_view("q", q)
+        n, hq, D = q.shape
+        qt, qh, _ = q.stride()
+        qo = fresh_like(q)
+        qp = q.data_ptr()
+    if k is not None:
+        k = heads_view("k", k)
+        n, hkv, D = k.shape
+        kt, kh, _ = k.stride()
+        ko = fresh_like(k)
+        kp = k.data_ptr()
+    if n and hq + hkv:
+        t, turns = (q if q is not None else k), rope.turns
+        dev = t.device
+        N.call_on(dev, "pia_rotary", N.ptr(qo), N.ptr(ko), qp, kp, qt, qh, kt, kh,
+                  positions.data_ptr(), 1 if positions.dtype == torch.int64 else 0,
+                  turns.data_ptr(), turns.numel(), rope.factor, 1 if rope.interleaved else 0,
+                  1 if transposed else 0, n, hq, hkv, D, N.dtype_code(t.dtype), N.stream_of(dev))
+    return qo, ko
 
 
 class _Rotary(torch.autograd.Function):
@@ -147,8 +161,10 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     [tokens]. Contiguous results; gradients flow to q and k in reverse mode. (A backward pass is
     captured into a graph only while no eager graph of the same leaves lives: torch's accumulation
     nodes keep the stream that made them, which is then part of the capture.)"""
-    given = [("q", q), ("positions", positions)] + ([] if k is None else [("k", k)])
-    dev = N.require_device(*(t for _, t in given), names=tuple(n for n, _ in given))
+    if k is None:
+        dev = N.require_device(q, positions, names=("q", "positions"))
+    else:
+        dev = N.require_device(q, k, positions, names=("q", "k", "positions"))
     q = heads_view("q", q)
     n, _, D = q.shape
     if k is not None:
@@ -160,8 +176,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
     N.dtype_code(q.dtype)
     if positions.shape != (n,) or positions.dtype not in (torch.int64, torch.int32):
         raise ValueError(f"positions must be int64 or int32 [{n}]")
-    if check_rope(rope, D) != dev:
-        raise ValueError(f"rope.turns is on {rope.turns.device}, expected {dev}")
+    check_rope(rope, D, dev)
     positions = positions.contiguous()
     if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
         return _Rotary.apply(q, k, positions, rope, False)
