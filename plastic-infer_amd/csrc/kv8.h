@@ -59,6 +59,18 @@ __device__ __forceinline__ float inverse(float scale) {
   return __uint_as_float((254u << 23) - __float_as_uint(scale));
 }
 
+// Multi-row attention on tiles in LDS (kv8_prefill.hip): whether a call takes it, and its launch
+// (arguments already checked by pia_kv8_attention).
+}  // namespace kv8
+bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
+                      const int32_t* cu_q, float scale);
+int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
+                       const uint8_t* vp, const float* ks, const float* vs, const int32_t* bt,
+                       int64_t bt_stride, const int32_t* lens, const int32_t* cu,
+                       const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
+                       int D, int P, int64_t num_pages, float scale_log2, hipStream_t s);
+namespace kv8 {
+
 inline bool pool_shape(int D, int P) {
   return D > 0 && D % 16 == 0 && D <= 256 && P > 0 && P % BLOCK == 0 && P <= 4096;
 }

@@ -1,0 +1,506 @@
+// Attention of many query rows per sequence (prefill, chunked prefill) over the 8-bit KV pool on the
+// matrix cores: bf16 or fp16 q (DT), head_dim 64 or 128, any page size of the pool.
+//
+// Work item (one workgroup of NW waves): one kv head and 32 NW / G consecutive query positions of one
+// sequence, i.e. up to 32 NW (position, q head) rows that share the kv head's keys: row r is position
+// s0 + r / G, head h * G + r % G. Wave w owns rows 32 w .. 32 w + 31, one 32 x 32 product block. The
+// keys go by tiles of 64 tokens (four blocks). Codes come from the pool into registers a tile
+// ahead, and on their way into LDS, in the middle of the tile before theirs, they are widened to
+// DT with their scale: once for all rows, where an operand widened at its use would be widened by
+// every wave. bf16 holds a code times its scale exactly; fp16 does for scales of 2^-15 .. 2^6 and
+// within 2^-25 below (values beyond 65504 are infinite there).
+//
+// Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
+// 8 (l / 32) + e; of C, lane l has column l % 32 and rows 8 i + 4 (l / 32) + j, i, j < 4)
+//   S^T = K . q^T  lane l has the scores of row l % 32 for tokens 8 i + 4 (l / 32) + j of each 32
+//   online softmax base 2, per row in fp32; a row's scores sit in two lanes (l, l ^ 32)
+//   O^T += V^T . P^T  the probabilities are the B operand straight from the score registers (rounded
+//                  to DT): of a block's tokens, lane half hh holds 4 hh + j and 8 + 4 hh + j. Rows of
+//                  the result are elements, so a lane has 4 D / 16 of them of its own row l % 32: what
+//                  a row's maximum and sum do to it needs no exchange between lanes.
+// LDS tiles (16-byte units, XORed with a term of their row): K [token][d]: unit u (d 8 u .. + 7) of
+// token t at u ^ t % 16 (head_dim 64: u ^ t / 2 % 8); V [d][token]: unit 2 m + hh (block m, tokens
+// 4 hh + j, then 8 + 4 hh + j) of element d at (2 m + hh) ^ (d / 4 % 8) ^ (d / 2 % 2). With the bank
+// rules of gfx950 (stores: 8 lanes over 32 banks; 16-byte reads: lanes {0-3, 12-15, 20-27} or the
+// others over 64) all of them are conflict-free but K stores at head_dim 64.
+#include <algorithm>
+
+#include "attn_tiles.h"
+#include "kv8.h"
+
+namespace pia {
+namespace {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+constexpr int P8_KT = 64;            // keys per tile: four blocks
+constexpr int P8_MAX_SEQS = 1024;    // sequences per launch (tile prefix in LDS)
+constexpr int P8_AHEAD = 4;          // LDS operand reads in flight ahead of the products
+constexpr int P8_RSRC_WORD3 = 0x00020000;
+constexpr float P8_RESCALE = 8.0f;   // log2: how far a row's maximum may run ahead of its reference
+
+struct PrefillArgs {
+  void* out;
+  const void* q;
+  int64_t q_stride;
+  const uint8_t *kp, *vp;
+  const float *ks, *vs;
+  const int32_t* bt;
+  int64_t bt_stride;
+  const int32_t *lens, *cu, *offs;
+  int64_t rows, num_pages;
+  float scale_log2;
+  int B, Hq, Hkv, G, P, ppt;
+};
+
+template <int DT>
+__device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, f32x16_t c) {
+  if constexpr (DT == PIA_DTYPE_F16)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(tile::f16x8_t, a),
+                                                  __builtin_bit_cast(tile::f16x8_t, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(tile::bf16x8_t, a),
+                                                   __builtin_bit_cast(tile::bf16x8_t, b), c, 0, 0,
+                                                   0);
+}
+
+// two codes (the low or high half of a word) times scale as two DT values
+template <int DT, bool HI>
+__device__ __forceinline__ uint32_t widen(uint32_t w, float scale) {
+  if constexpr (DT == PIA_DTYPE_F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+template <int DT>
+__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b, float scale) {
+  return make_uint4(widen<DT, false>(a, scale), widen<DT, true>(a, scale),
+                    widen<DT, false>(b, scale), widen<DT, true>(b, scale));
+}
+
+// sum of a pair of DT values onto c
+template <int DT>
+__device__ __forceinline__ float add_pair(uint32_t x, float c) {
+  typedef __bf16 bf2 __attribute__((ext_vector_type(2)));
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  if constexpr (DT == PIA_DTYPE_F16)
+    return __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, x), __builtin_bit_cast(h2, 0x3c003c00u), c,
+                                  false);
+  else
+    return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, x),
+                                           __builtin_bit_cast(bf2, 0x3f803f80u), c, false);
+}
+
+// the 16-bit values of a word that are NaN, as 0xffff each
+template <int DT>
+__device__ __forceinline__ uint32_t nan_pairs(uint32_t w) {
+  constexpr uint32_t INF = DT == PIA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
+  return ((w & 0x7fffu) > INF ? 0xffffu : 0u) | (((w >> 16) & 0x7fffu) > INF ? 0xffff0000u : 0u);
+}
+
+__device__ __forceinline__ float swap_halves(float x) {  // the value of lane l ^ 32
+  const unsigned u = __float_as_uint(x);
+  const auto r = __builtin_amdgcn_permlane32_swap(u, u, false, false);
+  return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
+}
+
+template <int D, int NW, int DT>
+__global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArgs a) {
+  constexpr int NT = 64 * NW, KS = D / 16, NB = D / 32, UK = D / 8;
+  constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
+  __shared__ __align__(16) uint4 ks_lds[2][P8_KT * UK];
+  __shared__ __align__(16) uint4 vs_lds[2][D * 8];
+  __shared__ int tile_pref[P8_MAX_SEQS + 1];
+  __shared__ int wsum[NW];
+  __shared__ int nan_tile[2];  // 1 + the last tile staged into a buffer with a NaN in V
+  const int lane = threadIdx.x & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+
+  // work items per sequence and their prefix
+  if (threadIdx.x == 0) tile_pref[0] = 0;
+  if (threadIdx.x < 2) nan_tile[threadIdx.x] = 0;
+  int carry = 0;
+  for (int c0 = 0; c0 < a.B; c0 += NT) {
+    const int i = c0 + threadIdx.x;
+    int incl = 0;
+    if (i < a.B) {
+      const int64_t r0 = a.cu[i], n = min(int64_t(a.cu[i + 1]), a.rows) - r0;
+      incl = r0 >= 0 && n > 0 ? int((n + a.ppt - 1) / a.ppt) : 0;
+    }
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const int y = __shfl_up(incl, o, 64);
+      if (lane >= o) incl += y;
+    }
+    if (lane == 63) wsum[wave] = incl;
+    __syncthreads();
+    int base = carry;
+    for (int x = 0; x < wave; ++x) base += wsum[x];
+    if (i < a.B) tile_pref[i + 1] = base + incl;
+#pragma unroll
+    for (int x = 0; x < NW; ++x) carry += wsum[x];
+    __syncthreads();
+  }
+  int h, j;
+  if (!xcd_item(blockIdx.x, carry, a.Hkv, h, j)) return;
+  int lo = 0, hi = a.B - 1;  // the sequence holding the item: the last with tile_pref[b] <= j
+  while (lo < hi) {
+    const int mid = (lo + hi + 1) >> 1;
+    if (tile_pref[mid] <= j) lo = mid; else hi = mid - 1;
+  }
+  const int b = __builtin_amdgcn_readfirstlane(lo);
+  h = __builtin_amdgcn_readfirstlane(h);
+  // the last positions of a sequence, which see the most keys, first
+  const int s0 = __builtin_amdgcn_readfirstlane((tile_pref[b + 1] - 1 - j) * a.ppt);
+  const int64_t row0 = a.cu[b];
+  const int n_b = int(min(int64_t(a.cu[b + 1]), a.rows) - row0);
+  const int kv_len =
+      int(min(int64_t(max(a.lens[b], 0)), min(a.bt_stride * a.P, int64_t(0x7ffffff0))));
+  const int off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
+  const int s_last = min(s0 + a.ppt, n_b) - 1;
+  const int kmax = a.offs ? max(0, min(kv_len, off + s_last + 1)) : kv_len;
+  const int nkt = (kmax + P8_KT - 1) / P8_KT;
+  const int nblk = (kv_len + 15) >> 4, PB = a.P / 16;
+  const int32_t* btb = a.bt + int64_t(b) * a.bt_stride;
+
+  // this lane's row and its q operands, d = 16 ks + 8 (l / 32) .. + 7
+  const int hh = lane >> 5, n32 = lane & 31, G = a.G;
+  const int r = 32 * wave + n32, pos = s0 + r / G;
+  const bool live = r < a.ppt * G && pos < n_b;
+  const int lim = !live ? 0 : a.offs ? min(kv_len, off + pos + 1) : kv_len;
+  uint4 qr[KS];
+  {
+    const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (row0 + (live ? pos : 0)) * a.q_stride +
+                         int64_t(h * G + (live ? r % G : 0)) * D;
+#pragma unroll
+    for (int k = 0; k < KS; ++k)
+      qr[k] = live ? *reinterpret_cast<const uint4*>(qp + 16 * k + 8 * hh)
+                   : make_uint4(0u, 0u, 0u, 0u);
+  }
+  // every row of the item sees at least the keys below lim_min (its first position's limit)
+  const int lim_min = a.offs ? max(0, min(kv_len, off + s0 + 1)) : kv_len;
+
+  // staging: wave w (of four) moves block w of a tile, K by lanes (token l % 16, chunks l / 16 and
+  // l / 16 + 4), V by lanes (elements 4 (l % 32) .. + 3, token groups l / 32 and l / 32 + 2)
+  const int blk = wave & 3;
+  const bool st_k = !SPLIT || wave < 4, st_v = !SPLIT || wave >= 4;
+  constexpr int NK = D == 128 ? 2 : 1;  // 16-byte loads of K per lane (head_dim 64: 64 chunks)
+  const int64_t tile_bytes = int64_t(D) * a.P;
+  const int kt_tok = lane & 15, kt_c = lane >> 4;
+  const uint32_t k_off = uint32_t((kt_c * a.P + kt_tok) * 16), k_next = uint32_t(64 * a.P);
+  constexpr int VL = D / 4;  // lanes of a token group
+  const bool v_lane = (lane & 31) < VL;
+  const uint32_t v_off = uint32_t(hh * 4 * D + 16 * (lane & (VL - 1)));
+  uint4 kr[NK], vr[2];
+  float k_sc = 1.f, v_sc = 1.f;
+  // (page, head) of the blocks of a tile in lanes 0 .. 3, -1 where there is none; and their places
+  struct Where {
+    int head, sub;
+  };
+  auto where = [&](int kt) {
+    Where w{-1, 0};
+    const int kb = 4 * kt + lane;
+    if (lane < 4 && kb < nblk) {
+      const int slot = kb / PB;
+      const int32_t id = btb[slot];
+      w.sub = kb - slot * PB;
+      w.head = uint32_t(id) < uint64_t(a.num_pages) ? id * a.Hkv + h : -1;
+    }
+    return w;
+  };
+  auto fetch = [&](const Where& w) {
+    const int head = __builtin_amdgcn_readlane(w.head, blk);
+    const int sub = __builtin_amdgcn_readlane(w.sub, blk);
+    const bool ok = head >= 0;
+    const int64_t page = (ok ? head : 0) * tile_bytes;
+    if (st_k) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a.kp + page + sub * 256), 0, ok ? int(tile_bytes) - sub * 256 : 0,
+          P8_RSRC_WORD3);
+#pragma unroll
+      for (int i = 0; i < NK; ++i)
+        kr[i] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, k_off + i * k_next, 0, 0));
+      k_sc = ok ? a.ks[int64_t(head) * PB + sub] : 1.f;
+    }
+    if (st_v) {
+      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+          const_cast<uint8_t*>(a.vp + page + int64_t(sub) * 16 * D), 0, ok ? 16 * D : 0,
+          P8_RSRC_WORD3);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        vr[i] = __builtin_bit_cast(
+            uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, v_off + i * 8 * D, 0, 0));
+      v_sc = ok ? a.vs[int64_t(head) * PB + sub] : 1.f;
+    }
+  };
+  auto stage = [&](int buf, int kt) {
+    if (st_k) {
+      const int t = 16 * blk + kt_tok;
+      const int sw = D == 128 ? t & 15 : (t >> 1) & 7;
+#pragma unroll
+      for (int i = 0; i < NK; ++i) {
+        const int u = 2 * (kt_c + 4 * i);
+        ks_lds[buf][t * UK + (u ^ sw)] = widen8<DT>(kr[i].x, kr[i].y, k_sc);
+        ks_lds[buf][t * UK + ((u + 1) ^ sw)] = widen8<DT>(kr[i].z, kr[i].w, k_sc);
+      }
+    }
+    if (st_v) {
+      // tokens past the context hold whatever the page held: zeros
+      const int nv = kv_len - (64 * kt + 16 * blk + 4 * hh);
+      if (64 * kt + 64 > kv_len) {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int n = nv - 8 * i;
+          const uint32_t keep = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+          vr[i].x &= keep;
+          vr[i].y &= keep;
+          vr[i].z &= keep;
+          vr[i].w &= keep;
+        }
+      }
+      const uint32_t w0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w};
+      const uint32_t w1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+      uint32_t any = 0;
+      if (v_lane) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int d = 4 * (lane & (VL - 1)) + e;
+          const int sw = ((d >> 2) & 7) ^ ((d >> 1) & 1);
+          vs_lds[buf][d * 8 + ((2 * blk + hh) ^ sw)] = widen8<DT>(w0[e], w1[e], v_sc);
+          any |= ((w0[e] & 0x7f7f7f7fu) + 0x01010101u) | ((w1[e] & 0x7f7f7f7fu) + 0x01010101u);
+        }
+      }
+      if (any & 0x80808080u) nan_tile[buf] = kt + 1;
+    }
+  };
+  // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
+  // bits enter by XOR, so one base per lane and a constant give any of them; bases of a buffer, so
+  // that they are computed where they are used and not kept.
+  const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (D == 128 ? n32 & 15 : (n32 >> 1) & 7));
+  const uint32_t v_base = n32 * 128 + 16 * (hh ^ (((n32 >> 2) & 7) ^ ((n32 >> 1) & 1)));
+  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // powers of two
+  auto kread = [&](int buf, int tb, int k) {
+    const uint32_t at = ((k_base + buf * K_BUF) ^ (32 * k)) + 32 * tb * UK * 16;
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(&ks_lds[0][0]) + at);
+  };
+  auto vread = [&](int buf, int nb, int s) {
+    const uint32_t at = ((v_base + buf * V_BUF) ^ (32 * s)) + 32 * nb * 128;
+    return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(&vs_lds[0][0]) + at);
+  };
+
+  float m = -INFINITY, l = 0.f;  // the row's reference point in raw score units; its lane's sum
+  f32x16_t acc[NB];
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int v = 0; v < 16; ++v) acc[nb][v] = 0.f;
+
+  Where w_cur = where(0), w_nxt = where(1), w_far = where(2);
+  fetch(w_cur);
+  stage(0, 0);
+  fetch(w_nxt);
+  __syncthreads();
+  for (int kt = 0; kt < nkt; ++kt) {
+    const int buf = kt & 1;
+    const int there = int(__ballot(lane < 4 && w_cur.head >= 0)) & 0xf;
+    const bool full = there == 0xf && (kt + 1) * P8_KT <= lim_min;
+    const Where w_next = where(kt + 3);
+
+    f32x16_t sc[2];
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) sc[tb][v] = 0.f;
+    {
+      // operands are read P8_AHEAD products ahead of their use, kept so through the scheduler
+      uint4 kq[P8_AHEAD];
+#pragma unroll
+      for (int i = 0; i < P8_AHEAD; ++i) kq[i] = kread(buf, i & 1, i >> 1);
+#pragma unroll
+      for (int i = 0; i < 2 * KS; ++i) {
+        const uint4 k = kq[i % P8_AHEAD];
+        if (i + P8_AHEAD < 2 * KS)
+          kq[i % P8_AHEAD] = kread(buf, (i + P8_AHEAD) & 1, (i + P8_AHEAD) >> 1);
+        sc[i & 1] = mfma32<DT>(k, qr[i >> 1], sc[i & 1]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, P8_AHEAD, 0);
+#pragma unroll
+      for (int i = 0; i < 2 * KS - P8_AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, P8_AHEAD, 0);
+    }
+
+    const int rel = lim - (kt * P8_KT + 4 * hh);
+    if (!full) {
+#pragma unroll
+      for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (!(32 * tb + 8 * (v >> 2) + (v & 3) < rel && ((there >> (2 * tb + (v >> 3))) & 1)))
+            sc[tb][v] = -INFINITY;
+    }
+    float mx = -INFINITY;
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v) mx = __builtin_elementwise_maximum(mx, sc[tb][v]);
+    mx = __builtin_elementwise_maximum(mx, swap_halves(mx));
+    const float mref = (mx - m) * a.scale_log2 > P8_RESCALE || mx != mx ? mx : m;
+    const float nm = mref == -INFINITY ? 0.f : -mref * a.scale_log2;
+    if (__ballot(m != mref)) {
+      const float alpha = m == mref ? 1.f : __builtin_amdgcn_exp2f((m - mref) * a.scale_log2);
+      l *= alpha;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[nb][v] *= alpha;
+    }
+    m = mref;
+    uint4 pk[4];  // block s: the B operand of its 16 tokens
+#pragma unroll
+    for (int s = 0; s < 4; ++s) {
+      uint32_t w[4];
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const int v = 8 * (s & 1) + 2 * i;
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], a.scale_log2, nm));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], a.scale_log2, nm));
+        w[i] = tile::pack16x2<DT>(p0, p1);
+        l = add_pair<DT>(w[i], l);
+      }
+      pk[s] = make_uint4(w[0], w[1], w[2], w[3]);
+    }
+    stage(buf ^ 1, kt + 1);
+    fetch(w_far);
+    if (!full && nan_tile[buf] == kt + 1) {  // the same for every wave of the workgroup
+      // Zero times NaN is NaN: V's NaN would reach rows that may not see its token. The rows that see
+      // one get it by a product of their places, then the tile's are made zeros.
+      constexpr uint32_t ONE = DT == PIA_DTYPE_F16 ? 0x3c00u : 0x3f80u;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb) {
+        __builtin_amdgcn_sched_barrier(0);  // one block at a time (registers)
+        f32x16_t hit;
+#pragma unroll
+        for (int v = 0; v < 16; ++v) hit[v] = 0.f;
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          __builtin_amdgcn_sched_barrier(0);
+          const uint4 x = vread(buf, nb, s);
+          uint32_t see[4];
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int t = 16 * s + 8 * (i >> 1) + 2 * (i & 1);
+            const bool here = (there >> s) & 1;
+            see[i] = (here && t < rel ? ONE : 0u) | (here && t + 1 < rel ? ONE << 16 : 0u);
+          }
+          constexpr uint32_t ONES = ONE * 0x10001u;
+          hit = mfma32<DT>(make_uint4(nan_pairs<DT>(x.x) & ONES, nan_pairs<DT>(x.y) & ONES,
+                                      nan_pairs<DT>(x.z) & ONES, nan_pairs<DT>(x.w) & ONES),
+                           make_uint4(see[0], see[1], see[2], see[3]), hit);
+        }
+#pragma unroll
+        for (int v = 0; v < 16; ++v)
+          if (hit[v] > 0.f) acc[nb][v] = __builtin_nanf("");
+      }
+      __syncthreads();
+      for (int u = threadIdx.x; u < D * 8; u += NT) {
+        uint4 x = vs_lds[buf][u];
+        x.x &= ~nan_pairs<DT>(x.x);
+        x.y &= ~nan_pairs<DT>(x.y);
+        x.z &= ~nan_pairs<DT>(x.z);
+        x.w &= ~nan_pairs<DT>(x.w);
+        vs_lds[buf][u] = x;
+      }
+      __syncthreads();
+    }
+    {
+      uint4 vq[P8_AHEAD];
+#pragma unroll
+      for (int i = 0; i < P8_AHEAD; ++i) vq[i] = vread(buf, i % NB, i / NB);
+#pragma unroll
+      for (int i = 0; i < 4 * NB; ++i) {
+        const uint4 v = vq[i % P8_AHEAD];
+        if (i + P8_AHEAD < 4 * NB)
+          vq[i % P8_AHEAD] = vread(buf, (i + P8_AHEAD) % NB, (i + P8_AHEAD) / NB);
+        acc[i % NB] = mfma32<DT>(v, pk[i / NB], acc[i % NB]);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x100, P8_AHEAD, 0);
+#pragma unroll
+      for (int i = 0; i < 4 * NB - P8_AHEAD; ++i) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      }
+      __builtin_amdgcn_sched_group_barrier(0x008, P8_AHEAD, 0);
+    }
+    __syncthreads();
+    w_cur = w_nxt;
+    w_nxt = w_far;
+    w_far = w_next;
+  }
+
+  l += swap_halves(l);
+  if (!live) return;
+  const float inv = l == 0.f ? 0.f : 1.f / l;
+  uint16_t* o = static_cast<uint16_t*>(a.out) + ((row0 + pos) * a.Hq + h * G + r % G) * D + 4 * hh;
+#pragma unroll
+  for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      uint32_t w[2];
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        w[e] = tile::pack16x2<DT>(l == 0.f ? 0.f : acc[nb][4 * i + 2 * e] * inv,
+                                  l == 0.f ? 0.f : acc[nb][4 * i + 2 * e + 1] * inv);
+      *reinterpret_cast<uint2*>(o + 32 * nb + 8 * i) = make_uint2(w[0], w[1]);
+    }
+}
+
+template <int D, int NW, int DT>
+void launch(const PrefillArgs& a, unsigned blocks, hipStream_t s) {
+  hipLaunchKernelGGL((kv8_prefill_kernel<D, NW, DT>), dim3(blocks), dim3(64 * NW), 0, s, a);
+}
+
+}  // namespace
+
+bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
+                      const int32_t* cu_q, float scale) {
+  const int G = Hq / Hkv;
+  // scale > 0: the kernel keeps its running max in raw score units
+  return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && (D == 64 || D == 128) &&
+         scale > 0.f && G <= 128 && cu_q != nullptr && num_seqs <= P8_MAX_SEQS &&
+         total_q_rows * G >= 64 * int64_t(num_seqs);
+}
+
+int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
+                       const uint8_t* vp, const float* ks, const float* vs, const int32_t* bt,
+                       int64_t bt_stride, const int32_t* lens, const int32_t* cu,
+                       const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
+                       int D, int P, int64_t num_pages, float scale_log2, hipStream_t s) {
+  const int G = Hq / Hkv;
+  const int64_t cus = device_cus();
+  const int wide_ppt = 256 / G;
+  const bool wide = (ceil_div(total_q_rows, wide_ppt) + num_seqs) * Hkv >= 2 * cus &&
+                    2 * total_q_rows >= int64_t(wide_ppt) * num_seqs;
+  const int ppt = (wide ? 256 : 128) / G;
+  const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * Hkv, 8) * 8;
+  if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many query rows");
+  PrefillArgs a{out, q, q_stride, kp, vp, ks, vs, bt, bt_stride, lens, cu, offs, total_q_rows,
+                num_pages, scale_log2, num_seqs, Hq, Hkv, G, P, ppt};
+#define PIA_P8(D, DT)                                   \
+  {                                                     \
+    if (wide) launch<D, 8, DT>(a, unsigned(blocks), s); \
+    else launch<D, 4, DT>(a, unsigned(blocks), s);      \
+  }
+  if (dtype == PIA_DTYPE_F16) {
+    if (D == 64) PIA_P8(64, PIA_DTYPE_F16) else PIA_P8(128, PIA_DTYPE_F16)
+  } else {
+    if (D == 64) PIA_P8(64, PIA_DTYPE_BF16) else PIA_P8(128, PIA_DTYPE_BF16)
+  }
+#undef PIA_P8
+  return check_launch("kv8_prefill");
+}
+
+}  // namespace pia

@@ -5,7 +5,8 @@ scale |q| . |k|, all in float64):
   half a step of the result's type;
   scores: (D + 8) roundings of fp32 at most, 2^-23 each, of z, and as much again by exp2 and the
     reference point, which a probability takes as a relative error: 2 (D + 8) 2^-23 z;
-  probabilities as two bf16 terms: 2^-16 of each (fp32 results: three terms, below 2^-23);
+  probabilities as two bf16 terms: 2^-16 of each (fp32 results: three terms, below 2^-23); calls
+    with many rows round them once to q's 16-bit type: half a step of it, 2^-8 or 2^-11 of each;
   the sums over n keys: n roundings of 2^-23 of what is summed, for p v and for p.
 All but the first times sum p |v|."""
 
@@ -28,9 +29,10 @@ STEP = {torch.bfloat16: 2.0 ** -8, torch.float16: 2.0 ** -11, torch.float32: 2.0
 LEAST = {torch.bfloat16: 2.0 ** -126, torch.float16: 2.0 ** -14, torch.float32: 2.0 ** -126}
 
 
-def _check(got, ref, mag, size, dtype, keys, dim):
+def _check(got, ref, mag, size, dtype, keys, dim, rows=False):
     assert got.dtype == dtype and got.shape == ref.shape
-    rel = (0.0 if dtype == torch.float32 else 2.0 ** -16) + 2.0 ** -22 + 2 * keys * 2.0 ** -23
+    rel = 0.0 if dtype == torch.float32 else STEP[dtype] if rows else 2.0 ** -16
+    rel = rel + 2.0 ** -22 + 2 * keys * 2.0 ** -23
     rel = rel + 2 * (dim + 8) * 2.0 ** -23 * size
     bound = STEP[dtype] * ref.abs().clamp_min(LEAST[dtype]) + rel * mag
     err = (got.double().cpu() - ref).abs()
@@ -114,7 +116,7 @@ def test_rows(dev, case, dtype):
     assert got.data_ptr() == out.data_ptr() and (out[cu[-1]:] == 5.0).all()
     ref, mag, size = O.attend(q[:cu[-1]], pool, tables.tolist(), lens, cu, offs,
                               1 / math.sqrt(dim))
-    _check(got[:cu[-1]], ref, mag, size, dtype, max(lens), dim)
+    _check(got[:cu[-1]], ref, mag, size, dtype, max(lens), dim, rows=True)
 
 
 def test_long_and_many(dev):
@@ -188,7 +190,7 @@ def test_what_a_row_may_not_see(dev):
     t[1, 2] = pages + 9
     got = run(clean, t)
     ref, mag, size = O.attend(q, clean, t.tolist(), lens, cu, offs, 1 / math.sqrt(dim))
-    _check(got, ref, mag, size, torch.bfloat16, 90, dim)
+    _check(got, ref, mag, size, torch.bfloat16, 90, dim, rows=True)
     t[0, :] = -1
     assert (run(clean, t)[:5] == 0).all()
     for value in (math.nan, math.inf):
@@ -292,7 +294,7 @@ def test_append_then_attend(dev):
     q, k, v = rows(37)
     q = kv8_append(q, k, v, pools, tables, i32(lens), cu_new=cu, rope=rope)
     got = paged_attention_kv8(q, pools, tables, i32(lens), cu_q=cu, q_pos_offsets=i32([0, 0]))
-    _check(got, *reference(q, cu.tolist(), [0, 0]), torch.bfloat16, 30, dim)
+    _check(got, *reference(q, cu.tolist(), [0, 0]), torch.bfloat16, 30, dim, rows=True)
     for _ in range(5):
         lens = [n + 1 for n in lens]
         q, k, v = rows(2)
