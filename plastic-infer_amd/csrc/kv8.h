@@ -29,15 +29,12 @@ __device__ __forceinline__ float scale_of(float bound) {
   return __uint_as_float(uint32_t(min(max(e, 27), 246)) << 23);
 }
 
-// Four values times inv (the inverse of a scale) as the e4m3 codes of a word: nearest
-// even, beyond the largest code the largest one, NaN and infinities the NaN code.
-__device__ __forceinline__ float clip(float x) {
-  const float c = fminf(fmaxf(x, -LARGEST), LARGEST);
-  return fabsf(x) < INFINITY ? c : __builtin_nanf("");
-}
+// Four values times inv (the inverse of a scale) as the e4m3 codes of a word, nearest even. A scale holds
+// its values within 448, so nothing is clipped; NaN and infinities become the NaN code, and so would
+// a finite value beyond 464 (only the largest fp32 values are, over a scale of 2^119).
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv) {
-  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(clip(a * inv), clip(b * inv), 0, false);
-  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(clip(c * inv), clip(d * inv), lo, true));
+  const int lo = __builtin_amdgcn_cvt_pk_fp8_f32(a * inv, b * inv, 0, false);
+  return uint32_t(__builtin_amdgcn_cvt_pk_fp8_f32(c * inv, d * inv, lo, true));
 }
 __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
   const auto lo = __builtin_amdgcn_cvt_pk_f32_fp8(int(w), false);
@@ -70,6 +67,22 @@ int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, co
                        const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
                        int D, int P, int64_t num_pages, float scale_log2, hipStream_t s);
 namespace kv8 {
+
+// The last of n numbers base(0) <= base(1) <= ... that is at or before id (the first where none is): 64
+// of them at once, one a lane; base reads what it needs. id is the same in all lanes.
+template <class Base>
+__device__ __forceinline__ int last_at(int n, int64_t id, Base base) {
+  const int lane = threadIdx.x & 63;
+  int lo = 0;
+  while (n > 1) {
+    const int step = (n + 63) >> 6, at = lane * step;
+    const uint64_t in = __ballot(at < n && base(lo + at) <= id);
+    const int last = in ? 63 - __builtin_clzll(in) : 0;
+    lo += last * step;
+    n = min(step, n - last * step);
+  }
+  return lo;
+}
 
 inline bool pool_shape(int D, int P) {
   return D > 0 && D % 16 == 0 && D <= 256 && P > 0 && P % BLOCK == 0 && P <= 4096;

@@ -37,187 +37,237 @@ struct AppendArgs {
   int num_seqs, pairs, inter, Hq, Hkv, D, P;
   double factor;
   float k_bound;
-  int k_vec, v_vec, k_pair, v_pair, whole, q_shares;
+  int k_vec, v_vec, k_pair, v_pair, whole, q_shares, stream;
 };
 
-// sequence whose numbers start last at or before id: base(b) = cu[b] / 16 + step b
-__device__ __forceinline__ int sequence_of(const int32_t* cu, int n, int64_t id, int step) {
-  int lo = 0, hi = n - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((cu[mid] >> 4) + int64_t(step) * mid <= id) lo = mid; else hi = mid - 1;
+// N consecutive elements as they are, in words; VEC: p is a vector of them (16 bytes at most)
+template <int DT, int N>
+struct Raw {
+  using T = typename Elem<DT>::T;
+  static constexpr int PER = 4 / int(sizeof(T)), W = N / PER;  // elements of a word, words
+  uint32_t w[W];
+  __device__ __forceinline__ void load(const T* p, bool vec) {
+    if (vec) {
+      if constexpr (W >= 4) {
+#pragma unroll
+        for (int i = 0; i < W; i += 4) {
+          const uint4 x = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint32_t*>(p) + i);
+          w[i] = x.x;
+          w[i + 1] = x.y;
+          w[i + 2] = x.z;
+          w[i + 3] = x.w;
+        }
+      } else {
+        const uint2 x = *reinterpret_cast<const uint2*>(p);
+        w[0] = x.x;
+        w[1] = x.y;
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < W; ++i) {
+        if constexpr (PER == 2) w[i] = uint32_t(p[2 * i]) | uint32_t(p[2 * i + 1]) << 16;
+        else w[i] = __float_as_uint(p[i]);
+      }
+    }
   }
-  return lo;
-}
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < W; ++i) w[i] = 0;
+  }
+  __device__ __forceinline__ float at(int e) const {
+    if constexpr (DT == PIA_DTYPE_F32) return __uint_as_float(w[e]);
+    else if constexpr (DT == PIA_DTYPE_BF16) return (e & 1) ? bf16_hi(w[e / 2]) : bf16_lo(w[e / 2]);
+    else return half_to_f32(uint16_t((e & 1) ? w[e / 2] >> 16 : w[e / 2]));
+  }
+  // most (magnitudes as whole numbers, in halves of a word for 16-bit types) with these elements
+  __device__ __forceinline__ uint32_t larger(uint32_t most) const {
+    typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+#pragma unroll
+    for (int i = 0; i < W; ++i) {
+      if constexpr (PER == 2)
+        most = __builtin_bit_cast(
+            uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, most),
+                                                __builtin_bit_cast(u16x2_t, w[i] & 0x7fff7fffu)));
+      else
+        most = max(most, w[i] & 0x7fffffffu);
+    }
+    return most;
+  }
+  // the largest finite magnitude
+  __device__ __forceinline__ float finite(float most) const {
+#pragma unroll
+    for (int e = 0; e < N; ++e) {
+      const float x = fabsf(at(e));
+      most = fmaxf(most, x < INFINITY ? x : 0.f);
+    }
+    return most;
+  }
+};
 
-__device__ __forceinline__ float finite_abs(float x) {
-  const float a = fabsf(x);
-  return a < INFINITY ? a : 0.f;
-}
-
-// 16 consecutive elements from p
-template <int DT>
-__device__ __forceinline__ void load16f(const typename Elem<DT>::T* p, bool vec, float (&x)[16]) {
-  if (vec) rope::load<DT, 16, true>(p, x);
-  else rope::load<DT, 16, false>(p, x);
+// The wave's largest finite magnitude: of whole numbers first, and only if that is not finite one
+// element after the other.
+template <int DT, int N, int C>
+__device__ __forceinline__ float largest(const Raw<DT, N> (&x)[C]) {
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < C; ++i) most = x[i].larger(most);
+  if constexpr (Raw<DT, N>::PER == 2) most = max(most & 0xffffu, most >> 16);
+#pragma unroll
+  for (int o = 32; o > 0; o >>= 1) most = max(most, uint32_t(__shfl_xor(int(most), o, 64)));
+  float r = DT == PIA_DTYPE_F32 ? __uint_as_float(most)
+            : DT == PIA_DTYPE_BF16 ? bf16_to_f32(uint16_t(most)) : half_to_f32(uint16_t(most));
+  if (r < INFINITY) return r;
+  r = 0.f;
+#pragma unroll
+  for (int i = 0; i < C; ++i) r = x[i].finite(r);
+  return wave_max(r);
 }
 
 // The K codes of one (block, kv head) of the 8-bit pool by one wave: lane (t, g) has token t's
-// elements 16 c .. 16 c + 15 for c = g, g + 4, ... o0: the block's offset of its first new token, n:
-// how many; r0: their first row; was: the block's scale, 0 where it holds no earlier tokens.
-template <int DT>
-__device__ void append8_k(const AppendArgs& a, const float2* tab, int tab_row, int h, int64_t r0,
-                          int o0, int n, int64_t head, int sub, float was) {
+// elements 16 c .. 16 c + 15 for c = g, g + 4, ... (NC of them). o0: the block's offset of its first
+// new token, n: how many; r0: their first row; was: the block's scale, 0 where it holds no earlier
+// tokens.
+template <int DT, int NC>
+__device__ __forceinline__ void append8_k(const AppendArgs& a, const float2* tab, int tab_row, int h,
+                                          int64_t r0, int o0, int n, int64_t head, int sub,
+                                          float was) {
   using T = typename Elem<DT>::T;
   const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = 2 * a.pairs;
-  {
-    const int t = lane & 15, g = lane >> 4;
-    const bool fresh = t >= o0 && t < o0 + n, old = t < o0;
-    const T* x = static_cast<const T*>(a.k) + (r0 + (fresh ? t - o0 : 0)) * a.k_tok + h * a.k_head;
-    uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.k_pages) +
-                                            head * D * P) + sub * 16 + t;
-    float* scale = a.k_scale + head * (P / 16) + sub;
-    float most = 0.f;
-    for (int c = g; fresh && 16 * c < D; c += 4) {
-      float v[16];
-      load16f<DT>(x + 16 * c, a.k_vec, v);
+  const int t = lane & 15, g = lane >> 4;
+  const bool fresh = t >= o0 && t < o0 + n, old = t < o0;
+  const T* x = static_cast<const T*>(a.k) + (r0 + (fresh ? t - o0 : 0)) * a.k_tok + h * a.k_head;
+  uint4* codes =
+      reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.k_pages) + head * D * P) + sub * 16 + t;
+  Raw<DT, 16> v[NC];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) most = fmaxf(most, finite_abs(v[e]));
-    }
-    const float now = fmaxf(was, kv8::scale_of(wave_max(most) * a.k_bound));
-    const float inv = kv8::inverse(now), ratio = was * inv;
-#pragma unroll 1
-    for (int c = g; 16 * c < D; c += 4) {  // loaded again, from the cache: in registers, D 256 spills
-      uint4 w;
-      if (fresh) {
-        float v[16];
-        load16f<DT>(x + 16 * c, a.k_vec, v);
-        if (16 * c < rd) {
-          const float2* cs = tab + (t - o0) * tab_row;
-          float r[16];
-          if (a.inter) {
-#pragma unroll
-            for (int e = 0; e < 16; e += 2) {
-              const bool in = 16 * c + e < rd;
-              const float2 f = in ? cs[8 * c + e / 2] : make_float2(1.f, 0.f);
-              r[e] = in ? rope::turn(v[e], -v[e + 1], f.x, f.y) : v[e];
-              r[e + 1] = in ? rope::turn(v[e + 1], v[e], f.x, f.y) : v[e + 1];
-            }
-          } else if (a.pairs % 16 == 0) {
-            const bool first = 16 * c < a.pairs;
-            const int other = first ? 16 * c + a.pairs : 16 * c - a.pairs;
-            const float sign = first ? -1.f : 1.f;
-            float p[16];
-            load16f<DT>(x + other, a.k_vec, p);
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const float2 f = cs[(first ? 16 * c : other) + e];
-              r[e] = rope::turn(v[e], sign * p[e], f.x, f.y);
-            }
-          } else {
-#pragma unroll
-            for (int e = 0; e < 16; ++e) {
-              const int d = 16 * c + e;
-              if (d < rd) {
-                const bool first = d < a.pairs;
-                const float2 f = cs[first ? d : d - a.pairs];
-                const float p = Elem<DT>::load(x, first ? d + a.pairs : d - a.pairs);
-                r[e] = rope::turn(v[e], first ? -p : p, f.x, f.y);
-              } else {
-                r[e] = v[e];
-              }
-            }
-          }
-#pragma unroll
-          for (int e = 0; e < 16; ++e) v[e] = r[e];
-        }
-        w = make_uint4(kv8::encode4(v[0], v[1], v[2], v[3], inv),
-                       kv8::encode4(v[4], v[5], v[6], v[7], inv),
-                       kv8::encode4(v[8], v[9], v[10], v[11], inv),
-                       kv8::encode4(v[12], v[13], v[14], v[15], inv));
-        codes[c * P] = w;
-      } else if (old && now != was) {
-        w = codes[c * P];
-        w.x = kv8::rescale4(w.x, ratio);
-        w.y = kv8::rescale4(w.y, ratio);
-        w.z = kv8::rescale4(w.z, ratio);
-        w.w = kv8::rescale4(w.w, ratio);
-        codes[c * P] = w;
-      }
-    }
-    if (lane == 0) *scale = now;
+  for (int i = 0; i < NC; ++i) {
+    const int c = g + 4 * i;
+    if (fresh && 16 * c < D) v[i].load(x + 16 * c, a.k_vec);
+    else v[i].zero();
   }
+  const float now = fmaxf(was, kv8::scale_of(largest(v) * a.k_bound));
+  const float inv = kv8::inverse(now), ratio = was * inv;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    const int c = g + 4 * i;
+    if (16 * c >= D) continue;
+    if (fresh) {
+      float r[16];
+      const float2* cs = tab + (t - o0) * tab_row;
+      if (16 * c >= rd) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) r[e] = v[i].at(e);
+      } else if (a.inter) {
+#pragma unroll
+        for (int e = 0; e < 16; e += 2) {
+          const float v0 = v[i].at(e), v1 = v[i].at(e + 1);
+          const bool in = 16 * c + e < rd;
+          const float2 f = in ? cs[8 * c + e / 2] : make_float2(1.f, 0.f);
+          r[e] = in ? rope::turn(v0, -v1, f.x, f.y) : v0;
+          r[e + 1] = in ? rope::turn(v1, v0, f.x, f.y) : v1;
+        }
+      } else if (a.pairs % 16 == 0) {
+        const bool first = 16 * c < a.pairs;
+        const int other = first ? 16 * c + a.pairs : 16 * c - a.pairs;
+        const float sign = first ? -1.f : 1.f;
+        // the partners: in this lane where they are 64 or 128 elements on, else from the cache
+        Raw<DT, 16> p;
+        if (NC >= 2 && a.pairs == 64) p = v[i ^ (NC >= 2 ? 1 : 0)];
+        else if (NC == 4 && a.pairs == 128) p = v[i ^ (NC == 4 ? 2 : 0)];
+        else p.load(x + other, a.k_vec);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const float2 f = cs[(first ? 16 * c : other) + e];
+          r[e] = rope::turn(v[i].at(e), sign * p.at(e), f.x, f.y);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) {
+          const int d = 16 * c + e;
+          r[e] = v[i].at(e);
+          if (d < rd) {
+            const bool first = d < a.pairs;
+            const float2 f = cs[first ? d : d - a.pairs];
+            const float p = Elem<DT>::load(x, first ? d + a.pairs : d - a.pairs);
+            r[e] = rope::turn(r[e], first ? -p : p, f.x, f.y);
+          }
+        }
+      }
+      codes[c * P] = make_uint4(kv8::encode4(r[0], r[1], r[2], r[3], inv),
+                                kv8::encode4(r[4], r[5], r[6], r[7], inv),
+                                kv8::encode4(r[8], r[9], r[10], r[11], inv),
+                                kv8::encode4(r[12], r[13], r[14], r[15], inv));
+    } else if (old && now != was) {
+      uint4 w = codes[c * P];
+      w.x = kv8::rescale4(w.x, ratio);
+      w.y = kv8::rescale4(w.y, ratio);
+      w.z = kv8::rescale4(w.z, ratio);
+      w.w = kv8::rescale4(w.w, ratio);
+      codes[c * P] = w;
+    }
+  }
+  if (lane == 0) a.k_scale[head * (P / 16) + sub] = now;
 }
 
 // Its V codes: lane (x, tg) has elements 64 i + 4 x .. + 3 of tokens 4 tg .. 4 tg + 3, one word of codes
 // for each element; a word that also holds earlier or stale tokens keeps theirs.
-template <int DT>
-__device__ void append8_v(const AppendArgs& a, int h, int64_t r0, int o0, int n, int64_t head,
-                          int sub, float was) {
+template <int DT, int NC>
+__device__ __forceinline__ void append8_v(const AppendArgs& a, int h, int64_t r0, int o0, int n,
+                                          int64_t head, int sub, float was) {
   using T = typename Elem<DT>::T;
   const int lane = threadIdx.x & 63, D = a.D, P = a.P;
-  {
-    const int x4 = (lane & 15) * 4, t0 = (lane >> 4) * 4;
-    uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.v_pages) + head * D * P +
-                                            (sub * 4 + (lane >> 4)) * 4 * D);
-    float* scale = a.v_scale + head * (P / 16) + sub;
-    // the 4 tokens' elements d .. d + 3, zeros where they are not new
-    auto load_v = [&](int d, float (&v)[4][4]) {
+  const int x4 = (lane & 15) * 4, t0 = (lane >> 4) * 4;
+  uint4* codes = reinterpret_cast<uint4*>(static_cast<uint8_t*>(a.v_pages) + head * D * P +
+                                          (sub * 4 + (lane >> 4)) * 4 * D);
+  Raw<DT, 4> v[4 * NC];
 #pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int t = t0 + j;
-        if (t >= o0 && t < o0 + n) {
-          const T* x = static_cast<const T*>(a.v) + (r0 + t - o0) * a.v_tok + h * a.v_head + d;
-          if (a.v_vec) rope::load<DT, 4, true>(x, v[j]);
-          else rope::load<DT, 4, false>(x, v[j]);
-        } else {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[j][e] = 0.f;
-        }
-      }
-    };
-    float most = 0.f;
-    for (int d = x4; d < D; d += 64) {
-      float v[4][4];
-      load_v(d, v);
-#pragma unroll
-      for (int j = 0; j < 4; ++j)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) most = fmaxf(most, finite_abs(v[j][e]));
-    }
-    const float now = fmaxf(was, kv8::scale_of(wave_max(most)));
-    const float inv = kv8::inverse(now), ratio = was * inv;
-    // bytes of a word: new tokens, and earlier ones that the scale moves
-    uint32_t fresh = 0, old = 0;
+  for (int i = 0; i < NC; ++i)
 #pragma unroll
     for (int j = 0; j < 4; ++j) {
-      const int t = t0 + j;
-      fresh |= t >= o0 && t < o0 + n ? 0xffu << (8 * j) : 0u;
-      old |= t < o0 ? 0xffu << (8 * j) : 0u;
+      const int t = t0 + j, d = 64 * i + x4;
+      if (d < D && t >= o0 && t < o0 + n)
+        v[4 * i + j].load(
+            static_cast<const T*>(a.v) + (r0 + t - o0) * a.v_tok + h * a.v_head + d, a.v_vec);
+      else
+        v[4 * i + j].zero();
     }
-    const bool moved = old != 0 && now != was;
-#pragma unroll 1
-    for (int d = x4; d < D && (fresh != 0 || moved); d += 64) {
-      float v[4][4];
-      load_v(d, v);
-      uint32_t w[4];
+  // bytes of a word: new tokens, and earlier ones that the scale moves
+  uint32_t fresh = 0, old = 0;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) w[e] = kv8::encode4(v[0][e], v[1][e], v[2][e], v[3][e], inv);
-      uint4* at = codes + d / 4;
-      if (fresh != 0xffffffffu) {
-        const uint4 c = *at;
-        const uint32_t before[4] = {c.x, c.y, c.z, c.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          uint32_t b = before[e];
-          if (moved) b = (kv8::rescale4(b, ratio) & old) | (b & ~old);
-          w[e] = (w[e] & fresh) | (b & ~fresh);
-        }
-      }
-      *at = make_uint4(w[0], w[1], w[2], w[3]);
-    }
-    if (lane == 0) *scale = now;
+  for (int j = 0; j < 4; ++j) {
+    const int t = t0 + j;
+    fresh |= t >= o0 && t < o0 + n ? 0xffu << (8 * j) : 0u;
+    old |= t < o0 ? 0xffu << (8 * j) : 0u;
   }
+  // codes that share their words with new ones: on their way while the scale is found
+  const bool part = (fresh | old) != 0 && fresh != 0xffffffffu;
+  uint4 before[NC];
+#pragma unroll
+  for (int i = 0; i < NC; ++i)
+    if (part && 64 * i + x4 < D) before[i] = codes[(64 * i + x4) / 4];
+  const float now = fmaxf(was, kv8::scale_of(largest(v)));
+  const float inv = kv8::inverse(now), ratio = was * inv;
+  const bool moved = old != 0 && now != was;
+#pragma unroll
+  for (int i = 0; i < NC; ++i) {
+    if (64 * i + x4 >= D || (fresh == 0 && !moved)) continue;
+    uint32_t w[4];
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      w[e] = kv8::encode4(v[4 * i].at(e), v[4 * i + 1].at(e), v[4 * i + 2].at(e),
+                          v[4 * i + 3].at(e), inv);
+    if (part) {
+      const uint32_t was4[4] = {before[i].x, before[i].y, before[i].z, before[i].w};
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        uint32_t b = was4[e];
+        if (moved) b = (kv8::rescale4(b, ratio) & old) | (b & ~old);
+        w[e] = (w[e] & fresh) | (b & ~fresh);
+      }
+    }
+    codes[(64 * i + x4) / 4] = make_uint4(w[0], w[1], w[2], w[3]);
+  }
+  if (lane == 0) a.v_scale[head * (P / 16) + sub] = now;
 }
 
 // K (which = 0) or V of one (block, kv head) of a pool of the model's type by one wave: a lane has
@@ -312,17 +362,19 @@ __device__ __forceinline__ void turn_q(const AppendArgs& a, const float2* tab, i
     const int h = h0 + int(hh);
     const T* x = static_cast<const T*>(a.q) + (r0 + t) * a.q_tok + h * a.q_head;
     T* o = static_cast<T*>(a.q_out) + ((r0 + t) * a.Hq + h) * a.D;
-    U::run(o, x, int(r - hh * per_head), tab + t * tab_row, a.pairs, a.D, 1.f);
+    U::run(o, x, int(r - hh * per_head), tab + t * tab_row, a.pairs, a.D, 1.f,
+           a.stream != 0);
   }
 }
 
-template <int DT, bool KV8, bool QVEC>
+// NC: 64-element parts of an 8-bit pool's head; 0: pools of the model's type
+template <int DT, int NC, bool QVEC>
 __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   extern __shared__ float2 tab[];
   int64_t id = blockIdx.x;
   int b = int(id), row_lo = int(id), n_b = 1;
   if (a.cu) {
-    b = sequence_of(a.cu, a.num_seqs, id, 2);
+    b = kv8::last_at(a.num_seqs, id, [&](int i) { return (a.cu[i] >> 4) + int64_t(2) * i; });
     row_lo = a.cu[b];
     n_b = a.cu[b + 1] - row_lo;
     id -= (row_lo >> 4) + int64_t(2) * b;
@@ -341,11 +393,14 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   // keys and values: what a wave needs of tables and scales is on its way before the angles
   const bool slots = !for_q && p0 >= 0 && p0 / a.P < a.bt_stride;  // else no position has one
   const int32_t* row = a.bt + b * a.bt_stride;
-  const int unit = (y - a.q_shares) * KA_WAVES + wave, which = unit & 1, h = unit >> 1;
+  // K heads first, in workgroups of their own: those of V need no angles
+  const int k_shares = (a.Hkv + KA_WAVES - 1) / KA_WAVES;
+  const int which = !for_q && y - a.q_shares >= k_shares;
+  const int h = (y - a.q_shares - (which ? k_shares : 0)) * KA_WAVES + wave;
   int64_t head = -1;
   float was = 0.f;
   const int sub = int(p0 % a.P) >> 4, o0 = int(p0 & 15);
-  if constexpr (KV8) {
+  if constexpr (NC > 0) {
     if (slots && h < a.Hkv) {
       const int32_t page = row[p0 / a.P];
       if (uint32_t(page) < uint64_t(a.num_pages)) {
@@ -356,11 +411,13 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   }
   // a row of the table more than the pairs: 16 tokens' entries of one pair then sit in 16 banks
   const int tab_row = a.pairs + 1;
-  for (int i = threadIdx.x; i < n * a.pairs; i += KA_THREADS) {
-    const int t = i / a.pairs, p = i - t * a.pairs;
-    tab[t * tab_row + p] = rope::cos_sin(a.turns[p], p0 + t, a.factor);
+  if (for_q || !which) {
+    for (int i = threadIdx.x; i < n * a.pairs; i += KA_THREADS) {
+      const int t = i / a.pairs, p = i - t * a.pairs;
+      tab[t * tab_row + p] = rope::cos_sin(a.turns[p], p0 + t, a.factor);
+    }
+    __syncthreads();
   }
-  __syncthreads();
   if (for_q) {
     const int h0 = int(int64_t(a.Hq) * y / a.q_shares);
     const int h1 = int(int64_t(a.Hq) * (y + 1) / a.q_shares);
@@ -370,33 +427,32 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   }
   if (!slots || h >= a.Hkv) return;
   const int m = int(min(int64_t(n), a.bt_stride * a.P - p0));
-  if constexpr (KV8) {
+  if constexpr (NC > 0) {
     if (head < 0) return;
-    if (which) append8_v<DT>(a, h, r0, o0, m, head, sub, was);
-    else append8_k<DT>(a, tab, tab_row, h, r0, o0, m, head, sub, was);
+    if (which) append8_v<DT, NC>(a, h, r0, o0, m, head, sub, was);
+    else append8_k<DT, NC>(a, tab, tab_row, h, r0, o0, m, head, sub, was);
   } else {
     append_plain<DT>(a, tab, tab_row, which, h, r0, p0, m, row);
   }
 }
 
-// Contexts of the 8-bit pool in logical order: one wave for each (block of 16 tokens, kv head).
+// Contexts of the 8-bit pool in logical order: one wave for each (block of 16 tokens, kv head). The
+// codes come in whole 256-byte runs, become values, and leave as whole rows: through LDS, because
+// the runs hold pieces of many rows, and lines that are written in pieces cost a third more.
 template <int DT>
 __global__ __launch_bounds__(256) void kv8_gather_kernel(
     typename Elem<DT>::T* __restrict__ k_out, typename Elem<DT>::T* __restrict__ v_out,
     const uint8_t* __restrict__ k_pages, const uint8_t* __restrict__ v_pages,
     const float* __restrict__ k_scale, const float* __restrict__ v_scale,
     const int32_t* __restrict__ bt, int64_t bt_stride, const int64_t* __restrict__ cu, int num_seqs,
-    int64_t total, int Hkv, int D, int P, int64_t num_pages) {
-  const int lane = threadIdx.x & 63;
-  const int64_t w = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+    int64_t total, int Hkv, int D, int P, int64_t num_pages, int stream) {
+  using T = typename Elem<DT>::T;
+  extern __shared__ __align__(16) unsigned char rows_lds[];
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t w = int64_t(blockIdx.x) * (blockDim.x >> 6) + wave;
   const int64_t id = w / Hkv;
   const int h = int(w - id * Hkv);
-  int lo = 0, hi = num_seqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if ((cu[mid] >> 4) + mid <= id) lo = mid; else hi = mid - 1;
-  }
-  const int b = lo;
+  const int b = kv8::last_at(num_seqs, id, [&](int i) { return (cu[i] >> 4) + i; });
   const int64_t first = cu[b], blk = id - ((first >> 4) + b);
   const int64_t len = min(cu[b + 1], total) - first;
   const int64_t n64 = min(len, bt_stride * P) - blk * 16;
@@ -407,17 +463,37 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(
   const int sub = int(blk % (P / 16));
   const int64_t head = int64_t(ok ? page : 0) * Hkv + h;
   const int64_t row0 = first + blk * 16;
-  const float ks = ok ? k_scale[head * (P / 16) + sub] : 0.f;
-  const float vs = ok ? v_scale[head * (P / 16) + sub] : 0.f;
   const int t = lane & 15, g = lane >> 4;
   const uint4 zero = make_uint4(0u, 0u, 0u, 0u);
+  // a row of the tile: D elements and 16 bytes, which spreads neighbouring rows over the banks
+  const int pitch = D * int(sizeof(T)) + 16, parts = D * int(sizeof(T)) / 16;
+  unsigned char* tile = rows_lds + wave * 16 * pitch;
+  uint4 kx[4], vx[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    kx[i] = vx[i] = zero;
+    const int c = g + 4 * i, d = 64 * i + 4 * t;
+    if (ok && 16 * c < D)
+      kx[i] = reinterpret_cast<const uint4*>(k_pages + head * D * P)[c * P + sub * 16 + t];
+    if (ok && d < D)
+      vx[i] = reinterpret_cast<const uint4*>(v_pages + head * D * P + (sub * 4 + g) * 4 * D)[d / 4];
+  }
+  const float ks = ok ? k_scale[head * (P / 16) + sub] : 0.f;
+  const float vs = ok ? v_scale[head * (P / 16) + sub] : 0.f;
+  auto leave = [&](T* out) {
+    for (int u = lane; u < n * parts; u += 64) {
+      const int r = u / parts, p = u - r * parts;
+      const auto x = *reinterpret_cast<const rope::u32x4_t*>(tile + r * pitch + 16 * p);
+      auto* to = reinterpret_cast<rope::u32x4_t*>(out + ((row0 + r) * Hkv + h) * D) + p;
+      if (stream) __builtin_nontemporal_store(x, to);
+      else *to = x;
+    }
+  };
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int c = g + 4 * i;
-    if (16 * c < D && t < n) {
-      const uint4 x = ok ? reinterpret_cast<const uint4*>(k_pages + head * D * P)[c * P + sub * 16 + t]
-                         : zero;
-      const uint32_t q[4] = {x.x, x.y, x.z, x.w};
+    if (16 * c < D) {
+      const uint32_t q[4] = {kx[i].x, kx[i].y, kx[i].z, kx[i].w};
       float r[16];
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
@@ -426,30 +502,30 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(
 #pragma unroll
         for (int j = 0; j < 4; ++j) r[4 * e + j] = f[j] * ks;
       }
-      rope::store<DT, 16, true>(k_out + ((row0 + t) * Hkv + h) * D + 16 * c, r);
+      rope::store<DT, 16, true>(reinterpret_cast<T*>(tile + t * pitch) + 16 * c, r);
     }
   }
+  __builtin_amdgcn_wave_barrier();  // one wave's LDS operations are done in order
+  leave(k_out);
+  __builtin_amdgcn_wave_barrier();
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     const int d = 64 * i + 4 * t;
     if (d < D) {
-      const uint4 x = ok ? reinterpret_cast<const uint4*>(v_pages + head * D * P +
-                                                          (sub * 4 + g) * 4 * D)[d / 4]
-                         : zero;
       float f[4][4];
-      kv8::decode4(x.x, f[0]);
-      kv8::decode4(x.y, f[1]);
-      kv8::decode4(x.z, f[2]);
-      kv8::decode4(x.w, f[3]);
+      kv8::decode4(vx[i].x, f[0]);
+      kv8::decode4(vx[i].y, f[1]);
+      kv8::decode4(vx[i].z, f[2]);
+      kv8::decode4(vx[i].w, f[3]);
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        if (4 * g + j < n) {
-          const float r[4] = {f[0][j] * vs, f[1][j] * vs, f[2][j] * vs, f[3][j] * vs};
-          rope::store<DT, 4, true>(v_out + ((row0 + 4 * g + j) * Hkv + h) * D + d, r);
-        }
+        const float r[4] = {f[0][j] * vs, f[1][j] * vs, f[2][j] * vs, f[3][j] * vs};
+        rope::store<DT, 4, true>(reinterpret_cast<T*>(tile + (4 * g + j) * pitch) + d, r);
       }
     }
   }
+  __builtin_amdgcn_wave_barrier();
+  leave(v_out);
 }
 
 }  // namespace
@@ -517,18 +593,25 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
   const int per_wg = KA_THREADS * 4 * (qvec ? int(v16) : 1) * (inter ? 1 : 2);
   a.q_shares = a.Hq ? int(std::min<int64_t>(
       a.Hq, ceil_div(int64_t(cu_new ? 16 : 1) * a.Hq * head_dim, per_wg))) : 0;
-  const int64_t shares = a.q_shares + ceil_div(2 * int64_t(num_kv_heads), KA_WAVES);
+  const int64_t shares = a.q_shares + 2 * ceil_div(int64_t(num_kv_heads), KA_WAVES);
+  a.stream = num_tokens * a.Hq * head_dim * elem >= rope::kStreamBytes;
   if (shares > 65535) return fail(PIA_EINVAL, "kv_append: too many heads");
   const dim3 grid{unsigned(blocks), unsigned(shares), 1u};
   const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1);
   hipStream_t s = as_stream(stream);
-#define PIA_KA(DT, KV8, QV) \
-  hipLaunchKernelGGL((kv_append_kernel<DT, KV8, QV>), grid, dim3(KA_THREADS), lds, s, a)
-#define PIA_KA_D(DT)                                                   \
-  if (kv8) {                                                           \
-    if (qvec) PIA_KA(DT, true, true); else PIA_KA(DT, true, false);    \
-  } else {                                                             \
-    if (qvec) PIA_KA(DT, false, true); else PIA_KA(DT, false, false);  \
+#define PIA_KA(DT, NC, QV) \
+  hipLaunchKernelGGL((kv_append_kernel<DT, NC, QV>), grid, dim3(KA_THREADS), lds, s, a)
+#define PIA_KA_Q(DT, NC) \
+  if (qvec) PIA_KA(DT, NC, true); else PIA_KA(DT, NC, false)
+#define PIA_KA_D(DT)                           \
+  if (!kv8) {                                  \
+    PIA_KA_Q(DT, 0);                           \
+  } else if (head_dim <= 64) {                 \
+    PIA_KA_Q(DT, 1);                           \
+  } else if (head_dim <= 128) {                \
+    PIA_KA_Q(DT, 2);                           \
+  } else {                                     \
+    PIA_KA_Q(DT, 4);                           \
   }
   if (dtype == PIA_DTYPE_F32) {
     PIA_KA_D(PIA_DTYPE_F32)
@@ -538,6 +621,7 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
     PIA_KA_D(PIA_DTYPE_BF16)
   }
 #undef PIA_KA_D
+#undef PIA_KA_Q
 #undef PIA_KA
   return check_launch("kv_append");
 }
@@ -562,15 +646,21 @@ extern "C" int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, con
   if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
     return fail(PIA_EINVAL, "kv8_gather: pools and outputs must be 16-byte aligned");
   const int64_t waves = (total_tokens / 16 + num_seqs) * int64_t(num_kv_heads);
-  const int64_t wgs = ceil_div(waves, 4);
+  const int elem = dtype == PIA_DTYPE_F32 ? 4 : 2;
+  const size_t tile = size_t(16) * (size_t(head_dim) * elem + 16);
+  const int per_wg = tile > 16384 ? 2 : 4;  // waves; their tiles stay within 64 KB
+  const size_t lds = per_wg * tile;
+  const int64_t wgs = ceil_div(waves, per_wg);
   if (wgs > 0x7fffffff) return fail(PIA_EINVAL, "kv8_gather: too many tokens");
   hipStream_t s = as_stream(stream);
+  const int stream_out =
+      2 * total_tokens * num_kv_heads * head_dim * elem >= rope::kStreamBytes;
 #define PIA_KG(DT)                                                                              \
-  hipLaunchKernelGGL((kv8_gather_kernel<DT>), dim3(unsigned(wgs)), dim3(256), 0, s,             \
+  hipLaunchKernelGGL((kv8_gather_kernel<DT>), dim3(unsigned(wgs)), dim3(64 * per_wg), lds, s,   \
                      static_cast<Elem<DT>::T*>(k_out), static_cast<Elem<DT>::T*>(v_out),        \
                      static_cast<const uint8_t*>(k_pages), static_cast<const uint8_t*>(v_pages), \
                      k_scales, v_scales, block_tables, bt_stride, cu_seqlens, num_seqs,         \
-                     total_tokens, num_kv_heads, head_dim, page_size, num_pages)
+                     total_tokens, num_kv_heads, head_dim, page_size, num_pages, stream_out)
   if (dtype == PIA_DTYPE_F32) PIA_KG(PIA_DTYPE_F32);
   else if (dtype == PIA_DTYPE_F16) PIA_KG(PIA_DTYPE_F16);
   else PIA_KG(PIA_DTYPE_BF16);

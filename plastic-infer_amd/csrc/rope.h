@@ -65,8 +65,11 @@ __device__ __forceinline__ void load(const typename Elem<DT>::T* p, float (&x)[V
     for (int i = 0; i < V; ++i) x[i] = Elem<DT>::load(p, i);
   }
 }
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+// stream: past the caches' usual order, for results larger than they are
 template <int DT, int V, bool VEC>
-__device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&x)[V]) {
+__device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&x)[V],
+                                      bool stream = false) {
   using T = typename Elem<DT>::T;
   if constexpr (VEC) {
     constexpr int W = V * int(sizeof(T)) < 16 ? V * int(sizeof(T)) : 16;
@@ -78,6 +81,13 @@ __device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&x)[
       Pack a;
 #pragma unroll
       for (int j = 0; j < W / int(sizeof(T)); ++j) Elem<DT>::store(a.v, j, x[i + j]);
+      if constexpr (W == 16) {
+        if (stream) {
+          __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, a),
+                                      reinterpret_cast<u32x4_t*>(p + i));
+          continue;
+        }
+      }
       *reinterpret_cast<Pack*>(p + i) = a;
     }
   } else {
@@ -99,7 +109,7 @@ struct Units {
   }
   // unit u of the head at x into the head at o; tab: the token's (cos, sin) of every pair
   __device__ __forceinline__ static void run(T* o, const T* x, int u, const float2* tab, int pairs,
-                                             int D, float sin_sign) {
+                                             int D, float sin_sign, bool stream) {
     const int nt = turned(pairs);
     if (u >= nt) {
       const int d = 2 * pairs + (u - nt) * V;
@@ -109,7 +119,7 @@ struct Units {
       }
       float a[V];
       load<DT, V, VEC>(x + d, a);
-      store<DT, V, VEC>(o + d, a);
+      store<DT, V, VEC>(o + d, a, stream);
       return;
     }
     float a[V];
@@ -123,7 +133,7 @@ struct Units {
         r[i] = turn(a[i], -a[i + 1], cs.x, s);
         r[i + 1] = turn(a[i + 1], a[i], cs.x, s);
       }
-      store<DT, V, VEC>(o + u * V, r);
+      store<DT, V, VEC>(o + u * V, r, stream);
     } else {
       float b[V], r0[V], r1[V];
       load<DT, V, VEC>(x + pairs + u * V, b);
@@ -134,11 +144,14 @@ struct Units {
         r0[i] = turn(a[i], -b[i], cs.x, s);
         r1[i] = turn(b[i], a[i], cs.x, s);
       }
-      store<DT, V, VEC>(o + u * V, r0);
-      store<DT, V, VEC>(o + pairs + u * V, r1);
+      store<DT, V, VEC>(o + u * V, r0, stream);
+      store<DT, V, VEC>(o + pairs + u * V, r1, stream);
     }
   }
 };
+
+// Results from this size on are stored past the caches' usual order: the L2s together hold 32 MB
+constexpr int64_t kStreamBytes = int64_t(32) << 20;
 
 // Whether a head's units are whole vectors at every stride (elements; bytes for the pointers)
 inline bool vectors(int elem, bool inter, int pairs, int D, const void* a, const void* b,

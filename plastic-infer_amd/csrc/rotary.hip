@@ -5,7 +5,8 @@
 //
 // The transposed map (the gradient's) is the same with s negated. Bound by HBM: every element is read
 // and written once. A workgroup takes a few tokens, computes their (cos, sin) into LDS once for all
-// heads of q and k, and then streams the heads in 16-byte vectors; fp32 arithmetic, one rounding.
+// heads of q and k, and then streams the heads in 16-byte vectors; fp32 arithmetic, one rounding. 8192
+// tokens of 32 + 8 heads of 128, bf16: 28.6 us, 5.9 TB/s (40 us with ordinary stores).
 #include <algorithm>
 
 #include "rope.h"
@@ -23,7 +24,7 @@ struct RotaryArgs {
   const void* positions;
   const double* turns;
   int64_t tokens;
-  int wide, pairs, Hq, Hkv, D, per_wg;
+  int wide, pairs, Hq, Hkv, D, per_wg, stream;
   double factor;
   float sin_sign;
 };
@@ -58,7 +59,7 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotaryArgs a) {
       x = static_cast<const T*>(a.k) + tok * a.k_tok + (h - a.Hq) * a.k_head;
       o = static_cast<T*>(a.k_out) + (tok * a.Hkv + h - a.Hq) * a.D;
     }
-    U::run(o, x, u, tab + t * a.pairs, a.pairs, a.D, a.sin_sign);
+    U::run(o, x, u, tab + t * a.pairs, a.pairs, a.D, a.sin_sign, a.stream != 0);
   }
 }
 
@@ -95,7 +96,8 @@ extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k
                                       k_head_stride));
   RotaryArgs a{q_out, k_out, q, k, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
                positions, turns, num_tokens, positions_i64 != 0, pairs, num_heads, num_kv_heads,
-               head_dim, 1, factor, transposed ? -1.f : 1.f};
+               head_dim, 1, num_tokens * H * head_dim * elem >= rope::kStreamBytes, factor,
+               transposed ? -1.f : 1.f};
   // tokens of a workgroup: one, or four where that still leaves four workgroups
   // for every compute unit (and the table 32 KiB)
   a.per_wg = num_tokens >= 16 * int64_t(device_cus()) ? 4 : 1;

@@ -193,7 +193,7 @@ def test_8bit_special_values(dev):
     k = torch.zeros(4, 1, 16)
     k[0, 0, 3], k[0, 0, 4], k[0, 0, 5] = math.nan, math.inf, 2.0
     k[1, 0, :] = -3.0
-    k[3, 0, 0], k[3, 0, 1] = 3.4028234e38, -1e-40
+    k[3, 0, 0], k[3, 0, 1], k[3, 0, 2] = 3.0e38, -1e-40, 3.4028234e38   # over 464 * 2^119: NaN
     v = torch.zeros(4, 1, 16)
     v[2, 0, 7] = -448.0
     pools = KV8Pools.allocate(1, 1, 16, 16, dev)
@@ -209,7 +209,7 @@ def test_8bit_special_values(dev):
     kv8_append(None, k[3:].to(dev), v[:1].to(dev), pools, table,
                torch.tensor([3], dtype=torch.int32, device=dev))
     x = O.Pool.from_device(pools).values("k")[0, 0]
-    assert x[2, 0] == 448.0 * 2.0 ** 119 and x[2, 1] == 0
+    assert x[2, 0] == 448.0 * 2.0 ** 119 and x[2, 1] == 0 and torch.isnan(x[2, 2])
     assert torch.isnan(x[0, 3:5]).all() and (x[1] == 0).all()
     # a block of zeros: the least scale, and the next token's takes over
     pools = KV8Pools.allocate(1, 1, 16, 16, dev)
