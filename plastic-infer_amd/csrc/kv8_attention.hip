@@ -38,7 +38,7 @@ constexpr int KA_WG_WAVES = 4;
 constexpr int KA_WGS_PER_CU = 2;   // two waves per SIMD
 constexpr int KA_RSRC_WORD3 = 0x00020000;
 constexpr float KA_RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
-constexpr int KA_JOIN_MIN = 128, KA_JOIN_MAX = 1024;  // threads of the joining workgroups
+constexpr int KA_JOIN_MANY = 128, KA_JOIN_FEW = 1024;  // threads of the joining workgroups
 
 struct AttnArgs {
   void* out;
@@ -74,9 +74,20 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b, int tokens) {
   return s;
 }
 
-// ranges of the waves: wave w of n takes steps first_of(w) .. first_of(w + 1) - 1 of total
+// 64-bit quotient of numbers that nearly always have 32 bits (the long division is 150 instructions)
+__device__ __forceinline__ int64_t quotient(int64_t a, int64_t b) {
+  if (((a | b) >> 32) == 0) return int64_t(uint32_t(a) / uint32_t(b));
+  return a / b;
+}
+// Ranges of the waves: total steps over n waves, one more for the first total % n of them. The first
+// step of wave w, and the wave that has step x.
 __device__ __forceinline__ int64_t first_of(int64_t w, int64_t n, int64_t total) {
-  return total * w / n;
+  const int64_t q = quotient(total, n);
+  return q * w + min(w, total - q * n);
+}
+__device__ __forceinline__ int64_t wave_of(int64_t x, int64_t n, int64_t total) {
+  const int64_t q = quotient(total, n), more = total - q * n, edge = (q + 1) * more;
+  return x < edge ? quotient(x, q + 1) : more + quotient(x - edge, q);
 }
 
 template <int DP>
@@ -188,7 +199,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   auto enter = [&](Cursor& c) {
     const int64_t per = pref[c.b + 1] - pref[c.b];
     c.steps = uniform(steps_of[c.b]);
-    c.items = uniform(int(per / (int64_t(c.steps) * a.Hkv)));
+    c.items = uniform(int(quotient(per, int64_t(c.steps) * a.Hkv)));
     c.kv_len = uniform(sequence(a, c.b, STEP).kv_len);
   };
   auto advance = [&](Cursor& c) {
@@ -211,10 +222,10 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     }
     cur.b = uniform(lo);
     enter(cur);
-    const int64_t at = x0 - pref[cur.b], seg = at / cur.steps;
+    const int64_t at = x0 - pref[cur.b], seg = quotient(at, cur.steps);
     cur.t = uniform(int(at - seg * cur.steps));
-    cur.i = uniform(int(seg % cur.items));
-    cur.h = uniform(int(seg / cur.items));
+    cur.h = uniform(int(quotient(seg, cur.items)));
+    cur.i = uniform(int(seg - int64_t(cur.h) * cur.items));
   }
 
   // pages: lane m < MB has block m of a step: its (page, head) and its place in the page, or -1
@@ -546,7 +557,8 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   }
 }
 
-// The items that were cut: their pieces joined, in the order of the waves. One workgroup per item.
+// The items that were cut: their pieces joined, in the order of the waves. A workgroup has rows_per_wg
+// rows of an item, all of them or, where there are few items with many pieces, one.
 // Items without keys are zeros.
 // the weight of a piece whose maximum is m against the joined one
 __device__ __forceinline__ float weight(float m, float joined) {
@@ -554,36 +566,34 @@ __device__ __forceinline__ float weight(float m, float joined) {
 }
 
 template <int QT, int DP>
-__global__ __launch_bounds__(KA_JOIN_MAX) void kv8_attention_join_kernel(AttnArgs a,
-                                                                              int64_t waves) {
+__global__ __launch_bounds__(KA_JOIN_FEW) void kv8_attention_join_kernel(AttnArgs a,
+                                                                         int64_t waves,
+                                                                         int rows_per_wg) {
   using T = typename Elem<QT>::T;
   constexpr int STEP = 16 * (DP > 128 ? 2 : 4);
-  int64_t id = blockIdx.x;
-  const int h = int(id % a.Hkv);
-  id /= a.Hkv;
+  int64_t id = blockIdx.x / unsigned(a.Hkv);
+  const int h = int(blockIdx.x - unsigned(id) * unsigned(a.Hkv));
   int b, i;
   if (a.cu) {
-    int lo = 0, hi = a.B - 1;  // items of sequence b are numbered from cu[b] G / 16 + b on
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t(a.cu[mid]) * a.G >> 4) + mid <= id) lo = mid; else hi = mid - 1;
-    }
-    b = lo;
+    // items of sequence b are numbered from cu[b] G / 16 + b on
+    b = kv8::last_at(a.B, id, [&](int k) { return (int64_t(a.cu[k]) * a.G >> 4) + k; });
     i = int(id - ((int64_t(a.cu[b]) * a.G >> 4) + b));
   } else {
     const int items = (a.G + 15) >> 4;
-    b = int(id / items);
+    b = int(uint32_t(id) / uint32_t(items));
     i = int(id - int64_t(b) * items);
   }
   const Seq s = sequence(a, b, STEP);
   if (i < 0 || i >= s.items) return;
-  const int rows = min(16, s.n * a.G - 16 * i);
+  const int r0 = blockIdx.y * rows_per_wg;
+  const int rows = min(min(16, s.n * a.G - 16 * i) - r0, rows_per_wg);
+  if (rows <= 0) return;
   const int64_t total = a.pref[a.B], nw = min(waves, total);
   const int64_t from = a.pref[b] + (int64_t(h) * s.items + i) * s.steps, to = from + s.steps;
   int64_t w0 = 0, w1 = 0;
   if (s.steps > 0) {
-    w0 = ((from + 1) * nw - 1) / total;
-    w1 = (to * nw - 1) / total;
+    w0 = wave_of(from, nw, total);
+    w1 = wave_of(to - 1, nw, total);
     if (w0 == w1) return;  // finished by its wave
   }
   const float* first = a.parts + (w0 * 2 + (s.steps > 0 && first_of(w0, nw, total) >= from ? 0 : 1)) *
@@ -593,11 +603,11 @@ __global__ __launch_bounds__(KA_JOIN_MAX) void kv8_attention_join_kernel(AttnArg
   const int per_row = a.D / 4, U = rows * per_row, np = int(w1 - w0) + 1;
   const int threads = blockDim.x;
   const int S = s.steps > 0 ? max(1, min(threads / U, np)) : 1;
-  __shared__ float4 o_s[KA_JOIN_MAX];
-  __shared__ float2 ml_s[KA_JOIN_MAX];
+  __shared__ float4 o_s[KA_JOIN_FEW];
+  __shared__ float2 ml_s[KA_JOIN_FEW];
   for (int u0 = 0; u0 < U; u0 += threads) {  // more than one turn: then S is 1
     const int u = u0 + threadIdx.x % min(U, threads), sp = threadIdx.x / min(U, threads);
-    const int r = u / per_row, d = 4 * (u - r * per_row);
+    const int rl = u / per_row, r = r0 + rl, d = 4 * (u - rl * per_row);
     const bool ok = u < U && sp < S;
     float M = -INFINITY, L = 0.f;
     float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -676,10 +686,15 @@ void launch(const AttnArgs& a, int64_t items, bool once, hipStream_t s) {
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, true>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, false>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
-  // few items: many pieces each, which the threads share; many: two or three
-  const int threads = items * 4 <= resident_waves() ? KA_JOIN_MAX : KA_JOIN_MIN;
-  hipLaunchKernelGGL((kv8_attention_join_kernel<QT, DP>), dim3(unsigned(items)), dim3(threads), 0, s,
-                     a, resident_waves());
+  // few items: many pieces each, which many threads share, on every compute unit; many: two or three
+  const bool few = items * 4 <= resident_waves();
+  const int rows = a.cu ? 16 : std::min(a.G, 16);
+  const int parts = few ? int(std::max<int64_t>(1, std::min<int64_t>(rows, device_cus() / items))) : 1;
+  const int rows_per_wg = (rows + parts - 1) / parts;
+  hipLaunchKernelGGL((kv8_attention_join_kernel<QT, DP>),
+                     dim3(unsigned(items), unsigned((rows + rows_per_wg - 1) / rows_per_wg)),
+                     dim3(few ? KA_JOIN_FEW : KA_JOIN_MANY), 0, s, a, resident_waves(),
+                     rows_per_wg);
 }
 
 }  // namespace

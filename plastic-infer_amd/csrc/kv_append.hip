@@ -283,9 +283,10 @@ __device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row
   T* pool = static_cast<T*>(which ? a.v_pages : a.k_pages);
   // a whole block in whole 16-byte vectors of one page
   if (n == 16 && a.whole && (which ? a.v_pair : a.k_pair)) {
-    const int32_t page = row[p0 / P];
+    const uint32_t slot = uint32_t(p0) / uint32_t(P);
+    const int32_t page = row[slot];
     if (uint32_t(page) >= uint64_t(a.num_pages)) return;
-    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + p0 % P;
+    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + (uint32_t(p0) - slot * uint32_t(P));
     struct alignas(2 * sizeof(T)) Two {
       T v[2];
     };
@@ -332,10 +333,10 @@ __device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row
     return;
   }
   for (int t = 0; t < n; ++t) {
-    const int64_t pos = p0 + t;
-    const int32_t page = row[pos / P];
+    const uint32_t pos = uint32_t(p0 + t), slot = pos / uint32_t(P);
+    const int32_t page = row[slot];
     if (uint32_t(page) >= uint64_t(a.num_pages)) continue;
-    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + pos % P;
+    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + (pos - slot * uint32_t(P));
     for (int d = lane; d < D; d += 64) {
       const T* xt = x + t * tok;
       T e = xt[d];
@@ -391,7 +392,8 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   const int y = blockIdx.y, wave = threadIdx.x >> 6;
   const bool for_q = y < a.q_shares;
   // keys and values: what a wave needs of tables and scales is on its way before the angles
-  const bool slots = !for_q && p0 >= 0 && p0 / a.P < a.bt_stride;  // else no position has one
+  const uint32_t slot = uint32_t(max(p0, int64_t(0))) / uint32_t(a.P);
+  const bool slots = !for_q && p0 >= 0 && slot < a.bt_stride;  // else no position has one
   const int32_t* row = a.bt + b * a.bt_stride;
   // K heads first, in workgroups of their own: those of V need no angles
   const int k_shares = (a.Hkv + KA_WAVES - 1) / KA_WAVES;
@@ -399,10 +401,10 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
   const int h = (y - a.q_shares - (which ? k_shares : 0)) * KA_WAVES + wave;
   int64_t head = -1;
   float was = 0.f;
-  const int sub = int(p0 % a.P) >> 4, o0 = int(p0 & 15);
+  const int sub = int(uint32_t(p0) - slot * uint32_t(a.P)) >> 4, o0 = int(p0 & 15);
   if constexpr (NC > 0) {
     if (slots && h < a.Hkv) {
-      const int32_t page = row[p0 / a.P];
+      const int32_t page = row[slot];
       if (uint32_t(page) < uint64_t(a.num_pages)) {
         head = int64_t(page) * a.Hkv + h;
         if (o0 > 0) was = (which ? a.v_scale : a.k_scale)[head * (a.P / 16) + sub];
@@ -449,8 +451,8 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(
   using T = typename Elem<DT>::T;
   extern __shared__ __align__(16) unsigned char rows_lds[];
   const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int64_t w = int64_t(blockIdx.x) * (blockDim.x >> 6) + wave;
-  const int64_t id = w / Hkv;
+  const uint32_t w = blockIdx.x * (blockDim.x >> 6) + wave;  // 32-bit quotients: the long ones took longer
+  const uint32_t id = w / uint32_t(Hkv);                     // than the copy
   const int h = int(w - id * Hkv);
   const int b = kv8::last_at(num_seqs, id, [&](int i) { return (cu[i] >> 4) + i; });
   const int64_t first = cu[b], blk = id - ((first >> 4) + b);
@@ -458,9 +460,10 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(
   const int64_t n64 = min(len, bt_stride * P) - blk * 16;
   if (n64 <= 0 || first < 0 || blk < 0) return;
   const int n = int(min(n64, int64_t(16)));
-  const int32_t page = bt[b * bt_stride + blk * 16 / P];
+  const uint32_t slot = uint32_t(blk) / uint32_t(P / 16);
+  const int sub = int(uint32_t(blk) - slot * uint32_t(P / 16));
+  const int32_t page = bt[b * bt_stride + slot];
   const bool ok = uint32_t(page) < uint64_t(num_pages);
-  const int sub = int(blk % (P / 16));
   const int64_t head = int64_t(ok ? page : 0) * Hkv + h;
   const int64_t row0 = first + blk * 16;
   const int t = lane & 15, g = lane >> 4;
@@ -646,12 +649,12 @@ extern "C" int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, con
   if (!aligned(k_out, 16) || !aligned(v_out, 16) || !aligned(k_pages, 16) || !aligned(v_pages, 16))
     return fail(PIA_EINVAL, "kv8_gather: pools and outputs must be 16-byte aligned");
   const int64_t waves = (total_tokens / 16 + num_seqs) * int64_t(num_kv_heads);
+  if (waves > 0x7fffffff) return fail(PIA_EINVAL, "kv8_gather: too many tokens");
   const int elem = dtype == PIA_DTYPE_F32 ? 4 : 2;
   const size_t tile = size_t(16) * (size_t(head_dim) * elem + 16);
   const int per_wg = tile > 16384 ? 2 : 4;  // waves; their tiles stay within 64 KB
   const size_t lds = per_wg * tile;
   const int64_t wgs = ceil_div(waves, per_wg);
-  if (wgs > 0x7fffffff) return fail(PIA_EINVAL, "kv8_gather: too many tokens");
   hipStream_t s = as_stream(stream);
   const int stream_out =
       2 * total_tokens * num_kv_heads * head_dim * elem >= rope::kStreamBytes;
