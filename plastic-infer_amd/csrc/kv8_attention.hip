@@ -228,20 +228,18 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     cur.i = uniform(int(seg - int64_t(cur.h) * cur.items));
   }
 
-  // pages: lane m < MB has block m of a step: its (page, head) and its place in the page, or -1
+  // Pages: lane m < MB has that of block m of a step (-1 where there is none) and the block's place in
+  // it. The ids are as loaded: what is made of them is made where they are used, a step later, so that
+  // no step waits for them (and with them for the K and V on their way).
   const int PB = a.P / 16, g = lane >> 4, n16 = lane & 15;
+  const uint32_t np = a.num_pages > 0x7fffffff ? 0x7fffffffu : uint32_t(a.num_pages);
   struct Where {
-    int head, sub;
+    int id, sub, h;
   };
   auto where = [&](const Cursor& c, bool real) {
-    Where r{-1, 0};
-    const int kb = c.t * MB + lane;
-    if (real && lane < MB && kb * 16 < c.kv_len) {
-      const int slot = kb / PB;
-      const int32_t id = a.bt[int64_t(c.b) * a.bt_stride + slot];
-      r.sub = kb - slot * PB;
-      r.head = uint32_t(id) < uint64_t(a.num_pages) ? id * a.Hkv + c.h : -1;
-    }
+    const int kb = c.t * MB + lane, slot = PB == 1 ? kb : kb / PB;
+    Where r{-1, kb - slot * PB, c.h};
+    if (real && lane < MB && kb * 16 < c.kv_len) r.id = a.bt[int64_t(c.b) * a.bt_stride + slot];
     return r;
   };
   const int64_t tile_bytes = int64_t(a.D) * a.P;
@@ -257,8 +255,9 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   auto load_k = [&](const Where& r) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-      const int head = __builtin_amdgcn_readlane(r.head, m), sub = __builtin_amdgcn_readlane(r.sub, m);
-      const bool ok = head >= 0;
+      const int id = __builtin_amdgcn_readlane(r.id, m), sub = __builtin_amdgcn_readlane(r.sub, m);
+      const bool ok = uint32_t(id) < np;
+      const int64_t head = int64_t(id) * a.Hkv + r.h;
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(a.kp + (ok ? head : 0) * tile_bytes + sub * 256), 0,
           ok ? int(tile_bytes) - sub * 256 : 0, KA_RSRC_WORD3);
@@ -271,8 +270,9 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   auto load_v = [&](const Where& r) {
 #pragma unroll
     for (int m = 0; m < MB; ++m) {
-      const int head = __builtin_amdgcn_readlane(r.head, m), sub = __builtin_amdgcn_readlane(r.sub, m);
-      const bool ok = head >= 0;
+      const int id = __builtin_amdgcn_readlane(r.id, m), sub = __builtin_amdgcn_readlane(r.sub, m);
+      const bool ok = uint32_t(id) < np;
+      const int64_t head = int64_t(id) * a.Hkv + r.h;
       const auto rs = __builtin_amdgcn_make_buffer_rsrc(
           const_cast<uint8_t*>(a.vp + (ok ? head : 0) * tile_bytes + int64_t(sub) * 16 * a.D), 0,
           ok ? 16 * a.D : 0, KA_RSRC_WORD3);
@@ -284,10 +284,9 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   };
   float sk = 1.f, sv = 1.f;  // lane m < MB: block m's scales
   auto load_scales = [&](const Where& r) {
-    const bool ok = r.head >= 0;
-    const int64_t at = ok ? int64_t(r.head) * PB + r.sub : 0;
-    sk = ok ? a.ks[at] : 1.f;
-    sv = ok ? a.vs[at] : 1.f;
+    const int64_t at = uint32_t(r.id) < np ? (int64_t(r.id) * a.Hkv + r.h) * PB + r.sub : 0;
+    sk = a.ks[at];
+    sv = a.vs[at];
   };
 
   Cursor nxt = cur;
@@ -356,7 +355,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     load_scales(w_nxt);
 
     // softmax, base 2
-    const int there = int(__ballot(lane < MB && w_cur.head >= 0)) & ((1 << MB) - 1);
+    const int there = int(__ballot(lane < MB && uint32_t(w_cur.id) < np)) & ((1 << MB) - 1);
     const int base = cur.t * STEP;
     const bool full = there == (1 << MB) - 1 && base + STEP <= lim_min;
     float mx = -INFINITY;

@@ -35,7 +35,15 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int P8_KT = 64;            // keys per tile: four blocks
 constexpr int P8_MAX_SEQS = 1024;    // sequences per launch (tile prefix in LDS)
-constexpr int P8_AHEAD = 4;          // LDS operand reads in flight ahead of the products
+#ifndef P8_NARROW
+#define P8_NARROW 0
+#endif
+#ifndef P8_AHEAD
+#define P8_AHEAD 4
+#endif
+#ifndef P8_PV_VALU
+#define P8_PV_VALU 2
+#endif
 constexpr int P8_RSRC_WORD3 = 0x00020000;
 constexpr float P8_RESCALE = 8.0f;   // log2: how far a row's maximum may run ahead of its reference
 
@@ -91,11 +99,9 @@ __device__ __forceinline__ float add_pair(uint32_t x, float c) {
                                            __builtin_bit_cast(bf2, 0x3f803f80u), c, false);
 }
 
-// the 16-bit values of a word that are NaN, as 0xffff each
-template <int DT>
-__device__ __forceinline__ uint32_t nan_pairs(uint32_t w) {
-  constexpr uint32_t INF = DT == PIA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
-  return ((w & 0x7fffu) > INF ? 0xffffu : 0u) | (((w >> 16) & 0x7fffu) > INF ? 0xffff0000u : 0u);
+// the bytes of a word of codes that hold the NaN code, as 1 each
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
 }
 
 __device__ __forceinline__ float swap_halves(float x) {  // the value of lane l ^ 32
@@ -108,17 +114,17 @@ template <int D, int NW, int DT>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArgs a) {
   constexpr int NT = 64 * NW, KS = D / 16, NB = D / 32, UK = D / 8;
   constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
-  __shared__ __align__(16) uint4 ks_lds[2][P8_KT * UK];
-  __shared__ __align__(16) uint4 vs_lds[2][D * 8];
+  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // bytes, powers of two
+  __shared__ __align__(16) unsigned char lds[2 * (K_BUF + V_BUF)];
   __shared__ int tile_pref[P8_MAX_SEQS + 1];
   __shared__ int wsum[NW];
-  __shared__ int nan_tile[2];  // 1 + the last tile staged into a buffer with a NaN in V
+  __shared__ int nan_seen;
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // work items per sequence and their prefix
   if (threadIdx.x == 0) tile_pref[0] = 0;
-  if (threadIdx.x < 2) nan_tile[threadIdx.x] = 0;
+  if (threadIdx.x == 0) nan_seen = 0;
   int carry = 0;
   for (int c0 = 0; c0 < a.B; c0 += NT) {
     const int i = c0 + threadIdx.x;
@@ -181,97 +187,125 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int lim_min = a.offs ? max(0, min(kv_len, off + s0 + 1)) : kv_len;
 
   // staging: wave w (of four) moves block w of a tile, K by lanes (token l % 16, chunks l / 16 and
-  // l / 16 + 4), V by lanes (elements 4 (l % 32) .. + 3, token groups l / 32 and l / 32 + 2)
+  // l / 16 + 4), V by lanes (elements 4 (l % 32) .. + 3, token groups l / 32 and l / 32 + 2). What a
+  // wave has of either: its loads' offset, and a base of its LDS addresses (the rest enters by XOR).
   const int blk = wave & 3;
-  const bool st_k = !SPLIT || wave < 4, st_v = !SPLIT || wave >= 4;
-  constexpr int NK = D == 128 ? 2 : 1;  // 16-byte loads of K per lane (head_dim 64: 64 chunks)
+  constexpr int VL = D / 4;  // lanes of a token group of V
   const int64_t tile_bytes = int64_t(D) * a.P;
-  const int kt_tok = lane & 15, kt_c = lane >> 4;
-  const uint32_t k_off = uint32_t((kt_c * a.P + kt_tok) * 16), k_next = uint32_t(64 * a.P);
-  constexpr int VL = D / 4;  // lanes of a token group
-  const bool v_lane = (lane & 31) < VL;
-  const uint32_t v_off = uint32_t(hh * 4 * D + 16 * (lane & (VL - 1)));
-  uint4 kr[NK], vr[2];
-  float k_sc = 1.f, v_sc = 1.f;
-  // (page, head) of the blocks of a tile in lanes 0 .. 3, -1 where there is none; and their places
-  struct Where {
-    int head, sub;
+  struct Part {
+    uint4 x[2];
+    float scale;
+    uint32_t off, base;
   };
+  auto k_part = [&]() {
+    const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = D == 128 ? t & 15 : (t >> 1) & 7;
+    return Part{{}, 1.f, uint32_t((c * a.P + (lane & 15)) * 16),
+                uint32_t(t * UK * 16 + 16 * ((2 * c) ^ sw))};
+  };
+  auto v_part = [&]() {
+    const int x = lane & (VL - 1);
+    return Part{{}, 1.f, uint32_t(hh * 4 * D + 16 * x),
+                2 * K_BUF + uint32_t(x * 4 * 128 + 16 * ((2 * blk + hh) ^ (x & 7)))};
+  };
+  const bool first4 = wave < 4;
+  Part pa = SPLIT && !first4 ? v_part() : k_part(), pb = v_part();  // pb: with four waves only
+  // Pages of the blocks of a tile in lanes 0 .. 3 (-1 where there is none) and the blocks' places in
+  // them. The ids are as loaded: what is made of them is made where they are used, tiles later, so
+  // that no tile waits for them (and with them for every load before).
+  struct Where {
+    int id, sub;
+  };
+  const uint32_t np = a.num_pages > 0x7fffffff ? 0x7fffffffu : uint32_t(a.num_pages);
   auto where = [&](int kt) {
     Where w{-1, 0};
-    const int kb = 4 * kt + lane;
-    if (lane < 4 && kb < nblk) {
-      const int slot = kb / PB;
-      const int32_t id = btb[slot];
-      w.sub = kb - slot * PB;
-      w.head = uint32_t(id) < uint64_t(a.num_pages) ? id * a.Hkv + h : -1;
-    }
+    const int kb = 4 * kt + lane, slot = PB == 1 ? kb : kb / PB;
+    w.sub = kb - slot * PB;
+    if (lane < 4 && kb < nblk) w.id = btb[slot];
     return w;
   };
-  auto fetch = [&](const Where& w) {
-    const int head = __builtin_amdgcn_readlane(w.head, blk);
-    const int sub = __builtin_amdgcn_readlane(w.sub, blk);
-    const bool ok = head >= 0;
-    const int64_t page = (ok ? head : 0) * tile_bytes;
-    if (st_k) {
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint8_t*>(a.kp + page + sub * 256), 0, ok ? int(tile_bytes) - sub * 256 : 0,
-          P8_RSRC_WORD3);
-#pragma unroll
-      for (int i = 0; i < NK; ++i)
-        kr[i] = __builtin_bit_cast(
-            uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, k_off + i * k_next, 0, 0));
-      k_sc = ok ? a.ks[int64_t(head) * PB + sub] : 1.f;
-    }
-    if (st_v) {
-      const auto rs = __builtin_amdgcn_make_buffer_rsrc(
-          const_cast<uint8_t*>(a.vp + page + int64_t(sub) * 16 * D), 0, ok ? 16 * D : 0,
-          P8_RSRC_WORD3);
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        vr[i] = __builtin_bit_cast(
-            uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, v_off + i * 8 * D, 0, 0));
-      v_sc = ok ? a.vs[int64_t(head) * PB + sub] : 1.f;
+  auto fetch_part = [&](Part& p, bool is_k, int id, int sub) {
+    const bool ok = uint32_t(id) < np;
+    const int64_t head = int64_t(id) * a.Hkv + h;
+    const int64_t at = (ok ? head : 0) * tile_bytes + (is_k ? sub * 256 : sub * 16 * D);
+    const int bytes = is_k ? int(tile_bytes) - sub * 256 : 16 * D;
+    const uint32_t step = is_k ? uint32_t(64 * a.P) : uint32_t(8 * D);
+    const auto rs = __builtin_amdgcn_make_buffer_rsrc(
+        const_cast<uint8_t*>((is_k ? a.kp : a.vp) + at), 0, ok ? bytes : 0, P8_RSRC_WORD3);
+    p.x[0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off, 0, 0));
+    if (D == 128 || !is_k)
+      p.x[1] =
+          __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off + step, 0, 0));
+    p.scale = (is_k ? a.ks : a.vs)[ok ? head * PB + sub : 0];
+  };
+  // K of one tile and V of another (with eight waves a wave has one of them)
+  auto fetch_next = [&](const Where& wk, const Where& wv) {
+    if constexpr (SPLIT) {
+      const int id = __builtin_amdgcn_readlane(first4 ? wk.id : wv.id, blk);
+      const int sub = __builtin_amdgcn_readlane(first4 ? wk.sub : wv.sub, blk);
+      fetch_part(pa, first4, id, sub);
+    } else {
+      fetch_part(pa, true, __builtin_amdgcn_readlane(wk.id, blk),
+                 __builtin_amdgcn_readlane(wk.sub, blk));
+      fetch_part(pb, false, __builtin_amdgcn_readlane(wv.id, blk),
+                 __builtin_amdgcn_readlane(wv.sub, blk));
     }
   };
-  auto stage = [&](int buf, int kt) {
-    if (st_k) {
-      const int t = 16 * blk + kt_tok;
-      const int sw = D == 128 ? t & 15 : (t >> 1) & 7;
+  auto put = [&](uint32_t at, const uint4& x) {
+    *reinterpret_cast<uint4*>(lds + at) = x;
+  };
+  auto stage_k = [&](const Part& p, int buf) {
+    const uint32_t base = p.base + buf * K_BUF;
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const int u = 2 * (kt_c + 4 * i);
-        ks_lds[buf][t * UK + (u ^ sw)] = widen8<DT>(kr[i].x, kr[i].y, k_sc);
-        ks_lds[buf][t * UK + ((u + 1) ^ sw)] = widen8<DT>(kr[i].z, kr[i].w, k_sc);
+    for (int i = 0; i < D / 64; ++i) {
+      put(base ^ (128 * i), widen8<DT>(p.x[i].x, p.x[i].y, p.scale));
+      put(base ^ (128 * i + 16), widen8<DT>(p.x[i].z, p.x[i].w, p.scale));
+    }
+  };
+  auto stage_v = [&](Part& p, int buf, int kt, bool places) {
+    // tokens past the context hold whatever the page held: zeros
+    if (64 * kt + 64 > kv_len) {
+      const int nv = kv_len - (64 * kt + 16 * blk + 4 * hh);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const int n = nv - 8 * i;
+        const uint32_t keep = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
+        p.x[i].x &= keep;
+        p.x[i].y &= keep;
+        p.x[i].z &= keep;
+        p.x[i].w &= keep;
       }
     }
-    if (st_v) {
-      // tokens past the context hold whatever the page held: zeros
-      const int nv = kv_len - (64 * kt + 16 * blk + 4 * hh);
-      if (64 * kt + 64 > kv_len) {
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int n = nv - 8 * i;
-          const uint32_t keep = n >= 4 ? 0xffffffffu : n <= 0 ? 0u : (1u << (8 * n)) - 1u;
-          vr[i].x &= keep;
-          vr[i].y &= keep;
-          vr[i].z &= keep;
-          vr[i].w &= keep;
-        }
-      }
-      const uint32_t w0[4] = {vr[0].x, vr[0].y, vr[0].z, vr[0].w};
-      const uint32_t w1[4] = {vr[1].x, vr[1].y, vr[1].z, vr[1].w};
+    // Zero times NaN is NaN, so a NaN of V would reach the rows that may not see its token. On tiles
+    // that not every row sees whole it is staged as zero; the end of the item puts it where it
+    // belongs, from tiles of the NaNs' places (places: a one for each).
+    float scale = p.scale;
+    if (places || 64 * kt + 64 > lim_min) {
       uint32_t any = 0;
-      if (v_lane) {
+      uint32_t* w = &p.x[0].x;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int d = 4 * (lane & (VL - 1)) + e;
-          const int sw = ((d >> 2) & 7) ^ ((d >> 1) & 1);
-          vs_lds[buf][d * 8 + ((2 * blk + hh) ^ sw)] = widen8<DT>(w0[e], w1[e], v_sc);
-          any |= ((w0[e] & 0x7f7f7f7fu) + 0x01010101u) | ((w1[e] & 0x7f7f7f7fu) + 0x01010101u);
-        }
+      for (int e = 0; e < 8; ++e) {
+        const uint32_t n = nan_codes(w[e]);
+        any |= n;
+        w[e] = places ? n * 0x38u : w[e] & ~(n * 0xffu);  // 0x38: the code of 1
       }
-      if (any & 0x80808080u) nan_tile[buf] = kt + 1;
+      if (places) scale = 1.f;
+      else if (any && (lane & 31) < VL) nan_seen = 1;
+    }
+    if ((lane & 31) < VL) {
+      const uint32_t base = p.base + buf * V_BUF;
+      put(base, widen8<DT>(p.x[0].x, p.x[1].x, scale));
+      put(base + 128, widen8<DT>(p.x[0].y, p.x[1].y, scale));
+      put((base ^ 16) + 256, widen8<DT>(p.x[0].z, p.x[1].z, scale));
+      put((base ^ 16) + 384, widen8<DT>(p.x[0].w, p.x[1].w, scale));
+    }
+  };
+  auto stage = [&](int buf, int kt, bool places) {
+    if constexpr (SPLIT) {
+      if (first4) stage_k(pa, buf);
+      else stage_v(pa, buf, kt, places);
+    } else {
+      stage_k(pa, buf);
+      stage_v(pb, buf, kt, places);
     }
   };
   // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
@@ -279,14 +313,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // that they are computed where they are used and not kept.
   const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (D == 128 ? n32 & 15 : (n32 >> 1) & 7));
   const uint32_t v_base = n32 * 128 + 16 * (hh ^ (((n32 >> 2) & 7) ^ ((n32 >> 1) & 1)));
-  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // powers of two
   auto kread = [&](int buf, int tb, int k) {
     const uint32_t at = ((k_base + buf * K_BUF) ^ (32 * k)) + 32 * tb * UK * 16;
-    return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(&ks_lds[0][0]) + at);
+    return *reinterpret_cast<const uint4*>(lds + at);
   };
   auto vread = [&](int buf, int nb, int s) {
     const uint32_t at = ((v_base + buf * V_BUF) ^ (32 * s)) + 32 * nb * 128;
-    return *reinterpret_cast<const uint4*>(reinterpret_cast<const char*>(&vs_lds[0][0]) + at);
+    return *reinterpret_cast<const uint4*>(lds + 2 * K_BUF + at);
   };
 
   float m = -INFINITY, l = 0.f;  // the row's reference point in raw score units; its lane's sum
@@ -296,57 +329,39 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
 #pragma unroll
     for (int v = 0; v < 16; ++v) acc[nb][v] = 0.f;
 
-  Where w_cur = where(0), w_nxt = where(1), w_far = where(2);
-  fetch(w_cur);
-  stage(0, 0);
-  fetch(w_nxt);
-  __syncthreads();
-  for (int kt = 0; kt < nkt; ++kt) {
-    const int buf = kt & 1;
-    const int there = int(__ballot(lane < 4 && w_cur.head >= 0)) & 0xf;
-    const bool full = there == 0xf && (kt + 1) * P8_KT <= lim_min;
-    const Where w_next = where(kt + 3);
-
-    f32x16_t sc[2];
+  // scores of a tile from its K, on their own
+  auto scores = [&](f32x16_t (&sc)[2], int buf) {
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
       for (int v = 0; v < 16; ++v) sc[tb][v] = 0.f;
-    {
-      // operands are read P8_AHEAD products ahead of their use, kept so through the scheduler
-      uint4 kq[P8_AHEAD];
 #pragma unroll
-      for (int i = 0; i < P8_AHEAD; ++i) kq[i] = kread(buf, i & 1, i >> 1);
+    for (int i = 0; i < 2 * KS; ++i)
+      sc[i & 1] = mfma32<DT>(kread(buf, i & 1, i >> 1), qr[i >> 1], sc[i & 1]);
+  };
+  auto largest = [&](const f32x16_t (&sc)[2]) {
+    float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 2 * KS; ++i) {
-        const uint4 k = kq[i % P8_AHEAD];
-        if (i + P8_AHEAD < 2 * KS)
-          kq[i % P8_AHEAD] = kread(buf, (i + P8_AHEAD) & 1, (i + P8_AHEAD) >> 1);
-        sc[i & 1] = mfma32<DT>(k, qr[i >> 1], sc[i & 1]);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, P8_AHEAD, 0);
+    for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
-      for (int i = 0; i < 2 * KS - P8_AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, P8_AHEAD, 0);
-    }
-
-    const int rel = lim - (kt * P8_KT + 4 * hh);
-    if (!full) {
+      for (int v = 0; v < 16; ++v) mx = __builtin_elementwise_maximum(mx, sc[tb][v]);
+    return mx;
+  };
+  // One tile. sc: its scores, mx: the largest of them (of the lane's) where none is hidden; sn, mx:
+  // the next tile's on return. A wave keeps its matrix core and its vector ALU busy at once: the
+  // next tile's scores are multiplied while this one's become probabilities, and this one's
+  // outputs while the tile after is staged.
+  auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int kt, int there) {
+    if (!(there == 0xf && (kt + 1) * P8_KT <= lim_min)) {
+      const int rel = lim - (kt * P8_KT + 4 * hh);
 #pragma unroll
       for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
         for (int v = 0; v < 16; ++v)
           if (!(32 * tb + 8 * (v >> 2) + (v & 3) < rel && ((there >> (2 * tb + (v >> 3))) & 1)))
             sc[tb][v] = -INFINITY;
+      mx = largest(sc);
     }
-    float mx = -INFINITY;
-#pragma unroll
-    for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-      for (int v = 0; v < 16; ++v) mx = __builtin_elementwise_maximum(mx, sc[tb][v]);
     mx = __builtin_elementwise_maximum(mx, swap_halves(mx));
     const float mref = (mx - m) * a.scale_log2 > P8_RESCALE || mx != mx ? mx : m;
     const float nm = mref == -INFINITY ? 0.f : -mref * a.scale_log2;
@@ -359,7 +374,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
         for (int v = 0; v < 16; ++v) acc[nb][v] *= alpha;
     }
     m = mref;
-    uint4 pk[4];  // block s: the B operand of its 16 tokens
+    scores(sn, (kt + 1) & 1);
+    const int buf = kt & 1;
+    uint4 pk[4];  // block s of the tile: the B operand of its 16 tokens, the probabilities
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
       uint32_t w[4];
@@ -373,22 +390,89 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       }
       pk[s] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    stage(buf ^ 1, kt + 1);
-    fetch(w_far);
-    if (!full && nan_tile[buf] == kt + 1) {  // the same for every wave of the workgroup
-      // Zero times NaN is NaN: V's NaN would reach rows that may not see its token. The rows that see
-      // one get it by a product of their places, then the tile's are made zeros.
+#pragma unroll
+    for (int i = 0; i < 4 * NB; ++i)
+      acc[i % NB] = mfma32<DT>(vread(buf, i % NB, i / NB), pk[i / NB], acc[i % NB]);
+    mx = largest(sn);
+    // kept so through the scheduler: operands read P8_AHEAD products ahead of their use, the vector
+    // work of the probabilities among the scores' products, the next maximum's among the outputs'
+    constexpr int QK = 2 * KS, PV = 4 * NB;
+    __builtin_amdgcn_sched_group_barrier(0x100, P8_AHEAD, 0);
+#pragma unroll
+    for (int i = 0; i < QK; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, 96 / QK, 0);
+    }
+#pragma unroll
+    for (int i = 0; i < PV; ++i) {
+      __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+      if (i + P8_AHEAD < PV) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+      __builtin_amdgcn_sched_group_barrier(0x402, P8_PV_VALU, 0);
+    }
+  };
+
+  // K is staged two tiles ahead of the outputs, for scores are a tile ahead, V one. With two buffers
+  // each, what a tile stages replaces what the tile before it has read, with a barrier between.
+  auto stage_next = [&](int kt) {
+    if constexpr (SPLIT) {
+      if (first4) stage_k(pa, kt & 1);
+      else stage_v(pa, (kt + 1) & 1, kt + 1, false);
+    } else {
+      stage_k(pa, kt & 1);
+      stage_v(pb, (kt + 1) & 1, kt + 1, false);
+    }
+  };
+  Where w0 = where(0), w1 = where(1), w2 = where(2), w3 = where(3);  // of tiles kt .. kt + 3
+  fetch_next(w0, w0);
+  stage(0, 0, false);
+  if (!SPLIT || first4) {  // K of tile 1; the other waves have nothing of it
+    fetch_part(pa, true, __builtin_amdgcn_readlane(w1.id, blk),
+               __builtin_amdgcn_readlane(w1.sub, blk));
+    stage_k(pa, 1);
+  }
+  fetch_next(w2, w1);
+  __syncthreads();
+  f32x16_t sa[2], sb[2];
+  scores(sa, 0);
+  float mx = largest(sa);
+  auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int kt) {
+    const int there = int(__ballot(lane < 4 && uint32_t(w0.id) < np)) & 0xf;
+    const Where w4 = where(kt + 4);
+    turn(sc, sn, mx, kt, there);
+    stage_next(kt);
+    fetch_next(w3, w2);
+    __syncthreads();
+    w0 = w1;
+    w1 = w2;
+    w2 = w3;
+    w3 = w4;
+  };
+  for (int kt = 0; kt < nkt; kt += 2) {
+    step(sa, sb, kt);
+    if (kt + 1 >= nkt) break;
+    step(sb, sa, kt + 1);
+  }
+
+  if (nan_seen) {  // the same for every wave: all stores to it are barriers ago
+#pragma unroll 1
+    for (int kt = max(lim_min, 0) / P8_KT; kt < nkt; ++kt) {
+      __syncthreads();
+      const Where w = where(kt);
+      fetch_next(w, w);
+      stage(0, kt, true);
+      __syncthreads();
+      const int there = int(__ballot(lane < 4 && uint32_t(w.id) < np)) & 0xf;
+      const int rel = lim - (kt * P8_KT + 4 * hh);
       constexpr uint32_t ONE = DT == PIA_DTYPE_F16 ? 0x3c00u : 0x3f80u;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb) {
-        __builtin_amdgcn_sched_barrier(0);  // one block at a time (registers)
         f32x16_t hit;
 #pragma unroll
         for (int v = 0; v < 16; ++v) hit[v] = 0.f;
 #pragma unroll
         for (int s = 0; s < 4; ++s) {
-          __builtin_amdgcn_sched_barrier(0);
-          const uint4 x = vread(buf, nb, s);
+          __builtin_amdgcn_sched_barrier(0);  // one operand at a time (registers)
           uint32_t see[4];
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
@@ -396,49 +480,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
             const bool here = (there >> s) & 1;
             see[i] = (here && t < rel ? ONE : 0u) | (here && t + 1 < rel ? ONE << 16 : 0u);
           }
-          constexpr uint32_t ONES = ONE * 0x10001u;
-          hit = mfma32<DT>(make_uint4(nan_pairs<DT>(x.x) & ONES, nan_pairs<DT>(x.y) & ONES,
-                                      nan_pairs<DT>(x.z) & ONES, nan_pairs<DT>(x.w) & ONES),
-                           make_uint4(see[0], see[1], see[2], see[3]), hit);
+          hit = mfma32<DT>(vread(0, nb, s), make_uint4(see[0], see[1], see[2], see[3]), hit);
         }
 #pragma unroll
         for (int v = 0; v < 16; ++v)
           if (hit[v] > 0.f) acc[nb][v] = __builtin_nanf("");
       }
-      __syncthreads();
-      for (int u = threadIdx.x; u < D * 8; u += NT) {
-        uint4 x = vs_lds[buf][u];
-        x.x &= ~nan_pairs<DT>(x.x);
-        x.y &= ~nan_pairs<DT>(x.y);
-        x.z &= ~nan_pairs<DT>(x.z);
-        x.w &= ~nan_pairs<DT>(x.w);
-        vs_lds[buf][u] = x;
-      }
-      __syncthreads();
     }
-    {
-      uint4 vq[P8_AHEAD];
-#pragma unroll
-      for (int i = 0; i < P8_AHEAD; ++i) vq[i] = vread(buf, i % NB, i / NB);
-#pragma unroll
-      for (int i = 0; i < 4 * NB; ++i) {
-        const uint4 v = vq[i % P8_AHEAD];
-        if (i + P8_AHEAD < 4 * NB)
-          vq[i % P8_AHEAD] = vread(buf, (i + P8_AHEAD) % NB, (i + P8_AHEAD) / NB);
-        acc[i % NB] = mfma32<DT>(v, pk[i / NB], acc[i % NB]);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x100, P8_AHEAD, 0);
-#pragma unroll
-      for (int i = 0; i < 4 * NB - P8_AHEAD; ++i) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
-      }
-      __builtin_amdgcn_sched_group_barrier(0x008, P8_AHEAD, 0);
-    }
-    __syncthreads();
-    w_cur = w_nxt;
-    w_nxt = w_far;
-    w_far = w_next;
   }
 
   l += swap_halves(l);
@@ -482,8 +530,9 @@ int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, co
   const int G = Hq / Hkv;
   const int64_t cus = device_cus();
   const int wide_ppt = 256 / G;
-  const bool wide = (ceil_div(total_q_rows, wide_ppt) + num_seqs) * Hkv >= 2 * cus &&
+  const bool wide_ = (ceil_div(total_q_rows, wide_ppt) + num_seqs) * Hkv >= 2 * cus &&
                     2 * total_q_rows >= int64_t(wide_ppt) * num_seqs;
+  const bool wide = wide_ && !P8_NARROW;
   const int ppt = (wide ? 256 : 128) / G;
   const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * Hkv, 8) * 8;
   if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many query rows");
