@@ -56,7 +56,7 @@ struct AttnArgs {
   int B, Hq, Hkv, G, D, P;
 };
 
-// A sequence's part of a call: its rows, the keys that some row of it may see and their steps.
+// A sequence's part of a call: its rows, the keys that some row of it may see (kv_len) and their steps.
 struct Seq {
   int64_t row0;
   int n, kv_len, off, items, steps;
@@ -68,9 +68,9 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b, int tokens) {
   s.n = s.row0 < 0 ? 0 : int(max(int64_t(0), min(n, a.rows - s.row0)));
   s.kv_len = int(min(int64_t(max(a.lens[b], 0)), min(a.bt_stride * a.P, int64_t(0x7ffffff0))));
   s.off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
-  const int64_t seen = a.offs ? min(int64_t(s.kv_len), int64_t(s.off) + s.n) : s.kv_len;
+  if (a.offs) s.kv_len = int(max(int64_t(0), min(int64_t(s.kv_len), int64_t(s.off) + s.n)));
   s.items = int((int64_t(s.n) * a.G + 15) >> 4);
-  s.steps = seen > 0 ? int((seen + tokens - 1) / tokens) : 0;
+  s.steps = (s.kv_len + tokens - 1) / tokens;
   return s;
 }
 
@@ -112,14 +112,17 @@ __device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b) {
   return make_uint4(widen<T, false>(a), widen<T, true>(a), widen<T, false>(b), widen<T, true>(b));
 }
 
-// eight consecutive q elements as NQ operands
+// eight consecutive q elements (which are there to be read) as NQ operands, zeros where not ok
 template <int QT>
 __device__ __forceinline__ void load_q(const typename Elem<QT>::T* p, bool ok,
                                        uint4 (&t)[Q<QT>::NQ]) {
   if constexpr (QT == PIA_DTYPE_F32) {
     float x[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = ok ? p[i] : 0.f;
+    for (int i = 0; i < 8; ++i) {
+      x[i] = p[i];
+      x[i] = ok ? x[i] : 0.f;
+    }
 #pragma unroll
     for (int k = 0; k < 3; ++k) {
       uint32_t w[4];
@@ -132,7 +135,11 @@ __device__ __forceinline__ void load_q(const typename Elem<QT>::T* p, bool ok,
       t[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
   } else {
-    t[0] = ok ? *reinterpret_cast<const uint4*>(p) : make_uint4(0u, 0u, 0u, 0u);
+    t[0] = *reinterpret_cast<const uint4*>(p);
+    t[0].x = ok ? t[0].x : 0u;
+    t[0].y = ok ? t[0].y : 0u;
+    t[0].z = ok ? t[0].z : 0u;
+    t[0].w = ok ? t[0].w : 0u;
   }
 }
 
@@ -145,13 +152,14 @@ __device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
   return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
 }
 
-// NT: K and V are read once by the call.
-template <int QT, int DP, bool NT>
+// ONCE: one position and one item per sequence and kv head, so K and V are read once by the call, and
+// all rows of an item see the same keys.
+template <int QT, int DP, bool ONCE>
 __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention_kernel(AttnArgs a) {
   using T = typename Elem<QT>::T;
   constexpr int NQ = Q<QT>::NQ, NP = Q<QT>::NP, KT16 = Q<QT>::KT;
   constexpr int MB = DP > 128 ? 2 : 4;  // blocks of a step (registers)
-  constexpr int STEP = 16 * MB, ND = DP / 64, AUX = NT ? 2 : 0;
+  constexpr int STEP = 16 * MB, ND = DP / 64, AUX = ONCE ? 2 : 0;
   __shared__ int64_t pref[KA_MAX_SEQS + 1];
   __shared__ int steps_of[KA_MAX_SEQS];
   __shared__ int64_t wsum[KA_WG_WAVES];
@@ -326,8 +334,21 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
           const int d = 16 * (g + 4 * i) + 8 * e;
           load_q<QT>(qp + (d < a.D ? d : 0), ok && d < a.D, qr[i][e]);
         }
-      lim = a.offs ? min(s.kv_len, s.off + pos + 1) : s.kv_len;
-      lim_min = a.offs ? min(s.kv_len, s.off + (16 * cur.i) / a.G + 1) : s.kv_len;
+      // q is waited for here, once an item: left to its use, the wait would be there in every step, and
+      // with it one for the step's K and V
+#pragma unroll
+      for (int i = 0; i < ND; ++i)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int n = 0; n < NQ; ++n)
+            asm volatile("" : "+v"(qr[i][e][n].x), "+v"(qr[i][e][n].y), "+v"(qr[i][e][n].z),
+                              "+v"(qr[i][e][n].w));
+      lim = lim_min = s.kv_len;
+      if (!ONCE && a.offs) {
+        lim = min(lim, s.off + pos + 1);
+        lim_min = min(lim_min, s.off + (16 * cur.i) / a.G + 1);
+      }
       m = -INFINITY;
       l = 0.f;
 #pragma unroll
@@ -350,9 +371,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
         }
       }
     }
-    const float sk_cur = sk, sv_cur = sv;
     load_k(w_nxt);
-    load_scales(w_nxt);
 
     // softmax, base 2
     const int there = int(__ballot(lane < MB && uint32_t(w_cur.id) < np)) & ((1 << MB) - 1);
@@ -361,7 +380,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     float mx = -INFINITY;
 #pragma unroll
     for (int b = 0; b < MB; ++b) {
-      const float f = a.scale_log2 * lane_value(sk_cur, b);
+      const float f = a.scale_log2 * lane_value(sk, b);
 #pragma unroll
       for (int j = 0; j < 4; ++j) s[b][j] *= f;
     }
@@ -409,7 +428,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
       uint32_t t[NP][4];
 #pragma unroll
       for (int b2 = 0; b2 < 2; ++b2) {
-        const float f = lane_value(sv_cur, 2 * c + b2);
+        const float f = lane_value(sv, 2 * c + b2);
 #pragma unroll
         for (int j2 = 0; j2 < 2; ++j2) {
           float u = p[2 * c + b2][2 * j2] * f, v = p[2 * c + b2][2 * j2 + 1] * f;
@@ -425,6 +444,9 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
 #pragma unroll
       for (int k = 0; k < NP; ++k) pt[c][k] = make_uint4(t[k][0], t[k][1], t[k][2], t[k][3]);
     }
+    // the next scales into the registers of these, whose last use this was: a copy of them, made for
+    // the step to come, would wait for them, and so for every load before
+    load_scales(w_nxt);
     // V of tokens past the context is whatever the page held: zeros
     if (base + STEP > cur.kv_len) {
 #pragma unroll
@@ -443,7 +465,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     // Zero times NaN is NaN, so a NaN of V would reach rows that may not see its token. Where rows
     // differ in what they see, NaN codes are taken out, and put into the rows that see them by a
     // product of their places.
-    if (a.offs && !full) {
+    if (!ONCE && a.offs && !full) {
       uint32_t any = 0;
 #pragma unroll
       for (int b = 0; b < MB; ++b)
