@@ -60,7 +60,7 @@ __device__ __forceinline__ float inverse(float scale) {
 // (arguments already checked by pia_kv8_attention).
 }  // namespace kv8
 bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
-                      const int32_t* cu_q, float scale);
+                      int64_t table_tokens, const int32_t* cu_q, float scale);
 int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
                        const uint8_t* vp, const float* ks, const float* vs, const int32_t* bt,
                        int64_t bt_stride, const int32_t* lens, const int32_t* cu,

@@ -769,8 +769,8 @@ extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, con
              reinterpret_cast<float*>(static_cast<char*>(workspace) + KA_PREF_BYTES),
              static_cast<int64_t*>(workspace), scale * 1.4426950408889634f, num_seqs, num_heads,
              num_kv_heads, G, head_dim, page_size};
-  if (kv8_prefill_path(dtype, num_heads, num_kv_heads, head_dim, num_seqs, total_q_rows, cu_q,
-                       scale))
+  if (kv8_prefill_path(dtype, num_heads, num_kv_heads, head_dim, num_seqs, total_q_rows,
+                       bt_stride * page_size, cu_q, scale))
     return launch_kv8_prefill(dtype, out, q, q_stride, a.kp, a.vp, a.ks, a.vs, block_tables,
                               bt_stride, kv_lens, cu_q, q_pos_offsets, num_seqs, total_q_rows,
                               num_heads, num_kv_heads, head_dim, page_size, num_pages,

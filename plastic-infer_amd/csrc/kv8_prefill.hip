@@ -1,5 +1,5 @@
 // Attention of many query rows per sequence (prefill, chunked prefill) over the 8-bit KV pool on the
-// matrix cores: bf16 or fp16 q (DT), head_dim 64 or 128, any page size of the pool.
+// matrix cores: bf16 or fp16 q (DT), head_dim 64, 96 or 128, any page size of the pool.
 //
 // Work item (one workgroup of NW waves): one kv head and 32 NW / G consecutive query positions of one
 // sequence, i.e. up to 32 NW (position, q head) rows that share the kv head's keys: row r is position
@@ -18,11 +18,18 @@
 //                  to DT): of a block's tokens, lane half hh holds 4 hh + j and 8 + 4 hh + j. Rows of
 //                  the result are elements, so a lane has 4 D / 16 of them of its own row l % 32: what
 //                  a row's maximum and sum do to it needs no exchange between lanes.
-// LDS tiles (16-byte units, XORed with a term of their row): K [token][d]: unit u (d 8 u .. + 7) of
-// token t at u ^ t % 16 (head_dim 64: u ^ t / 2 % 8); V [d][token]: unit 2 m + hh (block m, tokens
+// LDS tiles (16-byte units, XORed with a term of their row): K [token][d], 16 units to a token also at
+// head_dim 96: unit u (d 8 u .. + 7) of token t at u ^ t % 16 (head_dim 64: 8 units, u ^ t / 2 % 8); V [d][token]: unit 2 m + hh (block m, tokens
 // 4 hh + j, then 8 + 4 hh + j) of element d at (2 m + hh) ^ (d / 4 % 8) ^ (d / 2 % 2). With the bank
 // rules of gfx950 (stores: 8 lanes over 32 banks; 16-byte reads: lanes {0-3, 12-15, 20-27} or the
 // others over 64) all of them are conflict-free but K stores at head_dim 64.
+//
+// Measured: 8 sequences of 1024 new rows on 4096 keys, causal, 32 heads of 128 over 8, bf16: 627 us,
+// 0.99 PFLOP/s of 619 GFLOP (a large library product of this card: 1.3). No one unit bounds it: the
+// matrix cores are busy 40 % of the time, and of the rest a wave's exponentials and packing cost 50 us,
+// the widening and its LDS stores 90, the loads 15, the operands' LDS reads 35 (each taken out alone).
+// Scores a tile ahead brought it there from 700; loads two tiles ahead with exact waits, the widening
+// between the two products and half-tile turns of the waves left it as it is.
 #include <algorithm>
 
 #include "attn_tiles.h"
@@ -35,15 +42,8 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
 constexpr int P8_KT = 64;            // keys per tile: four blocks
 constexpr int P8_MAX_SEQS = 1024;    // sequences per launch (tile prefix in LDS)
-#ifndef P8_NARROW
-#define P8_NARROW 0
-#endif
-#ifndef P8_AHEAD
-#define P8_AHEAD 4
-#endif
-#ifndef P8_PV_VALU
-#define P8_PV_VALU 2
-#endif
+constexpr int P8_AHEAD = 4;           // LDS operands read ahead of their product
+constexpr int P8_PV_VALU = 2;         // vector instructions after each product of the outputs
 constexpr int P8_RSRC_WORD3 = 0x00020000;
 constexpr float P8_RESCALE = 8.0f;   // log2: how far a row's maximum may run ahead of its reference
 
@@ -112,9 +112,10 @@ __device__ __forceinline__ float swap_halves(float x) {  // the value of lane l 
 
 template <int D, int NW, int DT>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArgs a) {
-  constexpr int NT = 64 * NW, KS = D / 16, NB = D / 32, UK = D / 8;
+  constexpr int NT = 64 * NW, KS = D / 16, NB = D / 32;
+  constexpr int UK = D > 64 ? 16 : 8;  // 16-byte units of a K row in LDS
   constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
-  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // bytes, powers of two
+  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // bytes
   __shared__ __align__(16) unsigned char lds[2 * (K_BUF + V_BUF)];
   __shared__ int tile_pref[P8_MAX_SEQS + 1];
   __shared__ int wsum[NW];
@@ -198,12 +199,12 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     uint32_t off, base;
   };
   auto k_part = [&]() {
-    const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = D == 128 ? t & 15 : (t >> 1) & 7;
+    const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = D > 64 ? t & 15 : (t >> 1) & 7;
     return Part{{}, 1.f, uint32_t((c * a.P + (lane & 15)) * 16),
                 uint32_t(t * UK * 16 + 16 * ((2 * c) ^ sw))};
   };
   auto v_part = [&]() {
-    const int x = lane & (VL - 1);
+    const int x = lane & 31;  // below VL; the others load and drop
     return Part{{}, 1.f, uint32_t(hh * 4 * D + 16 * x),
                 2 * K_BUF + uint32_t(x * 4 * 128 + 16 * ((2 * blk + hh) ^ (x & 7)))};
   };
@@ -232,7 +233,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>((is_k ? a.kp : a.vp) + at), 0, ok ? bytes : 0, P8_RSRC_WORD3);
     p.x[0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off, 0, 0));
-    if (D == 128 || !is_k)
+    if (D > 64 || !is_k)
       p.x[1] =
           __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off + step, 0, 0));
     p.scale = (is_k ? a.ks : a.vs)[ok ? head * PB + sub : 0];
@@ -256,7 +257,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   auto stage_k = [&](const Part& p, int buf) {
     const uint32_t base = p.base + buf * K_BUF;
 #pragma unroll
-    for (int i = 0; i < D / 64; ++i) {
+    for (int i = 0; i < UK / 8; ++i) {
       put(base ^ (128 * i), widen8<DT>(p.x[i].x, p.x[i].y, p.scale));
       put(base ^ (128 * i + 16), widen8<DT>(p.x[i].z, p.x[i].w, p.scale));
     }
@@ -311,7 +312,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
   // bits enter by XOR, so one base per lane and a constant give any of them; bases of a buffer, so
   // that they are computed where they are used and not kept.
-  const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (D == 128 ? n32 & 15 : (n32 >> 1) & 7));
+  const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (D > 64 ? n32 & 15 : (n32 >> 1) & 7));
   const uint32_t v_base = n32 * 128 + 16 * (hh ^ (((n32 >> 2) & 7) ^ ((n32 >> 1) & 1)));
   auto kread = [&](int buf, int tb, int k) {
     const uint32_t at = ((k_base + buf * K_BUF) ^ (32 * k)) + 32 * tb * UK * 16;
@@ -513,13 +514,22 @@ void launch(const PrefillArgs& a, unsigned blocks, hipStream_t s) {
 
 }  // namespace
 
+// Against the kernel that streams codes to each 16 rows (2.4 us for 1M rows x keys at head_dim 128, 1.3
+// at 64, whatever the number of items): an item here takes 22 ns a key (head_dim 64: 18) alone or in
+// turn with another on its CU, however few items there are. So the rows (of all heads) have to fill a
+// third of the CUs with items. One sequence of 32 heads, head_dim 128, 4096 keys: 65 us there and 91
+// here at 8192 rows, 112 and 94 at 16384. Where contexts are short the other kernel's second launch
+// counts: 512 keys 18 us and 20 at 1024 rows, 21 and 20 at 2048, 39 and 20 at 16384. And an item's rows
+// cost the same when most are missing: 256 items of 16 rows (4096 keys) 63 us and 94, of 32 rows 98 and
+// 93.
 bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
-                      const int32_t* cu_q, float scale) {
+                      int64_t table_tokens, const int32_t* cu_q, float scale) {
   const int G = Hq / Hkv;
   // scale > 0: the kernel keeps its running max in raw score units
-  return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && (D == 64 || D == 128) &&
+  return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && (D == 64 || D == 96 || D == 128) &&
          scale > 0.f && G <= 128 && cu_q != nullptr && num_seqs <= P8_MAX_SEQS &&
-         total_q_rows * G >= 64 * int64_t(num_seqs);
+         total_q_rows * G >= 32 * int64_t(num_seqs) &&
+         total_q_rows * Hq >= (table_tokens <= 512 ? 8 : 48) * int64_t(device_cus());
 }
 
 int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
@@ -528,26 +538,26 @@ int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, co
                        const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
                        int D, int P, int64_t num_pages, float scale_log2, hipStream_t s) {
   const int G = Hq / Hkv;
-  const int64_t cus = device_cus();
-  const int wide_ppt = 256 / G;
-  const bool wide_ = (ceil_div(total_q_rows, wide_ppt) + num_seqs) * Hkv >= 2 * cus &&
-                    2 * total_q_rows >= int64_t(wide_ppt) * num_seqs;
-  const bool wide = wide_ && !P8_NARROW;
+  // Items of 256 rows halve what is widened for a row but come half as many: for long contexts that
+  // fill the CUs all the same. 32 sequences, 32 heads, 64 rows each: 90 us and 86 at 2048 keys, 322 and
+  // 279 at 8192; 128 rows: 95 and 101 at 1024 keys, 164 and 158 at 2048, 300 and 276 at 4096. At
+  // head_dim 64, where a tile's products are half, they lose everywhere (390 and 430 at 4096 keys).
+  const bool wide =
+      D == 128 && bt_stride * P >= 2048 &&
+      (ceil_div(total_q_rows, 128 / G) + num_seqs / 2) * Hkv >= 2 * int64_t(device_cus());
   const int ppt = (wide ? 256 : 128) / G;
   const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * Hkv, 8) * 8;
   if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many query rows");
   PrefillArgs a{out, q, q_stride, kp, vp, ks, vs, bt, bt_stride, lens, cu, offs, total_q_rows,
                 num_pages, scale_log2, num_seqs, Hq, Hkv, G, P, ppt};
-#define PIA_P8(D, DT)                                   \
-  {                                                     \
-    if (wide) launch<D, 8, DT>(a, unsigned(blocks), s); \
-    else launch<D, 4, DT>(a, unsigned(blocks), s);      \
+#define PIA_P8(DT)                                                 \
+  {                                                                \
+    if (wide) launch<128, 8, DT>(a, unsigned(blocks), s);          \
+    else if (D == 128) launch<128, 4, DT>(a, unsigned(blocks), s); \
+    else if (D == 96) launch<96, 4, DT>(a, unsigned(blocks), s);   \
+    else launch<64, 4, DT>(a, unsigned(blocks), s);                \
   }
-  if (dtype == PIA_DTYPE_F16) {
-    if (D == 64) PIA_P8(64, PIA_DTYPE_F16) else PIA_P8(128, PIA_DTYPE_F16)
-  } else {
-    if (D == 64) PIA_P8(64, PIA_DTYPE_BF16) else PIA_P8(128, PIA_DTYPE_BF16)
-  }
+  if (dtype == PIA_DTYPE_F16) PIA_P8(PIA_DTYPE_F16) else PIA_P8(PIA_DTYPE_BF16)
 #undef PIA_P8
   return check_launch("kv8_prefill");
 }

@@ -78,6 +78,8 @@ def _checked_shape(p: KV8Pools) -> tuple[int, int, int, int]:
         raise ValueError(f"pools.k must be [num_pages, H, D / 16, P, 16], got {tuple(p.k.shape)}")
     n, h, d, page = p.shape
     _check_shape(d, page)
+    if n == 0 or h == 0:
+        raise ValueError("8-bit pools need a page and a head")
     if p.v.shape != (n, h, page // 4, d, 4):
         raise ValueError(f"pools.v must be {(n, h, page // 4, d, 4)}, got {tuple(p.v.shape)}")
     if p.k.dtype != torch.float8_e4m3fn or p.v.dtype != torch.float8_e4m3fn:
@@ -111,7 +113,8 @@ def kv8_gather(pools: KV8Pools, block_tables: torch.Tensor, cu_seqlens: torch.Te
     """kv_gather of 8-bit pools: rows cu_seqlens[b]..cu_seqlens[b+1] of the results hold sequence
     b's tokens in logical order, [total_tokens, Hkv, D] in dtype (or that of the `out` buffers,
     whose first dimension is then the total). bf16 and fp32 hold the pool's values exactly.
-    max_seq_len: a bound of every length; 0 gathers nothing."""
+    max_seq_len: a bound of every length; 0 gathers nothing. Tokens of a page outside the pool are
+    zeros; rows past a sequence's table are left as they are."""
     num_pages, H, D, P = _check_pools(pools)
     dev = N.require_device(pools.k, block_tables, cu_seqlens,
                            names=("pools.k", "block_tables", "cu_seqlens"))
@@ -135,7 +138,7 @@ def kv8_gather(pools: KV8Pools, block_tables: torch.Tensor, cu_seqlens: torch.Te
                 or not (k_out.is_contiguous() and v_out.is_contiguous()):
             raise ValueError(f"out buffers must be contiguous [tokens, {H}, {D}] of one dtype")
     code = N.dtype_code(k_out.dtype)
-    if B and max_seq_len > 0 and bt.shape[1] > 0 and num_pages:
+    if B and max_seq_len > 0 and bt.shape[1] > 0:
         N.call_on(dev, "pia_kv8_gather", k_out.data_ptr(), v_out.data_ptr(), pools.k.data_ptr(),
                   pools.v.data_ptr(), pools.k_scale.data_ptr(), pools.v_scale.data_ptr(),
                   bt.data_ptr(), bt.shape[1], cu.data_ptr(), B, k_out.shape[0], H, D, P,
@@ -198,8 +201,6 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
         raise ValueError("out must be a contiguous, 16-byte aligned tensor of q's shape and dtype")
     if rows == 0 or B == 0:
         return out
-    if num_pages == 0:
-        return out.zero_()
     need = _workspace_bytes(D, dev.index)
     if workspace is None or workspace.numel() * workspace.element_size() < need \
             or workspace.data_ptr() % 16 or not workspace.is_contiguous():

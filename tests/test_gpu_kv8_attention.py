@@ -119,6 +119,43 @@ def test_rows(dev, case, dtype):
     _check(got[:cu[-1]], ref, mag, size, dtype, max(lens), dim, rows=True)
 
 
+MANY = [  # as ROWS, and the tables' width in tokens; rows of all heads from 2048 on
+    ([70, 1, 33], [70, 64, 200], "end", 32, 8, 128, 16, 0),
+    ([20, 0, 9], [500, 3, 130], "end", 96, 8, 96, 32, 0),
+    ([40, 30], [90, 20], [-3, 4], 40, 2, 64, 16, 0),
+    ([50], [45], None, 64, 64, 96, 48, 0),
+    ([17], [400], [2000], 128, 1, 128, 64, 0),
+    ([65, 40], [65, 300], "end", 128, 16, 64, 16, 600),
+    ([9, 12, 1, 30, 0, 17, 8, 9, 10, 6, 5, 11, 7, 9, 9, 13, 8, 9, 12, 7],
+     [9, 70, 33, 150, 8, 17, 128, 129, 40, 63, 64, 65, 80, 9, 100, 14, 20, 31, 12, 200], "end",
+     128, 32, 128, 16, 2048),
+]
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{sum(c[0])}of{max(c[1])}h{c[3]}/{c[4]}d{c[5]}w{c[7]}")
+def test_many_rows(dev, case, dtype):
+    new, lens, offs, hq, hkv, dim, page, width = case
+    tables, pages = _tables(lens, page, 2, sum(lens))
+    if width:
+        tables = torch.nn.functional.pad(tables, (0, width // page - tables.shape[1]), value=-1)
+    pool = O.Pool.random(pages, hkv, dim, page, seed=dim + hq + 2)
+    cu = [0]
+    for n in new:
+        cu.append(cu[-1] + n)
+    offs = [n - m for n, m in zip(lens, new)] if offs == "end" else offs
+    q = _rows(cu[-1] + 3, hq, dim, dtype, hq + 1)       # three rows behind the last sequence
+    out = torch.full(q.shape, 5.0, dtype=dtype, device=dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    got = paged_attention_kv8(q.to(dev), pool.to_device(dev), tables.to(dev), i32(lens),
+                              cu_q=i32(cu), q_pos_offsets=None if offs is None else i32(offs),
+                              out=out)
+    assert (out[cu[-1]:] == 5.0).all()
+    ref, mag, size = O.attend(q[:cu[-1]], pool, tables.tolist(), lens, cu, offs,
+                              1 / math.sqrt(dim))
+    _check(got[:cu[-1]], ref, mag, size, dtype, max(lens), dim, rows=True)
+
+
 def test_long_and_many(dev):
     """A long context (cut over all waves), and more sequences than one launch's tables hold:
     against the same values gathered, in fp32 (2^-8 for bf16 results, 2^-13 for what fp32 sums)."""
@@ -148,12 +185,18 @@ def test_long_and_many(dev):
             assert ((got[b].double().cpu() - ref).abs() <= 2.0 ** -8 * ref.abs() + 2.0 ** -9 * mag).all()
 
 
-def test_what_a_row_may_not_see(dev):
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("shape", [(1, 4, 128, 0), (8, 96, 128, 0), (8, 96, 64, 0), (8, 96, 96, 0),
+                                   (256, 1024, 128, 2048)],
+                         ids=lambda s: f"h{s[1]}/{s[0]}d{s[2]}w{s[3]}")
+def test_what_a_row_may_not_see(dev, shape, dtype):
     """Stale codes behind a context (NaN among them), pages outside the pool, and NaN keys and values
     of tokens that a row's limit hides leave its result alone; where they are seen, they show."""
-    dim, hkv, hq, page = 128, 1, 4, 16
+    (hkv, hq, dim, width), page = shape, 16
     lens, new = [37, 90], [5, 20]
     tables, pages = _tables(lens, page, 1, 7)
+    if width:
+        tables = torch.nn.functional.pad(tables, (0, width // page - tables.shape[1]), value=-1)
     clean = O.Pool.random(pages, hkv, dim, page, seed=3)
     dirty = O.Pool.random(pages, hkv, dim, page, seed=3)
     for b, n in enumerate(lens):     # past the context
@@ -161,8 +204,8 @@ def test_what_a_row_may_not_see(dev):
         for x in "kv":
             clean.codes[x][last, :, n % page or page:] = 0.0
             dirty.codes[x][last, :, n % page or page:] = math.nan
-    cu, offs = [0, 5, 25], [32, 70]
-    q = _rows(25, hq, dim, torch.bfloat16, 1)
+    cu, offs, g = [0, 5, 25], [32, 70], hq // hkv   # g heads share the first kv head
+    q = _rows(25, hq, dim, dtype, 1)
     i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
 
     def run(pool, t=tables):
@@ -171,26 +214,26 @@ def test_what_a_row_may_not_see(dev):
 
     want = run(clean)
     assert torch.equal(run(dirty), want)
-    # sequence 1, position 81: a NaN key, and a NaN value of elements 3 and 70
+    # sequence 1, position 81: a NaN key, and a NaN value of two elements
     i, o = int(tables[1, 81 // page]), 81 % page
     for x in "kv":
         bad = O.Pool.random(pages, hkv, dim, page, seed=3)
-        bad.codes[x][i, 0, o, [3, 70]] = math.nan
+        bad.codes[x][i, 0, o, [3, dim - 2]] = math.nan
         got = run(bad)
         sees = torch.zeros(25, dtype=torch.bool)
         sees[5 + 11:] = True
         assert torch.equal(got[~sees], want[~sees])
         if x == "k":
-            assert torch.isnan(got[sees]).all()
+            assert torch.isnan(got[sees][:, :g]).all() and torch.isfinite(got[:, g:]).all()
         else:
             hit = torch.isnan(got[sees])
-            assert hit[..., [3, 70]].all() and hit.sum() == 2 * hq * sees.sum()
+            assert hit[:, :g, [3, dim - 2]].all() and hit.sum() == 2 * g * sees.sum()
     # a page that is not there holds no keys
     t = tables.clone()
     t[1, 2] = pages + 9
     got = run(clean, t)
     ref, mag, size = O.attend(q, clean, t.tolist(), lens, cu, offs, 1 / math.sqrt(dim))
-    _check(got, ref, mag, size, torch.bfloat16, 90, dim, rows=True)
+    _check(got, ref, mag, size, dtype, 90, dim, rows=True)
     t[0, :] = -1
     assert (run(clean, t)[:5] == 0).all()
     for value in (math.nan, math.inf):
@@ -313,6 +356,7 @@ def test_refusals(dev):
            dict(q_pos_offsets=n[:1]), dict(q_pos_offsets=n.float()), dict(out=q.half()),
            dict(out=q[:1]), dict(q=q.clone().requires_grad_()),
            dict(pools=KV8Pools(pools.k, pools.v[:1], pools.k_scale, pools.v_scale)),
+           dict(pools=KV8Pools.allocate(0, 2, 32, 16, dev)),
            dict(pools=KV8Pools(pools.k.view(torch.uint8), pools.v, pools.k_scale, pools.v_scale))]
     for kw in bad:
         args = dict(q=q, pools=pools, block_tables=t, kv_lens=n) | kw
