@@ -26,6 +26,11 @@ overlap=False is the reference's order: ensure_experts, copy_missing, one FFN.
 The reference writes a zero K / V row for every layer before the real one
 (decode_step_moe_paged's dummy append, :119-122); each position is written once here, by the
 scatter, before attention reads it, so the zero writes are skipped.
+
+Over 8-bit pools (MoePagedDecoder's kv8_pools) a layer's RoPE, KV write and attention are kv8_append
+and paged_decode_attention_kv8: k is rotated, rounded once to e4m3 with its block's scale, and the
+rotation's cos and sin are exact to fp32 where the other path takes them from a table in the model
+dtype. Half the KV bytes of a bf16 pool.
 """
 
 from __future__ import annotations
@@ -39,7 +44,10 @@ import torch.nn.functional as F
 from ..kernel.moe_ops import moe_sum_reduce
 from ..kernel.norm_rope import add_rms_norm_rows, qk_norm_rope, rms_norm_rows
 from ..kernel.paged_kv import decode_workspace_bytes, paged_decode_append_attention
+from ..kernel.paged_kv8 import (KV8Pools, kv8_append, kv8_attention_workspace_bytes,
+                                paged_decode_attention_kv8)
 from ..kernel.pinned import alloc_pinned_exact
+from ..kernel.rotary import rope_params
 from ..moe.fused import fused_experts_decode_impl, fused_topk, routed_ffn_routes
 from ..moe.offload_cache import OffloadMoeCache
 from .attention import build_rope_cache
@@ -157,14 +165,31 @@ class DecodeBatch:
 class MoePagedDecoder:
     """Batched decode of a random-init or loaded MoE model over one KV pool shared by all
     layers (each layer's pages are distinct page ids, as KVStore lays them out) and an
-    OffloadMoeCache holding the routed experts."""
+    OffloadMoeCache holding the routed experts. The pool is k_pages and v_pages, or (with those
+    None) kv8_pools, which keeps the context in 8 bits."""
 
     def __init__(self, weights: dict[str, torch.Tensor], cfg: MoeModelConfig,
-                 moe_cache: OffloadMoeCache, k_pages: torch.Tensor, v_pages: torch.Tensor,
-                 max_batch: int, overlap: bool = True) -> None:
+                 moe_cache: OffloadMoeCache, k_pages: torch.Tensor | None,
+                 v_pages: torch.Tensor | None, max_batch: int, overlap: bool = True,
+                 kv8_pools: KV8Pools | None = None) -> None:
         self.w, self.cfg, self.cache = weights, cfg, moe_cache
         self.k_pages, self.v_pages = k_pages, v_pages
+        self.kv8_pools = kv8_pools
         self.overlap = overlap
+        self.layer_hook = None   # called as hook(layer, dict of the layer's tensors)
+        if kv8_pools is not None:
+            if k_pages is not None or v_pages is not None:
+                raise ValueError("kv8_pools take the place of k_pages and v_pages")
+            if kv8_pools.shape[1:3] != (cfg.n_kv_heads, cfg.head_dim):
+                raise ValueError(f"kv8_pools must hold {cfg.n_kv_heads} heads of {cfg.head_dim}, got "
+                                 f"{kv8_pools.shape[1:3]}")
+            self.device = dev = kv8_pools.k.device
+            self._rope = rope_params(cfg.head_dim, base=cfg.rope_base, device=dev)
+            self._ws = torch.empty(kv8_attention_workspace_bytes(cfg.head_dim, dev),
+                                   dtype=torch.uint8, device=dev)
+            return
+        if k_pages is None or v_pages is None:
+            raise ValueError("k_pages and v_pages, or kv8_pools, must be given")
         dev = k_pages.device
         self.device = dev
         self.cos, self.sin = build_rope_cache(cfg.max_seq_len, cfg.head_dim, base=cfg.rope_base,
@@ -173,7 +198,6 @@ class MoePagedDecoder:
         self._ws = torch.empty(max(1, decode_workspace_bytes(
             max_batch, cfg.n_heads, cfg.n_kv_heads, cfg.head_dim, P,
             math.ceil(cfg.max_seq_len / P))), dtype=torch.uint8, device=dev)
-        self.layer_hook = None   # called as hook(layer, dict of the layer's tensors)
 
     # ---- pieces --------------------------------------------------------------------------------
 
@@ -232,12 +256,29 @@ class MoePagedDecoder:
         x, routed = self._layer(l, x, h, batch, self._rope_rows(batch))
         return x + routed
 
-    def _rope_rows(self, batch: DecodeBatch) -> tuple[torch.Tensor, torch.Tensor]:
-        """The rows' cos / sin table rows [B, D]: every layer of a step takes the same."""
+    def _rope_rows(self, batch: DecodeBatch) -> tuple[torch.Tensor, torch.Tensor] | None:
+        """The rows' cos / sin table rows [B, D]: every layer of a step takes the same. None over
+        8-bit pools, where the append rotates."""
+        if self.kv8_pools is not None:
+            return None
         return self.cos[batch.positions], self.sin[batch.positions]
 
+    def _attend_kv8(self, l: int, q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                    qk_weights: tuple[torch.Tensor | None, torch.Tensor | None],
+                    batch: DecodeBatch) -> tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+        """(rotated q, normed k, attention) of a layer's new rows over the 8-bit pools, which take
+        k rotated and v."""
+        with torch.no_grad():
+            if qk_weights[0] is not None:
+                q, k = rms_norm_rows(q, qk_weights[0]), rms_norm_rows(k, qk_weights[1])
+            bt = batch.block_tables[l]
+            q = kv8_append(q, k, v, self.kv8_pools, bt, batch.context_lens, rope=self._rope)
+            return q, k, paged_decode_attention_kv8(q, self.kv8_pools, bt, batch.context_lens,
+                                                    workspace=self._ws)
+
     def _layer(self, l: int, x: torch.Tensor, h: torch.Tensor, batch: DecodeBatch,
-               rope: tuple[torch.Tensor, torch.Tensor]) -> tuple[torch.Tensor, torch.Tensor]:
+               rope: tuple[torch.Tensor, torch.Tensor] | None
+               ) -> tuple[torch.Tensor, torch.Tensor]:
         """A layer from its input x and that input's norm h: (x after attention, the routed
         experts' output), whose sum is the layer's output."""
         cfg, w = self.cfg, self.w
@@ -249,13 +290,16 @@ class MoePagedDecoder:
         v = F.linear(h, w[p + "self_attn.v_proj.weight"]).view(B, Hkv, D)
         qk_weights = (w[p + "self_attn.q_norm.weight"], w[p + "self_attn.k_norm.weight"]) \
             if cfg.qk_norm else (None, None)
-        q, k = qk_norm_rope(q, k, *qk_weights, *rope)
-        v = v.contiguous()
-        # the reference's _write_kv_layer then _attn_paged, as one call: the new token goes to
-        # its slot and the attention takes it from k / v directly
-        attn = paged_decode_append_attention(q, self.k_pages, self.v_pages,
-                                             batch.block_tables[l], batch.context_lens, k, v,
-                                             workspace=self._ws)
+        if self.kv8_pools is not None:
+            q, k, attn = self._attend_kv8(l, q, k, v, qk_weights, batch)
+        else:
+            q, k = qk_norm_rope(q, k, *qk_weights, *rope)
+            v = v.contiguous()
+            # the reference's _write_kv_layer then _attn_paged, as one call: the new token goes to
+            # its slot and the attention takes it from k / v directly
+            attn = paged_decode_append_attention(q, self.k_pages, self.v_pages,
+                                                 batch.block_tables[l], batch.context_lens, k, v,
+                                                 workspace=self._ws)
         x, h = add_rms_norm_rows(x, F.linear(attn.view(B, Hq * D),
                                              w[p + "self_attn.o_proj.weight"]),
                                  w[p + "post_attention_layernorm.weight"])
