@@ -161,7 +161,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   constexpr int MB = DP > 128 ? 2 : 4;  // blocks of a step (registers)
   constexpr int STEP = 16 * MB, ND = DP / 64, AUX = ONCE ? 2 : 0;
   __shared__ int64_t pref[KA_MAX_SEQS + 1];
-  __shared__ int steps_of[KA_MAX_SEQS];
+  __shared__ int4 seq_of[KA_MAX_SEQS];  // first row (below 2^31), rows, keys, offset
   __shared__ int64_t wsum[KA_WG_WAVES];
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   constexpr int NTH = 64 * KA_WG_WAVES;
@@ -174,7 +174,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     int64_t incl = 0;
     if (b < a.B) {
       const Seq s = sequence(a, b, STEP);
-      steps_of[b] = s.steps;
+      seq_of[b] = make_int4(int(s.row0), s.n, s.kv_len, s.off);
       incl = int64_t(s.items) * a.Hkv * s.steps;
     }
 #pragma unroll
@@ -205,10 +205,10 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     int b, h, i, t, items, steps, kv_len;
   };
   auto enter = [&](Cursor& c) {
-    const int64_t per = pref[c.b + 1] - pref[c.b];
-    c.steps = uniform(steps_of[c.b]);
-    c.items = uniform(int(quotient(per, int64_t(c.steps) * a.Hkv)));
-    c.kv_len = uniform(sequence(a, c.b, STEP).kv_len);
+    const int4 s = seq_of[c.b];
+    c.kv_len = uniform(s.z);
+    c.steps = (c.kv_len + STEP - 1) / STEP;
+    c.items = uniform(int((int64_t(s.y) * a.G + 15) >> 4));
   };
   auto advance = [&](Cursor& c) {
     if (++c.t < c.steps) return;
@@ -320,9 +320,10 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
     if (!opened) {
       opened = true;
       begun = x;
-      const Seq s = sequence(a, cur.b, STEP);
-      row0 = s.row0;
-      rows_left = s.n * a.G - 16 * cur.i;
+      const int4 s = seq_of[cur.b];
+      const int off = uniform(s.w);
+      row0 = uniform(s.x);
+      rows_left = uniform(s.y) * a.G - 16 * cur.i;
       const int r = 16 * cur.i + n16, pos = r / a.G;
       const bool ok = n16 < rows_left;
       const T* qp = static_cast<const T*>(a.q) + (row0 + (ok ? pos : 0)) * a.q_stride +
@@ -344,10 +345,10 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
           for (int n = 0; n < NQ; ++n)
             asm volatile("" : "+v"(qr[i][e][n].x), "+v"(qr[i][e][n].y), "+v"(qr[i][e][n].z),
                               "+v"(qr[i][e][n].w));
-      lim = lim_min = s.kv_len;
+      lim = lim_min = cur.kv_len;
       if (!ONCE && a.offs) {
-        lim = min(lim, s.off + pos + 1);
-        lim_min = min(lim_min, s.off + (16 * cur.i) / a.G + 1);
+        lim = min(lim, off + pos + 1);
+        lim_min = min(lim_min, off + (16 * cur.i) / a.G + 1);
       }
       m = -INFINITY;
       l = 0.f;

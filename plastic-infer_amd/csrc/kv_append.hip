@@ -22,6 +22,10 @@ namespace {
 constexpr int KA_THREADS = 256;
 constexpr int KA_WAVES = KA_THREADS / 64;
 
+// bytes of a wave's tile: 16 tokens of 128 elements
+template <int DT>
+constexpr int KA_TILE = 16 * 128 * int(sizeof(typename Elem<DT>::T));
+
 struct AppendArgs {
   void* q_out;
   const void *q, *k, *v;
@@ -271,83 +275,109 @@ __device__ __forceinline__ void append8_v(const AppendArgs& a, int h, int64_t r0
 }
 
 // K (which = 0) or V of one (block, kv head) of a pool of the model's type by one wave: a lane has
-// two elements of all the block's tokens, so that a full block goes out in 16-byte stores.
-template <int DT>
-__device__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row, int which, int h,
-                             int64_t r0, int64_t p0, int n, const int32_t* row) {
+// E consecutive elements of the block's n tokens (NT at most; all loads go out before any is used, those
+// past n are the last token's again). A whole block goes out in the pool's order, 16 bytes a lane and
+// a KB of consecutive ones a store, through a tile in LDS (K and V of 5000 tokens, 8 heads of 128 in
+// bf16: 20 us, and 22 straight from the lanes that have them, 64 bytes apart); of others each element
+// goes to its place. Token by token, with a page looked up and a row loaded for each, a prompt's
+// ragged ends took longer than all its blocks: the same call is 12.5 us, 3.3 TB/s, without.
+template <int DT, int E, int NT>
+__device__ __forceinline__ void append_plain(const AppendArgs& a, const float2* tab, int tab_row,
+                                             int which, int h, int64_t r0, int64_t p0, int n,
+                                             const int32_t* row, unsigned char* tile) {
   using T = typename Elem<DT>::T;
-  constexpr int TV = 16 / int(sizeof(T));
+  constexpr int TV = 16 / int(sizeof(T)), N = 2 * 16 / TV;
   const int lane = threadIdx.x & 63, D = a.D, P = a.P, rd = which ? 0 : 2 * a.pairs;
   const int64_t tok = which ? a.v_tok : a.k_tok;
   const T* x = static_cast<const T*>(which ? a.v : a.k) + r0 * tok + h * (which ? a.v_head : a.k_head);
   T* pool = static_cast<T*>(which ? a.v_pages : a.k_pages);
-  // a whole block in whole 16-byte vectors of one page
-  if (n == 16 && a.whole && (which ? a.v_pair : a.k_pair)) {
-    const uint32_t slot = uint32_t(p0) / uint32_t(P);
+  struct alignas(E * sizeof(T)) Part {
+    T v[E];
+  };
+  struct alignas(16) Pack {
+    T x[TV];
+  };
+  // lane t: where token t's first element goes, -1 where its page is not in the pool
+  int64_t to = -1;
+  if (lane < n) {
+    const uint32_t pos = uint32_t(p0 + lane), slot = pos / uint32_t(P);
     const int32_t page = row[slot];
-    if (uint32_t(page) >= uint64_t(a.num_pages)) return;
-    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + (uint32_t(p0) - slot * uint32_t(P));
-    struct alignas(2 * sizeof(T)) Two {
-      T v[2];
-    };
-    struct alignas(16) Pack {
-      T x[TV];
-    };
-    for (int d = 2 * lane; d < D; d += 128) {
-      Two own[16], other[16];
-      const bool turned = d < rd, first = d < a.pairs;
-      const int od = first ? d + a.pairs : d - a.pairs;
-#pragma unroll
-      for (int t = 0; t < 16; ++t) own[t] = *reinterpret_cast<const Two*>(x + t * tok + d);
-      if (turned && !a.inter) {
-#pragma unroll
-        for (int t = 0; t < 16; ++t) other[t] = *reinterpret_cast<const Two*>(x + t * tok + od);
-      }
-      Pack o[2][16 / TV];
-#pragma unroll
-      for (int t = 0; t < 16; ++t) {
-        T e0 = own[t].v[0], e1 = own[t].v[1];
-        if (turned) {
-          const float2* cs = tab + t * tab_row;
-          const float v0 = Elem<DT>::load(own[t].v, 0), v1 = Elem<DT>::load(own[t].v, 1);
-          if (a.inter) {
-            const float2 f = cs[d / 2];
-            Elem<DT>::store(&e0, 0, rope::turn(v0, -v1, f.x, f.y));
-            Elem<DT>::store(&e1, 0, rope::turn(v1, v0, f.x, f.y));
-          } else {
-            const float2 f0 = cs[first ? d : od], f1 = cs[(first ? d : od) + 1];
-            const float w0 = Elem<DT>::load(other[t].v, 0), w1 = Elem<DT>::load(other[t].v, 1);
-            Elem<DT>::store(&e0, 0, rope::turn(v0, first ? -w0 : w0, f0.x, f0.y));
-            Elem<DT>::store(&e1, 0, rope::turn(v1, first ? -w1 : w1, f1.x, f1.y));
-          }
-        }
-        o[0][t / TV].x[t % TV] = e0;
-        o[1][t / TV].x[t % TV] = e1;
-      }
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < 16 / TV; ++i)
-          reinterpret_cast<Pack*>(to + int64_t(d + e) * P)[i] = o[e][i];
-    }
-    return;
+    if (uint32_t(page) < uint64_t(a.num_pages))
+      to = (int64_t(page) * a.Hkv + h) * D * P + (pos - slot * uint32_t(P));
   }
-  for (int t = 0; t < n; ++t) {
-    const uint32_t pos = uint32_t(p0 + t), slot = pos / uint32_t(P);
-    const int32_t page = row[slot];
-    if (uint32_t(page) >= uint64_t(a.num_pages)) continue;
-    T* to = pool + (int64_t(page) * a.Hkv + h) * D * P + (pos - slot * uint32_t(P));
-    for (int d = lane; d < D; d += 64) {
-      const T* xt = x + t * tok;
-      T e = xt[d];
-      if (d < rd) {
-        const bool first = a.inter ? !(d & 1) : d < a.pairs;
-        const int od = a.inter ? d ^ 1 : first ? d + a.pairs : d - a.pairs;
-        const float p = Elem<DT>::load(xt, od);
-        const float2 f = tab[t * tab_row + (a.inter ? d >> 1 : first ? d : od)];
-        Elem<DT>::store(&e, 0, rope::turn(Elem<DT>::load(xt, d), first ? -p : p, f.x, f.y));
+  auto to_of = [&](int t) {
+    return int64_t(uint64_t(uint32_t(__builtin_amdgcn_readlane(int(to >> 32), t))) << 32 |
+                   uint32_t(__builtin_amdgcn_readlane(int(to), t)));
+  };
+  for (int d0 = 0; d0 < D; d0 += 64 * E) {
+    const bool in = d0 + E * lane < D;
+    const int d = in ? d0 + E * lane : 0;
+    const bool turned = d < rd, first = a.inter ? !(d & 1) : d < a.pairs;
+    const int od = a.inter ? (E == 2 ? d : d ^ 1) : first ? d + a.pairs : d - a.pairs;
+    Part own[NT], other[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t)
+      own[t] = *reinterpret_cast<const Part*>(x + min(t, n - 1) * tok + d);
+    if (turned && !(E == 2 && a.inter)) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+        other[t] = *reinterpret_cast<const Part*>(x + min(t, n - 1) * tok + od);
+    }
+    if (turned && E == 2 && a.inter) {
+#pragma unroll
+      for (int t = 0; t < NT; ++t) {
+        const float2 f = tab[t * tab_row + d / 2];
+        const float v0 = Elem<DT>::load(own[t].v, 0), v1 = Elem<DT>::load(own[t].v, E - 1);
+        own[t].v[0] = rope::narrow<DT>(rope::turn(v0, -v1, f.x, f.y));
+        own[t].v[E - 1] = rope::narrow<DT>(rope::turn(v1, v0, f.x, f.y));
       }
-      to[int64_t(d) * P] = e;
+    } else if (turned) {
+      const float2* cs = tab + (a.inter ? d >> 1 : first ? d : od);
+      const float sign = first ? -1.f : 1.f;
+#pragma unroll
+      for (int t = 0; t < NT; ++t)
+#pragma unroll
+        for (int e = 0; e < E; ++e) {
+          const float2 f = cs[t * tab_row + e];
+          own[t].v[e] = rope::narrow<DT>(rope::turn(Elem<DT>::load(own[t].v, e),
+                                                    sign * Elem<DT>::load(other[t].v, e), f.x, f.y));
+        }
+    }
+    if constexpr (E == 2 && NT == 16) {
+      if (n == 16 && a.whole) {
+        const int64_t base = to_of(0);  // one page: P is a multiple of 16
+        if (base < 0) return;
+        // 16-byte units of the tile, in the pool's order; a lane writes N of them in a row. The order
+        // within N is XORed so that eight lanes' units fall into different banks either way.
+        auto place = [&](int u) {
+          return reinterpret_cast<Pack*>(tile) + ((u & ~(N - 1)) | ((u ^ (u >> 3)) & (N - 1)));
+        };
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+#pragma unroll
+          for (int i = 0; i < 16 / TV; ++i) {
+            Pack o;
+#pragma unroll
+            for (int j = 0; j < TV; ++j) o.x[j] = own[TV * i + j].v[e];
+            *place(N * lane + e * (16 / TV) + i) = o;
+          }
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int i = 0; i < N; ++i) {
+          const int u = lane + 64 * i, at = d0 + u / (16 / TV);
+          if (at < D)
+            reinterpret_cast<Pack*>(pool + base + int64_t(at) * P)[u % (16 / TV)] = *place(u);
+        }
+        __builtin_amdgcn_wave_barrier();
+        continue;
+      }
+    }
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+      const int64_t base = t < n ? to_of(t) : -1;
+      if (base < 0 || !in) continue;
+#pragma unroll
+      for (int e = 0; e < E; ++e) pool[base + int64_t(d + e) * P] = own[t].v[e];
     }
   }
 }
@@ -434,7 +464,15 @@ __global__ __launch_bounds__(KA_THREADS) void kv_append_kernel(AppendArgs a) {
     if (which) append8_v<DT, NC>(a, h, r0, o0, m, head, sub, was);
     else append8_k<DT, NC>(a, tab, tab_row, h, r0, o0, m, head, sub, was);
   } else {
-    append_plain<DT>(a, tab, tab_row, which, h, r0, p0, m, row);
+    unsigned char* tile = reinterpret_cast<unsigned char*>(tab + 16 * tab_row) + wave * KA_TILE<DT>;
+    const bool two = which ? a.v_pair : a.k_pair;
+    if (m == 1) {
+      if (two) append_plain<DT, 2, 1>(a, tab, tab_row, which, h, r0, p0, m, row, tile);
+      else append_plain<DT, 1, 1>(a, tab, tab_row, which, h, r0, p0, m, row, tile);
+    } else {
+      if (two) append_plain<DT, 2, 16>(a, tab, tab_row, which, h, r0, p0, m, row, tile);
+      else append_plain<DT, 1, 16>(a, tab, tab_row, which, h, r0, p0, m, row, tile);
+    }
   }
 }
 
@@ -600,7 +638,8 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
   a.stream = num_tokens * a.Hq * head_dim * elem >= rope::kStreamBytes;
   if (shares > 65535) return fail(PIA_EINVAL, "kv_append: too many heads");
   const dim3 grid{unsigned(blocks), unsigned(shares), 1u};
-  const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1);
+  const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1) +
+                     (cu_new && !kv8 ? size_t(KA_WAVES * 16 * 128 * elem) : 0);  // the tiles
   hipStream_t s = as_stream(stream);
 #define PIA_KA(DT, NC, QV) \
   hipLaunchKernelGGL((kv_append_kernel<DT, NC, QV>), grid, dim3(KA_THREADS), lds, s, a)

@@ -45,6 +45,15 @@ __device__ __forceinline__ float turn(float x, float y, float c, float s) {
   return r;
 }
 
+// x rounded to nearest even, by the instruction that does it (bf16: two elements at once; in integer
+// arithmetic with a branch for NaN it is ten, and the rotation bound by them)
+template <int DT>
+__device__ __forceinline__ typename Elem<DT>::T narrow(float x) {
+  if constexpr (DT == PIA_DTYPE_BF16) return __builtin_bit_cast(uint16_t, static_cast<__bf16>(x));
+  else if constexpr (DT == PIA_DTYPE_F16) return f32_to_half(x);
+  else return x;
+}
+
 // V consecutive elements of a 16- or 32-bit row as floats, by 16-byte vectors (VEC) or one by one
 template <int DT, int V, bool VEC>
 __device__ __forceinline__ void load(const typename Elem<DT>::T* p, float (&x)[V]) {
@@ -80,7 +89,7 @@ __device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&x)[
     for (int i = 0; i < V; i += W / int(sizeof(T))) {
       Pack a;
 #pragma unroll
-      for (int j = 0; j < W / int(sizeof(T)); ++j) Elem<DT>::store(a.v, j, x[i + j]);
+      for (int j = 0; j < W / int(sizeof(T)); ++j) a.v[j] = narrow<DT>(x[i + j]);
       if constexpr (W == 16) {
         if (stream) {
           __builtin_nontemporal_store(__builtin_bit_cast(u32x4_t, a),
@@ -92,7 +101,7 @@ __device__ __forceinline__ void store(typename Elem<DT>::T* p, const float (&x)[
     }
   } else {
 #pragma unroll
-    for (int i = 0; i < V; ++i) Elem<DT>::store(p, i, x[i]);
+    for (int i = 0; i < V; ++i) p[i] = narrow<DT>(x[i]);
   }
 }
 
