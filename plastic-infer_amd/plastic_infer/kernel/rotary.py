@@ -151,7 +151,9 @@ class _Rotary(torch.autograd.Function):
         positions, turns = ctx.saved_tensors
         factor, interleaved, transposed = ctx.form
         rope = RopeParams(turns, factor, interleaved)
-        return *_Rotary.apply(gq, gk, positions, rope, not transposed), None, None, None
+        # a graph of the gradient is wanted only by who differentiates it again
+        run = _Rotary.apply if torch.is_grad_enabled() else _launch
+        return *run(gq, gk, positions, rope, not transposed), None, None, None
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
