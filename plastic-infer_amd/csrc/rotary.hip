@@ -6,7 +6,7 @@
 // The transposed map (the gradient's) is the same with s negated. Bound by HBM: every element is read
 // and written once. A workgroup takes a few tokens, computes their (cos, sin) into LDS once for all
 // heads of q and k, and then streams the heads in 16-byte vectors; fp32 arithmetic, one rounding. 8192
-// tokens of 32 + 8 heads of 128, bf16: 28.6 us, 5.9 TB/s (40 us with ordinary stores).
+// tokens of 32 + 8 heads of 128, bf16: 29 to 35 us, 4.8 to 5.8 TB/s (40 us with ordinary stores).
 #include <algorithm>
 
 #include "rope.h"
