@@ -588,7 +588,8 @@ int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, const void* v_
 /* Attention over the 8-bit pool: q / out [total_q_rows, num_heads, head_dim], rows of sequence b =
  * cu_q[b] .. cu_q[b + 1] (NULL: row b). Row s of b attends keys j < kv_lens[b] and, with
  * q_pos_offsets, j <= q_pos_offsets[b] + s; q head h reads kv head h / (num_heads / num_kv_heads).
- * A row without a key is zeros; a page id outside the pool holds no keys. q rows are q_stride
+ * A row without a key is zeros; a page id outside the pool holds no keys; rows behind the last
+ * sequence's are left. q rows are q_stride
  * elements apart (whole 16-byte vectors), out is contiguous. workspace: 16-byte aligned, of
  * pia_kv8_attention_workspace_bytes(head_dim) bytes, any content; calls that share one are ordered on one
  * stream. */

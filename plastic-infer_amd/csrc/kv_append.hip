@@ -643,8 +643,12 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
   a.stream = num_tokens * a.Hq * head_dim * elem >= rope::kStreamBytes;
   if (shares > 65535) return fail(PIA_EINVAL, "kv_append: too many heads");
   const dim3 grid{unsigned(blocks), unsigned(shares), 1u};
-  const size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1) +
-                     (cu_new && !kv8 ? size_t(KA_WAVES * 16 * 128 * elem) : 0);  // the tiles
+  size_t lds = sizeof(float2) * size_t(cu_new ? 16 : 1) * size_t(pairs + 1);
+  if (cu_new && !kv8 && a.whole) {  // and the tiles, if a launch may have that much (pairs to 255)
+    const size_t tiles = size_t(KA_WAVES) * 16 * 128 * elem;
+    if (lds + tiles <= 65536) lds += tiles;
+    else a.whole = 0;
+  }
   hipStream_t s = as_stream(stream);
 #define PIA_KA(DT, NC, QV) \
   hipLaunchKernelGGL((kv_append_kernel<DT, NC, QV>), grid, dim3(KA_THREADS), lds, s, a)

@@ -79,7 +79,9 @@ def kv_append(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor, k_pages:
     (cu_new None: row b) are the last tokens of sequence b, whose context_lens[b] counts them. k,
     rotated at its place in the context by rope (None: as it is), and v go to their slots of
     block_tables[b] in pools [num_pages, Hkv, D, P] of their dtype. Returns q [tokens, Hq, D]
-    rotated likewise (None without q). Tokens of pages outside the pool are not written."""
+    rotated likewise (None without q). Tokens of pages outside the pool are not written; rows of no
+    sequence are read nowhere and hold nothing in the returned q. The pages that take new tokens
+    belong to one sequence each."""
     _check_pool(k_pages, v_pages)
     if k.dtype != k_pages.dtype:
         raise ValueError("k and v must have the pools' dtype")

@@ -181,6 +181,7 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
         q = q.contiguous()
         if q.data_ptr() % 16:   # a contiguous view that starts between vectors
             q = q.clone()
+    stride = q.stride(0) if rows > 1 else Hq * D   # of a single row it says nothing
     if block_tables.dtype != torch.int32 or block_tables.dim() != 2:
         raise ValueError("block_tables must be int32 [B, max_pages]")
     B = block_tables.shape[0]
@@ -209,7 +210,7 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
     bt, lens = block_tables.contiguous(), kv_lens.contiguous()
     cu = None if cu_q is None else cu_q.contiguous()
     offs = None if q_pos_offsets is None else q_pos_offsets.contiguous()
-    N.call_on(dev, "pia_kv8_attention", out.data_ptr(), q.data_ptr(), q.stride(0),
+    N.call_on(dev, "pia_kv8_attention", out.data_ptr(), q.data_ptr(), stride,
               pools.k.data_ptr(), pools.v.data_ptr(), pools.k_scale.data_ptr(),
               pools.v_scale.data_ptr(), bt.data_ptr(), bt.shape[1], lens.data_ptr(), N.ptr(cu),
               N.ptr(offs), B, rows, Hq, Hkv, D, P, num_pages, scale, code, workspace.data_ptr(),

@@ -279,6 +279,9 @@ def test_strides_scale_workspace_streams_and_graphs(dev):
     assert torch.equal(paged_decode_attention_kv8(odd, pools, t, lens_t, scale=0.05), want)
     flip = paged_decode_attention_kv8(-wide[:, :hq], pools, t, lens_t, scale=-0.05)
     assert torch.equal(flip, want)
+    row = torch.as_strided(wide, (1, hq, dim), (3, dim, 1))     # one row: its stride says nothing
+    assert torch.equal(paged_decode_attention_kv8(row, pools, t[:1], lens_t[:1], scale=0.05),
+                       paged_decode_attention_kv8(wide[:1, :hq], pools, t[:1], lens_t[:1], scale=0.05))
     wt = tables.repeat(1, 2).to(dev)[:, ::2]     # a strided table
     st = torch.stack([tables, tables], -1).flatten(1).to(dev)[:, ::2]
     assert wt.shape == st.shape
@@ -311,6 +314,89 @@ def test_strides_scale_workspace_streams_and_graphs(dev):
         b = paged_decode_attention_kv8(wide[:, :hq], pools, t, lens_t, scale=0.1)
         torch.cuda.synchronize()
         assert torch.equal(out, a) and torch.equal(two, b), i
+
+
+def test_more_sequences_than_a_launch_takes(dev):
+    """1100 sequences of 0 to 3 rows, their pages shared by every fourth of them."""
+    dim, hkv, hq, page, n = 64, 1, 4, 16, 1100
+    new, lens = [b % 4 for b in range(n)], [b % 4 + (5 * b) % 40 for b in range(n)]
+    tables = torch.tensor([[(3 * (b // 4) + i) % 50 for i in range(3)] for b in range(n)],
+                          dtype=torch.int32)
+    pool = O.Pool.random(50, hkv, dim, page, seed=8)
+    cu = [0] + torch.tensor(new).cumsum(0).tolist()
+    q = _rows(cu[-1], hq, dim, torch.bfloat16, 6)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    offs = [m - k for m, k in zip(lens, new)]
+    got = paged_attention_kv8(q.to(dev), pool.to_device(dev), tables.to(dev), i32(lens), cu_q=i32(cu),
+                              q_pos_offsets=i32(offs))
+    pick = list(range(0, n, 37)) + [1022, 1023, 1024, 1025, n - 1]
+    for b in pick:
+        r = slice(cu[b], cu[b + 1])
+        ref, mag, size = O.attend(q[r], pool, [tables[b].tolist()], [lens[b]], [0, new[b]], [offs[b]],
+                                  1 / math.sqrt(dim))
+        _check(got[r], ref, mag, size, torch.bfloat16, 43, dim)
+
+
+def test_pools_beyond_32_bits(dev):
+    """Pages whose bytes lie past 2^32: append, gather and all attention kernels as on a small pool."""
+    dim, hkv, hq, page = 128, 8, 32, 16
+    pages = 2 ** 32 // (dim * hkv * page) + 40
+    far, near = (KV8Pools.allocate(n, hkv, dim, page, dev) for n in (pages, 40))
+    tables = torch.arange(40, dtype=torch.int32, device=dev).view(2, 20)
+    rope = rope_params(dim, device=dev)
+    g = torch.Generator().manual_seed(3)
+    q, k, v = (torch.randn(500, h, dim, generator=g).to(torch.bfloat16).to(dev) for h in (hq, hkv, hkv))
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    cu, lens = i32([0, 220, 500]), i32([220, 280])
+    out = []
+    for pools, t in ((far, tables + (pages - 40)), (near, tables)):
+        r = kv8_append(q, k, v, pools, t, lens, cu, rope)
+        out.append([r, *kv8_gather(pools, t, cu.long(), 280),
+                    paged_attention_kv8(r, pools, t, lens, cu, i32([0, 0])),
+                    paged_attention_kv8(r[:6], pools, t, lens, i32([0, 2, 6]), i32([218, 276])),
+                    paged_decode_attention_kv8(r[:2], pools, t, lens)])
+    for a, b in zip(*out):
+        assert torch.equal(a, b) and a.abs().max() > 0
+
+
+@pytest.mark.parametrize("rows", [4, 200])
+def test_rows_captured_and_on_two_streams(dev, rows):
+    """A captured call replayed with other contexts and rows between eager ones, and two calls on
+    streams of their own at once, each with its workspace."""
+    dim, hkv, hq, page, B = 128, 4, 16, 16, 2
+    pool = O.Pool.random(2 * 30, hkv, dim, page, seed=6).to_device(dev)
+    t = torch.randperm(60, generator=torch.Generator().manual_seed(1)).int().view(B, 30).to(dev)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q = _rows(B * rows, hq, dim, torch.bfloat16, 3).to(dev)
+    lens, cu, offs = i32([470, 300]), i32([0, rows, 2 * rows]), i32([470 - rows, 300 - rows])
+    ws = [torch.empty(kv8_attention_workspace_bytes(dim), dtype=torch.uint8, device=dev)
+          for _ in range(2)]
+
+    def call(w=None, out=None):
+        return paged_attention_kv8(q, pool, t, lens, cu, offs, out=out, workspace=w)
+
+    out = call(ws[0])
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(ws[0], out)
+    for i in range(3):
+        q.mul_(-1.1)
+        lens.sub_(i32([3, 17]))
+        offs.sub_(i32([3, 17]))
+        cu[1] -= 1
+        out.zero_()
+        graph.replay()
+        want = call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want), i
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s, w in zip(streams, ws):
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            got.append([call(w) for _ in range(4)])
+    torch.cuda.synchronize()
+    assert all(torch.equal(x, want) for y in got for x in y)
 
 
 def test_append_then_attend(dev):

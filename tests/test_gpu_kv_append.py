@@ -52,11 +52,17 @@ CASES = [  # new rows, context, Hq, Hkv, D, rotated, P
     ([5, 64], [11, 32], 2, 2, 256, 256, 16),
     ([19], [3], 2, 1, 16, 16, 16),
 ]
+FLOAT_CASES = CASES + [  # head sizes of float pools alone
+    ([40, 17], [0, 30], 1, 2, 512, 512, 16),
+    ([33, 3], [5, 0], 2, 1, 200, 130, 32),
+    ([50, 1], [2, 9], 2, 2, 33, 6, 16),
+    ([1, 1], [2, 31], 1, 3, 65, 65 - 1, 16),
+]
 
 
 @pytest.mark.parametrize("dtype", list(STEP))
 @pytest.mark.parametrize("interleaved", [False, True])
-@pytest.mark.parametrize("case", CASES, ids=lambda c: f"{c[0]}+{c[1]}d{c[4]}r{c[5]}p{c[6]}")
+@pytest.mark.parametrize("case", FLOAT_CASES, ids=lambda c: f"{c[0]}+{c[1]}d{c[4]}r{c[5]}p{c[6]}")
 def test_float_pools(dev, case, interleaved, dtype):
     """The pools of rotary_embed followed by kv_scatter, and nothing else written."""
     new, ctx, hq, hkv, dim, rd, page = case
@@ -306,6 +312,23 @@ def test_strides_streams_and_graphs(dev):
         for a, b in ((pools.k, same.k), (pools.v, same.v)):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), i
         assert torch.equal(pools.k_scale, same.k_scale) and torch.equal(pools.v_scale, same.v_scale)
+
+
+def test_rows_behind_the_last_sequence(dev):
+    """A padded batch: rows of no sequence go nowhere, whichever pool."""
+    g = torch.Generator().manual_seed(4)
+    q, k, v = (torch.randn(40, h, 64, generator=g).to(torch.bfloat16).to(dev) for h in (4, 2, 2))
+    tables, lens, cu, pages = _batch([17, 3], [0, 14], 16, 3)
+    args = (tables.to(dev), lens.to(dev), cu.to(dev), rope_params(64, device=dev))
+    a, b = (KV8Pools.allocate(pages, 2, 64, 16, dev) for _ in range(2))
+    got, want = kv8_append(q, k, v, a, *args), kv8_append(q[:20], k[:20], v[:20], b, *args)
+    assert torch.equal(got[:20], want)
+    assert torch.equal(a.k.view(torch.uint8), b.k.view(torch.uint8))
+    assert torch.equal(a.v.view(torch.uint8), b.v.view(torch.uint8))
+    pools = [torch.zeros(pages, 2, 64, 16, dtype=torch.bfloat16, device=dev) for _ in range(4)]
+    got, want = kv_append(q, k, v, *pools[:2], *args), kv_append(q[:20], k[:20], v[:20], *pools[2:], *args)
+    assert torch.equal(got[:20], want)
+    assert torch.equal(pools[0], pools[2]) and torch.equal(pools[1], pools[3])
 
 
 def test_refusals(dev):
