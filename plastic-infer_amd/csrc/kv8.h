@@ -60,12 +60,13 @@ __device__ __forceinline__ float inverse(float scale) {
 // (arguments already checked by pia_kv8_attention).
 }  // namespace kv8
 bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
-                      int64_t table_tokens, const int32_t* cu_q, float scale);
+                      const int32_t* cu_q, float scale);
 int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
                        const uint8_t* vp, const float* ks, const float* vs, const int32_t* bt,
                        int64_t bt_stride, const int32_t* lens, const int32_t* cu,
                        const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
-                       int D, int P, int64_t num_pages, float scale_log2, hipStream_t s);
+                       int D, int P, int64_t num_pages, float scale_log2, float* parts,
+                       int64_t part_rows, hipStream_t s);
 namespace kv8 {
 
 // The last of n numbers base(0) <= base(1) <= ... that is at or before id (the first where none is): 64

@@ -772,12 +772,12 @@ extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, con
              reinterpret_cast<float*>(static_cast<char*>(workspace) + KA_PREF_BYTES),
              static_cast<int64_t*>(workspace), scale * 1.4426950408889634f, num_seqs, num_heads,
              num_kv_heads, G, head_dim, page_size};
-  if (kv8_prefill_path(dtype, num_heads, num_kv_heads, head_dim, num_seqs, total_q_rows,
-                       bt_stride * page_size, cu_q, scale))
+  if (kv8_prefill_path(dtype, num_heads, num_kv_heads, head_dim, num_seqs, total_q_rows, cu_q,
+                       scale))
     return launch_kv8_prefill(dtype, out, q, q_stride, a.kp, a.vp, a.ks, a.vs, block_tables,
                               bt_stride, kv_lens, cu_q, q_pos_offsets, num_seqs, total_q_rows,
                               num_heads, num_kv_heads, head_dim, page_size, num_pages,
-                              a.scale_log2, s);
+                              a.scale_log2, a.parts, resident_waves() * 2 * 16, s);
   const bool once = !cu_q && G <= 16;
   // more sequences than a launch's tables hold: by parts, one after the other on the stream
   for (int b0 = 0; b0 < num_seqs; b0 += KA_MAX_SEQS) {

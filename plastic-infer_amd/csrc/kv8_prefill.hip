@@ -4,10 +4,11 @@
 // Work item (one workgroup of NW waves): one kv head and 32 NW / G consecutive query positions of one
 // sequence, i.e. up to 32 NW (position, q head) rows that share the kv head's keys: row r is position
 // s0 + r / G, head h * G + r % G. Wave w owns rows 32 w .. 32 w + 31, one 32 x 32 product block. The
-// keys go by tiles of 64 tokens (four blocks). Codes come from the pool into registers a tile
-// ahead, and on their way into LDS, in the middle of the tile before theirs, they are widened to
-// DT with their scale: once for all rows, where an operand widened at its use would be widened by
-// every wave. bf16 holds a code times its scale exactly; fp16 does for scales of 2^-15 .. 2^6 and
+// keys go by tiles of 64 tokens (four blocks); where there are few items, each is cut along its keys
+// into pieces (workgroups of their own), whose outputs, maxima and sums a second kernel joins in order.
+// Codes come from the pool into registers a tile ahead, and on their way into LDS, at the end of the
+// tile before theirs, they are widened to DT with their scale: once for all rows, where an operand
+// widened at its use would be widened by every wave. bf16 holds a code times its scale exactly; fp16 does for scales of 2^-15 .. 2^6 and
 // within 2^-25 below (values beyond 65504 are infinite there).
 //
 // Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
@@ -44,6 +45,7 @@ constexpr int P8_KT = 64;            // keys per tile: four blocks
 constexpr int P8_MAX_SEQS = 1024;    // sequences per launch (tile prefix in LDS)
 constexpr int P8_AHEAD = 4;           // LDS operands read ahead of their product
 constexpr int P8_PV_VALU = 2;         // vector instructions after each product of the outputs
+constexpr int P8_MAX_CUTS = 64;      // pieces of an item
 constexpr int P8_RSRC_WORD3 = 0x00020000;
 constexpr float P8_RESCALE = 8.0f;   // log2: how far a row's maximum may run ahead of its reference
 
@@ -58,7 +60,8 @@ struct PrefillArgs {
   const int32_t *lens, *cu, *offs;
   int64_t rows, num_pages;
   float scale_log2;
-  int B, Hq, Hkv, G, P, ppt;
+  int B, Hq, Hkv, G, P, ppt, cuts;
+  float* parts;
 };
 
 template <int DT>
@@ -149,7 +152,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     __syncthreads();
   }
   int h, j;
-  if (!xcd_item(blockIdx.x, carry, a.Hkv, h, j)) return;
+  if (!xcd_item(blockIdx.x, carry * a.cuts, a.Hkv, h, j)) return;
+  const int piece = a.cuts == 1 ? 0 : uint32_t(j) % uint32_t(a.cuts);  // of the item's keys
+  if (a.cuts > 1) j = uint32_t(j) / uint32_t(a.cuts);
   int lo = 0, hi = a.B - 1;  // the sequence holding the item: the last with tile_pref[b] <= j
   while (lo < hi) {
     const int mid = (lo + hi + 1) >> 1;
@@ -166,7 +171,15 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
   const int s_last = min(s0 + a.ppt, n_b) - 1;
   const int kmax = a.offs ? max(0, min(kv_len, off + s_last + 1)) : kv_len;
-  const int nkt = (kmax + P8_KT - 1) / P8_KT;
+  // its tiles kt0 .. nkt - 1: all, or the piece's
+  int kt0 = 0, nkt = (kmax + P8_KT - 1) / P8_KT;
+  if (a.cuts > 1) {
+    const uint32_t n = nkt;  // times 64 pieces: 2^31 at most
+    kt0 = int(n * uint32_t(piece) / uint32_t(a.cuts));
+    nkt = int(n * uint32_t(piece + 1) / uint32_t(a.cuts));
+  }
+  kt0 = __builtin_amdgcn_readfirstlane(kt0);
+  nkt = __builtin_amdgcn_readfirstlane(nkt);
   const int nblk = (kv_len + 15) >> 4, PB = a.P / 16;
   const int32_t* btb = a.bt + int64_t(b) * a.bt_stride;
 
@@ -352,7 +365,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // the next tile's on return. A wave keeps its matrix core and its vector ALU busy at once: the
   // next tile's scores are multiplied while this one's become probabilities, and this one's
   // outputs while the tile after is staged.
-  auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int kt, int there) {
+  auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int kt, int buf, int there) {
     if (!(there == 0xf && (kt + 1) * P8_KT <= lim_min)) {
       const int rel = lim - (kt * P8_KT + 4 * hh);
 #pragma unroll
@@ -375,8 +388,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
         for (int v = 0; v < 16; ++v) acc[nb][v] *= alpha;
     }
     m = mref;
-    scores(sn, (kt + 1) & 1);
-    const int buf = kt & 1;
+    scores(sn, buf ^ 1);
     uint4 pk[4];  // block s of the tile: the B operand of its 16 tokens, the probabilities
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
@@ -415,18 +427,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
 
   // K is staged two tiles ahead of the outputs, for scores are a tile ahead, V one. With two buffers
   // each, what a tile stages replaces what the tile before it has read, with a barrier between.
-  auto stage_next = [&](int kt) {
+  auto stage_next = [&](int kt, int buf) {
     if constexpr (SPLIT) {
-      if (first4) stage_k(pa, kt & 1);
-      else stage_v(pa, (kt + 1) & 1, kt + 1, false);
+      if (first4) stage_k(pa, buf);
+      else stage_v(pa, buf ^ 1, kt + 1, false);
     } else {
-      stage_k(pa, kt & 1);
-      stage_v(pb, (kt + 1) & 1, kt + 1, false);
+      stage_k(pa, buf);
+      stage_v(pb, buf ^ 1, kt + 1, false);
     }
   };
-  Where w0 = where(0), w1 = where(1), w2 = where(2), w3 = where(3);  // of tiles kt .. kt + 3
+  Where w0 = where(kt0), w1 = where(kt0 + 1), w2 = where(kt0 + 2), w3 = where(kt0 + 3);  // kt .. kt + 3
   fetch_next(w0, w0);
-  stage(0, 0, false);
+  stage(0, kt0, false);
   if (!SPLIT || first4) {  // K of tile 1; the other waves have nothing of it
     fetch_part(pa, true, __builtin_amdgcn_readlane(w1.id, blk),
                __builtin_amdgcn_readlane(w1.sub, blk));
@@ -437,11 +449,11 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   f32x16_t sa[2], sb[2];
   scores(sa, 0);
   float mx = largest(sa);
-  auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int kt) {
+  auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int kt, int buf) {
     const int there = int(__ballot(lane < 4 && uint32_t(w0.id) < np)) & 0xf;
     const Where w4 = where(kt + 4);
-    turn(sc, sn, mx, kt, there);
-    stage_next(kt);
+    turn(sc, sn, mx, kt, buf, there);
+    stage_next(kt, buf);
     fetch_next(w3, w2);
     __syncthreads();
     w0 = w1;
@@ -449,15 +461,15 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     w2 = w3;
     w3 = w4;
   };
-  for (int kt = 0; kt < nkt; kt += 2) {
-    step(sa, sb, kt);
+  for (int kt = kt0; kt < nkt; kt += 2) {
+    step(sa, sb, kt, 0);
     if (kt + 1 >= nkt) break;
-    step(sb, sa, kt + 1);
+    step(sb, sa, kt + 1, 1);
   }
 
   if (nan_seen) {  // the same for every wave: all stores to it are barriers ago
 #pragma unroll 1
-    for (int kt = max(lim_min, 0) / P8_KT; kt < nkt; ++kt) {
+    for (int kt = max(kt0, lim_min / P8_KT); kt < nkt; ++kt) {
       __syncthreads();
       const Where w = where(kt);
       fetch_next(w, w);
@@ -492,6 +504,19 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
 
   l += swap_halves(l);
   if (!live) return;
+  if (a.cuts > 1) {  // the piece as it is, to be joined: its outputs, then its maximum and sum
+    const int64_t R = a.rows * a.Hq, at = piece * R + (row0 + pos) * a.Hq + h * G + r % G;
+    float* o = a.parts + at * D + 4 * hh;
+#pragma unroll
+    for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        *reinterpret_cast<float4*>(o + 32 * nb + 8 * i) =
+            make_float4(acc[nb][4 * i], acc[nb][4 * i + 1], acc[nb][4 * i + 2], acc[nb][4 * i + 3]);
+    if (hh == 0)
+      reinterpret_cast<float2*>(a.parts + a.cuts * R * D)[at] = make_float2(m * a.scale_log2, l);
+    return;
+  }
   const float inv = l == 0.f ? 0.f : 1.f / l;
   uint16_t* o = static_cast<uint16_t*>(a.out) + ((row0 + pos) * a.Hq + h * G + r % G) * D + 4 * hh;
 #pragma unroll
@@ -507,49 +532,100 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     }
 }
 
+// The pieces of every row joined, in order: a thread has four elements of one.
+template <int DT>
+__global__ __launch_bounds__(256) void kv8_prefill_join_kernel(PrefillArgs a, int D) {
+  const int64_t x = int64_t(blockIdx.x) * 256 + threadIdx.x, R = a.rows * a.Hq;
+  const int64_t at = uint32_t(x) / uint32_t(D / 4);  // below 2^31
+  const int d = 4 * int(x - at * (D / 4));
+  const int64_t row = uint32_t(at) / uint32_t(a.Hq);
+  if (at >= R || row < a.cu[0] || row >= a.cu[a.B]) return;
+  const float2* ml = reinterpret_cast<const float2*>(a.parts + a.cuts * R * D);
+  float M = -INFINITY, L = 0.f;
+  float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+  constexpr int N = 4;  // pieces on their way at once; past the end: the last again, without weight
+  for (int p0 = 0; p0 < a.cuts; p0 += N) {
+    float2 pm[N];
+    float4 po[N];
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      const int64_t i = min(p0 + k, a.cuts - 1) * R + at;
+      pm[k] = ml[i];
+      po[k] = *reinterpret_cast<const float4*>(a.parts + i * D + d);
+    }
+#pragma unroll
+    for (int k = 0; k < N; ++k) {
+      if (p0 + k >= a.cuts) break;
+      const float to = __builtin_elementwise_maximum(M, pm[k].x);
+      const float f0 = M == to ? 1.f : __builtin_amdgcn_exp2f(M - to);
+      const float f = pm[k].x == to ? 1.f : __builtin_amdgcn_exp2f(pm[k].x - to);
+      L = L * f0 + pm[k].y * f;
+      o = make_float4(fmaf(po[k].x, f, o.x * f0), fmaf(po[k].y, f, o.y * f0),
+                      fmaf(po[k].z, f, o.z * f0), fmaf(po[k].w, f, o.w * f0));
+      M = to;
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  const uint2 w = make_uint2(tile::pack16x2<DT>(L == 0.f ? 0.f : o.x * inv, L == 0.f ? 0.f : o.y * inv),
+                             tile::pack16x2<DT>(L == 0.f ? 0.f : o.z * inv, L == 0.f ? 0.f : o.w * inv));
+  *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * D + d) = w;
+}
+
 template <int D, int NW, int DT>
 void launch(const PrefillArgs& a, unsigned blocks, hipStream_t s) {
   hipLaunchKernelGGL((kv8_prefill_kernel<D, NW, DT>), dim3(blocks), dim3(64 * NW), 0, s, a);
+  if (a.cuts > 1)
+    hipLaunchKernelGGL((kv8_prefill_join_kernel<DT>),
+                       dim3(unsigned(ceil_div(a.rows * a.Hq * (D / 4), 256))), dim3(256), 0, s, a, D);
 }
 
 }  // namespace
 
-// Against the kernel that streams codes to each 16 rows (2.4 us for 1M rows x keys at head_dim 128, 1.3
-// at 64, whatever the number of items): an item here takes 22 ns a key (head_dim 64: 18) alone or in
-// turn with another on its CU, however few items there are. So the rows (of all heads) have to fill a
-// third of the CUs with items. One sequence of 32 heads, head_dim 128, 4096 keys: 65 us there and 91
-// here at 8192 rows, 112 and 94 at 16384. Where contexts are short the other kernel's second launch
-// counts: 512 keys 18 us and 20 at 1024 rows, 21 and 20 at 2048, 39 and 20 at 16384. And an item's rows
-// cost the same when most are missing: 256 items of 16 rows (4096 keys) 63 us and 94, of 32 rows 98 and
-// 93.
+// Against the kernel that streams codes to each 16 rows: that one takes 2.4 us for 1M rows x keys at
+// head_dim 128 (1.3 at 64), this one 0.6 (0.5) where its items are full and long, and their rows cost
+// the same when most are missing. In us there and here, 4096 keys, 8 kv heads of 128, rows of a kv head
+// and sequence: one sequence, 32 rows 20.0 and 19.5, 64 rows 25 and 20, 256 rows 30 and 25, 4096 rows
+// 175 and 87; 16 sequences, 32 rows 39 and 52, 64 rows 61 and 48, 4096 rows 1694 and 530. Only a few rows
+// on few heads lose a microsecond or two from 64 rows on (one sequence, 512 keys: 13.7 and 15.3); below
+// two rows to a compute unit there would not be pieces enough for all of them.
 bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t total_q_rows,
-                      int64_t table_tokens, const int32_t* cu_q, float scale) {
+                      const int32_t* cu_q, float scale) {
   const int G = Hq / Hkv;
   // scale > 0: the kernel keeps its running max in raw score units
   return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && (D == 64 || D == 96 || D == 128) &&
          scale > 0.f && G <= 128 && cu_q != nullptr && num_seqs <= P8_MAX_SEQS &&
-         total_q_rows * G >= 32 * int64_t(num_seqs) &&
-         total_q_rows * Hq >= (table_tokens <= 512 ? 8 : 48) * int64_t(device_cus());
+         total_q_rows * G >= 64 * int64_t(num_seqs) &&
+         total_q_rows * Hq >= 2 * int64_t(device_cus());
 }
 
 int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, const uint8_t* kp,
                        const uint8_t* vp, const float* ks, const float* vs, const int32_t* bt,
                        int64_t bt_stride, const int32_t* lens, const int32_t* cu,
                        const int32_t* offs, int num_seqs, int64_t total_q_rows, int Hq, int Hkv,
-                       int D, int P, int64_t num_pages, float scale_log2, hipStream_t s) {
+                       int D, int P, int64_t num_pages, float scale_log2, float* parts,
+                       int64_t part_rows, hipStream_t s) {
   const int G = Hq / Hkv;
   // Items of 256 rows halve what is widened for a row but come half as many: for long contexts that
   // fill the CUs all the same. 32 sequences, 32 heads, 64 rows each: 90 us and 86 at 2048 keys, 322 and
   // 279 at 8192; 128 rows: 95 and 101 at 1024 keys, 164 and 158 at 2048, 300 and 276 at 4096. At
   // head_dim 64, where a tile's products are half, they lose everywhere (390 and 430 at 4096 keys).
-  const bool wide =
-      D == 128 && bt_stride * P >= 2048 &&
-      (ceil_div(total_q_rows, 128 / G) + num_seqs / 2) * Hkv >= 2 * int64_t(device_cus());
+  const int64_t cus = device_cus(), tiles = ceil_div(bt_stride * P, P8_KT);
+  const int64_t items = std::max<int64_t>(1, (ceil_div(total_q_rows, 128 / G) + num_seqs / 2) * Hkv);
+  const bool wide = D == 128 && bt_stride * P >= 2048 && items >= 2 * cus;
   const int ppt = (wide ? 256 : 128) / G;
-  const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * Hkv, 8) * 8;
+  // Fewer items than CUs: their keys are cut into pieces, to two on every CU of 16 tiles each (if the
+  // table is full), or one of 4, as far as the workspace has rows for them. One sequence of 32 heads of
+  // 128 on 32768 keys: 128 rows 650 us whole and 88 cut, 512 rows 666 and 288. 64 pieces of 8 tiles a
+  // row take 52 us there where 32 of 16 take 43; pieces of 2 tiles cost more than they bring (4096 keys,
+  // 2048 rows of 64 heads: 34 us, and 25 with 8), and so does a cut of items that fill the CUs (512
+  // keys, 32768 rows: 30 and 21).
+  const int64_t most = std::max(std::min(2 * cus / items, tiles / 16), std::min(cus / items, tiles / 4));
+  const int cuts = int(std::max<int64_t>(
+      1, std::min(std::min<int64_t>(most, P8_MAX_CUTS), part_rows / (total_q_rows * Hq))));
+  const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * cuts * Hkv, 8) * 8;
   if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many query rows");
   PrefillArgs a{out, q, q_stride, kp, vp, ks, vs, bt, bt_stride, lens, cu, offs, total_q_rows,
-                num_pages, scale_log2, num_seqs, Hq, Hkv, G, P, ppt};
+                num_pages, scale_log2, num_seqs, Hq, Hkv, G, P, ppt, cuts, parts};
 #define PIA_P8(DT)                                                 \
   {                                                                \
     if (wide) launch<128, 8, DT>(a, unsigned(blocks), s);          \

@@ -119,7 +119,7 @@ def test_rows(dev, case, dtype):
     _check(got[:cu[-1]], ref, mag, size, dtype, max(lens), dim, rows=True)
 
 
-MANY = [  # as ROWS, and the tables' width in tokens; rows of all heads from 2048 on
+MANY = [  # as ROWS, and the tables' width in tokens; a kv head's rows 64 a sequence
     ([70, 1, 33], [70, 64, 200], "end", 32, 8, 128, 16, 0),
     ([20, 0, 9], [500, 3, 130], "end", 96, 8, 96, 32, 0),
     ([40, 30], [90, 20], [-3, 4], 40, 2, 64, 16, 0),
@@ -129,6 +129,13 @@ MANY = [  # as ROWS, and the tables' width in tokens; rows of all heads from 204
     ([9, 12, 1, 30, 0, 17, 8, 9, 10, 6, 5, 11, 7, 9, 9, 13, 8, 9, 12, 7],
      [9, 70, 33, 150, 8, 17, 128, 129, 40, 63, 64, 65, 80, 9, 100, 14, 20, 31, 12, 200], "end",
      128, 32, 128, 16, 2048),
+    ([10, 12, 1, 30, 0, 17, 28, 19, 20, 6, 15, 21, 17, 19, 29, 13, 28, 19, 12, 17],
+     [10, 70, 33, 150, 8, 17, 128, 129, 40, 63, 64, 65, 80, 19, 100, 14, 30, 31, 12, 200], "end",
+     128, 32, 128, 16, 2048),
+    ([70], [700], "end", 16, 2, 128, 16, 0),              # cut along the keys
+    ([33, 40], [900, 10], "end", 16, 2, 64, 32, 8192),
+    ([65, 2, 0], [300, 1000, 40], None, 16, 2, 96, 48, 1200),
+    ([40], [600], [-20], 32, 4, 128, 16, 1600),
 ]
 
 
@@ -187,7 +194,8 @@ def test_long_and_many(dev):
 
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(1, 4, 128, 0), (8, 96, 128, 0), (8, 96, 64, 0), (8, 96, 96, 0),
-                                   (256, 1024, 128, 2048)],
+                                   (176, 1056, 128, 2048),
+                                   (8, 96, 128, 2048), (8, 96, 64, 4096)],
                          ids=lambda s: f"h{s[1]}/{s[0]}d{s[2]}w{s[3]}")
 def test_what_a_row_may_not_see(dev, shape, dtype):
     """Stale codes behind a context (NaN among them), pages outside the pool, and NaN keys and values
