@@ -27,7 +27,7 @@
 //
 // Measured: 8 sequences of 1024 new rows on 4096 keys, causal, 32 heads of 128 over 8, bf16: 627 us,
 // 0.99 PFLOP/s of 619 GFLOP (a large library product of this card: 1.3). No one unit bounds it: the
-// matrix cores are busy 40 % of the time, and of the rest a wave's exponentials and packing cost 50 us,
+// matrix cores are busy 46 % of the time, and of the rest a wave's exponentials and packing cost 50 us,
 // the widening and its LDS stores 90, the loads 15, the operands' LDS reads 35 (each taken out alone).
 // Scores a tile ahead brought it there from 700; loads two tiles ahead with exact waits, the widening
 // between the two products and half-tile turns of the waves left it as it is.
