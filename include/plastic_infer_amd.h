@@ -562,7 +562,7 @@ int pia_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t q
  *     v_pages [num_pages, num_kv_heads, page_size / 4, head_dim, 4]
  *     scales f32 [num_pages, num_kv_heads, page_size / 16], one per block of 16 tokens and head.
  * A block's scale is the smallest power of two (at least 2^-100) that holds, in 448 steps of it,
- * the largest finite element of its new tokens (rotated k: times sqrt(2) * factor, a bound of what
+ * the largest finite element of its new tokens (rotated k: times sqrt(2) * |factor|, a bound of what
  * the rotation makes of it), or the scale it had if that is larger and the block holds earlier
  * tokens, whose codes are rounded to the scale when it grows. Codes round to nearest even; NaN,
  * infinities and what is beyond 464 times the largest scale, 2^119, become the NaN code.

@@ -753,7 +753,8 @@ extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, con
   if (!cu_q && total_q_rows != num_seqs)
     return fail(PIA_EINVAL, "kv8_attention: without cu_q one row per sequence");
   if (num_seqs == 0 || total_q_rows == 0) return 0;
-  if (num_pages * num_kv_heads > 0x7fffffff || total_q_rows * num_heads > 0x7fffffff)
+  if (num_pages > 0x7fffffff || num_pages * num_kv_heads > 0x7fffffff || total_q_rows > 0x3fffffff ||
+      total_q_rows * num_heads > 0x7ffffff0)
     return fail(PIA_EINVAL, "kv8_attention: pool or rows too large");
   if (!out || !q || !k_pages || !v_pages || !k_scales || !v_scales || !kv_lens ||
       (bt_stride && !block_tables) || !workspace)

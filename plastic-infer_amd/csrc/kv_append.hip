@@ -16,6 +16,7 @@
 // 32 + 8 heads, fp16, 8-bit pool: 47 us, 4.7 TB/s (a large copy of this card: 5.2). 256 single tokens
 // of 32 + 8 heads, 8-bit pool: 7.4 us.
 #include <algorithm>
+#include <cmath>
 
 #include "kv8.h"
 #include "rope.h"
@@ -592,7 +593,7 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
   if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
     return fail(PIA_EUNSUPPORTED, "kv_append: dtype must be bf16, fp16 or fp32");
   if (num_tokens < 0 || num_seqs < 0 || num_heads < 0 || num_kv_heads <= 0 || head_dim <= 0 ||
-      page_size <= 0 || num_pages < 0 || bt_stride < 0 || pairs < 0 ||
+      page_size <= 0 || num_pages < 0 || num_pages > 0x7fffffff || bt_stride < 0 || pairs < 0 ||
       2 * int64_t(pairs) > head_dim)
     return fail(PIA_EINVAL, "kv_append: invalid size");
   if (head_dim > 512) return fail(PIA_EUNSUPPORTED, "kv_append: head_dim over 512");
@@ -616,8 +617,8 @@ extern "C" int pia_kv_append(void* q_out, const void* q, int64_t q_token_stride,
               !aligned(v_scales, 4)))
     return fail(PIA_EINVAL, "kv_append: pools must be 16-byte aligned");
   const int64_t v16 = 16 / elem;
-  // c: a rotated element is at most sqrt(2) times the factor times the head's largest element
-  const float bound = pairs ? float(1.4142135623730951 * factor) : 1.f;
+  // c: a rotated element is at most sqrt(2) times the factor's size times the head's largest element
+  const float bound = pairs ? float(1.4142135623730951 * std::abs(factor)) : 1.f;
   AppendArgs a{q_out, q, k, v, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
                v_token_stride, v_head_stride, k_pages, v_pages, k_scales, v_scales, block_tables,
                bt_stride, context_lens, cu_new, num_tokens, turns, num_pages, num_seqs, pairs,
@@ -685,7 +686,8 @@ extern "C" int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, con
                               int dtype, void* stream) {
   if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
     return fail(PIA_EUNSUPPORTED, "kv8_gather: dtype must be bf16, fp16 or fp32");
-  if (num_seqs < 0 || total_tokens < 0 || num_kv_heads <= 0 || num_pages <= 0 || bt_stride < 0)
+  if (num_seqs < 0 || total_tokens < 0 || num_kv_heads <= 0 || num_pages <= 0 ||
+      num_pages > 0x7fffffff || bt_stride < 0)
     return fail(PIA_EINVAL, "kv8_gather: invalid size");
   if (!kv8::pool_shape(head_dim, page_size))
     return fail(PIA_EUNSUPPORTED,

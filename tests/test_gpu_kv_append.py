@@ -16,7 +16,7 @@ import kv8_oracle as O
 from plastic_infer.kernel.kv_append import kv_append
 from plastic_infer.kernel.paged_kv import kv_scatter
 from plastic_infer.kernel.paged_kv8 import KV8Pools, kv8_append, kv8_gather
-from plastic_infer.kernel.rotary import rope_params, rotary_embed
+from plastic_infer.kernel.rotary import RopeParams, rope_params, rotary_embed
 
 pytestmark = pytest.mark.gpu
 
@@ -312,6 +312,19 @@ def test_strides_streams_and_graphs(dev):
         for a, b in ((pools.k, same.k), (pools.v, same.v)):
             assert torch.equal(a.view(torch.uint8), b.view(torch.uint8)), i
         assert torch.equal(pools.k_scale, same.k_scale) and torch.equal(pools.v_scale, same.v_scale)
+
+
+def test_a_negative_factor_turns_the_negative(dev):
+    """k rotated times -1.5 is -k rotated times 1.5: the same codes and scales."""
+    g = torch.Generator().manual_seed(5)
+    k, v = (torch.randn(20, 2, 64, generator=g).to(torch.bfloat16).to(dev) for _ in "kv")
+    tables, lens, cu, pages = _batch([17, 3], [0, 14], 16, 3)
+    turns = rope_params(64, device=dev).turns
+    a, b = (KV8Pools.allocate(pages, 2, 64, 16, dev) for _ in range(2))
+    for pools, x, f in ((a, k, -1.5), (b, -k, 1.5)):
+        kv8_append(None, x, v, pools, tables.to(dev), lens.to(dev), cu.to(dev), RopeParams(turns, f))
+    assert (a.k.float().abs().amax() > 100) and torch.equal(a.k_scale, b.k_scale)
+    assert torch.equal(a.k.float(), b.k.float())     # zeros of either sign are equal
 
 
 def test_rows_behind_the_last_sequence(dev):

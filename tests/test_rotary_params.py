@@ -120,6 +120,7 @@ def test_kv8_entry_point_refusals():
     assert attend(dtype=7)[0] == -2 and attend(d=8)[0] == -2 and attend(p=8)[0] == -2
     assert attend(hq=3)[0] == -1 and attend(rows=3)[0] == -1 and attend(pages=0)[0] == -1
     assert attend(rows=0, seqs=0)[0] == 0
+    assert attend(pages=2 ** 31)[1].endswith("too large") and attend(rows=2 ** 30, seqs=2 ** 30)[0] == -1
     assert "null" in attend()[1]
     assert N.query("pia_kv8_attention_workspace_bytes", 0) == 0
     assert N.query("pia_kv8_attention_workspace_bytes", 300) == 0
