@@ -1,5 +1,5 @@
 // Attention of many query rows per sequence (prefill, chunked prefill) over the 8-bit KV pool on the
-// matrix cores: bf16 or fp16 q (DT), head_dim 64, 96 or 128, any page size of the pool.
+// matrix cores: bf16 or fp16 q (DT), head_dim to 128 (DP: 64, 96, 128), any page size of the pool.
 //
 // Work item (one workgroup of NW waves): one kv head and 32 NW / G consecutive query positions of one
 // sequence, i.e. up to 32 NW (position, q head) rows that share the kv head's keys: row r is position
@@ -8,8 +8,10 @@
 // into pieces (workgroups of their own), whose outputs, maxima and sums a second kernel joins in order.
 // Codes come from the pool into registers a tile ahead, and on their way into LDS, at the end of the
 // tile before theirs, they are widened to DT with their scale: once for all rows, where an operand
-// widened at its use would be widened by every wave. bf16 holds a code times its scale exactly; fp16 does for scales of 2^-15 .. 2^6 and
-// within 2^-25 below (values beyond 65504 are infinite there).
+// widened at its use would be widened by every wave. bf16 holds a code times its scale exactly; fp16
+// does for scales of 2^-15 .. 2^6 and within 2^-25 below (values beyond 65504 are infinite there). A
+// head_dim below DP is made up with zeros of K and q; V's rows behind it are whatever LDS holds and end
+// in outputs that nobody writes.
 //
 // Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
 // 8 (l / 32) + e; of C, lane l has column l % 32 and rows 8 i + 4 (l / 32) + j, i, j < 4)
@@ -17,16 +19,16 @@
 //   online softmax base 2, per row in fp32; a row's scores sit in two lanes (l, l ^ 32)
 //   O^T += V^T . P^T  the probabilities are the B operand straight from the score registers (rounded
 //                  to DT): of a block's tokens, lane half hh holds 4 hh + j and 8 + 4 hh + j. Rows of
-//                  the result are elements, so a lane has 4 D / 16 of them of its own row l % 32: what
+//                  the result are elements, so a lane has 4 DP / 16 of them of its own row l % 32: what
 //                  a row's maximum and sum do to it needs no exchange between lanes.
 // LDS tiles (16-byte units, XORed with a term of their row): K [token][d], 16 units to a token also at
-// head_dim 96: unit u (d 8 u .. + 7) of token t at u ^ t % 16 (head_dim 64: 8 units, u ^ t / 2 % 8); V [d][token]: unit 2 m + hh (block m, tokens
+// DP 96: unit u (d 8 u .. + 7) of token t at u ^ t % 16 (DP 64: 8 units, u ^ t / 2 % 8); V [d][token]: unit 2 m + hh (block m, tokens
 // 4 hh + j, then 8 + 4 hh + j) of element d at (2 m + hh) ^ (d / 4 % 8) ^ (d / 2 % 2). With the bank
 // rules of gfx950 (stores: 8 lanes over 32 banks; 16-byte reads: lanes {0-3, 12-15, 20-27} or the
-// others over 64) all of them are conflict-free but K stores at head_dim 64.
+// others over 64) all of them are conflict-free but K stores at DP 64.
 //
-// Measured: 8 sequences of 1024 new rows on 4096 keys, causal, 32 heads of 128 over 8, bf16: 627 us,
-// 0.99 PFLOP/s of 619 GFLOP (a large library product of this card: 1.3). No one unit bounds it: the
+// Measured: 8 sequences of 1024 new rows on 4096 keys, causal, 32 heads of 128 over 8, bf16: 625 to
+// 645 us on several machines, 0.96 to 0.99 PFLOP/s of 619 GFLOP (a large library product of this card: 1.3). No one unit bounds it: the
 // matrix cores are busy 46 % of the time, and of the rest a wave's exponentials and packing cost 50 us,
 // the widening and its LDS stores 90, the loads 15, the operands' LDS reads 35 (each taken out alone).
 // Scores a tile ahead brought it there from 700; loads two tiles ahead with exact waits, the widening
@@ -60,7 +62,7 @@ struct PrefillArgs {
   const int32_t *lens, *cu, *offs;
   int64_t rows, num_pages;
   float scale_log2;
-  int B, Hq, Hkv, G, P, ppt, cuts;
+  int B, Hq, Hkv, G, D, P, ppt, cuts;
   float* parts;
 };
 
@@ -113,12 +115,12 @@ __device__ __forceinline__ float swap_halves(float x) {  // the value of lane l 
   return __uint_as_float((threadIdx.x & 32) ? r[0] : r[1]);
 }
 
-template <int D, int NW, int DT>
+template <int DP, int NW, int DT>
 __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArgs a) {
-  constexpr int NT = 64 * NW, KS = D / 16, NB = D / 32;
-  constexpr int UK = D > 64 ? 16 : 8;  // 16-byte units of a K row in LDS
+  constexpr int NT = 64 * NW, KS = DP / 16, NB = DP / 32;
+  constexpr int UK = DP > 64 ? 16 : 8;  // 16-byte units of a K row in LDS
   constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
-  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = D * 128;  // bytes
+  constexpr uint32_t K_BUF = P8_KT * UK * 16, V_BUF = DP * 128;  // bytes
   __shared__ __align__(16) unsigned char lds[2 * (K_BUF + V_BUF)];
   __shared__ int tile_pref[P8_MAX_SEQS + 1];
   __shared__ int wsum[NW];
@@ -184,6 +186,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int32_t* btb = a.bt + int64_t(b) * a.bt_stride;
 
   // this lane's row and its q operands, d = 16 ks + 8 (l / 32) .. + 7
+  const int D = NW == 8 ? DP : a.D;  // 8 waves: as a constant, it takes 1 % less
   const int hh = lane >> 5, n32 = lane & 31, G = a.G;
   const int r = 32 * wave + n32, pos = s0 + r / G;
   const bool live = r < a.ppt * G && pos < n_b;
@@ -194,7 +197,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
                          int64_t(h * G + (live ? r % G : 0)) * D;
 #pragma unroll
     for (int k = 0; k < KS; ++k)
-      qr[k] = live ? *reinterpret_cast<const uint4*>(qp + 16 * k + 8 * hh)
+      qr[k] = live && 16 * k < D ? *reinterpret_cast<const uint4*>(qp + 16 * k + 8 * hh)
                    : make_uint4(0u, 0u, 0u, 0u);
   }
   // every row of the item sees at least the keys below lim_min (its first position's limit)
@@ -204,7 +207,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // l / 16 + 4), V by lanes (elements 4 (l % 32) .. + 3, token groups l / 32 and l / 32 + 2). What a
   // wave has of either: its loads' offset, and a base of its LDS addresses (the rest enters by XOR).
   const int blk = wave & 3;
-  constexpr int VL = D / 4;  // lanes of a token group of V
+  const int VL = D / 4;  // lanes of a token group of V
   const int64_t tile_bytes = int64_t(D) * a.P;
   struct Part {
     uint4 x[2];
@@ -212,7 +215,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     uint32_t off, base;
   };
   auto k_part = [&]() {
-    const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = D > 64 ? t & 15 : (t >> 1) & 7;
+    const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = DP > 64 ? t & 15 : (t >> 1) & 7;
     return Part{{}, 1.f, uint32_t((c * a.P + (lane & 15)) * 16),
                 uint32_t(t * UK * 16 + 16 * ((2 * c) ^ sw))};
   };
@@ -246,7 +249,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     const auto rs = __builtin_amdgcn_make_buffer_rsrc(
         const_cast<uint8_t*>((is_k ? a.kp : a.vp) + at), 0, ok ? bytes : 0, P8_RSRC_WORD3);
     p.x[0] = __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off, 0, 0));
-    if (D > 64 || !is_k)
+    if (DP > 64 || !is_k)
       p.x[1] =
           __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off + step, 0, 0));
     p.scale = (is_k ? a.ks : a.vs)[ok ? head * PB + sub : 0];
@@ -325,7 +328,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
   // bits enter by XOR, so one base per lane and a constant give any of them; bases of a buffer, so
   // that they are computed where they are used and not kept.
-  const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (D > 64 ? n32 & 15 : (n32 >> 1) & 7));
+  const uint32_t k_base = n32 * UK * 16 + 16 * (hh ^ (DP > 64 ? n32 & 15 : (n32 >> 1) & 7));
   const uint32_t v_base = n32 * 128 + 16 * (hh ^ (((n32 >> 2) & 7) ^ ((n32 >> 1) & 1)));
   auto kread = [&](int buf, int tb, int k) {
     const uint32_t at = ((k_base + buf * K_BUF) ^ (32 * k)) + 32 * tb * UK * 16;
@@ -511,8 +514,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
       for (int i = 0; i < 4; ++i)
-        *reinterpret_cast<float4*>(o + 32 * nb + 8 * i) =
-            make_float4(acc[nb][4 * i], acc[nb][4 * i + 1], acc[nb][4 * i + 2], acc[nb][4 * i + 3]);
+        if (32 * nb + 8 * i < D)
+          *reinterpret_cast<float4*>(o + 32 * nb + 8 * i) = make_float4(
+              acc[nb][4 * i], acc[nb][4 * i + 1], acc[nb][4 * i + 2], acc[nb][4 * i + 3]);
     if (hh == 0)
       reinterpret_cast<float2*>(a.parts + a.cuts * R * D)[at] = make_float2(m * a.scale_log2, l);
     return;
@@ -523,6 +527,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   for (int nb = 0; nb < NB; ++nb)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
+      if (32 * nb + 8 * i >= D) continue;
       uint32_t w[2];
 #pragma unroll
       for (int e = 0; e < 2; ++e)
@@ -534,7 +539,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
 
 // The pieces of every row joined, in order: a thread has four elements of one.
 template <int DT>
-__global__ __launch_bounds__(256) void kv8_prefill_join_kernel(PrefillArgs a, int D) {
+__global__ __launch_bounds__(256) void kv8_prefill_join_kernel(PrefillArgs a) {
+  const int D = a.D;
   const int64_t x = int64_t(blockIdx.x) * 256 + threadIdx.x, R = a.rows * a.Hq;
   const int64_t at = uint32_t(x) / uint32_t(D / 4);  // below 2^31
   const int d = 4 * int(x - at * (D / 4));
@@ -571,12 +577,12 @@ __global__ __launch_bounds__(256) void kv8_prefill_join_kernel(PrefillArgs a, in
   *reinterpret_cast<uint2*>(static_cast<uint16_t*>(a.out) + at * D + d) = w;
 }
 
-template <int D, int NW, int DT>
+template <int DP, int NW, int DT>
 void launch(const PrefillArgs& a, unsigned blocks, hipStream_t s) {
-  hipLaunchKernelGGL((kv8_prefill_kernel<D, NW, DT>), dim3(blocks), dim3(64 * NW), 0, s, a);
+  hipLaunchKernelGGL((kv8_prefill_kernel<DP, NW, DT>), dim3(blocks), dim3(64 * NW), 0, s, a);
   if (a.cuts > 1)
     hipLaunchKernelGGL((kv8_prefill_join_kernel<DT>),
-                       dim3(unsigned(ceil_div(a.rows * a.Hq * (D / 4), 256))), dim3(256), 0, s, a, D);
+                       dim3(unsigned(ceil_div(a.rows * a.Hq * (a.D / 4), 256))), dim3(256), 0, s, a);
 }
 
 }  // namespace
@@ -592,7 +598,7 @@ bool kv8_prefill_path(int dtype, int Hq, int Hkv, int D, int num_seqs, int64_t t
                       const int32_t* cu_q, float scale) {
   const int G = Hq / Hkv;
   // scale > 0: the kernel keeps its running max in raw score units
-  return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && (D == 64 || D == 96 || D == 128) &&
+  return (dtype == PIA_DTYPE_BF16 || dtype == PIA_DTYPE_F16) && D <= 128 &&
          scale > 0.f && G <= 128 && cu_q != nullptr && num_seqs <= P8_MAX_SEQS &&
          total_q_rows * G >= 64 * int64_t(num_seqs) &&
          total_q_rows * Hq >= 2 * int64_t(device_cus());
@@ -625,12 +631,12 @@ int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, co
   const int64_t blocks = ceil_div((ceil_div(total_q_rows, ppt) + num_seqs) * cuts * Hkv, 8) * 8;
   if (blocks > 0x7fffffff) return fail(PIA_EINVAL, "kv8_attention: too many query rows");
   PrefillArgs a{out, q, q_stride, kp, vp, ks, vs, bt, bt_stride, lens, cu, offs, total_q_rows,
-                num_pages, scale_log2, num_seqs, Hq, Hkv, G, P, ppt, cuts, parts};
+                num_pages, scale_log2, num_seqs, Hq, Hkv, G, D, P, ppt, cuts, parts};
 #define PIA_P8(DT)                                                 \
   {                                                                \
     if (wide) launch<128, 8, DT>(a, unsigned(blocks), s);          \
-    else if (D == 128) launch<128, 4, DT>(a, unsigned(blocks), s); \
-    else if (D == 96) launch<96, 4, DT>(a, unsigned(blocks), s);   \
+    else if (D > 96) launch<128, 4, DT>(a, unsigned(blocks), s);   \
+    else if (D > 64) launch<96, 4, DT>(a, unsigned(blocks), s);    \
     else launch<64, 4, DT>(a, unsigned(blocks), s);                \
   }
   if (dtype == PIA_DTYPE_F16) PIA_P8(PIA_DTYPE_F16) else PIA_P8(PIA_DTYPE_BF16)

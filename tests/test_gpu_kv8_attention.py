@@ -136,6 +136,10 @@ MANY = [  # as ROWS, and the tables' width in tokens; a kv head's rows 64 a sequ
     ([33, 40], [900, 10], "end", 16, 2, 64, 32, 8192),
     ([65, 2, 0], [300, 1000, 40], None, 16, 2, 96, 48, 1200),
     ([40], [600], [-20], 32, 4, 128, 16, 1600),
+    ([70, 30], [70, 90], "end", 8, 1, 80, 16, 0),         # padded heads
+    ([33, 40], [700, 50], "end", 16, 2, 112, 32, 0),
+    ([70], [300], None, 16, 2, 48, 16, 0),
+    ([18, 25], [18, 29], "end", 20, 2, 16, 48, 0),
 ]
 
 
@@ -195,7 +199,8 @@ def test_long_and_many(dev):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("shape", [(1, 4, 128, 0), (8, 96, 128, 0), (8, 96, 64, 0), (8, 96, 96, 0),
                                    (176, 1056, 128, 2048),
-                                   (8, 96, 128, 2048), (8, 96, 64, 4096)],
+                                   (8, 96, 128, 2048), (8, 96, 64, 4096),
+                                   (8, 96, 112, 0), (8, 96, 80, 2048), (8, 96, 48, 0)],
                          ids=lambda s: f"h{s[1]}/{s[0]}d{s[2]}w{s[3]}")
 def test_what_a_row_may_not_see(dev, shape, dtype):
     """Stale codes behind a context (NaN among them), pages outside the pool, and NaN keys and values
