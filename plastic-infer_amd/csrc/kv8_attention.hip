@@ -21,7 +21,10 @@
 // resident wave, whatever the batch looks like. The next step's K and V are on their way while a
 // step is computed, across items too. An item that lies in one range is finished there; pieces of
 // the others (at most two a wave) go to the workspace, and a second kernel joins them in order, so
-// results do not depend on timing.
+// results do not depend on timing. Items of three steps at most (by the table's width) are not cut: a
+// wave takes those that begin in its range, and there is no second kernel. In us, cut and whole: one
+// sequence of 64 keys 10.4 and 8.4 (the call from Python 13.5 and 10.5), of 192 10.6 and 11.4 (13.5 and
+// 11.3), of 256 10.6 and 13.1; 256 sequences of 192 24.3 and 22.4.
 //
 // Measured (both kernels): 256 sequences of 512 to 8192 keys, 32 heads of 128 over 8, bf16: 372-382 us,
 // 6.0-6.2 TB/s, the first kernel alone at the 6.4 that reads reach. Two of 100000 and 131072 keys,
@@ -43,6 +46,7 @@ constexpr int KA_MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
 constexpr int KA_WG_WAVES = 4;
 constexpr int KA_WGS_PER_CU = 2;   // two waves per SIMD
 constexpr int KA_RSRC_WORD3 = 0x00020000;
+constexpr int KA_WHOLE = 3;  // steps of a table whose items are not cut
 constexpr float KA_RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
 constexpr int KA_JOIN_MANY = 128, KA_JOIN_FEW = 512;  // threads of the joining workgroups
 
@@ -59,7 +63,7 @@ struct AttnArgs {
   float* parts;
   int64_t* pref;
   float scale_log2;
-  int B, Hq, Hkv, G, D, P;
+  int B, Hq, Hkv, G, D, P, whole;  // whole: no item is cut
 };
 
 // A sequence's part of a call: its rows, the keys that some row of it may see (kv_len) and their steps.
@@ -200,10 +204,38 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   if (blockIdx.x == 0)  // for the kernel that joins the pieces
     for (int b = threadIdx.x; b <= a.B; b += NTH) a.pref[b] = pref[b];
   const int64_t total = carry;
+  if (a.whole) {  // nothing will be joined: rows of sequences without keys are zeros
+    for (int b = blockIdx.x; b < a.B; b += gridDim.x) {
+      const int4 s = seq_of[b];
+      if (s.z > 0) continue;
+      uint4* o = reinterpret_cast<uint4*>(static_cast<T*>(a.out) + int64_t(s.x) * a.Hq * a.D);
+      const int64_t n = int64_t(s.y) * a.Hq * a.D * int(sizeof(T)) / 16;
+      for (int64_t i = threadIdx.x; i < n; i += NTH) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
+  }
   const int64_t nw = min(int64_t(gridDim.x) * KA_WG_WAVES, total);
   const int64_t w = int64_t(wave) * gridDim.x + blockIdx.x;  // few steps: over all compute units
   if (w >= nw) return;
-  const int64_t x0 = first_of(w, nw, total), x1 = first_of(w + 1, nw, total);
+  auto seq_at = [&](int64_t x) {  // the last sequence that starts at or before x (and is not empty)
+    int lo = 0, hi = a.B - 1;
+    while (lo < hi) {
+      const int mid = (lo + hi + 1) >> 1;
+      if (pref[mid] <= x) lo = mid; else hi = mid - 1;
+    }
+    return lo;
+  };
+  int64_t x0 = first_of(w, nw, total), x1 = first_of(w + 1, nw, total);
+  if (a.whole) {  // the items that begin in the range
+    auto item_from = [&](int64_t x) {
+      if (x >= total) return total;
+      const int b = seq_at(x), steps = (seq_of[b].z + STEP - 1) / STEP;
+      const int t = int(uint32_t(x - pref[b]) % uint32_t(steps));
+      return t ? x + steps - t : x;
+    };
+    x0 = item_from(x0);
+    x1 = item_from(x1);
+    if (x0 >= x1) return;
+  }
   const int count = uniform(int(min(x1 - x0, int64_t(0x7fffffff))));
 
   // where a wave is: step t of item i of kv head h of sequence b
@@ -229,12 +261,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
   };
   Cursor cur;
   {
-    int lo = 0, hi = a.B - 1;  // the last sequence that starts at or before x0 (and is not empty)
-    while (lo < hi) {
-      const int mid = (lo + hi + 1) >> 1;
-      if (pref[mid] <= x0) lo = mid; else hi = mid - 1;
-    }
-    cur.b = uniform(lo);
+    cur.b = uniform(seq_at(x0));
     enter(cur);
     const int64_t at = x0 - pref[cur.b], seg = quotient(at, cur.steps);
     cur.t = uniform(int(at - seg * cur.steps));
@@ -710,6 +737,7 @@ void launch(const AttnArgs& a, int64_t items, bool once, hipStream_t s) {
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, true>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
   else
     hipLaunchKernelGGL((kv8_attention_kernel<QT, DP, false>), dim3(wgs), dim3(64 * KA_WG_WAVES), 0, s, a);
+  if (a.whole) return;
   // few items: many pieces each, which many threads share, on every compute unit; many: two or three
   const bool few = items * 4 <= resident_waves();
   const int rows = a.cu ? 16 : std::min(a.G, 16);
@@ -772,7 +800,8 @@ extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, con
              kv_lens, cu_q, q_pos_offsets, total_q_rows, num_pages,
              reinterpret_cast<float*>(static_cast<char*>(workspace) + KA_PREF_BYTES),
              static_cast<int64_t*>(workspace), scale * 1.4426950408889634f, num_seqs, num_heads,
-             num_kv_heads, G, head_dim, page_size};
+             num_kv_heads, G, head_dim, page_size,
+             ceil_div(bt_stride * page_size, DP > 128 ? 32 : 64) <= KA_WHOLE};
   if (kv8_prefill_path(dtype, num_heads, num_kv_heads, head_dim, num_seqs, total_q_rows, cu_q,
                        scale))
     return launch_kv8_prefill(dtype, out, q, q_stride, a.kp, a.vp, a.ks, a.vs, block_tables,

@@ -93,6 +93,9 @@ ROWS = [  # new rows, lens, offsets (None: no causal limit), Hq, Hkv, D, P
     ([3, 2], [10, 30], None, 6, 2, 96, 16),
     ([5, 5], [90, 20], [-3, 4], 20, 1, 64, 16),
     ([6], [100], [2000], 4, 2, 256, 16),
+    ([3, 2, 0, 5, 1], [0, 192, 7, 0, 1], "end", 8, 2, 128, 16),
+    ([2, 9], [0, 90], [4, -5], 40, 2, 256, 32),
+    ([4, 4], [193, 0], "end", 8, 2, 128, 16),
     ([130, 65], [130, 400], "end", 16, 2, 128, 16),
 ]
 
