@@ -9,7 +9,7 @@
 // Codes come from the pool into registers a tile ahead, and on their way into LDS, at the end of the
 // tile before theirs, they are widened to DT with their scale: once for all rows, where an operand
 // widened at its use would be widened by every wave. bf16 holds a code times its scale exactly; fp16
-// does for scales of 2^-15 .. 2^6 and within 2^-25 below (values beyond 65504 are infinite there). A
+// does for scales of 2^-15 .. 2^7 and within 2^-25 below (values beyond 65504 count as that there). A
 // head_dim below DP is made up with zeros of K and q; V's rows behind it are whatever LDS holds and end
 // in outputs that nobody writes.
 //
@@ -39,6 +39,7 @@
 // Scores a tile ahead brought it there from 700; loads two tiles ahead with exact waits, the widening
 // between the two products and half-tile turns of the waves left it as it is.
 #include <algorithm>
+#include <type_traits>
 
 #include "attn_tiles.h"
 #include "kv8.h"
@@ -94,6 +95,20 @@ template <int DT>
 __device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b, float scale) {
   return make_uint4(widen<DT, false>(a, scale), widen<DT, true>(a, scale),
                     widen<DT, false>(b, scale), widen<DT, true>(b, scale));
+}
+
+// fp16 infinities as the largest values: what no fp16 holds of a code times its scale (fp16 tensors
+// round to 65536 at most, half a step from there). An infinity would be NaN in rows that do not see it.
+__device__ __forceinline__ uint32_t finite16(uint32_t w) {
+  return w - ((w & 0x7fffu) == 0x7c00u ? 1u : 0u) - ((w & 0x7fff0000u) == 0x7c000000u ? 0x10000u : 0u);
+}
+// a uint4 of DT values as it is, or finite
+template <bool FIX>
+__device__ __forceinline__ uint4 kept(const uint4& x) {
+  if constexpr (FIX)
+    return make_uint4(finite16(x.x), finite16(x.y), finite16(x.z), finite16(x.w));
+  else
+    return x;
 }
 
 // sum of a pair of DT values onto c
@@ -275,13 +290,21 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   auto put = [&](uint32_t at, const uint4& x) {
     *reinterpret_cast<uint4*>(lds + at) = x;
   };
+  // a block whose values may pass 65504 (448 times its scale): the same for the whole wave
+  auto large = [&](float scale) {
+    return DT == PIA_DTYPE_F16 && __builtin_amdgcn_readfirstlane(int(scale > 128.f));
+  };
   auto stage_k = [&](const Part& p, int buf) {
     const uint32_t base = p.base + buf * K_BUF;
+    auto all = [&](auto fix) {
 #pragma unroll
-    for (int i = 0; i < UK / 8; ++i) {
-      put(base ^ (128 * i), widen8<DT>(p.x[i].x, p.x[i].y, p.scale));
-      put(base ^ (128 * i + 16), widen8<DT>(p.x[i].z, p.x[i].w, p.scale));
-    }
+      for (int i = 0; i < UK / 8; ++i) {
+        put(base ^ (128 * i), kept<fix()>(widen8<DT>(p.x[i].x, p.x[i].y, p.scale)));
+        put(base ^ (128 * i + 16), kept<fix()>(widen8<DT>(p.x[i].z, p.x[i].w, p.scale)));
+      }
+    };
+    if (large(p.scale)) all(std::true_type{});
+    else all(std::false_type{});
   };
   auto stage_v = [&](Part& p, int buf, int kt, bool places) {
     // tokens past the context hold whatever the page held: zeros
@@ -313,12 +336,16 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       if (places) scale = 1.f;
       else if (any && (lane & 31) < VL) nan_seen = 1;
     }
-    if ((lane & 31) < VL) {
+    auto all = [&](auto fix) {
       const uint32_t base = p.base + buf * V_BUF;
-      put(base, widen8<DT>(p.x[0].x, p.x[1].x, scale));
-      put(base + 128, widen8<DT>(p.x[0].y, p.x[1].y, scale));
-      put((base ^ 16) + 256, widen8<DT>(p.x[0].z, p.x[1].z, scale));
-      put((base ^ 16) + 384, widen8<DT>(p.x[0].w, p.x[1].w, scale));
+      put(base, kept<fix()>(widen8<DT>(p.x[0].x, p.x[1].x, scale)));
+      put(base + 128, kept<fix()>(widen8<DT>(p.x[0].y, p.x[1].y, scale)));
+      put((base ^ 16) + 256, kept<fix()>(widen8<DT>(p.x[0].z, p.x[1].z, scale)));
+      put((base ^ 16) + 384, kept<fix()>(widen8<DT>(p.x[0].w, p.x[1].w, scale)));
+    };
+    if ((lane & 31) < VL) {
+      if (large(scale)) all(std::true_type{});
+      else all(std::false_type{});
     }
   };
   auto stage = [&](int buf, int kt, bool places) {

@@ -260,6 +260,48 @@ def test_what_a_row_may_not_see(dev, shape, dtype):
         q[7, 2, 5] = 0.0
 
 
+@pytest.mark.parametrize("dim,width", [(64, 0), (128, 0), (80, 2048)])
+def test_values_beyond_fp16(dev, dim, width):
+    """Many rows of fp16: values that fp16 does not hold (65504 itself becomes 65536 in the pool) count
+    as 65504 where they are seen and leave other rows alone; NaN stays NaN."""
+    hkv, hq, page, lens = 4, 48, 16, [90]
+    tables, pages = _tables(lens, page, 1, 9)
+    if width:
+        tables = torch.nn.functional.pad(tables, (0, width // page - tables.shape[1]), value=-1)
+    q = _rows(60, hq, dim, torch.float16, 2)
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    i, o = int(tables[0, 81 // page]), 81 % page
+
+    def pool(big):
+        p = O.Pool.random(pages, hkv, dim, page, seed=4)
+        p.codes["v"][i, 0] /= 8      # exact in e4m3, and within fp16 at the scale
+        p.codes["v"][i, 0] = O.e4m3(p.codes["v"][i, 0])
+        p.scale["v"][i, 0, 0] = 256.0
+        p.codes["v"][i, 0, o, 3], p.codes["v"][i, 0, o, dim - 2] = big, -big
+        return p
+
+    def run(p):
+        return paged_attention_kv8(q.to(dev), p.to_device(dev), tables.to(dev), i32(lens),
+                                   cu_q=i32([0, 60]), q_pos_offsets=i32([30])).cpu()
+
+    sees = torch.arange(60) + 30 >= 81
+    for big, held in ((256.0, 65504.0 / 256), (448.0, 65504.0 / 256)):
+        got = run(pool(big))
+        ref, mag, size = O.attend(q, pool(held), tables.tolist(), lens, [0, 60], [30],
+                                  1 / math.sqrt(dim))
+        assert torch.isfinite(got).all()
+        _check(got, ref, mag, size, torch.float16, 90, dim, rows=True)
+    bad = pool(256.0)
+    bad.codes["v"][i, 0, o, 5] = math.nan
+    hit = torch.isnan(run(bad))
+    assert hit[sees][:, :hq // hkv, 5].all() and hit.sum() == sees.sum() * (hq // hkv)
+    high = pool(256.0)
+    high.codes["k"][i, 0, o], high.scale["k"][i, 0, 0] = 256.0, 256.0
+    a, b = run(high), run(pool(256.0))
+    assert torch.equal(a[(torch.arange(60) + 30) < (81 // page) * page],
+                       b[(torch.arange(60) + 30) < (81 // page) * page])
+
+
 def test_scales_far_apart(dev):
     """Blocks whose scales differ by 2^40, in either pool, and probabilities near one and near zero."""
     dim, page = 64, 16
