@@ -462,7 +462,8 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
       uint32_t t[NP][4];
 #pragma unroll
       for (int b2 = 0; b2 < 2; ++b2) {
-        const float f = lane_value(sv, 2 * c + b2);
+        // a block that is not there has no scale: what load_scales has for it is any block's, NaN perhaps
+        const float f = (there >> (2 * c + b2)) & 1 ? lane_value(sv, 2 * c + b2) : 0.f;
 #pragma unroll
         for (int j2 = 0; j2 < 2; ++j2) {
           float u = p[2 * c + b2][2 * j2] * f, v = p[2 * c + b2][2 * j2 + 1] * f;

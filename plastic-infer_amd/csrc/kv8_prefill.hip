@@ -231,17 +231,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int64_t tile_bytes = int64_t(D) * a.P;
   struct Part {
     uint4 x[2];
-    float scale;
+    float scale;  // of a block that is not there: any block's, NaN perhaps
+    bool there;
     uint32_t off, base;
   };
   auto k_part = [&]() {
     const int t = 16 * blk + (lane & 15), c = lane >> 4, sw = DP > 64 ? t & 15 : (t >> 1) & 7;
-    return Part{{}, 1.f, uint32_t((c * a.P + (lane & 15)) * 16),
+    return Part{{}, 1.f, false, uint32_t((c * a.P + (lane & 15)) * 16),
                 uint32_t(t * UK * 16 + 16 * ((2 * c) ^ sw))};
   };
   auto v_part = [&]() {
     const int x = lane & 31;  // below VL; the others load and drop
-    return Part{{}, 1.f, uint32_t(hh * 4 * D + 16 * x),
+    return Part{{}, 1.f, false, uint32_t(hh * 4 * D + 16 * x),
                 2 * K_BUF + uint32_t(x * 4 * 128 + 16 * ((2 * blk + hh) ^ (x & 7)))};
   };
   const bool first4 = wave < 4;
@@ -273,6 +274,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       p.x[1] =
           __builtin_bit_cast(uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, p.off + step, 0, 0));
     p.scale = (is_k ? a.ks : a.vs)[ok ? head * PB + sub : 0];
+    p.there = ok;
   };
   // K of one tile and V of another (with eight waves a wave has one of them)
   auto fetch_next = [&](const Where& wk, const Where& wv) {
@@ -323,7 +325,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     // Zero times NaN is NaN, so a NaN of V would reach the rows that may not see its token. On tiles
     // that not every row sees whole it is staged as zero; the end of the item puts it where it
     // belongs, from tiles of the NaNs' places (places: a one for each).
-    float scale = p.scale;
+    float scale = p.there ? p.scale : 1.f;  // times zeros (K's scores are hidden, whatever they are)
     if (places || 64 * kt + 64 > lim_min) {
       uint32_t any = 0;
       uint32_t* w = &p.x[0].x;
