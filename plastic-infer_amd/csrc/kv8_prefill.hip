@@ -7,10 +7,10 @@
 // keys go by tiles of 64 tokens (four blocks); where there are few items, each is cut along its keys
 // into pieces (workgroups of their own), whose outputs, maxima and sums a second kernel joins in order.
 // Codes come from the pool into registers a tile ahead, and on their way into LDS, at the end of the
-// tile before theirs, they are widened to DT with their scale: once for all rows, where an operand
-// widened at its use would be widened by every wave. bf16 holds a code times its scale exactly; fp16
-// does for scales of 2^-15 .. 2^7 and within 2^-25 below (values beyond 65504 count as that there). A
-// head_dim below DP is made up with zeros of K and q; V's rows behind it are whatever LDS holds and end
+// tile before theirs, they are widened to DT: once for all rows, where an operand widened at its use
+// would be widened by every wave. bf16 holds a code times its scale exactly. fp16 does only for scales of
+// 2^-15 .. 2^7, so its K is codes, whose scale enters the scores in fp32 (1 to 2 % of the time); its V is
+// within 2^-25 below those scales, and beyond 65504 counts as that. A head_dim below DP is made up with zeros of K and q; V's rows behind it are whatever LDS holds and end
 // in outputs that nobody writes.
 //
 // Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
@@ -145,6 +145,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   __shared__ int tile_pref[P8_MAX_SEQS + 1];
   __shared__ int wsum[NW];
   __shared__ int nan_seen;
+  // fp16: the K scales of four tiles' blocks. A tile's are read while the one before it is computed, and
+  // those two tiles on are put down meanwhile.
+  constexpr bool HALF = DT == PIA_DTYPE_F16;
+  __shared__ __align__(16) float k_scale[HALF ? 4 : 1][4];
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
@@ -296,17 +300,15 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   auto large = [&](float scale) {
     return DT == PIA_DTYPE_F16 && __builtin_amdgcn_readfirstlane(int(scale > 128.f));
   };
-  auto stage_k = [&](const Part& p, int buf) {
+  auto stage_k = [&](const Part& p, int buf, int kt) {
     const uint32_t base = p.base + buf * K_BUF;
-    auto all = [&](auto fix) {
+    const float scale = HALF ? 1.f : p.scale;
 #pragma unroll
-      for (int i = 0; i < UK / 8; ++i) {
-        put(base ^ (128 * i), kept<fix()>(widen8<DT>(p.x[i].x, p.x[i].y, p.scale)));
-        put(base ^ (128 * i + 16), kept<fix()>(widen8<DT>(p.x[i].z, p.x[i].w, p.scale)));
-      }
-    };
-    if (large(p.scale)) all(std::true_type{});
-    else all(std::false_type{});
+    for (int i = 0; i < UK / 8; ++i) {
+      put(base ^ (128 * i), widen8<DT>(p.x[i].x, p.x[i].y, scale));
+      put(base ^ (128 * i + 16), widen8<DT>(p.x[i].z, p.x[i].w, scale));
+    }
+    if (HALF && lane == 0) k_scale[kt & 3][blk] = p.there ? p.scale : 1.f;
   };
   auto stage_v = [&](Part& p, int buf, int kt, bool places) {
     // tokens past the context hold whatever the page held: zeros
@@ -352,10 +354,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   };
   auto stage = [&](int buf, int kt, bool places) {
     if constexpr (SPLIT) {
-      if (first4) stage_k(pa, buf);
+      if (first4) stage_k(pa, buf, kt);
       else stage_v(pa, buf, kt, places);
     } else {
-      stage_k(pa, buf);
+      stage_k(pa, buf, kt);
       stage_v(pb, buf, kt, places);
     }
   };
@@ -373,7 +375,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     return *reinterpret_cast<const uint4*>(lds + 2 * K_BUF + at);
   };
 
-  float m = -INFINITY, l = 0.f;  // the row's reference point in raw score units; its lane's sum
+  // bf16: the row's reference point m is in units of the products q . K. fp16: K is codes, and m, like
+  // `unit`, what a block's products have to be multiplied by, in those of the exponent.
+  float m = -INFINITY, l = 0.f;  // l: the lane's sum
+  float4 unit = make_float4(0.f, 0.f, 0.f, 0.f);  // fp16: of the tile whose scores are there
+  auto unit_of = [&](int kt) {
+    if constexpr (HALF) {
+      // never 0: hidden scores are -inf
+      auto f = [&](float x) { return fmaxf(x * a.scale_log2, 1.17549435e-38f); };
+      const float4 x = *reinterpret_cast<const float4*>(k_scale[kt & 3]);
+      unit = make_float4(f(x.x), f(x.y), f(x.z), f(x.w));
+    }
+  };
   f32x16_t acc[NB];
 #pragma unroll
   for (int nb = 0; nb < NB; ++nb)
@@ -391,6 +404,17 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       sc[i & 1] = mfma32<DT>(kread(buf, i & 1, i >> 1), qr[i >> 1], sc[i & 1]);
   };
   auto largest = [&](const f32x16_t (&sc)[2]) {
+    if constexpr (HALF) {
+      float b[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int s = 0; s < 4; ++s)
+#pragma unroll
+        for (int v = 0; v < 8; ++v)
+          b[s] = __builtin_elementwise_maximum(b[s], sc[s >> 1][8 * (s & 1) + v]);
+      return __builtin_elementwise_maximum(
+          __builtin_elementwise_maximum(b[0] * unit.x, b[1] * unit.y),
+          __builtin_elementwise_maximum(b[2] * unit.z, b[3] * unit.w));
+    }
     float mx = -INFINITY;
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
@@ -398,6 +422,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       for (int v = 0; v < 16; ++v) mx = __builtin_elementwise_maximum(mx, sc[tb][v]);
     return mx;
   };
+  const float m_unit = HALF ? 1.f : a.scale_log2;
   // One tile. sc: its scores, mx: the largest of them (of the lane's) where none is hidden; sn, mx:
   // the next tile's on return. A wave keeps its matrix core and its vector ALU busy at once: the
   // next tile's scores are multiplied while this one's become probabilities, and this one's
@@ -414,10 +439,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       mx = largest(sc);
     }
     mx = __builtin_elementwise_maximum(mx, swap_halves(mx));
-    const float mref = (mx - m) * a.scale_log2 > P8_RESCALE || mx != mx ? mx : m;
-    const float nm = mref == -INFINITY ? 0.f : -mref * a.scale_log2;
+    const float mref = (mx - m) * m_unit > P8_RESCALE || mx != mx ? mx : m;
+    const float nm = mref == -INFINITY ? 0.f : -mref * m_unit;
     if (__ballot(m != mref)) {
-      const float alpha = m == mref ? 1.f : __builtin_amdgcn_exp2f((m - mref) * a.scale_log2);
+      const float alpha = m == mref ? 1.f : __builtin_amdgcn_exp2f((m - mref) * m_unit);
       l *= alpha;
 #pragma unroll
       for (int nb = 0; nb < NB; ++nb)
@@ -429,12 +454,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     uint4 pk[4];  // block s of the tile: the B operand of its 16 tokens, the probabilities
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
+      const float u = !HALF ? a.scale_log2 : s == 0 ? unit.x : s == 1 ? unit.y : s == 2 ? unit.z : unit.w;
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         const int v = 8 * (s & 1) + 2 * i;
-        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], a.scale_log2, nm));
-        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], a.scale_log2, nm));
+        const float p0 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v], u, nm));
+        const float p1 = __builtin_amdgcn_exp2f(fmaf(sc[s >> 1][v + 1], u, nm));
         w[i] = tile::pack16x2<DT>(p0, p1);
         l = add_pair<DT>(w[i], l);
       }
@@ -443,6 +469,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
 #pragma unroll
     for (int i = 0; i < 4 * NB; ++i)
       acc[i % NB] = mfma32<DT>(vread(buf, i % NB, i / NB), pk[i / NB], acc[i % NB]);
+    unit_of(kt + 1);
     mx = largest(sn);
     // kept so through the scheduler: operands read P8_AHEAD products ahead of their use, the vector
     // work of the probabilities among the scores' products, the next maximum's among the outputs'
@@ -466,10 +493,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // each, what a tile stages replaces what the tile before it has read, with a barrier between.
   auto stage_next = [&](int kt, int buf) {
     if constexpr (SPLIT) {
-      if (first4) stage_k(pa, buf);
+      if (first4) stage_k(pa, buf, kt + 2);
       else stage_v(pa, buf ^ 1, kt + 1, false);
     } else {
-      stage_k(pa, buf);
+      stage_k(pa, buf, kt + 2);
       stage_v(pb, buf ^ 1, kt + 1, false);
     }
   };
@@ -479,12 +506,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   if (!SPLIT || first4) {  // K of tile 1; the other waves have nothing of it
     fetch_part(pa, true, __builtin_amdgcn_readlane(w1.id, blk),
                __builtin_amdgcn_readlane(w1.sub, blk));
-    stage_k(pa, 1);
+    stage_k(pa, 1, kt0 + 1);
   }
   fetch_next(w2, w1);
   __syncthreads();
   f32x16_t sa[2], sb[2];
   scores(sa, 0);
+  unit_of(kt0);
   float mx = largest(sa);
   auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int kt, int buf) {
     const int there = int(__ballot(lane < 4 && uint32_t(w0.id) < np)) & 0xf;
@@ -552,7 +580,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
           *reinterpret_cast<float4*>(o + 32 * nb + 8 * i) = make_float4(
               acc[nb][4 * i], acc[nb][4 * i + 1], acc[nb][4 * i + 2], acc[nb][4 * i + 3]);
     if (hh == 0)
-      reinterpret_cast<float2*>(a.parts + a.cuts * R * D)[at] = make_float2(m * a.scale_log2, l);
+      reinterpret_cast<float2*>(a.parts + a.cuts * R * D)[at] = make_float2(m * m_unit, l);
     return;
   }
   const float inv = l == 0.f ? 0.f : 1.f / l;
