@@ -23,7 +23,11 @@
 //                  maximum and sum do to it needs no exchange between lanes.
 // The probabilities are rounded to DT once, and the sum is of the rounded ones: half a step of DT each,
 // as much as the result's own rounding (bf16, the case below: 0.0020 of the norm from exact results,
-// 0.0017 for exactly computed ones rounded). A second term would be half as many products again.
+// 0.0017 for exactly computed ones rounded). A second term would be half as many products again (fp16
+// with two bf16 terms: 895 us where this takes 750). fp16 has no more than 29 binades of normal numbers for
+// them: a row's reference follows its maximum tile by tile, up and down, so that a tile's largest has
+// them all below it, and what the rest loses is bounded at the end of an item, which is done again where
+// that is too much (8 % of the time for the references; an item that is done again takes 3.3 times as long).
 // LDS tiles (16-byte units, XORed with a term of their row): K [token][d], 16 units to a token also at
 // DP 96: unit u (d 8 u .. + 7) of token t at u ^ t % 16 (DP 64: 8 units, u ^ t / 2 % 8); V [d][token]:
 // unit 2 m + hh (block m, tokens 4 hh + j, then 8 + 4 hh + j) of element d at
@@ -56,6 +60,14 @@ constexpr int P8_PV_VALU = 2;         // vector instructions after each product 
 constexpr int P8_MAX_CUTS = 64;      // pieces of an item
 constexpr int P8_RSRC_WORD3 = 0x00020000;
 constexpr float P8_RESCALE = 8.0f;   // log2: how far a row's maximum may run ahead of its reference
+// fp16, where a tile's largest probability has to be near the top of the type's range: how far a row's
+// maximum in the tile may be from its reference, on either side, the exponent of the reference's
+// probability, and how far below the largest maximum so far a reference may be (fp32 outputs hold
+// 2^(13 + 60) times 2^31 keys of 2^16)
+constexpr float P8_NEAR_HALF = 2.0f, P8_UP_HALF = 13.0f, P8_FLOOR_HALF = 60.0f;
+constexpr float P8_LEAST_HALF = 6.103515625e-5f;  // 2^-14: the least normal number
+constexpr float P8_REST = 16777216.f;             // 2^24, one over the least number
+constexpr float P8_V_HALF = 0.0625f;              // the largest V scale that the rounding below takes
 
 struct PrefillArgs {
   void* out;
@@ -149,12 +161,14 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   // those two tiles on are put down meanwhile.
   constexpr bool HALF = DT == PIA_DTYPE_F16;
   __shared__ __align__(16) float k_scale[HALF ? 4 : 1][4];
+  __shared__ uint32_t v_most[4];  // fp16: the largest V scale of each block of the tiles so far
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 
   // work items per sequence and their prefix
   if (threadIdx.x == 0) tile_pref[0] = 0;
   if (threadIdx.x == 0) nan_seen = 0;
+  if (threadIdx.x < 4) v_most[threadIdx.x] = 0;
   int carry = 0;
   for (int c0 = 0; c0 < a.B; c0 += NT) {
     const int i = c0 + threadIdx.x;
@@ -328,6 +342,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     // that not every row sees whole it is staged as zero; the end of the item puts it where it
     // belongs, from tiles of the NaNs' places (places: a one for each).
     float scale = p.there ? p.scale : 1.f;  // times zeros (K's scores are hidden, whatever they are)
+    if (HALF && lane == 0 && p.there)
+      __hip_atomic_fetch_max(&v_most[blk], __float_as_uint(scale), __ATOMIC_RELAXED,
+                             __HIP_MEMORY_SCOPE_WORKGROUP);
     if (places || 64 * kt + 64 > lim_min) {
       uint32_t any = 0;
       uint32_t* w = &p.x[0].x;
@@ -423,24 +440,41 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     return mx;
   };
   const float m_unit = HALF ? 1.f : a.scale_log2;
+  auto minus = [&](float x) {  // what a score takes to its probability's exponent
+    return x == -INFINITY ? 0.f : HALF ? P8_UP_HALF - x : -x * m_unit;
+  };
+  float top = -INFINITY;  // fp16: the largest of the row's maxima
+  auto reference = [&](float mx) {
+    if constexpr (!HALF) return (mx - m) * m_unit > P8_RESCALE || mx != mx ? mx : m;
+    top = __builtin_elementwise_maximum(top, mx);
+    const float d = mx - m;
+    return fabsf(d) <= P8_NEAR_HALF || mx == -INFINITY
+               ? m : __builtin_elementwise_maximum(mx, top - P8_FLOOR_HALF);
+  };
+  auto unit_at = [&](int s) {
+    return !HALF ? a.scale_log2 : s == 0 ? unit.x : s == 1 ? unit.y : s == 2 ? unit.z : unit.w;
+  };
+  auto hide = [&](f32x16_t (&sc)[2], int kt, int there) {  // what the row may not see
+    const int rel = lim - (kt * P8_KT + 4 * hh);
+#pragma unroll
+    for (int tb = 0; tb < 2; ++tb)
+#pragma unroll
+      for (int v = 0; v < 16; ++v)
+        if (!(32 * tb + 8 * (v >> 2) + (v & 3) < rel && ((there >> (2 * tb + (v >> 3))) & 1)))
+          sc[tb][v] = -INFINITY;
+  };
   // One tile. sc: its scores, mx: the largest of them (of the lane's) where none is hidden; sn, mx:
   // the next tile's on return. A wave keeps its matrix core and its vector ALU busy at once: the
   // next tile's scores are multiplied while this one's become probabilities, and this one's
   // outputs while the tile after is staged.
   auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int kt, int buf, int there) {
     if (!(there == 0xf && (kt + 1) * P8_KT <= lim_min)) {
-      const int rel = lim - (kt * P8_KT + 4 * hh);
-#pragma unroll
-      for (int tb = 0; tb < 2; ++tb)
-#pragma unroll
-        for (int v = 0; v < 16; ++v)
-          if (!(32 * tb + 8 * (v >> 2) + (v & 3) < rel && ((there >> (2 * tb + (v >> 3))) & 1)))
-            sc[tb][v] = -INFINITY;
+      hide(sc, kt, there);
       mx = largest(sc);
     }
     mx = __builtin_elementwise_maximum(mx, swap_halves(mx));
-    const float mref = (mx - m) * m_unit > P8_RESCALE || mx != mx ? mx : m;
-    const float nm = mref == -INFINITY ? 0.f : -mref * m_unit;
+    const float mref = reference(mx);
+    const float nm = minus(mref);
     if (__ballot(m != mref)) {
       const float alpha = m == mref ? 1.f : __builtin_amdgcn_exp2f((m - mref) * m_unit);
       l *= alpha;
@@ -454,7 +488,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     uint4 pk[4];  // block s of the tile: the B operand of its 16 tokens, the probabilities
 #pragma unroll
     for (int s = 0; s < 4; ++s) {
-      const float u = !HALF ? a.scale_log2 : s == 0 ? unit.x : s == 1 ? unit.y : s == 2 ? unit.z : unit.w;
+      const float u = unit_at(s);
       uint32_t w[4];
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
@@ -530,6 +564,62 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     step(sa, sb, kt, 0);
     if (kt + 1 >= nkt) break;
     step(sb, sa, kt + 1, 1);
+  }
+
+  // fp16: rounding takes up to 2^-25 from each probability below the normal numbers, where the largest of
+  // its tile is 2^11 at least. The lost ones of 64 keys are 2^-30 of that largest one then, and those of all
+  // keys 2^-30 of the row's sum: times values of up to 28 (448 times the limit), less than half of the least
+  // fp16 number. For larger values the item is done again with its row's own maximum, each probability below
+  // the normal numbers as two: what fp16 holds of it, and 2^24 times the rest.
+  if constexpr (HALF) {
+    const float most = __uint_as_float(max(max(v_most[0], v_most[1]), max(v_most[2], v_most[3])));
+    if (!(most <= P8_V_HALF)) {  // the same for all waves
+      m = top;
+      const float nm = minus(m);
+      l = 0.f;
+#pragma unroll
+      for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+        for (int v = 0; v < 16; ++v) acc[nb][v] = 0.f;
+#pragma unroll 1
+      for (int i = 2 * kt0; i < 2 * nkt; ++i) {  // the rests of all tiles first
+        const bool rest = i < kt0 + nkt;
+        const int kt = rest ? i - kt0 : i - nkt;
+        __syncthreads();
+        const Where w = where(kt);
+        fetch_next(w, w);
+        stage(0, kt, false);
+        __syncthreads();
+        if (i == kt0 + nkt)
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+#pragma unroll
+            for (int v = 0; v < 16; ++v) acc[nb][v] *= 1.f / P8_REST;
+        scores(sa, 0);
+        unit_of(kt);
+        hide(sa, kt, int(__ballot(lane < 4 && uint32_t(w.id) < np)) & 0xf);
+#pragma unroll
+        for (int s = 0; s < 4; ++s) {
+          uint32_t x[4];
+#pragma unroll
+          for (int k = 0; k < 4; ++k) {
+            float r[2];
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const float p = __builtin_amdgcn_exp2f(
+                  fmaf(sa[s >> 1][8 * (s & 1) + 2 * k + e], unit_at(s), nm));
+              const float less = p < P8_LEAST_HALF ? (p - half_to_f32(f32_to_half(p))) * P8_REST : 0.f;
+              r[e] = rest ? less : p;
+              l += rest ? p : 0.f;
+            }
+            x[k] = tile::pack16x2<DT>(r[0], r[1]);
+          }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb)
+            acc[nb] = mfma32<DT>(vread(0, nb, s), make_uint4(x[0], x[1], x[2], x[3]), acc[nb]);
+        }
+      }
+    }
   }
 
   if (nan_seen) {  // the same for every wave: all stores to it are barriers ago
