@@ -85,6 +85,11 @@ __device__ __forceinline__ int last_at(int n, int64_t id, Base base) {
   return lo;
 }
 
+// Keys that row `pos` of a sequence sees of the first `keys`, with its first row at position off (any int)
+__device__ __forceinline__ int seen(int keys, int off, int pos) {
+  return int(max(int64_t(0), min(int64_t(keys), int64_t(off) + pos + 1)));
+}
+
 inline bool pool_shape(int D, int P) {
   return D > 0 && D % 16 == 0 && D <= 256 && P > 0 && P % BLOCK == 0 && P <= 4096;
 }

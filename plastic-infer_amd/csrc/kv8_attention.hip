@@ -77,8 +77,8 @@ __device__ __forceinline__ Seq sequence(const AttnArgs& a, int b, int tokens) {
   const int64_t n = a.cu ? int64_t(a.cu[b + 1]) - s.row0 : 1;
   s.n = s.row0 < 0 ? 0 : int(max(int64_t(0), min(n, a.rows - s.row0)));
   s.kv_len = int(min(int64_t(max(a.lens[b], 0)), min(a.bt_stride * a.P, int64_t(0x7ffffff0))));
-  s.off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
-  if (a.offs) s.kv_len = int(max(int64_t(0), min(int64_t(s.kv_len), int64_t(s.off) + s.n)));
+  s.off = a.offs ? a.offs[b] : 0;
+  if (a.offs) s.kv_len = kv8::seen(s.kv_len, s.off, s.n - 1);
   s.items = int((int64_t(s.n) * a.G + 15) >> 4);
   s.steps = (s.kv_len + tokens - 1) / tokens;
   return s;
@@ -380,8 +380,8 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
                               "+v"(qr[i][e][n].w));
       lim = lim_min = cur.kv_len;
       if (!ONCE && a.offs) {
-        lim = min(lim, off + pos + 1);
-        lim_min = min(lim_min, off + (16 * cur.i) / a.G + 1);
+        lim = kv8::seen(lim, off, pos);
+        lim_min = kv8::seen(lim_min, off, (16 * cur.i) / a.G);
       }
       m = -INFINITY;
       l = 0.f;

@@ -208,9 +208,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int n_b = int(min(int64_t(a.cu[b + 1]), a.rows) - row0);
   const int kv_len =
       int(min(int64_t(max(a.lens[b], 0)), min(a.bt_stride * a.P, int64_t(0x7ffffff0))));
-  const int off = a.offs ? max(min(a.offs[b], 0x3fffffff), -0x3fffffff) : 0;
+  const int off = a.offs ? a.offs[b] : 0;
   const int s_last = min(s0 + a.ppt, n_b) - 1;
-  const int kmax = a.offs ? max(0, min(kv_len, off + s_last + 1)) : kv_len;
+  const int kmax = a.offs ? kv8::seen(kv_len, off, s_last) : kv_len;
   // its tiles kt0 .. nkt - 1: all, or the piece's
   int kt0 = 0, nkt = (kmax + P8_KT - 1) / P8_KT;
   if (a.cuts > 1) {
@@ -228,7 +228,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   const int hh = lane >> 5, n32 = lane & 31, G = a.G;
   const int r = 32 * wave + n32, pos = s0 + r / G;
   const bool live = r < a.ppt * G && pos < n_b;
-  const int lim = !live ? 0 : a.offs ? min(kv_len, off + pos + 1) : kv_len;
+  const int lim = !live ? 0 : a.offs ? kv8::seen(kv_len, off, pos) : kv_len;
   uint4 qr[KS];
   {
     const uint16_t* qp = static_cast<const uint16_t*>(a.q) + (row0 + (live ? pos : 0)) * a.q_stride +
@@ -239,7 +239,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
                    : make_uint4(0u, 0u, 0u, 0u);
   }
   // every row of the item sees at least the keys below lim_min (its first position's limit)
-  const int lim_min = a.offs ? max(0, min(kv_len, off + s0 + 1)) : kv_len;
+  const int lim_min = a.offs ? kv8::seen(kv_len, off, s0) : kv_len;
 
   // staging: wave w (of four) moves block w of a tile, K by lanes (token l % 16, chunks l / 16 and
   // l / 16 + 4), V by lanes (elements 4 (l % 32) .. + 3, token groups l / 32 and l / 32 + 2). What a
