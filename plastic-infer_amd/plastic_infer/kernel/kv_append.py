@@ -10,7 +10,7 @@ import torch
 
 from .. import _native as N
 from .paged_kv import _check_pool
-from .rotary import RopeParams, check_rope, fresh_like, heads_view
+from .rotary import RopeParams, check_rope, derived, fresh_like, heads_view
 
 
 def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
@@ -24,9 +24,9 @@ def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
                            *(() if q is None else (q,)), *(() if cu_new is None else (cu_new,)),
                            names=("k", "v", "k_pages", "v_pages", "block_tables", "context_lens",
                                   "cu_new" if q is None else "q", "cu_new"))
-    if torch.is_grad_enabled() and (k.requires_grad or v.requires_grad
-                                    or (q is not None and q.requires_grad)):
-        raise ValueError("an append has no gradient: call it under torch.no_grad()")
+    if derived(q, k, v):
+        raise ValueError("an append has no gradient: call it under torch.no_grad(), on tensors "
+                         "without a tangent")
     k, v = heads_view("k", k), heads_view("v", v)
     n = k.shape[0]
     if k.shape != (n, Hkv, D) or v.shape != (n, Hkv, D):

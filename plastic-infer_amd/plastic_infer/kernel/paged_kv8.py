@@ -16,7 +16,7 @@ import torch
 
 from .. import _native as N
 from .kv_append import append_call
-from .rotary import RopeParams, fresh_like
+from .rotary import RopeParams, derived, fresh_like
 
 BLOCK = 16   # tokens that share a scale
 
@@ -172,9 +172,9 @@ def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out,
         raise ValueError(f"q must be [rows, Hq, {D}] with Hq a multiple of {Hkv}, got "
                          f"{tuple(q.shape)}")
     code = N.dtype_code(q.dtype)
-    if torch.is_grad_enabled() and q.requires_grad:
+    if derived(q):
         raise ValueError("attention over the 8-bit cache has no gradient: call it under "
-                         "torch.no_grad()")
+                         "torch.no_grad(), on a q without a tangent")
     rows, Hq, _ = q.shape
     token, head, elem = q.stride()
     if elem != 1 or head != D or token * q.element_size() % 16 or q.data_ptr() % 16:

@@ -12,6 +12,7 @@ import math
 from dataclasses import dataclass
 
 import torch
+from torch.autograd import forward_ad
 
 from .. import _native as N
 
@@ -94,6 +95,15 @@ def check_rope(rope: RopeParams, head_dim: int, dev: torch.device) -> None:
         raise ValueError(f"rope rotates {2 * t.numel()} elements of a head of {head_dim}")
 
 
+def derived(*tensors: torch.Tensor | None) -> bool:
+    """Whether a derivative in either mode is to be taken of any of them (tangents are looked up only
+    inside a dual level)."""
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        return True
+    return getattr(forward_ad, "_current_level", -1) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def fresh_like(t: torch.Tensor) -> torch.Tensor:
     """A contiguous tensor of t's shape and type (empty_like takes half the time of empty)."""
     if t.is_contiguous():
@@ -134,15 +144,37 @@ def _launch(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Ten
     return qo, ko
 
 
+def _rotate(q: torch.Tensor | None, k: torch.Tensor | None, positions: torch.Tensor,
+            rope: RopeParams, transposed: bool) -> tuple[torch.Tensor | None, torch.Tensor | None]:
+    # a node of the graph is made only for what somebody differentiates
+    if derived(q, k):
+        return _Rotary.apply(q, k, positions, rope, transposed)
+    return _launch(q, k, positions, rope, transposed)
+
+
 class _Rotary(torch.autograd.Function):
-    """The map is linear in q and k: its gradient is the transposed map, and so on."""
+    """The map is linear in q and k: its derivative along a tangent is itself, its gradient the
+    transposed map, and so on."""
 
     @staticmethod
     def forward(ctx, q, k, positions, rope, transposed):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(positions, rope.turns)
+        ctx.save_for_forward(positions, rope.turns)
         ctx.form = (rope.factor, rope.interleaved, transposed)
-        return _launch(q, k, positions, rope, transposed)
+        out = _launch(q, k, positions, rope, transposed)
+        ctx.shapes = [None if o is None else o.shape for o in out]
+        return out
+
+    @staticmethod
+    def jvp(ctx, tq, tk, *_):
+        positions, turns = ctx.saved_tensors
+        factor, interleaved, transposed = ctx.form
+        t = tq if tq is not None else tk
+        # of the two one may come without a tangent, and its result needs one
+        tq, tk = (x if x is not None or s is None else t.new_zeros(s)
+                  for x, s in zip((tq, tk), ctx.shapes))
+        return _rotate(tq, tk, positions, RopeParams(turns, factor, interleaved), transposed)
 
     @staticmethod
     def backward(ctx, gq, gk):
@@ -151,16 +183,14 @@ class _Rotary(torch.autograd.Function):
         positions, turns = ctx.saved_tensors
         factor, interleaved, transposed = ctx.form
         rope = RopeParams(turns, factor, interleaved)
-        # a graph of the gradient is wanted only by who differentiates it again
-        run = _Rotary.apply if torch.is_grad_enabled() else _launch
-        return *run(gq, gk, positions, rope, not transposed), None, None, None
+        return *_rotate(gq, gk, positions, rope, not transposed), None, None, None
 
 
 def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tensor,
                  rope: RopeParams) -> tuple[torch.Tensor, torch.Tensor | None]:
     """(q, k) rotated at their rows' positions. q [tokens, Hq, D], k [tokens, Hkv, D] or None, of one
     dtype (bf16, fp16 or fp32), tokens and heads at any strides; positions int64 or int32
-    [tokens]. Contiguous results; gradients flow to q and k in reverse mode. (A backward pass is
+    [tokens]. Contiguous results; derivatives of q and k in both modes. (A backward pass is
     captured into a graph only while no eager graph of the same leaves lives: torch's accumulation
     nodes keep the stream that made them, which is then part of the capture.)"""
     if k is None:
@@ -180,9 +210,7 @@ def rotary_embed(q: torch.Tensor, k: torch.Tensor | None, positions: torch.Tenso
         raise ValueError(f"positions must be int64 or int32 [{n}]")
     check_rope(rope, D, dev)
     positions = positions.contiguous()
-    if torch.is_grad_enabled() and (q.requires_grad or (k is not None and k.requires_grad)):
-        return _Rotary.apply(q, k, positions, rope, False)
-    return _launch(q, k, positions, rope, False)
+    return _rotate(q, k, positions, rope, False)
 
 
 __all__ = ["RopeParams", "rope_params", "rotary_embed"]
