@@ -64,11 +64,20 @@ def _check_shape(head_dim: int, page_size: int) -> None:
 
 
 def _check_pools(p: KV8Pools) -> tuple[int, int, int, int]:
-    """(num_pages, Hkv, D, P) of valid pools, checked once for each KV8Pools."""
-    shape = p.__dict__.get("_shape")
-    if shape is None:
-        shape = p.__dict__["_shape"] = _checked_shape(p)
-    return shape
+    """(num_pages, Hkv, D, P) of valid pools. Looked at on every call (2 us): tensors can be resized."""
+    k, v, ks, vs = p.k, p.v, p.k_scale, p.v_scale
+    index = k.get_device()
+    if k.dim() == 5 and index >= 0 and v.get_device() == index and ks.get_device() == index \
+            and vs.get_device() == index:   # the usual case: nothing to report
+        n, h, c, page, e = k.shape
+        if n and h and e == 16 and 0 < c <= 16 and 0 < page <= 4096 and page % BLOCK == 0 \
+                and v.shape == (n, h, page // 4, 16 * c, 4) \
+                and ks.shape == vs.shape == (n, h, page // BLOCK) \
+                and k.dtype == v.dtype == torch.float8_e4m3fn \
+                and ks.dtype == vs.dtype == torch.float32 and k.is_contiguous() \
+                and v.is_contiguous() and ks.is_contiguous() and vs.is_contiguous():
+            return n, h, 16 * c, page
+    return _checked_shape(p)
 
 
 def _checked_shape(p: KV8Pools) -> tuple[int, int, int, int]:
@@ -162,12 +171,13 @@ def kv8_attention_workspace_bytes(head_dim: int, device: torch.device | None = N
 
 def _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out, workspace):
     num_pages, Hkv, D, P = _check_pools(pools)
-    dev = N.require_device(pools.k, q, block_tables, kv_lens,
-                           names=("pools.k", "q", "block_tables", "kv_lens"))
+    tensors, names = [pools.k, q, block_tables, kv_lens], ["pools.k", "q", "block_tables", "kv_lens"]
     for name, t in (("cu_q", cu_q), ("q_pos_offsets", q_pos_offsets), ("out", out),
                     ("workspace", workspace)):
         if t is not None:
-            N.require_device(pools.k, t, names=("pools.k", name))
+            tensors.append(t)
+            names.append(name)
+    dev = N.require_device(*tensors, names=tuple(names))
     if q.dim() != 3 or q.shape[2] != D or q.shape[1] == 0 or q.shape[1] % Hkv:
         raise ValueError(f"q must be [rows, Hq, {D}] with Hq a multiple of {Hkv}, got "
                          f"{tuple(q.shape)}")
