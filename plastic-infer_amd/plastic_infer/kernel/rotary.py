@@ -178,6 +178,7 @@ class _Rotary(torch.autograd.Function):
 
     @staticmethod
     def backward(ctx, gq, gk):
+        gq, gk = (g if need else None for g, need in zip((gq, gk), ctx.needs_input_grad))
         if gq is None and gk is None:
             return None, None, None, None, None
         positions, turns = ctx.saved_tensors
