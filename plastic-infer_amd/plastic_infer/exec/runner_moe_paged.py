@@ -47,7 +47,7 @@ from ..kernel.paged_kv import decode_workspace_bytes, paged_decode_append_attent
 from ..kernel.paged_kv8 import (KV8Pools, kv8_append, kv8_attention_workspace_bytes,
                                 paged_decode_attention_kv8)
 from ..kernel.pinned import alloc_pinned_exact
-from ..kernel.rotary import rope_params
+from ..kernel.rotary import rope_params, rotary_embed
 from ..moe.fused import fused_experts_decode_impl, fused_topk, routed_ffn_routes
 from ..moe.offload_cache import OffloadMoeCache
 from .attention import build_rope_cache
@@ -166,7 +166,13 @@ class MoePagedDecoder:
     """Batched decode of a random-init or loaded MoE model over one KV pool shared by all
     layers (each layer's pages are distinct page ids, as KVStore lays them out) and an
     OffloadMoeCache holding the routed experts. The pool is k_pages and v_pages, or (with those
-    None) kv8_pools, which keeps the context in 8 bits."""
+    None) kv8_pools, which keeps the context in 8 bits. There the append rotates, at each row's
+    place in its context: context_lens - 1, which DecodeBatch.positions is to hold, is not read
+    from it.
+
+    layer_hook, if set, is called as hook(layer, dict) with the layer's tensors: q rotated; k as the
+    layer hands it on (rotated for float pools, normed and not yet rotated for 8-bit ones) and
+    k_rotated, the same over either pool; v, attn, moe_in, topk_weights, topk_ids, routed."""
 
     def __init__(self, weights: dict[str, torch.Tensor], cfg: MoeModelConfig,
                  moe_cache: OffloadMoeCache, k_pages: torch.Tensor | None,
@@ -176,7 +182,7 @@ class MoePagedDecoder:
         self.k_pages, self.v_pages = k_pages, v_pages
         self.kv8_pools = kv8_pools
         self.overlap = overlap
-        self.layer_hook = None   # called as hook(layer, dict of the layer's tensors)
+        self.layer_hook = None
         if kv8_pools is not None:
             if k_pages is not None or v_pages is not None:
                 raise ValueError("kv8_pools take the place of k_pages and v_pages")
@@ -307,9 +313,13 @@ class MoePagedDecoder:
         topk_w, topk_ids = fused_topk(h, logits, cfg.n_experts_per_tok, True)
         routed, info = self._routed(l, h, topk_w, topk_ids)
         if self.layer_hook is not None:
-            self.layer_hook(l, {"q": q, "k": k, "v": v, "attn": attn, "moe_in": h,
-                                "topk_weights": topk_w, "topk_ids": topk_ids, "routed": routed,
-                                **info})
+            turned = k
+            if self.kv8_pools is not None:
+                with torch.no_grad():
+                    turned, _ = rotary_embed(k, None, batch.context_lens - 1, self._rope)
+            self.layer_hook(l, {"q": q, "k": k, "k_rotated": turned, "v": v, "attn": attn,
+                                "moe_in": h, "topk_weights": topk_w, "topk_ids": topk_ids,
+                                "routed": routed, **info})
         return x, routed
 
 
