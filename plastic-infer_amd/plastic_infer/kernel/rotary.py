@@ -85,6 +85,17 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
     return RopeParams((freq / (2 * math.pi)).to(device), factor, bool(interleaved))
 
 
+def derived(*tensors: torch.Tensor | None) -> bool:
+    """Whether a derivative in either mode is to be taken of any of them (tangents are looked up only
+    inside a dual level)."""
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return getattr(forward_ad, "_current_level", -1) >= 0 and any(
+        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+
+
 def check_rope(rope: RopeParams, head_dim: int, dev: torch.device) -> None:
     t = rope.turns
     if not t.is_cuda or t.get_device() != dev.index:
@@ -93,15 +104,8 @@ def check_rope(rope: RopeParams, head_dim: int, dev: torch.device) -> None:
         raise ValueError("rope.turns must be a contiguous float64 [pairs] tensor")
     if 2 * t.numel() > head_dim:
         raise ValueError(f"rope rotates {2 * t.numel()} elements of a head of {head_dim}")
-
-
-def derived(*tensors: torch.Tensor | None) -> bool:
-    """Whether a derivative in either mode is to be taken of any of them (tangents are looked up only
-    inside a dual level)."""
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        return True
-    return getattr(forward_ad, "_current_level", -1) >= 0 and any(
-        t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors)
+    if derived(t):
+        raise ValueError("rope.turns has no gradient: detach it")
 
 
 def fresh_like(t: torch.Tensor) -> torch.Tensor:
