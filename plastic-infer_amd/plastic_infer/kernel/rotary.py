@@ -48,8 +48,8 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
     rd = head_dim if rotary_dim is None else int(rotary_dim)
     if head_dim <= 0 or rd < 0 or rd > head_dim or rd % 2:
         raise ValueError(f"rotary_dim must be even and within head_dim {head_dim}, got {rd}")
-    if not base > 0:
-        raise ValueError("base must be positive")
+    if not 0 < base < math.inf:
+        raise ValueError("base must be positive and finite")
     i = torch.arange(0, rd, 2, dtype=torch.float64)
     factor = 1.0
     kind = None if scaling is None else scaling.get("type")
@@ -58,9 +58,11 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
                  "yarn": {"type", "factor", "original_length", "beta_fast", "beta_slow"}}
         if kind not in known or set(scaling) - known[kind]:
             raise ValueError(f"unknown rotary scaling {scaling!r}")
+        if "factor" not in scaling or (kind == "yarn" and "original_length" not in scaling):
+            raise ValueError(f"incomplete rotary scaling {scaling!r}")
         by = float(scaling["factor"])
-        if not by >= 1.0:
-            raise ValueError("the scaling factor must be at least 1")
+        if not 1.0 <= by < math.inf:
+            raise ValueError("the scaling factor must be at least 1 and finite")
     if kind == "ntk" and rd > 2:
         base = base * by ** (rd / (rd - 2))
     freq = base ** (-i / rd) if rd else i
@@ -71,11 +73,15 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
         if n <= 0 or base == 1.0:
             raise ValueError("yarn needs a positive original_length and a base other than 1")
 
+        fast, slow = (float(scaling.get(x, d)) for x, d in (("beta_fast", 32), ("beta_slow", 1)))
+        if not 0 < slow <= fast < math.inf:
+            raise ValueError("yarn's beta_slow must be positive and at most beta_fast")
+
         def pair_of(turns):   # the pair that turns so often within n positions
             return rd * math.log(n / (turns * 2 * math.pi)) / (2 * math.log(base))
 
-        low = max(math.floor(pair_of(scaling.get("beta_fast", 32))), 0)
-        high = min(math.ceil(pair_of(scaling.get("beta_slow", 1))), rd - 1)
+        low = max(math.floor(pair_of(fast)), 0)
+        high = min(math.ceil(pair_of(slow)), rd - 1)
         ramp = ((torch.arange(rd // 2, dtype=torch.float64) - low) / max(high - low, 1e-3))
         ramp = ramp.clamp(0.0, 1.0)
         freq = freq / by * ramp + freq * (1.0 - ramp)
