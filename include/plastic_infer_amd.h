@@ -589,10 +589,10 @@ int pia_kv8_gather(void* k_out, void* v_out, const void* k_pages, const void* v_
  * cu_q[b] .. cu_q[b + 1] (NULL: row b). Row s of b attends keys j < kv_lens[b] and, with
  * q_pos_offsets, j <= q_pos_offsets[b] + s; q head h reads kv head h / (num_heads / num_kv_heads).
  * A row without a key is zeros; a page id outside the pool holds no keys; rows behind the last
- * sequence's are left. q rows are q_stride
- * elements apart (whole 16-byte vectors), out is contiguous. workspace: 16-byte aligned, of
- * pia_kv8_attention_workspace_bytes(head_dim) bytes, any content; calls that share one are ordered on one
- * stream. */
+ * sequence's are left. q rows are q_stride elements apart (whole 16-byte vectors), out is contiguous
+ * and may be q itself (dense rows), which it must not overlap otherwise. workspace: 16-byte aligned, of
+ * pia_kv8_attention_workspace_bytes(head_dim) bytes, any content; calls that share one are ordered on
+ * one stream. */
 int64_t pia_kv8_attention_workspace_bytes(int head_dim);
 int pia_kv8_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
                       const void* v_pages, const float* k_scales, const float* v_scales,

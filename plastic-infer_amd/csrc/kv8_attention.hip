@@ -750,6 +750,16 @@ void launch(const AttnArgs& a, int64_t items, bool once, hipStream_t s) {
                      rows_per_wg);
 }
 
+// Whether `out` (bytes) holds any byte of n rows of `row` bytes, `stride` bytes apart from q on
+bool holds_rows(uintptr_t out, int64_t bytes, uintptr_t q, int64_t n, int64_t row, int64_t stride) {
+  if (stride <= 0) n = 1;
+  // the first row that ends behind out's beginning
+  const int64_t to = int64_t(out) - int64_t(q) - row;
+  const int64_t r = to < 0 || n == 1 ? 0 : to / stride + 1;
+  const int64_t from = int64_t(q) + r * stride;
+  return r < n && from < int64_t(out) + bytes && from + row > int64_t(out);
+}
+
 }  // namespace
 }  // namespace pia
 
@@ -792,6 +802,11 @@ extern "C" int pia_kv8_attention(void* out, const void* q, int64_t q_stride, con
   if (!aligned(q, 16) || !aligned(out, 16) || (q_stride * elem) % 16 || !aligned(k_pages, 16) ||
       !aligned(v_pages, 16) || !aligned(workspace, 16))
     return fail(PIA_EINVAL, "kv8_attention: q rows, out, pools and workspace must be 16-byte aligned");
+  // every row is read before it is written, by whoever writes it, but not before others are
+  const int64_t row = int64_t(num_heads) * head_dim * elem;
+  if (!(out == q && q_stride * elem == row) &&
+      holds_rows(uintptr_t(out), total_q_rows * row, uintptr_t(q), total_q_rows, row, q_stride * elem))
+    return fail(PIA_EINVAL, "kv8_attention: out overlaps q");
   if (workspace_bytes < pia_kv8_attention_workspace_bytes(head_dim))
     return fail(PIA_EINVAL, "kv8_attention: workspace too small");
   const int G = num_heads / num_kv_heads, DP = padded(head_dim);

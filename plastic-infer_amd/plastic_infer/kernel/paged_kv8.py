@@ -247,7 +247,8 @@ def paged_attention_kv8(q: torch.Tensor, pools: KV8Pools, block_tables: torch.Te
     """paged_attention over 8-bit pools. q: [rows, Hq, D], rows of sequence b = cu_q[b]..cu_q[b+1]
     (cu_q None: one row per sequence). Row s of b attends keys j < kv_lens[b] and, when
     q_pos_offsets is given, j <= q_pos_offsets[b] + s; a row without a key is zeros. Rows behind
-    the last sequence are left as they were in `out`."""
+    the last sequence are left as they were in `out`, which may be q itself and must not overlap it
+    otherwise."""
     return _attention(q, pools, block_tables, kv_lens, cu_q, q_pos_offsets, scale, out, workspace)
 
 
