@@ -44,6 +44,23 @@ __device__ __forceinline__ void decode4(uint32_t w, float (&x)[4]) {
   x[2] = hi[0];
   x[3] = hi[1];
 }
+// two codes (the low or high half of a word) times scale as two 16-bit values of type T
+template <int T, bool HI>
+__device__ __forceinline__ uint32_t widen(uint32_t w, float scale) {
+  if constexpr (T == PIA_DTYPE_F16)
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
+  else
+    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
+}
+template <int T>
+__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b, float scale = 1.f) {
+  return make_uint4(widen<T, false>(a, scale), widen<T, true>(a, scale),
+                    widen<T, false>(b, scale), widen<T, true>(b, scale));
+}
+// the bytes of a word of codes that hold the NaN code, as 1 each
+__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
+  return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
+}
 // a word's codes times ratio (a power of two, at most 1), rounded to codes again
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
   float x[4];

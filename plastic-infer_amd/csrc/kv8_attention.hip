@@ -109,19 +109,6 @@ template <> struct Q<PIA_DTYPE_BF16> { static constexpr int NQ = 1, NP = 2, KT =
 template <> struct Q<PIA_DTYPE_F16> { static constexpr int NQ = 1, NP = 2, KT = PIA_DTYPE_F16; };
 template <> struct Q<PIA_DTYPE_F32> { static constexpr int NQ = 3, NP = 3, KT = PIA_DTYPE_BF16; };
 
-// two codes (the low or high half of a word) as two 16-bit values
-template <int T, bool HI>
-__device__ __forceinline__ uint32_t widen(uint32_t w) {
-  if constexpr (T == PIA_DTYPE_F16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, 1.f, HI));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, 1.f, HI));
-}
-template <int T>
-__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b) {
-  return make_uint4(widen<T, false>(a), widen<T, true>(a), widen<T, false>(b), widen<T, true>(b));
-}
-
 // eight consecutive q elements (which are there to be read) as NQ operands, zeros where not ok
 template <int QT>
 __device__ __forceinline__ void load_q(const typename Elem<QT>::T* p, bool ok,
@@ -157,11 +144,6 @@ __device__ __forceinline__ int uniform(int x) { return __builtin_amdgcn_readfirs
 __device__ __forceinline__ float lane_value(float x, int lane) {
   return __uint_as_float(__builtin_amdgcn_readlane(__float_as_uint(x), lane));
 }
-// the bytes of a word that hold the NaN code, as 0x80 each
-__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
-  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
-}
-
 // ONCE: one position and one item per sequence and kv head, so K and V are read once by the call, and
 // all rows of an item see the same keys.
 template <int QT, int DP, bool ONCE>
@@ -397,7 +379,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
 #pragma unroll
       for (int i = 0; i < ND; ++i) {
         const uint4 k = kr[b][i];
-        const uint4 lo = widen8<KT16>(k.x, k.y), hi = widen8<KT16>(k.z, k.w);
+        const uint4 lo = kv8::widen8<KT16>(k.x, k.y), hi = kv8::widen8<KT16>(k.z, k.w);
 #pragma unroll
         for (int n = NQ - 1; n >= 0; --n) {
           s[b] = tile::mfma16<KT16>(lo, qr[i][0][n], s[b]);
@@ -506,8 +488,8 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
       for (int b = 0; b < MB; ++b)
 #pragma unroll
         for (int i = 0; i < ND; ++i)
-          any |= nan_bytes(vr[b][i].x) | nan_bytes(vr[b][i].y) | nan_bytes(vr[b][i].z) |
-                 nan_bytes(vr[b][i].w);
+          any |= kv8::nan_codes(vr[b][i].x) | kv8::nan_codes(vr[b][i].y) |
+                 kv8::nan_codes(vr[b][i].z) | kv8::nan_codes(vr[b][i].w);
       if (__ballot(any != 0)) {
         const int rel = lim - (base + 4 * g);
 #pragma unroll 1
@@ -531,13 +513,13 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
                 for (int e = 0; e < 4; ++e)
                   if (nb == 4 * i + e) {
                     uint32_t* q4 = reinterpret_cast<uint32_t*>(&vr[b][i]);
-                    wd = nan_bytes(q4[e]);
-                    q4[e] &= ~((wd >> 7) * 0xffu);
+                    wd = kv8::nan_codes(q4[e]);
+                    q4[e] &= ~(wd * 0xffu);
                   }
-              at[b2] = (wd >> 7) * 0x38u;  // the code of 1
+              at[b2] = wd * 0x38u;  // the code of 1
             }
             hit = tile::mfma16<PIA_DTYPE_BF16>(make_uint4(see[0], see[1], see[2], see[3]),
-                                               widen8<PIA_DTYPE_BF16>(at[0], at[1]), hit);
+                                               kv8::widen8<PIA_DTYPE_BF16>(at[0], at[1]), hit);
           }
 #pragma unroll
           for (int k = 0; k < 4 * ND; ++k)
@@ -554,7 +536,7 @@ __global__ __launch_bounds__(64 * KA_WG_WAVES, KA_WGS_PER_CU) void kv8_attention
       for (int i = 0; i < ND; ++i)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint4 v = widen8<PIA_DTYPE_BF16>(tile32::word(vr[2 * c][i], e),
+          const uint4 v = kv8::widen8<PIA_DTYPE_BF16>(tile32::word(vr[2 * c][i], e),
                                                  tile32::word(vr[2 * c + 1][i], e));
 #pragma unroll
           for (int k = NP - 1; k >= 0; --k)

@@ -95,20 +95,6 @@ __device__ __forceinline__ f32x16_t mfma32(const uint4& a, const uint4& b, f32x1
                                                    0);
 }
 
-// two codes (the low or high half of a word) times scale as two DT values
-template <int DT, bool HI>
-__device__ __forceinline__ uint32_t widen(uint32_t w, float scale) {
-  if constexpr (DT == PIA_DTYPE_F16)
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(w, scale, HI));
-  else
-    return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(w, scale, HI));
-}
-template <int DT>
-__device__ __forceinline__ uint4 widen8(uint32_t a, uint32_t b, float scale) {
-  return make_uint4(widen<DT, false>(a, scale), widen<DT, true>(a, scale),
-                    widen<DT, false>(b, scale), widen<DT, true>(b, scale));
-}
-
 // fp16 infinities as the largest values: what no fp16 holds of a code times its scale (fp16 tensors
 // round to 65536 at most, half a step from there). An infinity would be NaN in rows that do not see it.
 __device__ __forceinline__ uint32_t finite16(uint32_t w) {
@@ -134,11 +120,6 @@ __device__ __forceinline__ float add_pair(uint32_t x, float c) {
   else
     return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(bf2, x),
                                            __builtin_bit_cast(bf2, 0x3f803f80u), c, false);
-}
-
-// the bytes of a word of codes that hold the NaN code, as 1 each
-__device__ __forceinline__ uint32_t nan_codes(uint32_t w) {
-  return (((w & 0x7f7f7f7fu) + 0x01010101u) >> 7) & 0x01010101u;
 }
 
 __device__ __forceinline__ float swap_halves(float x) {  // the value of lane l ^ 32
@@ -319,8 +300,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     const float scale = HALF ? 1.f : p.scale;
 #pragma unroll
     for (int i = 0; i < UK / 8; ++i) {
-      put(base ^ (128 * i), widen8<DT>(p.x[i].x, p.x[i].y, scale));
-      put(base ^ (128 * i + 16), widen8<DT>(p.x[i].z, p.x[i].w, scale));
+      put(base ^ (128 * i), kv8::widen8<DT>(p.x[i].x, p.x[i].y, scale));
+      put(base ^ (128 * i + 16), kv8::widen8<DT>(p.x[i].z, p.x[i].w, scale));
     }
     if (HALF && lane == 0) k_scale[kt & 3][blk] = p.there ? p.scale : 1.f;
   };
@@ -350,7 +331,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
       uint32_t* w = &p.x[0].x;
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const uint32_t n = nan_codes(w[e]);
+        const uint32_t n = kv8::nan_codes(w[e]);
         any |= n;
         w[e] = places ? n * 0x38u : w[e] & ~(n * 0xffu);  // 0x38: the code of 1
       }
@@ -359,10 +340,10 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
     }
     auto all = [&](auto fix) {
       const uint32_t base = p.base + buf * V_BUF;
-      put(base, kept<fix()>(widen8<DT>(p.x[0].x, p.x[1].x, scale)));
-      put(base + 128, kept<fix()>(widen8<DT>(p.x[0].y, p.x[1].y, scale)));
-      put((base ^ 16) + 256, kept<fix()>(widen8<DT>(p.x[0].z, p.x[1].z, scale)));
-      put((base ^ 16) + 384, kept<fix()>(widen8<DT>(p.x[0].w, p.x[1].w, scale)));
+      put(base, kept<fix()>(kv8::widen8<DT>(p.x[0].x, p.x[1].x, scale)));
+      put(base + 128, kept<fix()>(kv8::widen8<DT>(p.x[0].y, p.x[1].y, scale)));
+      put((base ^ 16) + 256, kept<fix()>(kv8::widen8<DT>(p.x[0].z, p.x[1].z, scale)));
+      put((base ^ 16) + 384, kept<fix()>(kv8::widen8<DT>(p.x[0].w, p.x[1].w, scale)));
     };
     if ((lane & 31) < VL) {
       if (large(scale)) all(std::true_type{});
