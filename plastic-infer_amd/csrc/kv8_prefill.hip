@@ -297,7 +297,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   };
   auto stage_k = [&](const Part& p, int buf, int kt) {
     const uint32_t base = p.base + buf * K_BUF;
-    const float scale = HALF ? 1.f : p.scale;
+    const float scale = HALF && p.scale == p.scale ? 1.f : p.scale;  // NaN stays, in K
 #pragma unroll
     for (int i = 0; i < UK / 8; ++i) {
       put(base ^ (128 * i), kv8::widen8<DT>(p.x[i].x, p.x[i].y, scale));

@@ -83,3 +83,23 @@ def test_gather(dev, bad):
     cu = torch.tensor([0] + lens).cumsum(0).to(dev)
     want, got = (kv8_gather(p.to_device(dev), tables.to(dev), cu, 130) for p in (clean, dirty))
     assert all(torch.equal(a, b) for a, b in zip(want, got))
+
+
+@pytest.mark.parametrize("bad", BAD)
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("hq,hkv,dim", [(8, 2, 128), (96, 8, 128), (96, 8, 64), (8, 2, 256)])
+def test_a_k_scale_that_is_none_shows_where_it_is_seen(dev, hq, hkv, dim, dtype, bad):
+    """The block of positions 80..95 of one head: rows that see a key of it are NaN (with an infinite scale
+    a row may be finite, where its products with them are all negative), others are as they were."""
+    n, rows, page, g = 130, 66, 16, hq // hkv
+    tables, pages = _tables([n], page, 0, 3)
+    clean, dirty = (O.Pool.random(pages, hkv, dim, page, seed=5) for _ in range(2))
+    dirty.scale["k"][int(tables[0, 5]), 1] = bad
+    i32 = lambda x: torch.tensor(x, dtype=torch.int32, device=dev)  # noqa: E731
+    q = _rows(rows, hq, dim, dtype, dim).to(dev)
+    want, got = (paged_attention_kv8(q, p.to_device(dev), tables.to(dev), i32([n]), i32([0, rows]),
+                                     i32([n - rows])) for p in (clean, dirty))
+    sees = torch.arange(rows) + n - rows >= 80
+    assert torch.equal(got[~sees], want[~sees])
+    assert torch.equal(got[:, :g], want[:, :g]) and torch.equal(got[:, 2 * g:], want[:, 2 * g:])
+    assert torch.isnan(got[sees][:, g:2 * g]).all() or bad == math.inf
