@@ -24,7 +24,8 @@
 // results do not depend on timing. Items of three steps at most (by the table's width) are not cut: a
 // wave takes those that begin in its range, and there is no second kernel. In us, cut and whole: one
 // sequence of 64 keys 10.4 and 8.4 (the call from Python 13.5 and 10.5), of 192 10.6 and 11.4 (13.5 and
-// 11.3), of 256 10.6 and 13.1; 256 sequences of 192 24.3 and 22.4.
+// 11.3), of 256 10.6 and 13.1; 256 sequences of 192 24.3 and 22.4. A short context under a wide table is
+// cut all the same: the host does not know the keys.
 //
 // Measured (both kernels): 256 sequences of 512 to 8192 keys, 32 heads of 128 over 8, bf16: 372-382 us,
 // 6.0-6.2 TB/s, the first kernel alone at the 6.4 that reads reach. Two of 100000 and 131072 keys,

@@ -10,8 +10,8 @@
 // tile before theirs, they are widened to DT: once for all rows, where an operand widened at its use
 // would be widened by every wave. bf16 holds a code times its scale exactly. fp16 does only for scales of
 // 2^-15 .. 2^7, so its K is codes, whose scale enters the scores in fp32 (1 to 2 % of the time); its V is
-// within 2^-25 below those scales, and beyond 65504 counts as that. A head_dim below DP is made up with zeros of K and q; V's rows behind it are whatever LDS holds and end
-// in outputs that nobody writes.
+// within 2^-25 below those scales, and beyond 65504 counts as that. A head_dim below DP is made up with
+// zeros of K and q; V's rows behind it are whatever LDS holds and end in outputs that nobody writes.
 //
 // Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
 // 8 (l / 32) + e; of C, lane l has column l % 32 and rows 8 i + 4 (l / 32) + j, i, j < 4)
@@ -24,10 +24,10 @@
 // The probabilities are rounded to DT once, and the sum is of the rounded ones: half a step of DT each,
 // as much as the result's own rounding (bf16, the case below: 0.0020 of the norm from exact results,
 // 0.0017 for exactly computed ones rounded). A second term would be half as many products again (fp16
-// with two bf16 terms: 895 us where this takes 750). fp16 has no more than 29 binades of normal numbers for
-// them: a row's reference follows its maximum tile by tile, up and down, so that a tile's largest has
-// them all below it, and what the rest loses is bounded at the end of an item, which is done again where
-// that is too much (8 % of the time for the references; an item that is done again takes 3.3 times as long).
+// with two bf16 terms: 890 us, and 660 with one on the same machine). fp16 has 29 binades of normal numbers
+// for them: a row's reference follows its maximum from tile to tile, up and down, so that a tile's largest
+// has at least 25 of them below it (8 % of the time where heads' scores spread unlike). What the rest loses
+// is bounded at the end of an item, which is done again where that is too much: 3.3 times as long.
 // LDS tiles (16-byte units, XORed with a term of their row): K [token][d], 16 units to a token also at
 // DP 96: unit u (d 8 u .. + 7) of token t at u ^ t % 16 (DP 64: 8 units, u ^ t / 2 % 8); V [d][token]:
 // unit 2 m + hh (block m, tokens 4 hh + j, then 8 + 4 hh + j) of element d at
@@ -757,7 +757,8 @@ int launch_kv8_prefill(int dtype, void* out, const void* q, int64_t q_stride, co
   // 128 on 32768 keys: 128 rows 650 us whole and 88 cut, 512 rows 666 and 288. 64 pieces of 8 tiles a
   // row take 52 us there where 32 of 16 take 43; pieces of 2 tiles cost more than they bring (4096 keys,
   // 2048 rows of 64 heads: 34 us, and 25 with 8), and so does a cut of items that fill the CUs (512
-  // keys, 32768 rows: 30 and 21).
+  // keys, 32768 rows: 30 and 21). Under a table that is not full the pieces are shorter than that: 128 rows on
+  // 512 keys take 18 us with their own table, 23 with one of 4096 tokens, 31 of 32768.
   const int64_t most = std::max(std::min(2 * cus / items, tiles / 16), std::min(cus / items, tiles / 4));
   const int cuts = int(std::max<int64_t>(
       1, std::min(std::min<int64_t>(most, P8_MAX_CUTS), part_rows / (total_q_rows * Hq))));

@@ -353,7 +353,9 @@ __device__ __forceinline__ void append_plain(const AppendArgs& a, const float2* 
         const int64_t base = to_of(0);  // one page: P is a multiple of 16
         if (base < 0) return;
         // 16-byte units of the tile, in the pool's order; a lane writes N of them in a row. The order
-        // within N is XORed so that eight lanes' units fall into different banks either way.
+        // within N is XORed so that eight lanes' units fall into different banks either way (K and V
+        // alone count no conflict; those of the whole call, 6 cycles to an instruction, are of q's
+        // lanes, which read 32 or 64 bytes of the table each).
         auto place = [&](int u) {
           return reinterpret_cast<Pack*>(tile) + ((u & ~(N - 1)) | ((u ^ (u >> 3)) & (N - 1)));
         };
