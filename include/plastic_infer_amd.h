@@ -549,6 +549,16 @@ int pia_rotary(void* q_out, void* k_out, const void* q, const void* k, int64_t q
                double factor, int interleaved, int transposed, int64_t num_tokens, int num_heads,
                int num_kv_heads, int head_dim, int dtype, void* stream);
 
+/* The same with a position on each of num_axes axes (time, height, width): positions
+ * [num_axes, num_tokens], contiguous, and pair i turns by its position on axis axes[i] (i32[pairs]). A
+ * pair whose axis is outside [0, num_axes) is turned as at position 0. */
+int pia_rotary_axes(void* q_out, void* k_out, const void* q, const void* k, int64_t q_token_stride,
+                    int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+                    const void* positions, int positions_i64, const int32_t* axes, int num_axes,
+                    const double* turns, int pairs, double factor, int interleaved,
+                    int transposed, int64_t num_tokens, int num_heads, int num_kv_heads,
+                    int head_dim, int dtype, void* stream);
+
 /* ---------------------------------------------------------------------------------------------
  * Append with the rotary positions applied. Rows cu_new[b] .. cu_new[b + 1] of q / k / v (cu_new
  * NULL: row b) are the last tokens of sequence b, whose context_lens[b] counts them; a row's

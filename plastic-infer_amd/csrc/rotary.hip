@@ -3,6 +3,9 @@
 //
 //   (a, b) -> (a c - b s, b c + a s), c = factor cos(2 pi p f), s = factor sin(2 pi p f)
 //
+// With several axes (time, height, width of images and video) a token has a position on each, and p is
+// that of the pair's own axis: only the table of (cos, sin) differs, by two loads for each of its entries.
+//
 // The transposed map (the gradient's) is the same with s negated. Bound by HBM: every element is read
 // and written once. A workgroup takes a few tokens, computes their (cos, sin) into LDS once for all
 // heads of q and k, and then streams the heads in 16-byte vectors; fp32 arithmetic, one rounding. 8192
@@ -22,14 +25,15 @@ struct RotaryArgs {
   const void *q, *k;
   int64_t q_tok, q_head, k_tok, k_head;
   const void* positions;
+  const int32_t* axes;  // several axes: the axis of each pair, positions [num_axes, tokens]
   const double* turns;
   int64_t tokens;
-  int wide, pairs, Hq, Hkv, D, per_wg, stream;
+  int num_axes, wide, pairs, Hq, Hkv, D, per_wg, stream;
   double factor;
   float sin_sign;
 };
 
-template <int DT, bool INTER, bool VEC>
+template <int DT, bool INTER, bool VEC, bool AXES>
 __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotaryArgs a) {
   using T = typename Elem<DT>::T;
   using U = rope::Units<DT, INTER, VEC>;
@@ -38,8 +42,16 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotaryArgs a) {
   const int nt = int(min(int64_t(a.per_wg), a.tokens - t0));
   for (int i = threadIdx.x; i < nt * a.pairs; i += RT_THREADS) {
     const int t = i / a.pairs, p = i - t * a.pairs;
-    const int64_t pos = a.wide ? static_cast<const int64_t*>(a.positions)[t0 + t]
-                               : int64_t(static_cast<const int32_t*>(a.positions)[t0 + t]);
+    int64_t at = t0 + t;
+    bool there = true;
+    if constexpr (AXES) {
+      const int axis = a.axes[p];
+      there = axis >= 0 && axis < a.num_axes;
+      at += (there ? axis : 0) * a.tokens;
+    }
+    int64_t pos = a.wide ? static_cast<const int64_t*>(a.positions)[at]
+                         : int64_t(static_cast<const int32_t*>(a.positions)[at]);
+    if (AXES && !there) pos = 0;
     tab[i] = rope::cos_sin(a.turns[p], pos, a.factor);
   }
   __syncthreads();
@@ -63,17 +75,12 @@ __global__ __launch_bounds__(RT_THREADS) void rotary_kernel(RotaryArgs a) {
   }
 }
 
-}  // namespace
-}  // namespace pia
-
-using namespace pia;
-
-extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k,
-                          int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
-                          int64_t k_head_stride, const void* positions, int positions_i64,
-                          const double* turns, int pairs, double factor, int interleaved,
-                          int transposed, int64_t num_tokens, int num_heads, int num_kv_heads,
-                          int head_dim, int dtype, void* stream) {
+int rotate(void* q_out, void* k_out, const void* q, const void* k, int64_t q_token_stride,
+           int64_t q_head_stride, int64_t k_token_stride, int64_t k_head_stride,
+           const void* positions, int positions_i64, const int32_t* axes, int num_axes,
+           const double* turns, int pairs, double factor, int interleaved, int transposed,
+           int64_t num_tokens, int num_heads, int num_kv_heads, int head_dim, int dtype,
+           void* stream) {
   if (dtype != PIA_DTYPE_F32 && dtype != PIA_DTYPE_F16 && dtype != PIA_DTYPE_BF16)
     return fail(PIA_EUNSUPPORTED, "rotary: dtype must be bf16, fp16 or fp32");
   if (num_tokens < 0 || num_heads < 0 || num_kv_heads < 0 || head_dim <= 0 || pairs < 0 ||
@@ -95,7 +102,7 @@ extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k
       (!num_kv_heads || rope::vectors(elem, inter, pairs, head_dim, k, k_out, k_token_stride,
                                       k_head_stride));
   RotaryArgs a{q_out, k_out, q, k, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
-               positions, turns, num_tokens, positions_i64 != 0, pairs, num_heads, num_kv_heads,
+               positions, axes, turns, num_tokens, num_axes, positions_i64 != 0, pairs, num_heads, num_kv_heads,
                head_dim, 1, num_tokens * H * head_dim * elem >= rope::kStreamBytes, factor,
                transposed ? -1.f : 1.f};
   // tokens of a workgroup: one, or four where that still leaves four workgroups
@@ -109,13 +116,16 @@ extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k
   const dim3 grid{unsigned(ceil_div(num_tokens, a.per_wg)), unsigned(gy), 1u};
   const size_t lds = sizeof(float2) * size_t(a.per_wg) * size_t(pairs);
   hipStream_t s = as_stream(stream);
-#define PIA_RT(DT, I, V) \
-  hipLaunchKernelGGL((rotary_kernel<DT, I, V>), grid, dim3(RT_THREADS), lds, s, a)
+#define PIA_RT(DT, I, V)                                                                      \
+  if (axes)                                                                                   \
+    hipLaunchKernelGGL((rotary_kernel<DT, I, V, true>), grid, dim3(RT_THREADS), lds, s, a);   \
+  else                                                                                        \
+    hipLaunchKernelGGL((rotary_kernel<DT, I, V, false>), grid, dim3(RT_THREADS), lds, s, a)
 #define PIA_RT_D(DT)                                                   \
   if (inter) {                                                         \
-    if (vec) PIA_RT(DT, true, true); else PIA_RT(DT, true, false);     \
+    if (vec) { PIA_RT(DT, true, true); } else { PIA_RT(DT, true, false); }     \
   } else {                                                             \
-    if (vec) PIA_RT(DT, false, true); else PIA_RT(DT, false, false);   \
+    if (vec) { PIA_RT(DT, false, true); } else { PIA_RT(DT, false, false); }   \
   }
   if (dtype == PIA_DTYPE_F32) {
     PIA_RT_D(PIA_DTYPE_F32)
@@ -127,4 +137,34 @@ extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k
 #undef PIA_RT_D
 #undef PIA_RT
   return check_launch("rotary");
+}
+
+}  // namespace
+}  // namespace pia
+
+using namespace pia;
+
+extern "C" int pia_rotary(void* q_out, void* k_out, const void* q, const void* k,
+                          int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                          int64_t k_head_stride, const void* positions, int positions_i64,
+                          const double* turns, int pairs, double factor, int interleaved,
+                          int transposed, int64_t num_tokens, int num_heads, int num_kv_heads,
+                          int head_dim, int dtype, void* stream) {
+  return rotate(q_out, k_out, q, k, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+                positions, positions_i64, nullptr, 1, turns, pairs, factor, interleaved, transposed,
+                num_tokens, num_heads, num_kv_heads, head_dim, dtype, stream);
+}
+
+extern "C" int pia_rotary_axes(void* q_out, void* k_out, const void* q, const void* k,
+                               int64_t q_token_stride, int64_t q_head_stride,
+                               int64_t k_token_stride, int64_t k_head_stride,
+                               const void* positions, int positions_i64, const int32_t* axes,
+                               int num_axes, const double* turns, int pairs, double factor,
+                               int interleaved, int transposed, int64_t num_tokens, int num_heads,
+                               int num_kv_heads, int head_dim, int dtype, void* stream) {
+  if (num_axes <= 0) return fail(PIA_EINVAL, "rotary: invalid number of axes");
+  if (pairs > 0 && num_tokens > 0 && !axes) return fail(PIA_EINVAL, "rotary: null pointer");
+  return rotate(q_out, k_out, q, k, q_token_stride, q_head_stride, k_token_stride, k_head_stride,
+                positions, positions_i64, pairs > 0 ? axes : nullptr, num_axes, turns, pairs, factor,
+                interleaved, transposed, num_tokens, num_heads, num_kv_heads, head_dim, dtype, stream);
 }

@@ -79,6 +79,8 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pia_prefill_hit_compact": (_I, [_P, _P, _P, _P, _L, _L, _I, _P]),
     "pia_rotary": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _P, _I, _P, _I, _D, _I, _I, _L, _I, _I, _I,
                         _I, _P]),
+    "pia_rotary_axes": (_I, [_P, _P, _P, _P, _L, _L, _L, _L, _P, _I, _P, _I, _P, _I, _D, _I, _I, _L,
+                             _I, _I, _I, _I, _P]),
     "pia_kv_append": (_I, [_P, _P, _L, _L, _P, _L, _L, _P, _L, _L, _P, _P, _P, _P, _P, _L, _P, _P,
                            _L, _I, _P, _I, _D, _I, _I, _I, _I, _I, _L, _I, _P]),
     "pia_kv8_gather": (_I, [_P, _P, _P, _P, _P, _P, _P, _L, _P, _I, _L, _I, _I, _I, _L, _I, _P]),
@@ -89,7 +91,7 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pia_hbm_read_rows_probe": (_I, [_P, _L, _I, _I, _P, _P]),
 }
 
-EXPECTED_ABI = 10
+EXPECTED_ABI = 11
 
 _HIP = torch.version.hip is not None
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

@@ -47,6 +47,9 @@ def append_call(q: torch.Tensor | None, k: torch.Tensor, v: torch.Tensor,
         raise ValueError("cu_new must be int32 [B + 1]")
     if rope is not None:
         check_rope(rope, D, dev)
+        if rope.axes is not None:
+            raise ValueError("an append turns by the place in the context: rotate positions with "
+                             "several axes by rotary_embed, and append with rope None")
     out = None
     if q is not None:
         q = heads_view("q", q)
