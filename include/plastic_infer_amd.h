@@ -613,6 +613,43 @@ int pia_kv8_attention(void* out, const void* q, int64_t q_stride, const void* k_
                       int64_t workspace_bytes, void* stream);
 
 /* ---------------------------------------------------------------------------------------------
+ * Attention with a sliding window and sinks over the float pools (those of pia_paged_attention). Rows of
+ * sequence b are q[cu_q[b] .. cu_q[b + 1]) (NULL: row b); row s of b stands at position
+ * p = q_pos_offsets[b] + s (NULL: the rows are the context's last, p = kv_lens[b] - rows + s) and attends
+ * the keys j < kv_lens[b], j <= p with p - j < window or j < sinks. Softmax, heads, pages outside the
+ * pool, rows without a key (zeros) and non-finite values as in pia_paged_attention; entries of a block
+ * table whose tokens no row sees are not dereferenced. Rows behind the last sequence's are left. q rows are q_stride
+ * elements apart (heads contiguous), out is contiguous and may be q itself (dense rows), which it must
+ * not overlap otherwise. head_dim to 512, page_size to 4096. workspace: 16-byte aligned, of
+ * pia_window_attention_workspace_bytes(head_dim) bytes (0: none), any content; calls that share one are
+ * ordered on one stream. No counterpart in the reference.
+ * ------------------------------------------------------------------------------------------- */
+int64_t pia_window_attention_workspace_bytes(int head_dim);
+int pia_window_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
+                         const void* v_pages, const int32_t* block_tables, int64_t bt_stride,
+                         const int32_t* kv_lens, const int32_t* cu_q, const int32_t* q_pos_offsets,
+                         int window, int sinks, int num_seqs, int64_t total_q_rows, int num_heads,
+                         int num_kv_heads, int head_dim, int page_size, int64_t num_pages,
+                         float scale, int dtype, void* workspace, int64_t workspace_bytes,
+                         void* stream);
+
+/* Attention behind shared prefixes over the float pools. Group g is the sequences
+ * cu_seqs[g] .. cu_seqs[g + 1] (not decreasing; NULL: num_groups is 1 (or 0) and the group all of them); its prefix
+ * is the first prefix_lens[g] tokens of prefix_tables[g] (pt_stride entries a row). Row s of sequence b
+ * attends the whole prefix of b's group (none: no prefix) and the sequence's own keys j < kv_lens[b] of
+ * block_tables[b], with q_pos_offsets j <= q_pos_offsets[b] + s. All else as pia_window_attention.
+ * workspace: 16-byte aligned, of pia_prefix_attention_workspace_bytes for so many rows or more. */
+int64_t pia_prefix_attention_workspace_bytes(int64_t total_q_rows, int num_heads, int head_dim);
+int pia_prefix_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
+                         const void* v_pages, const int32_t* prefix_tables, int64_t pt_stride,
+                         const int32_t* prefix_lens, const int32_t* cu_seqs, int num_groups,
+                         const int32_t* block_tables, int64_t bt_stride, const int32_t* kv_lens,
+                         const int32_t* cu_q, const int32_t* q_pos_offsets, int num_seqs,
+                         int64_t total_q_rows, int num_heads, int num_kv_heads, int head_dim,
+                         int page_size, int64_t num_pages, float scale, int dtype, void* workspace,
+                         int64_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------------------------------------
  * HBM streaming-read probe. No counterpart in the reference: a measurement aid for the
  * rooflines of the kernels above (bench.py --workload hbm-read times it over fresh regions and
  * fits fixed cost + rate). src: 16-byte aligned device memory of `bytes` bytes (a positive

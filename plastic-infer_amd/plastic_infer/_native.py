@@ -87,6 +87,12 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pia_kv8_attention_workspace_bytes": (_L, [_I]),
     "pia_kv8_attention": (_I, [_P, _P, _L, _P, _P, _P, _P, _P, _L, _P, _P, _P, _I, _L, _I, _I, _I,
                                _I, _L, _F, _I, _P, _L, _P]),
+    "pia_window_attention_workspace_bytes": (_L, [_I]),
+    "pia_window_attention": (_I, [_P, _P, _L, _P, _P, _P, _L, _P, _P, _P, _I, _I, _I, _L, _I, _I, _I,
+                                  _I, _L, _F, _I, _P, _L, _P]),
+    "pia_prefix_attention_workspace_bytes": (_L, [_L, _I, _I]),
+    "pia_prefix_attention": (_I, [_P, _P, _L, _P, _P, _P, _L, _P, _P, _I, _P, _L, _P, _P, _P, _I, _L,
+                                  _I, _I, _I, _I, _L, _F, _I, _P, _L, _P]),
     "pia_hbm_read_probe": (_I, [_P, _L, _P, _L, _P, _P]),
     "pia_hbm_read_rows_probe": (_I, [_P, _L, _I, _I, _P, _P]),
 }

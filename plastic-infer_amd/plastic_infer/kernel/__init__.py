@@ -33,6 +33,16 @@ from .paged_kv8 import (
     paged_attention_kv8,
     paged_decode_attention_kv8,
 )
+from .paged_prefix import (
+    paged_prefix_attention,
+    paged_prefix_decode_attention,
+    prefix_attention_workspace_bytes,
+)
+from .paged_window import (
+    paged_window_attention,
+    paged_window_decode_attention,
+    window_attention_workspace_bytes,
+)
 from .rotary import RopeParams, rope_params, rotary_embed
 
 __all__ = [
@@ -45,5 +55,7 @@ __all__ = [
     "pages_chunks_copy",
     "KV8Pools", "kv8_append", "kv8_attention_workspace_bytes", "kv8_gather", "kv_append",
     "paged_attention_kv8", "paged_decode_attention_kv8",
+    "paged_prefix_attention", "paged_prefix_decode_attention", "prefix_attention_workspace_bytes",
+    "paged_window_attention", "paged_window_decode_attention", "window_attention_workspace_bytes",
     "RopeParams", "rope_params", "rotary_embed",
 ]
