@@ -3,16 +3,15 @@
 //   window  the row at position p sees tokens j <= p of its sequence with p - j < window or j < sinks
 //   prefix  a row sees all tokens of its group's prefix and then those of its own sequence
 //
-// Both are two stretches of keys: the first `head` tokens of one table (the sinks in the sequence's own, or
-// the prefix's), which every row sees whole but where a causal limit cuts the sinks, and tokens lo .. lim - 1
-// of the sequence's table, with limits that move with the row. The kernels differ in how they share the
-// work; what a row sees they all take from here.
+// The kernels differ in how they share the work; what a row sees they all take from here.
 #pragma once
 
 #include "pia_internal.h"
 
 namespace pia {
 namespace reach {
+
+constexpr int FAR = 0x7ffffff0;  // beyond every token
 
 struct Args {
   void* out;
@@ -30,11 +29,22 @@ struct Args {
   int64_t pt_stride;
   const int32_t *plens, *gs;  // gs null: one group of all sequences
   int groups;
+  // of the kernels that share work
+  int first, count;  // the sequences (by_group: groups) of a launch
+  int by_group;      // a "sequence" is a group: all its rows, over its prefix
+  int whole;         // no item is cut
+  float* parts;      // pieces of items, by wave
+  int64_t* pref;
+  // Pieces of rows, for rows * Hq of them: unnormalised outputs [cuts, rows * Hq, D], then (reference
+  // point in log2 units, sum) [cuts, rows * Hq]. dst: where results go instead of out; src: the
+  // prefix's, to be joined with what the kernel has.
+  float *dst, *src;
+  int dst_cuts, src_cuts;
 };
 
 // tokens of a table that are there
 __device__ __forceinline__ int held(int len, int64_t stride, int P) {
-  return int(min(int64_t(max(len, 0)), min(stride * P, int64_t(0x7ffffff0))));
+  return int(min(int64_t(max(len, 0)), min(stride * P, int64_t(FAR))));
 }
 
 // The group of sequence b (-1: none)
@@ -49,35 +59,68 @@ __device__ __forceinline__ int group_of(const Args& a, int b) {
   return a.gs[lo] <= b && b < a.gs[lo + 1] ? lo : -1;
 }
 
-// A sequence: its rows and tokens, the position of its first row (window) or the causal offset
+// A sequence: its rows and tokens, and the position of its first row where rows are limited by theirs
 struct Seq {
   int64_t row0;
-  int n, len;
-  int off;
+  int n, len, off;
   bool causal;
 };
+// the first row of sequence b <= B
+__device__ __forceinline__ int64_t row_of(const Args& a, int b) { return a.cu ? a.cu[b] : b; }
+__device__ __forceinline__ int edge_of(const Args& a, int g) {  // the first sequence of group g
+  return a.gs ? min(max(a.gs[g], 0), a.B) : g == 0 ? 0 : a.B;
+}
 __device__ __forceinline__ Seq sequence(const Args& a, int b) {
   Seq s;
-  s.row0 = a.cu ? a.cu[b] : b;
-  const int64_t n = a.cu ? int64_t(a.cu[b + 1]) - s.row0 : 1;
+  s.row0 = row_of(a, b);
+  const int64_t n = row_of(a, b + 1) - s.row0;
   s.n = s.row0 < 0 ? 0 : int(max(int64_t(0), min(n, a.rows - s.row0)));
   s.len = held(a.lens[b], a.bt_stride, a.P);
   s.causal = a.offs || a.window;
   s.off = a.offs ? a.offs[b] : a.window ? s.len - s.n : 0;
   return s;
 }
-// Row pos of a sequence sees tokens lo .. lim - 1, and (window) the first `sinks` of those below lim
+__device__ __forceinline__ Seq group(const Args& a, int g) {
+  Seq s;
+  s.row0 = row_of(a, edge_of(a, g));
+  const int64_t n = row_of(a, edge_of(a, g + 1)) - s.row0;
+  s.n = s.row0 < 0 ? 0 : int(max(int64_t(0), min(n, a.rows - s.row0)));
+  s.len = held(a.plens[g], a.pt_stride, a.P);
+  s.off = 0;
+  s.causal = false;
+  return s;
+}
+// Row pos of a sequence sees tokens lowest .. limit - 1 and (window) the first `sinks` of those below limit
 __device__ __forceinline__ int limit(const Seq& s, int pos) {
   return s.causal ? int(max(int64_t(0), min(int64_t(s.len), int64_t(s.off) + pos + 1))) : s.len;
 }
 __device__ __forceinline__ int lowest(const Args& a, const Seq& s, int pos) {
   if (!a.window) return 0;
-  return int(max(int64_t(0), min(int64_t(0x7ffffff0), int64_t(s.off) + pos + 1 - a.window)));
+  return int(max(int64_t(0), min(int64_t(FAR), int64_t(s.off) + pos + 1 - a.window)));
+}
+
+// The prefix's pieces of a row of sequence b, if it has any
+__device__ __forceinline__ bool has_prefix(const Args& a, int b) {
+  const int g = group_of(a, b);
+  return g >= 0 && held(a.plens[g], a.pt_stride, a.P) > 0;
+}
+// the weight of a piece whose reference is m against the joined one
+__device__ __forceinline__ float weight(float m, float joined) {
+  return m == joined ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - joined);
 }
 
 }  // namespace reach
 
 // Any head_dim to 512, page size and group: one wave for each row and head (reach_general.hip)
 int launch_reach_general(const reach::Args& a, int dtype, hipStream_t s);
+
+// Items of 16 rows over a contiguous range of their steps for each resident wave (reach_stream.h), for the
+// sequences or (by_group) for the groups. tokens: a bound of the tokens that an item walks.
+int launch_reach_stream_f32(const reach::Args& a, int64_t tokens, hipStream_t s);
+int launch_reach_stream_f16(const reach::Args& a, int64_t tokens, hipStream_t s);
+int launch_reach_stream_bf16(const reach::Args& a, int64_t tokens, hipStream_t s);
+// bytes of its pieces by wave, and of the numbers before them
+int64_t reach_stream_parts_bytes(int D);
+int64_t reach_stream_pref_bytes();
 
 }  // namespace pia

@@ -53,12 +53,44 @@ int check(const reach::Args& a, int dtype, const char* name) {
   return 0;
 }
 
+int check_workspace(const void* ws, int64_t bytes, int64_t need, const char* name) {
+  if (need == 0) return 0;
+  if (!ws || bytes < need || !aligned(ws, 16)) {
+    set_error("%s: workspace missing, too small or not 16-byte aligned", name);
+    return PIA_EINVAL;
+  }
+  return 0;
+}
+// Whether the streaming kernel takes a call; what it does not is the general kernel's
+bool streams(const reach::Args& a, int dtype) {
+  const int64_t e = elem_bytes(dtype);
+  return a.D % 16 == 0 && a.D <= 256 && a.P % 16 == 0 && aligned(a.q, 16) && aligned(a.out, 16) &&
+         a.q_stride * e % 16 == 0 && aligned(a.kp, 16) && aligned(a.vp, 16) &&
+         // workgroups of the joining kernel
+         ((a.rows * a.G >> 4) + a.B + a.groups + 2) * a.Hkv < (1 << 25);
+}
+int stream_call(const reach::Args& a, int dtype, int64_t tokens, hipStream_t s) {
+  return dtype == PIA_DTYPE_F32   ? launch_reach_stream_f32(a, tokens, s)
+         : dtype == PIA_DTYPE_F16 ? launch_reach_stream_f16(a, tokens, s)
+                                  : launch_reach_stream_bf16(a, tokens, s);
+}
+// The streaming kernel's part of a workspace; where it ends
+char* place(reach::Args& a, void* workspace) {
+  char* p = static_cast<char*>(workspace);
+  a.pref = reinterpret_cast<int64_t*>(p);
+  a.parts = reinterpret_cast<float*>(p + reach_stream_pref_bytes());
+  return p + reach_stream_pref_bytes() + reach_stream_parts_bytes(a.D);
+}
+
 }  // namespace
 }  // namespace pia
 
 using namespace pia;
 
-extern "C" int64_t pia_window_attention_workspace_bytes(int head_dim) { return 0; }
+extern "C" int64_t pia_window_attention_workspace_bytes(int head_dim) {
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 16) return 0;
+  return reach_stream_pref_bytes() + reach_stream_parts_bytes(head_dim);
+}
 
 extern "C" int pia_window_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
                                     const void* v_pages, const int32_t* block_tables,
@@ -70,18 +102,30 @@ extern "C" int pia_window_attention(void* out, const void* q, int64_t q_stride, 
                                     int64_t workspace_bytes, void* stream) {
   if (window <= 0 || sinks < 0)
     return fail(PIA_EINVAL, "window_attention: window must be positive and sinks not negative");
-  const reach::Args a{out, q, q_stride, k_pages, v_pages, block_tables, bt_stride, kv_lens, cu_q,
-                      q_pos_offsets, total_q_rows, num_pages, 0, scale * 1.4426950408889634f, num_seqs,
-                      num_heads, num_kv_heads, num_kv_heads > 0 ? num_heads / num_kv_heads : 0,
-                      head_dim, page_size, window, sinks, nullptr, 0, nullptr, nullptr, 0};
-  const int rc = check(a, dtype, "window_attention");
+  reach::Args a{out, q, q_stride, k_pages, v_pages, block_tables, bt_stride, kv_lens, cu_q,
+                q_pos_offsets, total_q_rows, num_pages, 0, scale * 1.4426950408889634f, num_seqs,
+                num_heads, num_kv_heads, num_kv_heads > 0 ? num_heads / num_kv_heads : 0,
+                head_dim, page_size, window, sinks};
+  int rc = check(a, dtype, "window_attention");
+  if (!rc)
+    rc = check_workspace(workspace, workspace_bytes, pia_window_attention_workspace_bytes(head_dim),
+                         "window_attention");
   if (rc) return rc < 0 ? rc : 0;
-  return launch_reach_general(a, dtype, as_stream(stream));
+  if (!streams(a, dtype)) return launch_reach_general(a, dtype, as_stream(stream));
+  place(a, workspace);
+  // tokens that an item walks: the sinks' and the window's, of the table's
+  const int64_t tokens = std::min(bt_stride * page_size,
+                                  int64_t(window) + sinks + std::min<int64_t>(total_q_rows, 16));
+  return stream_call(a, dtype, tokens, as_stream(stream));
 }
 
 extern "C" int64_t pia_prefix_attention_workspace_bytes(int64_t total_q_rows, int num_heads,
                                                         int head_dim) {
-  return 0;
+  if (head_dim <= 0 || head_dim > 256 || head_dim % 16 || total_q_rows <= 0 || num_heads <= 0)
+    return 0;
+  // the prefix's pieces of all rows behind the streaming kernel's
+  return reach_stream_pref_bytes() + reach_stream_parts_bytes(head_dim) +
+         total_q_rows * num_heads * (head_dim + 2) * int64_t(sizeof(float));
 }
 
 extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
@@ -102,12 +146,29 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
   const bool some = num_groups > 0 && pt_stride > 0;
   if (some && (!prefix_tables || !prefix_lens))
     return fail(PIA_EINVAL, "prefix_attention: null pointer");
-  const reach::Args a{out, q, q_stride, k_pages, v_pages, block_tables, bt_stride, kv_lens, cu_q,
-                      q_pos_offsets, total_q_rows, num_pages, 0, scale * 1.4426950408889634f, num_seqs,
-                      num_heads, num_kv_heads, num_kv_heads > 0 ? num_heads / num_kv_heads : 0,
-                      head_dim, page_size, 0, 0, some ? prefix_tables : nullptr, pt_stride,
-                      prefix_lens, cu_seqs, some ? num_groups : 0};
-  const int rc = check(a, dtype, "prefix_attention");
+  reach::Args a{out, q, q_stride, k_pages, v_pages, block_tables, bt_stride, kv_lens, cu_q,
+                q_pos_offsets, total_q_rows, num_pages, 0, scale * 1.4426950408889634f, num_seqs,
+                num_heads, num_kv_heads, num_kv_heads > 0 ? num_heads / num_kv_heads : 0,
+                head_dim, page_size, 0, 0, some ? prefix_tables : nullptr, pt_stride, prefix_lens,
+                cu_seqs, some ? num_groups : 0};
+  int rc = check(a, dtype, "prefix_attention");
+  if (!rc)
+    rc = check_workspace(
+        workspace, workspace_bytes,
+        pia_prefix_attention_workspace_bytes(total_q_rows, num_heads, head_dim), "prefix_attention");
   if (rc) return rc < 0 ? rc : 0;
-  return launch_reach_general(a, dtype, as_stream(stream));
+  hipStream_t s = as_stream(stream);
+  if (!streams(a, dtype)) return launch_reach_general(a, dtype, s);
+  float* rows = reinterpret_cast<float*>(place(a, workspace));
+  if (some) {  // the prefix's part of all rows, then the rest
+    reach::Args g = a;
+    g.by_group = 1;
+    g.dst = rows;
+    g.dst_cuts = 1;
+    rc = stream_call(g, dtype, pt_stride * page_size, s);
+    if (rc) return rc;
+    a.src = rows;
+    a.src_cuts = 1;
+  }
+  return stream_call(a, dtype, bt_stride * page_size, s);
 }
