@@ -11,7 +11,7 @@
 namespace pia {
 namespace reach {
 
-constexpr int FAR = 0x7ffffff0;  // beyond every token
+constexpr int FAR = 0x7ffff000;  // beyond every token, with room for a few tiles behind it
 
 struct Args {
   void* out;
@@ -119,7 +119,13 @@ int launch_reach_general(const reach::Args& a, int dtype, hipStream_t s);
 int launch_reach_stream_f32(const reach::Args& a, int64_t tokens, hipStream_t s);
 int launch_reach_stream_f16(const reach::Args& a, int64_t tokens, hipStream_t s);
 int launch_reach_stream_bf16(const reach::Args& a, int64_t tokens, hipStream_t s);
-// bytes of its pieces by wave, and of the numbers before them
+// Tiles in LDS for 128 or 256 rows at a time (reach_tiles.hip), 16-bit pools: whether a call's shape is taken,
+// into how many pieces (at most `most`) it would cut each item of so many rows, and its launch. Pieces
+// go to dst; those of sequences are joined there, those of groups are not.
+bool reach_tiles_shape(const reach::Args& a, int dtype);
+int reach_tiles_cuts(const reach::Args& a, int64_t tokens, int64_t most);
+int launch_reach_tiles(const reach::Args& a, int dtype, int cuts, hipStream_t s);
+// bytes of the streaming kernel's pieces by wave, and of the numbers before them
 int64_t reach_stream_parts_bytes(int D);
 int64_t reach_stream_pref_bytes();
 

@@ -17,6 +17,10 @@ bool holds_rows(uintptr_t out, int64_t bytes, uintptr_t q, int64_t n, int64_t ro
   return r < n && from < int64_t(out) + bytes && from + row > int64_t(out);
 }
 
+// rows of a kv head and sequence (group) from which tiles in LDS take the call
+constexpr int64_t TILE_ROWS = 64;
+constexpr int64_t PREFIX_ROWS = 65536;
+
 int elem_bytes(int dtype) { return dtype == PIA_DTYPE_F32 ? 4 : 2; }
 
 // What both entry points ask of their arguments; 0: the call can run, 1: there is nothing to do
@@ -74,12 +78,30 @@ int stream_call(const reach::Args& a, int dtype, int64_t tokens, hipStream_t s) 
          : dtype == PIA_DTYPE_F16 ? launch_reach_stream_f16(a, tokens, s)
                                   : launch_reach_stream_bf16(a, tokens, s);
 }
-// The streaming kernel's part of a workspace; where it ends
-char* place(reach::Args& a, void* workspace) {
+// A workspace: the streaming kernel's numbers, its pieces by wave, and (prefix) pieces of rows
+void place(reach::Args& a, void* workspace) {
   char* p = static_cast<char*>(workspace);
   a.pref = reinterpret_cast<int64_t*>(p);
   a.parts = reinterpret_cast<float*>(p + reach_stream_pref_bytes());
-  return p + reach_stream_pref_bytes() + reach_stream_parts_bytes(a.D);
+}
+int64_t piece_bytes(int64_t rows, int Hq, int D) {  // of one piece of all rows
+  return rows * Hq * (D + 2) * int64_t(sizeof(float));
+}
+// Room for the prefix's pieces: one of all rows, and as many as bring its items onto all compute units
+int64_t prefix_bytes(int64_t rows, int Hq, int D) {
+  return std::max(piece_bytes(rows, Hq, D), piece_bytes(PREFIX_ROWS, 1, D));
+}
+
+// Whether n sequences (groups) have rows enough for tiles in LDS
+bool tiled(const reach::Args& a, int dtype, int64_t n) {
+  return reach_tiles_shape(a, dtype) && a.rows * a.G >= TILE_ROWS * n;
+}
+// Tiles for the sequences of a call, with pieces in `bytes` from dst on
+int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t bytes, hipStream_t s) {
+  const int cuts = reach_tiles_cuts(a, tokens, bytes / piece_bytes(a.rows, a.Hq, a.D));
+  a.dst = cuts > 1 ? dst : nullptr;
+  a.dst_cuts = cuts;
+  return launch_reach_tiles(a, dtype, cuts, s);
 }
 
 }  // namespace
@@ -116,6 +138,9 @@ extern "C" int pia_window_attention(void* out, const void* q, int64_t q_stride, 
   // tokens that an item walks: the sinks' and the window's, of the table's
   const int64_t tokens = std::min(bt_stride * page_size,
                                   int64_t(window) + sinks + std::min<int64_t>(total_q_rows, 16));
+  if (cu_q && tiled(a, dtype, num_seqs))
+    return tile_call(a, dtype, tokens, a.parts, reach_stream_parts_bytes(head_dim),
+                     as_stream(stream));
   return stream_call(a, dtype, tokens, as_stream(stream));
 }
 
@@ -123,9 +148,8 @@ extern "C" int64_t pia_prefix_attention_workspace_bytes(int64_t total_q_rows, in
                                                         int head_dim) {
   if (head_dim <= 0 || head_dim > 256 || head_dim % 16 || total_q_rows <= 0 || num_heads <= 0)
     return 0;
-  // the prefix's pieces of all rows behind the streaming kernel's
   return reach_stream_pref_bytes() + reach_stream_parts_bytes(head_dim) +
-         total_q_rows * num_heads * (head_dim + 2) * int64_t(sizeof(float));
+         prefix_bytes(total_q_rows, num_heads, head_dim);
 }
 
 extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
@@ -159,16 +183,27 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
   if (rc) return rc < 0 ? rc : 0;
   hipStream_t s = as_stream(stream);
   if (!streams(a, dtype)) return launch_reach_general(a, dtype, s);
-  float* rows = reinterpret_cast<float*>(place(a, workspace));
+  place(a, workspace);
+  const int64_t prefix_tokens = pt_stride * page_size, tokens = bt_stride * page_size;
+  const int64_t parts = reach_stream_parts_bytes(head_dim),
+                shared = prefix_bytes(total_q_rows, num_heads, head_dim);
+  // many rows of a sequence: they share their own keys' tiles too, and need no pieces
+  if (cu_q && tiled(a, dtype, num_seqs))
+    return tile_call(a, dtype, prefix_tokens + tokens, a.parts, parts + shared, s);
   if (some) {  // the prefix's part of all rows, then the rest
     reach::Args g = a;
     g.by_group = 1;
-    g.dst = rows;
+    g.dst = a.src = a.parts + parts / int64_t(sizeof(float));
     g.dst_cuts = 1;
-    rc = stream_call(g, dtype, pt_stride * page_size, s);
+    if (tiled(a, dtype, num_groups)) {
+      g.dst_cuts = reach_tiles_cuts(g, prefix_tokens,
+                                    shared / piece_bytes(total_q_rows, num_heads, head_dim));
+      rc = launch_reach_tiles(g, dtype, g.dst_cuts, s);
+    } else {
+      rc = stream_call(g, dtype, prefix_tokens, s);
+    }
     if (rc) return rc;
-    a.src = rows;
-    a.src_cuts = 1;
+    a.src_cuts = g.dst_cuts;
   }
-  return stream_call(a, dtype, bt_stride * page_size, s);
+  return stream_call(a, dtype, tokens, s);
 }
