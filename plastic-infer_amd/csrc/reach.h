@@ -35,11 +35,14 @@ struct Args {
   int whole;         // no item is cut
   float* parts;      // pieces of items, by wave
   int64_t* pref;
-  // Pieces of rows, for rows * Hq of them: unnormalised outputs [cuts, rows * Hq, D], then (reference
-  // point in log2 units, sum) [cuts, rows * Hq]. dst: where results go instead of out; src: the
-  // prefix's, to be joined with what the kernel has.
-  float *dst, *src;
-  int dst_cuts, src_cuts;
+  // Pieces of rows: unnormalised outputs [n, rows * Hq, D] and (reference point in log2 units, sum)
+  // [n, rows * Hq]. dst: where results go instead of out; src: src_cuts pieces of the prefix and behind
+  // them one of the rest.
+  float* dst;
+  float2* dst_ml;
+  const float* src;
+  const float2* src_ml;
+  int src_cuts;
 };
 
 // tokens of a table that are there

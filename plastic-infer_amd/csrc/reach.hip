@@ -87,9 +87,10 @@ void place(reach::Args& a, void* workspace) {
 int64_t piece_bytes(int64_t rows, int Hq, int D) {  // of one piece of all rows
   return rows * Hq * (D + 2) * int64_t(sizeof(float));
 }
-// Room for the prefix's pieces: one of all rows, and as many as bring its items onto all compute units
+// Room for pieces of the prefix and one of the rest: two of all rows, or as many as bring the prefix's
+// items onto all compute units
 int64_t prefix_bytes(int64_t rows, int Hq, int D) {
-  return std::max(piece_bytes(rows, Hq, D), piece_bytes(PREFIX_ROWS, 1, D));
+  return std::max(2 * piece_bytes(rows, Hq, D), piece_bytes(PREFIX_ROWS, 1, D));
 }
 
 // Whether n sequences (groups) have rows enough for tiles in LDS
@@ -100,7 +101,7 @@ bool tiled(const reach::Args& a, int dtype, int64_t n) {
 int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t bytes, hipStream_t s) {
   const int cuts = reach_tiles_cuts(a, tokens, bytes / piece_bytes(a.rows, a.Hq, a.D));
   a.dst = cuts > 1 ? dst : nullptr;
-  a.dst_cuts = cuts;
+  a.dst_ml = reinterpret_cast<float2*>(dst + cuts * a.rows * a.Hq * a.D);
   return launch_reach_tiles(a, dtype, cuts, s);
 }
 
@@ -193,17 +194,20 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
   if (some) {  // the prefix's part of all rows, then the rest
     reach::Args g = a;
     g.by_group = 1;
-    g.dst = a.src = a.parts + parts / int64_t(sizeof(float));
-    g.dst_cuts = 1;
-    if (tiled(a, dtype, num_groups)) {
-      g.dst_cuts = reach_tiles_cuts(g, prefix_tokens,
-                                    shared / piece_bytes(total_q_rows, num_heads, head_dim));
-      rc = launch_reach_tiles(g, dtype, g.dst_cuts, s);
-    } else {
-      rc = stream_call(g, dtype, prefix_tokens, s);
-    }
+    const bool tiles = tiled(a, dtype, num_groups);
+    const int64_t R = total_q_rows * num_heads;
+    const int cuts =
+        !tiles ? 1 : reach_tiles_cuts(g, prefix_tokens,
+                                      shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
+    g.dst = a.parts + parts / int64_t(sizeof(float));
+    g.dst_ml = reinterpret_cast<float2*>(g.dst + (cuts + 1) * R * head_dim);
+    rc = tiles ? launch_reach_tiles(g, dtype, cuts, s) : stream_call(g, dtype, prefix_tokens, s);
     if (rc) return rc;
-    a.src_cuts = g.dst_cuts;
+    a.src = g.dst;
+    a.src_ml = g.dst_ml;
+    a.src_cuts = cuts;
+    a.dst = g.dst + cuts * R * head_dim;
+    a.dst_ml = g.dst_ml + cuts * R;
   }
   return stream_call(a, dtype, tokens, s);
 }

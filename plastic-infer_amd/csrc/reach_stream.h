@@ -207,33 +207,12 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     for (int w = 0; w < WG_WAVES; ++w) carry += wsum[w];
     __syncthreads();
   }
-  if (blockIdx.x == 0 && !a.whole)  // for the kernel that joins the pieces
+  if (blockIdx.x == 0 && (a.src || !a.whole))  // for the kernel that joins the pieces
     for (int b = threadIdx.x; b <= a.count; b += NTH) a.pref[b] = pref[b];
   const int64_t total = carry;
-  const int64_t R = a.rows * a.Hq;
-
-  // what a lane has of row `row` and q head `head`, elements 16 nb + 4 kd + j: joined with the prefix's
-  // pieces and written
-  auto finish = [&](f32x4_t (&o)[NB], float m, float l, int64_t row, int head, bool prefix) {
+  // what a lane has of row `row` and q head `head`, elements 16 nb + 4 kd + j
+  auto finish = [&](f32x4_t (&o)[NB], float m, float l, int64_t row, int head) {
     const int64_t at = row * a.Hq + head;
-    if (prefix) {
-      const float2* ml = reinterpret_cast<const float2*>(a.src + a.src_cuts * R * D);
-      for (int c = 0; c < a.src_cuts; ++c) {
-        const float2 x = ml[c * R + at];
-        const float to = __builtin_elementwise_maximum(m, x.x);
-        const float f0 = reach::weight(m, to), f = reach::weight(x.x, to);
-        const float* p = a.src + (c * R + at) * D + 4 * kd;
-        l = l * f0 + x.y * f;
-        m = to;
-#pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          if (!FULL && 16 * nb >= D) continue;
-          const float4 y = *reinterpret_cast<const float4*>(p + 16 * nb);
-          o[nb] = f32x4_t{fmaf(y.x, f, o[nb][0] * f0), fmaf(y.y, f, o[nb][1] * f0),
-                          fmaf(y.z, f, o[nb][2] * f0), fmaf(y.w, f, o[nb][3] * f0)};
-        }
-      }
-    }
     if (a.dst) {
       float* p = a.dst + at * D + 4 * kd;
 #pragma unroll
@@ -241,7 +220,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
         if (FULL || 16 * nb < D)
           *reinterpret_cast<float4*>(p + 16 * nb) =
               make_float4(o[nb][0], o[nb][1], o[nb][2], o[nb][3]);
-      if (kd == 0) reinterpret_cast<float2*>(a.dst + a.dst_cuts * R * D)[at] = make_float2(m, l);
+      if (kd == 0) a.dst_ml[at] = make_float2(m, l);
       return;
     }
     T* out = static_cast<T*>(a.out) + at * D + 4 * kd;
@@ -253,17 +232,16 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       }
   };
   f32x4_t acc[NB];
-  if (a.whole) {  // nothing will be joined: rows of sequences without steps, 16 at a time
+  if (a.whole && !a.src) {  // nothing will be joined: rows of sequences without steps, 16 at a time
     for (int b = blockIdx.x; b < a.count; b += gridDim.x) {
       if (pref[b + 1] != pref[b]) continue;
       const int4 s = seqs[b];
-      const bool prefix = a.src && reach::has_prefix(a, a.first + b);
       const int64_t n = int64_t(s.y) * a.Hq;
       for (int64_t r = wave * 16 + n16; r < n; r += 16 * WG_WAVES) {
         const int64_t pos = r / a.Hq;
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) acc[nb] = f32x4_t{0.f, 0.f, 0.f, 0.f};
-        finish(acc, -INFINITY, 0.f, s.x + pos, int(r - pos * a.Hq), prefix);
+        finish(acc, -INFINITY, 0.f, s.x + pos, int(r - pos * a.Hq));
       }
     }
   }
@@ -421,7 +399,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
   int lim = 0, lo = 0, hs = 0, lim_all = 0, lo_all = 0, hs_all = 0, lim_any = 0, lo_any = 0, hs_any = 0;
   int64_t row = 0;
   int head = 0;
-  bool live = false, prefix = false;
+  bool live = false;
   float m = -INFINITY, l = 0.f;
   bool opened = false;
   int begun = 0;  // step of the range at which the item began
@@ -439,7 +417,6 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       live = n16 < rows_left;
       row = s.row0 + (live ? pos : 0);
       head = cur.h * a.G + (live ? r - pos * a.G : 0);
-      prefix = a.src && reach::has_prefix(a, a.first + cur.b);
       const int p0 = 16 * cur.i / a.G, p1 = min((16 * cur.i + 15) / a.G, s.n - 1);
       lim_all = reach::limit(s, p0);
       lim_any = reach::limit(s, p1);
@@ -689,7 +666,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     if (cur.t + 1 == cur.steps || x + 1 == count) {
       const float lsum = tile32::sum_col4(l), mr = m == -INFINITY ? m : m - SHIFT<DT>;
       if (cur.t + 1 == cur.steps && cur.t == x - begun) {
-        if (live) finish(acc, mr, lsum, row, head, prefix);
+        if (live) finish(acc, mr, lsum, row, head);
       } else {
         float* part = a.parts + (w * 2 + (begun == 0 ? 0 : 1)) * part_floats<DP>;
         if (live) {
@@ -712,9 +689,10 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
   }
 }
 
-// The items that were cut: their pieces joined, in the order of the waves, and the prefix's behind them. A
+// The items that were cut: their pieces joined, in the order of the waves. Behind a prefix all items, which
+// are pieces of rows where they were not cut (the one behind the prefix's), joined with the prefix's. A
 // workgroup has rows_per_wg rows of an item, all of them or, where there are few items with many pieces,
-// one. Items without keys of their own are the prefix's, or zeros.
+// one. Items without keys are zeros.
 template <int DT, int DP>
 __global__ __launch_bounds__(JOIN_FEW) void reach_stream_join_kernel(Args a, int64_t waves,
                                                                      int rows_per_wg) {
@@ -756,20 +734,25 @@ __global__ __launch_bounds__(JOIN_FEW) void reach_stream_join_kernel(Args a, int
   const int64_t total = a.pref[a.count], nw = min(waves, total), R = a.rows * a.Hq;
   const int64_t from = a.pref[b] + (int64_t(h) * items_of(s.n, a.G) + i) * steps, to = from + steps;
   int64_t w0 = 0, w1 = 0;
-  if (steps > 0) {
+  bool cut = false;
+  if (steps > 0 && !a.whole) {
     w0 = wave_of(from, nw, total);
     w1 = wave_of(to - 1, nw, total);
-    if (w0 == w1) return;  // finished by its wave
+    cut = w0 != w1;
   }
-  const bool prefix = a.src && reach::has_prefix(a, a.first + b);
+  if (steps > 0 && !cut && !a.src) return;  // finished by its wave
   const float* first =
-      a.parts + (w0 * 2 + (steps > 0 && first_of(w0, nw, total) >= from ? 0 : 1)) * part_floats<DP>;
+      a.parts + (w0 * 2 + (cut && first_of(w0, nw, total) >= from ? 0 : 1)) * part_floats<DP>;
+  // pieces of rows: the prefix's, and the item's own where it was not cut
+  const int own = steps > 0 && !cut ? 1 : 0;
+  const int c0 = a.src && reach::has_prefix(a, a.first + b) ? 0 : a.src_cuts,
+            c1 = a.src ? a.src_cuts + own : 0;
   // S lanes in a row have four elements u of the item (row r, elements d .. d + 3) and every S-th piece
   // each, eight of them on their way at once; they meet by exchanges, in a fixed order.
   const int per_row = a.D / 4, U = rows * per_row, np = int(w1 - w0) + 1;
   const int threads = blockDim.x;
   int S = 1;
-  while (S < 64 && 2 * S * U <= threads && 16 * S < np && steps > 0) S *= 2;
+  while (S < 64 && 2 * S * U <= threads && 16 * S < np && cut) S *= 2;
   const int sp = threadIdx.x & (S - 1);
   for (int u0 = 0; u0 < U; u0 += threads / S) {
     const int u = u0 + int(threadIdx.x) / S, rl = u / per_row, r = r0 + rl, d = 4 * (u - rl * per_row);
@@ -784,7 +767,7 @@ __global__ __launch_bounds__(JOIN_FEW) void reach_stream_join_kernel(Args a, int
                       fmaf(x.w, f, o.w * f0));
       M = to;
     };
-    if (steps > 0) {
+    if (cut) {
       constexpr int N = 8;
       for (int p0 = sp; p0 < np; p0 += N * S) {
         float pm[N], pl[N];
@@ -820,14 +803,25 @@ __global__ __launch_bounds__(JOIN_FEW) void reach_stream_join_kernel(Args a, int
     if (sp) continue;
     const int rr = 16 * i + r, pos = rr / a.G;
     const int64_t at = (s.row0 + pos) * a.Hq + h * a.G + rr - pos * a.G;
-    if (prefix)
-      for (int c = 0; c < a.src_cuts; ++c) {
-        const float2 x = reinterpret_cast<const float2*>(a.src + a.src_cuts * R * a.D)[c * R + at];
-        add(x.x, x.y, *reinterpret_cast<const float4*>(a.src + (c * R + at) * a.D + d));
+    if (c0 < c1) {
+      constexpr int N = 8;  // on their way at once
+      for (int p0 = c0; p0 < c1; p0 += N) {
+        float2 pm[N];
+        float4 po[N];
+#pragma unroll
+        for (int j = 0; j < N; ++j) {
+          const int64_t c = min(p0 + j, c1 - 1) * R + at;
+          pm[j] = a.src_ml[c];
+          po[j] = *reinterpret_cast<const float4*>(a.src + c * a.D + d);
+        }
+#pragma unroll
+        for (int j = 0; j < N; ++j)
+          if (p0 + j < c1) add(pm[j].x, pm[j].y, po[j]);
       }
-    if (a.dst) {
+    }
+    if (a.dst && !a.src) {
       *reinterpret_cast<float4*>(a.dst + at * a.D + d) = o;
-      if (d == 0) reinterpret_cast<float2*>(a.dst + a.dst_cuts * R * a.D)[at] = make_float2(M, L);
+      if (d == 0) a.dst_ml[at] = make_float2(M, L);
       continue;
     }
     const float x[4] = {o.x, o.y, o.z, o.w};
@@ -849,7 +843,7 @@ void launch_shape(const Args& a, int64_t items, bool alike, hipStream_t s) {
     if (full) PIA_RS(false, true); else PIA_RS(false, false);
   }
 #undef PIA_RS
-  if (a.whole) return;
+  if (a.whole && !a.src) return;
   // few items: many pieces each, which many threads share, on every compute unit; many: two or three
   const bool few = items * 4 <= resident_waves();
   const int rows = a.cu || a.by_group ? 16 : std::min(a.G, 16);

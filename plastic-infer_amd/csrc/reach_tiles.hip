@@ -179,14 +179,19 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   kt0 = __builtin_amdgcn_readfirstlane(kt0);
   nkt = __builtin_amdgcn_readfirstlane(nkt);
 
-  // this lane's row
+  // this lane's row; what it sees is made where it is used, on the tiles that not all rows see whole
   const int D = a.D;
   const int hh = lane >> 5, n32 = lane & 31, G = a.G;
-  const int r = 32 * wave + n32, pos = s0 + r / G;
-  const bool live = r < a.ppt * G && pos < s.n;
-  const int lim = live ? reach::limit(s, pos) : 0;
-  const int lo = live ? reach::lowest(a, s, pos) : 0;
-  const int hs = !live ? 0 : a.window ? min(head, lim) : head;
+  struct Row {
+    int r, pos;
+    bool live;
+  };
+  auto row_now = [&]() {
+    int x = lane & 31;
+    asm volatile("" : "+v"(x));
+    const int r = 32 * wave + x, pos = s0 + r / G;
+    return Row{r, pos, r < a.ppt * G && pos < s.n};
+  };
 
   // q through LDS: element NU e + u of a row to unit u, place e
   uint4 qr[KS];
@@ -212,7 +217,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     }
     __syncthreads();
 #pragma unroll
-    for (int k = 0; k < KS; ++k) qr[k] = *reinterpret_cast<const uint4*>(lds + q_at(r, 2 * k + hh));
+    for (int k = 0; k < KS; ++k)
+      qr[k] = *reinterpret_cast<const uint4*>(lds + q_at(32 * wave + n32, 2 * k + hh));
     __syncthreads();
   }
 
@@ -234,17 +240,20 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     auto first = [](int n) { return (1u << min(max(n, 0), 8)) - 1u; };
     return (first(x.to - t) & ~first(x.from - t)) | first(x.below - t);
   };
+  auto reach_of_row = [&](int it) {
+    const Row x = row_now();
+    const int lim = reach::limit(s, x.pos);
+    const Reach y = reach_of(it, reach::lowest(a, s, x.pos), lim, a.window ? min(head, lim) : head);
+    return x.live ? y : Reach{0, 0, 0};
+  };
   // whether every row sees all of a tile (of the blocks that are there)
   auto seen_whole = [&](int it) {
     const Reach x = reach_of(it, lo_all, lim_all, hs_all);
     return x.below >= RT_KT || (x.from <= 0 && x.to >= RT_KT);
   };
-  // Pages of the blocks of a tile in lanes 0 .. 3 (-1 where no row sees any of it) and the blocks' places
-  // in them. The ids are as loaded: what is made of them is made where they are used, tiles later, so
-  // that no tile waits for them (and with them for every load before).
-  struct Where {
-    int id, sub;
-  };
+  // Pages of the blocks of a tile in lanes 0 .. 3 (-1 where no row sees any of it). The ids are as
+  // loaded: what is made of them is made where they are used, tiles later, so that no tile waits for them
+  // (and with them for every load before).
   const uint32_t np = uint32_t(a.num_pages);
   const int PB = a.P / 16;
   auto where = [&](int it) {
@@ -252,9 +261,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     const int t = 16 * lane, kb = (first_token(it) >> 4) + lane, slot = PB == 1 ? kb : kb / PB;
     const bool in = (it < nkt) & (lane < 4) &
                     (((t + 16 > x.from) & (t < x.to)) | (t < x.below));
-    Where w{-1, kb - slot * PB};
-    if (in) w.id = (in_head(it) ? head_table : own)[slot];
-    return w;
+    int id = -1;
+    if (in) id = (in_head(it) ? head_table : own)[slot];
+    return id;
   };
 
   // staging: wave w (of four) moves block w of a tile
@@ -270,27 +279,39 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   // V: lanes 8 c + 2 x + half take row c % 4 + 4 x + 16 (c / 4), and those 32 on
   const int vd = ((lane >> 3) & 3) + 4 * ((lane >> 1) & 3) + 16 * (lane >> 5), vh = lane & 1;
   const uint32_t v_off = uint32_t(vd) * row_bytes + 16 * vh;
+  // where they go: K's first token (bits 2 and 3 of the token exchanged), V's first row
+  const int k_tok = TL * tg, k_row = 16 * blk + ((k_tok & 3) | ((k_tok & 4) << 1) | ((k_tok & 8) >> 1));
+  const uint32_t k_st = k_row * UK * 16 + 16 * (du ^ (DP > 64 ? k_row & 15 : (k_row >> 1) & 7));
+  const uint32_t v_st = 2 * K_BUF + vd * 128 + 16 * ((2 * blk + vh) ^ ((vd >> 1) & 7));
   const int tile_bytes = D * a.P * 2;
   const int64_t page_bytes = int64_t(tile_bytes) * a.Hkv;
   const char* kp = static_cast<const char*>(a.kp) + int64_t(h) * tile_bytes;
   const char* vp = static_cast<const char*>(a.vp) + int64_t(h) * tile_bytes;
-  auto rsrc = [&](const char* pool, const Where& w) {
-    const int id = __builtin_amdgcn_readlane(w.id, blk), sub = __builtin_amdgcn_readlane(w.sub, blk);
+  auto rsrc = [&](const char* pool, int ids, int it) {
+    const int id = __builtin_amdgcn_readlane(ids, blk), kb = (first_token(it) >> 4) + blk;
+    const int sub = PB == 1 ? 0 : kb % PB;
     const bool ok = uint32_t(id) < np;
     // elements behind head_dim lie past the descriptor's end, and are zeros
     return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pool) + (ok ? id : 0) * page_bytes + sub * 32,
                                              0, ok ? tile_bytes - sub * 32 : 0, RT_RSRC_WORD3);
+  };
+  // a lane's term, hidden, so that what is added to it is added at its use: kept for all uses, the sums were
+  // spilled, and a wait for a spilled register is one for every load before it
+  auto now = [](uint32_t x) {
+    asm volatile("" : "+v"(x));
+    return x;
   };
   // word i of a part (a constant)
   auto word = [](Part& p, int i) -> uint32_t& {
     uint4& x = p.x[i >> 2];
     return (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
   };
-  auto fetch_k = [&](Part& p, const Where& w) {
-    const auto rs = rsrc(kp, w);
+  auto fetch_k = [&](Part& p, int ids, int it) {
+    const auto rs = rsrc(kp, ids, it);
+    const uint32_t o = now(k_off);
 #pragma unroll
     for (int e = 0; e < KL; ++e) {
-      const uint32_t at = k_off + uint32_t(e * NU) * row_bytes;
+      const uint32_t at = o + uint32_t(e * NU) * row_bytes;
       if constexpr (TL == 4) {
         const auto y = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
         word(p, 2 * e) = y[0];
@@ -300,16 +321,18 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       }
     }
   };
-  auto fetch_v = [&](Part& p, const Where& w) {
-    const auto rs = rsrc(vp, w);
+  auto fetch_v = [&](Part& p, int ids, int it) {
+    const auto rs = rsrc(vp, ids, it);
+    const uint32_t o = now(v_off);
 #pragma unroll
     for (int i = 0; i < VL; ++i)
       p.x[i] = __builtin_bit_cast(
-          uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, v_off + uint32_t(32 * i) * row_bytes, 0, 0));
+          uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + uint32_t(32 * i) * row_bytes, 0, 0));
   };
   auto put = [&](uint32_t at, const uint4& x) { *reinterpret_cast<uint4*>(lds + at) = x; };
   auto stage_k = [&](Part& p, int buf) {
     if (!k_lane) return;
+    const uint32_t o = now(k_st) + buf * K_BUF;
 #pragma unroll
     for (int t = 0; t < TL; ++t) {
       uint32_t w[4];
@@ -318,10 +341,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
         w[f] = __builtin_amdgcn_perm(word(p, (2 * f + 1) * (TL / 2) + (t >> 1)),
                                      word(p, 2 * f * (TL / 2) + (t >> 1)),
                                      (t & 1) ? 0x07060302u : 0x05040100u);
-      const int tok = TL * tg + t;  // bits 2 and 3 exchanged
-      const int row = 16 * blk + ((tok & 3) | ((tok & 4) << 1) | ((tok & 8) >> 1));
-      put(buf * K_BUF + row * UK * 16 + 16 * (du ^ (DP > 64 ? row & 15 : (row >> 1) & 7)),
-          make_uint4(w[0], w[1], w[2], w[3]));
+      // row t on, whose swizzle differs by t (DP 64: by none)
+      put(((o ^ (DP > 64 ? 16 * t : 0)) + t * UK * 16), make_uint4(w[0], w[1], w[2], w[3]));
     }
   };
   // kind 0: V itself, but zeros for what is not finite on tiles that some row does not see whole (zero
@@ -352,11 +373,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       }
       if (odd) odd_seen = 1;
     }
+    const uint32_t o = now(v_st) + buf * V_BUF;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) {
-      const int d = vd + 32 * i;
-      put(2 * K_BUF + buf * V_BUF + d * 128 + 16 * ((2 * blk + vh) ^ ((d >> 1) & 7)), p.x[i]);
-    }
+    for (int i = 0; i < VL; ++i) put(o + 4096 * i, p.x[i]);
   };
   // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
   // bits enter by XOR, so one base per lane and a constant give any of them
@@ -397,7 +416,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     return mx;
   };
   auto hide = [&](f32x16_t (&sc)[2], int it, int there) {  // what the row may not see
-    const Reach x = reach_of(it, lo, lim, hs);
+    const Reach x = reach_of_row(it);
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
@@ -469,39 +488,33 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       // never 0, which an infinite V would make NaN
       if (__ballot(least < RT_LEAST_HALF)) {
         typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
-        uint4 rest[4];
-        bool any = false;
 #pragma unroll
         for (int s4 = 0; s4 < 4; ++s4) {
-          uint32_t* w = &pk[s4].x;
-          uint32_t* z = &rest[s4].x;
+          __builtin_amdgcn_sched_barrier(0);  // one operand at a time (registers)
+          uint32_t z[4];
+          uint32_t any = 0;
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            float x[2];
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const float p = sc[s4 >> 1][8 * (s4 & 1) + 2 * i + e];
-              const float q16 = half_to_f32(uint16_t(w[i] >> (16 * e)));
-              x[e] = p > 0.f && p < RT_LEAST_HALF ? (p - q16) * RT_REST : 0.f;
-              any |= x[e] != 0.f;
-            }
-            z[i] = tile::pack16x2<DT>(x[0], x[1]);
+            uint32_t& w = i == 0 ? pk[s4].x : i == 1 ? pk[s4].y : i == 2 ? pk[s4].z : pk[s4].w;
+            const float p0 = sc[s4 >> 1][8 * (s4 & 1) + 2 * i], p1 = sc[s4 >> 1][8 * (s4 & 1) + 2 * i + 1];
+            const float x0 = (p0 - half_to_f32(uint16_t(w))) * RT_REST;
+            const float x1 = (p1 - half_to_f32(uint16_t(w >> 16))) * RT_REST;
+            z[i] = tile::pack16x2<DT>(p0 < RT_LEAST_HALF ? x0 : 0.f, p1 < RT_LEAST_HALF ? x1 : 0.f);
+            any |= z[i] & 0x7fff7fffu;
             const uint32_t low =
-                min(__float_as_uint(sc[s4 >> 1][8 * (s4 & 1) + 2 * i]), 1u) |
-                (min(__float_as_uint(sc[s4 >> 1][8 * (s4 & 1) + 2 * i + 1]), 1u) << 16);
-            w[i] = __builtin_bit_cast(
-                uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w[i]),
-                                                    __builtin_bit_cast(u16x2_t, low)));
+                min(__float_as_uint(p0), 1u) | (min(__float_as_uint(p1), 1u) << 16);
+            w = __builtin_bit_cast(uint32_t,
+                                   __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w),
+                                                             __builtin_bit_cast(u16x2_t, low)));
           }
-        }
-        if (__ballot(any)) {
+          if (!__ballot(any != 0)) continue;
 #pragma unroll
           for (int nb = 0; nb < NB; ++nb) {
+            __builtin_amdgcn_sched_barrier(0);
             f32x16_t t;
 #pragma unroll
             for (int v = 0; v < 16; ++v) t[v] = 0.f;
-#pragma unroll
-            for (int s4 = 0; s4 < 4; ++s4) t = mfma32<DT>(vread(buf, nb, s4), rest[s4], t);
+            t = mfma32<DT>(vread(buf, nb, s4), make_uint4(z[0], z[1], z[2], z[3]), t);
 #pragma unroll
             for (int v = 0; v < 16; ++v) {
               // an infinite V enters by the first terms alone
@@ -529,14 +542,15 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   // each, what a tile stages replaces what the tile before it has read, with a barrier between.
   const bool first4 = wave < 4;
   Part pa, pb;  // SPLIT: K or V in pa; else K in pa, V in pb
-  Where w0 = where(kt0), w1 = where(kt0 + 1), w2 = where(kt0 + 2), w3 = where(kt0 + 3);
-  auto fetch = [&](const Where& wk, const Where& wv) {
+  int w0 = where(kt0), w1 = where(kt0 + 1), w2 = where(kt0 + 2), w3 = where(kt0 + 3);
+  // K of tile it_k and V of the one before (with eight waves a wave has one of them)
+  auto fetch = [&](int wk, int wv, int it_k) {
     if constexpr (SPLIT) {
-      if (first4) fetch_k(pa, wk);
-      else fetch_v(pa, wv);
+      if (first4) fetch_k(pa, wk, it_k);
+      else fetch_v(pa, wv, it_k - 1);
     } else {
-      fetch_k(pa, wk);
-      fetch_v(pb, wv);
+      fetch_k(pa, wk, it_k);
+      fetch_v(pb, wv, it_k - 1);
     }
   };
   auto stage = [&](int buf_k, int buf_v, int it_v) {
@@ -548,23 +562,23 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       stage_v(pb, buf_v, it_v, 0);
     }
   };
-  fetch(w0, w0);
-  stage(0, 0, kt0);
-  if (!SPLIT || first4) {  // K of the second tile; the other waves have nothing of it
-    fetch_k(pa, w1);
-    stage_k(pa, 1);
+  fetch(w1, w0, kt0 + 1);
+  stage(1, 0, kt0);
+  if (!SPLIT || first4) {  // K of the first tile; the other waves have nothing of it
+    fetch_k(pa, w0, kt0);
+    stage_k(pa, 0);
   }
-  fetch(w2, w1);
+  fetch(w2, w1, kt0 + 2);
   __syncthreads();
   f32x16_t sa[2], sb[2];
   scores(sa, 0);
   float mx = largest(sa);
   auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int it, int buf) {
-    const int there = int(__ballot(lane < 4 && uint32_t(w0.id) < np)) & 0xf;
-    const Where w4 = where(it + 4);
+    const int there = int(__ballot(lane < 4 && uint32_t(w0) < np)) & 0xf;
+    const int w4 = where(it + 4);
     turn(sc, sn, mx, it, buf, there);
     stage(buf, buf ^ 1, it + 1);
-    fetch(w3, w2);
+    fetch(w3, w2, it + 3);
     __syncthreads();
     w0 = w1;
     w1 = w2;
@@ -581,14 +595,14 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
 #pragma unroll 1
     for (int it = kt0; it < nkt; ++it) {
       if (seen_whole(it)) continue;
-      const Where w = where(it);
-      const int there = int(__ballot(lane < 4 && uint32_t(w.id) < np)) & 0xf;
-      const Reach x = reach_of(it, lo, lim, hs);
+      const int w = where(it);
+      const int there = int(__ballot(lane < 4 && uint32_t(w) < np)) & 0xf;
+      const Reach x = reach_of_row(it);
 #pragma unroll 1
       for (int kind = 1; kind <= 3; ++kind) {
         __syncthreads();
         if (!SPLIT || !first4) {
-          fetch_v(SPLIT ? pa : pb, w);
+          fetch_v(SPLIT ? pa : pb, w, it);
           stage_v(SPLIT ? pa : pb, 0, it, kind);
         }
         __syncthreads();
@@ -617,8 +631,9 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   }
 
   l += swap_halves(l);
-  if (!live) return;
-  const int64_t at = (row0 + pos) * a.Hq + h * G + r % G, R = a.rows * a.Hq;
+  const Row own_row = row_now();
+  if (!own_row.live) return;
+  const int64_t at = (row0 + own_row.pos) * a.Hq + h * G + own_row.r % G, R = a.rows * a.Hq;
   if (a.dst) {  // the piece as it is, to be joined: its outputs, then its reference and sum
     float* o = a.dst + (piece * R + at) * D + 4 * hh;
 #pragma unroll
@@ -629,7 +644,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
           *reinterpret_cast<float4*>(o + 32 * nb + 8 * i) = make_float4(
               acc[nb][4 * i], acc[nb][4 * i + 1], acc[nb][4 * i + 2], acc[nb][4 * i + 3]);
     if (hh == 0)
-      reinterpret_cast<float2*>(a.dst + a.dst_cuts * R * D)[piece * R + at] =
+      a.dst_ml[piece * R + at] =
           make_float2(m == -INFINITY ? m : m * a.scale_log2 - RT_SHIFT<DT>, l);
     return;
   }
@@ -658,7 +673,6 @@ __global__ __launch_bounds__(256) void reach_tiles_join_kernel(TileArgs a) {
   const int d = 4 * int(x - at * (D / 4));
   const int64_t row = at / a.Hq;
   if (at >= R || row < a.cu[a.first] || row >= a.cu[a.first + a.count]) return;
-  const float2* ml = reinterpret_cast<const float2*>(a.dst + a.cuts * R * D);
   float M = -INFINITY, L = 0.f;
   float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
   constexpr int N = 4;  // pieces on their way at once; past the end: the last again, without weight
@@ -668,7 +682,7 @@ __global__ __launch_bounds__(256) void reach_tiles_join_kernel(TileArgs a) {
 #pragma unroll
     for (int k = 0; k < N; ++k) {
       const int64_t i = min(p0 + k, a.cuts - 1) * R + at;
-      pm[k] = ml[i];
+      pm[k] = a.dst_ml[i];
       po[k] = *reinterpret_cast<const float4*>(a.dst + i * D + d);
     }
 #pragma unroll
