@@ -33,6 +33,9 @@ struct Args {
   int first, count;  // the sequences (by_group: groups) of a launch
   int by_group;      // a "sequence" is a group: all its rows, over its prefix
   int whole;         // no item is cut
+  int splits;        // workgroups of an item; 0: none are an item's
+  unsigned long long* counters;  // of an item's workgroups, and the launch's token in them
+  unsigned long long token;
   float* parts;      // pieces of items, by wave
   int64_t* pref;
   // Pieces of rows: unnormalised outputs [n, rows * Hq, D] and (reference point in log2 units, sum)
@@ -128,6 +131,8 @@ int launch_reach_stream_bf16(const reach::Args& a, int64_t tokens, hipStream_t s
 bool reach_tiles_shape(const reach::Args& a, int dtype);
 int reach_tiles_cuts(const reach::Args& a, int64_t tokens, int64_t most);
 int launch_reach_tiles(const reach::Args& a, int dtype, int cuts, hipStream_t s);
+// a number that no other launch has, in the upper 48 bits
+unsigned long long reach_token();
 // bytes of the streaming kernel's pieces by wave, and of the numbers before them
 int64_t reach_stream_parts_bytes(int D);
 int64_t reach_stream_pref_bytes();

@@ -1,6 +1,8 @@
 // Entry points of windowed attention and of attention behind a shared prefix: checks of the arguments
 // and the choice of a kernel.
 #include <algorithm>
+#include <atomic>
+#include <random>
 
 #include "reach.h"
 
@@ -106,6 +108,15 @@ int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t byte
 }
 
 }  // namespace
+
+unsigned long long reach_token() {
+  static std::atomic<unsigned long long> next{[] {
+    std::random_device r;
+    return (static_cast<unsigned long long>(r()) << 32) | r();
+  }()};
+  return next.fetch_add(1, std::memory_order_relaxed) << 16;
+}
+
 }  // namespace pia
 
 using namespace pia;

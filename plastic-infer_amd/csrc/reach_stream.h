@@ -46,6 +46,8 @@ constexpr int WG_WAVES = 4;
 constexpr int WGS_PER_CU = 2;   // two waves per SIMD
 constexpr int WHOLE = 3;        // steps of items that are not cut
 constexpr float RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
+constexpr int MAX_SPLITS = 64;  // workgroups of an item
+constexpr int ITEM_STEPS = 8;   // steps of a wave above which even ranges for all waves are better
 constexpr int JOIN_MANY = 128, JOIN_FEW = 512;  // threads of the joining workgroups
 
 // log2 of what probabilities are scaled by: fp16's terms then go down to 2^-32 of the largest
@@ -152,6 +154,37 @@ __device__ __forceinline__ Unit<UB> load_unit(const void* p) {
   return __builtin_bit_cast(Unit<UB>, v);
 }
 
+// Stores and loads of what workgroups on other XCDs read or wrote in this launch
+__device__ __forceinline__ void put_far(float* p, float v) {
+  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float get_far(const float* p) {
+  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+// Counts a workgroup in at its item's counter, which holds (token of the launch, arrivals); true for the last
+// of n. What it held before (another launch's, or anything) is replaced by whoever comes first. The last one
+// leaves it at no arrivals, for a graph that replays the launch with its token. 48 random bits of a token: what
+// an unused workspace holds is taken for it once in 2^48.
+__device__ __forceinline__ bool arrive(unsigned long long* counter, unsigned long long token, int n) {
+  unsigned long long seen =
+      __hip_atomic_load(counter, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  for (;;) {
+    const bool ours = (seen >> 16) == (token >> 16);
+    const unsigned long long to = ours ? seen + 1 : token + 1;
+    if (!ours) {
+      if (__hip_atomic_compare_exchange_strong(counter, &seen, to, __ATOMIC_RELAXED, __ATOMIC_RELAXED,
+                                               __HIP_MEMORY_SCOPE_AGENT))
+        return n == 1;
+      continue;  // another one of this launch put the token there
+    }
+    const unsigned long long before =
+        __hip_atomic_fetch_add(counter, 1ull, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    if (int(before & 0xffffu) + 1 < n) return false;
+    __hip_atomic_store(counter, token, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    return true;
+  }
+}
+
 // A row's four outputs o (of sum l), normalised
 template <int DT>
 __device__ __forceinline__ void store4(typename Elem<DT>::T* out, const float (&o)[4], float l) {
@@ -165,23 +198,83 @@ __device__ __forceinline__ void store4(typename Elem<DT>::T* out, const float (&
   *reinterpret_cast<Pack*>(out) = pk;
 }
 
-// ALIKE: all rows of an item see the same tokens. FULL: head_dim is DP.
-template <int DT, int DP, bool ALIKE, bool FULL>
+// ALIKE: all rows of an item see the same tokens. FULL: head_dim is DP. ITEM: a workgroup takes one of a.splits
+// runs of an item's steps, and the last of an item's workgroups joins them.
+template <int DT, int DP, bool ALIKE, bool FULL, bool ITEM>
 __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel(Args a) {
   using F = Form<DT, DP>;
   using T = typename F::T;
   constexpr int TU = F::TU, STEP = F::STEP, MB = F::MB, NI = F::NI, NB = F::NB, NU = F::NU;
-  constexpr int NTH = 64 * WG_WAVES;
+  constexpr int NW = WG_WAVES, NTH = 64 * NW;
   constexpr bool F32 = F::F32;
-  __shared__ int64_t pref[MAX_SEQS + 1];
-  __shared__ int4 seqs[MAX_SEQS];  // first row (below 2^30), rows, tokens, offset
-  __shared__ int64_t wsum[WG_WAVES];
-  __shared__ __align__(16) T qs[WG_WAVES][64 * F::QS];
-  __shared__ float ps[ALIKE ? 1 : WG_WAVES][ALIKE ? 1 : 16 * (STEP + 1)];
+  __shared__ int64_t pref[ITEM ? 1 : MAX_SEQS + 1];
+  __shared__ int4 seqs[ITEM ? 1 : MAX_SEQS];  // first row (below 2^30), rows, tokens, offset
+  __shared__ int64_t wsum[NW];
+  __shared__ __align__(16) T qs[ITEM ? 1 : NW][64 * F::QS];
+  __shared__ float ps[ALIKE ? 1 : NW][ALIKE ? 1 : 16 * (STEP + 1)];
+  // ITEM: items of the sequences before each; the waves' pieces
+  __shared__ int item_pref[ITEM ? MAX_SEQS + 1 : 1];
+  constexpr int RS = DP + 4;
+  __shared__ __align__(16) float red[ITEM ? NW * 16 * RS : 4];
+  __shared__ float red_m[ITEM ? NW * 16 : 1], red_l[ITEM ? NW * 16 : 1];
+  __shared__ int is_last;
   const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
   const int kd = lane >> 4, n16 = lane & 15;
   const int D = FULL ? DP : a.D;
 
+  // where a wave is: step t of item i of kv head h of sequence b; tiles nh .. of the item begin at t0
+  struct Cursor {
+    int b, h, i, t, items, steps, nh, t0, end;
+  };
+  int64_t total = 0;
+  Seq mine{};  // ITEM: the sequence
+  Cursor cur{};
+  int split = 0, item = 0;  // ITEM: which of the item's runs, and the item's number
+  if constexpr (ITEM) {
+    int j;
+    const unsigned id = blockIdx.x / unsigned(a.splits);
+    split = int(blockIdx.x - id * unsigned(a.splits));
+    if (a.cu || a.by_group) {
+      if (threadIdx.x == 0) item_pref[0] = 0;
+      int carry = 0;
+      for (int c0 = 0; c0 < a.count; c0 += NTH) {
+        const int b = c0 + threadIdx.x;
+        int incl = b < a.count ? items_of(seq_at(a, b).n, a.G) : 0;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+          const int y = __shfl_up(incl, o, 64);
+          if (lane >= o) incl += y;
+        }
+        if (lane == 63) wsum[wave] = incl;
+        __syncthreads();
+        int base = carry;
+        for (int w = 0; w < wave; ++w) base += int(wsum[w]);
+        if (b < a.count) item_pref[b + 1] = base + incl;
+#pragma unroll
+        for (int w = 0; w < NW; ++w) carry += int(wsum[w]);
+        __syncthreads();
+      }
+      if (!xcd_item(id, carry, a.Hkv, cur.h, j)) return;
+      int lo = 0, hi = a.count - 1;  // the last sequence with item_pref[b] <= j
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (item_pref[mid] <= j) lo = mid; else hi = mid - 1;
+      }
+      cur.b = uniform(lo);
+      cur.h = uniform(cur.h);
+      cur.i = uniform(item_pref[cur.b + 1] - 1 - j);  // the last rows first
+      item = uniform(j * a.Hkv + cur.h);
+    } else {
+      const unsigned ips = unsigned(a.G + 15) >> 4, k = id / ips;
+      cur.i = int(id - k * ips);
+      cur.b = int(k / unsigned(a.Hkv));
+      cur.h = int(k - unsigned(cur.b) * unsigned(a.Hkv));
+      if (cur.b >= a.count) return;
+      item = int(id);
+    }
+    mine = seq_at(a, cur.b);
+  }
+  if constexpr (!ITEM) {
   // steps of the sequences before each
   if (threadIdx.x == 0) pref[0] = 0;
   int64_t carry = 0;
@@ -209,7 +302,8 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
   }
   if (blockIdx.x == 0 && (a.src || !a.whole))  // for the kernel that joins the pieces
     for (int b = threadIdx.x; b <= a.count; b += NTH) a.pref[b] = pref[b];
-  const int64_t total = carry;
+  total = carry;
+  }
   // what a lane has of row `row` and q head `head`, elements 16 nb + 4 kd + j
   auto finish = [&](f32x4_t (&o)[NB], float m, float l, int64_t row, int head) {
     const int64_t at = row * a.Hq + head;
@@ -232,7 +326,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       }
   };
   f32x4_t acc[NB];
-  if (a.whole && !a.src) {  // nothing will be joined: rows of sequences without steps, 16 at a time
+  if (!ITEM && a.whole && !a.src) {  // nothing will be joined: rows of sequences without steps, 16 at a time
     for (int b = blockIdx.x; b < a.count; b += gridDim.x) {
       if (pref[b + 1] != pref[b]) continue;
       const int4 s = seqs[b];
@@ -245,9 +339,9 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       }
     }
   }
-  const int64_t nw = min(int64_t(gridDim.x) * WG_WAVES, total);
+  const int64_t nw = ITEM ? 1 : min(int64_t(gridDim.x) * WG_WAVES, total);
   const int64_t w = int64_t(wave) * gridDim.x + blockIdx.x;  // few steps: over all compute units
-  if (w >= nw) return;
+  if (!ITEM && w >= nw) return;
   auto seq_with = [&](int64_t x) {  // the last sequence that starts at or before x (and is not empty)
     int lo = 0, hi = a.count - 1;
     while (lo < hi) {
@@ -257,6 +351,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     return lo;
   };
   auto get = [&](int b) {
+    if constexpr (ITEM) return mine;
     const int4 x = seqs[b];
     Seq s;
     s.row0 = uniform(x.x);
@@ -266,8 +361,12 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     s.causal = !a.by_group && (a.offs || a.window);
     return s;
   };
-  int64_t x0 = first_of(w, nw, total), x1 = first_of(w + 1, nw, total);
-  if (a.whole) {  // the items that begin in the range
+  int64_t x0 = 0, x1 = 0;
+  if constexpr (!ITEM) {
+  x0 = first_of(w, nw, total);
+  x1 = first_of(w + 1, nw, total);
+  }
+  if (!ITEM && a.whole) {  // the items that begin in the range
     auto item_from = [&](int64_t x) {
       if (x >= total) return total;
       const int b = seq_with(x), steps = steps_of(a, get(b), STEP);
@@ -278,12 +377,8 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     x1 = item_from(x1);
     if (x0 >= x1) return;
   }
-  const int count = uniform(int(min(x1 - x0, int64_t(0x7fffffff))));
+  int count = uniform(int(min(x1 - x0, int64_t(0x7fffffff))));
 
-  // where a wave is: step t of item i of kv head h of sequence b; tiles nh .. of the item begin at t0
-  struct Cursor {
-    int b, h, i, t, items, steps, nh, t0, end;
-  };
   auto open = [&](Cursor& c) {
     const Seq s = get(c.b);
     c.t0 = a.window ? max(c.nh, reach::lowest(a, s, 16 * c.i / a.G) / STEP) : 0;
@@ -296,7 +391,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     c.nh = head_tiles(a, s, STEP);
   };
   auto advance = [&](Cursor& c) {
-    if (++c.t < c.steps) return;
+    if (++c.t < c.steps || ITEM) return;
     c.t = 0;
     if (++c.i == c.items) {
       c.i = 0;
@@ -311,8 +406,20 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     open(c);
   };
   auto tile_of = [&](const Cursor& c) { return c.t < c.nh ? c.t : c.t0 + c.t - c.nh; };
-  Cursor cur;
-  {
+  int pieces = 0;  // ITEM: waves that have steps
+  if constexpr (ITEM) {
+    cur.nh = head_tiles(a, mine, STEP);
+    open(cur);
+    const int tiles = (cur.end + STEP - 1) / STEP;
+    const int all = min(cur.nh, tiles) + max(0, tiles - max(cur.t0, cur.nh));
+    const int from = int(int64_t(all) * split / a.splits),
+              steps = int(int64_t(all) * (split + 1) / a.splits) - from;
+    pieces = min(steps, NW);
+    const int q = steps / NW, r = steps - q * NW;
+    cur.t = from + wave * q + min(wave, r);
+    count = q + (wave < r ? 1 : 0);
+    cur.steps = cur.t + count;
+  } else {
     cur.b = uniform(seq_with(x0));
     enter(cur);
     const int64_t at = x0 - pref[cur.b], seg = quotient(at, cur.steps);
@@ -387,10 +494,44 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     }
   };
 
+  // q of an item: vectors of 16 bytes by lanes, element (r, d) to [(d % 4) 16 + r][d / 4]
+  T* q_lds = &qs[ITEM ? 0 : wave][0];
+  auto stage_q = [&](const Seq& s, int rows_left) {
+    constexpr int VE = 16 / F::E, PER = DP / VE, N = ITEM ? NTH : 64;
+    const int me = ITEM ? int(threadIdx.x) : lane;
+#pragma unroll
+    for (int y = 0; y < (16 * PER + N - 1) / N; ++y) {
+      const int v = y * N + me, rr = v / PER, d = v % PER * VE;
+      if (16 * PER % N != 0 && v >= 16 * PER) break;
+      const int fr = 16 * cur.i + rr, fp = fr / a.G;
+      const bool ok = rr < rows_left && (FULL || d < D);
+      const T* p = static_cast<const T*>(a.q) + (s.row0 + (ok ? fp : 0)) * a.q_stride +
+                   int64_t(cur.h * a.G + (ok ? fr - fp * a.G : 0)) * D + (ok ? d : 0);
+      uint4 z = *reinterpret_cast<const uint4*>(p);
+      z.x = ok ? z.x : 0u;
+      z.y = ok ? z.y : 0u;
+      z.z = ok ? z.z : 0u;
+      z.w = ok ? z.w : 0u;
+      if constexpr (F32) {
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          q_lds[(e * 16 + rr) * F::QS + d / 4] = __uint_as_float(tile32::word(z, e));
+      } else {
+        // d, d + 4 are neighbours of one lane
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const uint32_t lo16 = tile32::word(z, e >> 1), hi16 = tile32::word(z, 2 + (e >> 1));
+          *reinterpret_cast<uint32_t*>(&q_lds[(e * 16 + rr) * F::QS + d / 4]) =
+              __builtin_amdgcn_perm(hi16, lo16, (e & 1) ? 0x07060302u : 0x05040100u);
+        }
+      }
+    }
+  };
+
   Cursor nxt = cur;
   if (count > 1) advance(nxt);
   Cursor far = nxt;
-  Where w_cur = where(cur, true), w_nxt = where(nxt, count > 1);
+  Where w_cur = where(cur, count > 0), w_nxt = where(nxt, count > 1);
   load_k(w_cur);
   load_v(w_cur);
 
@@ -403,8 +544,10 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
   float m = -INFINITY, l = 0.f;
   bool opened = false;
   int begun = 0;  // step of the range at which the item began
-  T* q_lds = &qs[wave][0];
-
+  if constexpr (ITEM) {
+    stage_q(mine, mine.n * a.G - 16 * cur.i);
+    __syncthreads();
+  }
   for (int x = 0; x < count; ++x) {
     if (x + 2 < count) advance(far);
     const Where w_far = where(far, x + 2 < count);
@@ -427,37 +570,12 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       lim = ALIKE ? lim_all : reach::limit(s, min(pos, s.n - 1));
       lo = ALIKE ? lo_all : reach::lowest(a, s, min(pos, s.n - 1));
       hs = a.window ? min(a.sinks, lim) : 0;
-      // q: vectors of 16 bytes by lanes, element (r, d) to [(d % 4) 16 + r][d / 4]
-      constexpr int VE = 16 / F::E, PER = DP / VE;
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int y = 0; y < 16 * PER / 64; ++y) {
-        const int v = y * 64 + lane, rr = v / PER, d = v % PER * VE;
-        const int fr = 16 * cur.i + rr, fp = fr / a.G;
-        const bool ok = rr < rows_left && (FULL || d < D);
-        const T* p = static_cast<const T*>(a.q) + (s.row0 + (ok ? fp : 0)) * a.q_stride +
-                     int64_t(cur.h * a.G + (ok ? fr - fp * a.G : 0)) * D + (ok ? d : 0);
-        uint4 z = *reinterpret_cast<const uint4*>(p);
-        z.x = ok ? z.x : 0u;
-        z.y = ok ? z.y : 0u;
-        z.z = ok ? z.z : 0u;
-        z.w = ok ? z.w : 0u;
-        if constexpr (F32) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e)
-            q_lds[(e * 16 + rr) * F::QS + d / 4] = __uint_as_float(tile32::word(z, e));
-        } else {
-          // d, d + 4 are neighbours of one lane
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            const uint32_t lo16 = tile32::word(z, e >> 1), hi16 = tile32::word(z, 2 + (e >> 1));
-            *reinterpret_cast<uint32_t*>(&q_lds[(e * 16 + rr) * F::QS + d / 4]) =
-                __builtin_amdgcn_perm(hi16, lo16, (e & 1) ? 0x07060302u : 0x05040100u);
-          }
-        }
+      if constexpr (!ITEM) {
+        __builtin_amdgcn_wave_barrier();
+        stage_q(s, rows_left);
+        __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
+        __builtin_amdgcn_wave_barrier();
       }
-      __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-      __builtin_amdgcn_wave_barrier();
       m = -INFINITY;
       l = 0.f;
 #pragma unroll
@@ -510,30 +628,33 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     }
     load_k(w_nxt);
 
-    // token c of unit(4 kd + v) is token tok0 + token_of(v, c) of the step
-    const int tok0 = (F::UB == 8 ? 2 : 4) * TU * kd;
-    auto token_of = [](int v, int c) {
-      return F::UB == 8 ? TU * (8 * (v >> 1) + (v & 1)) + c : TU * v + c;
-    };
+    // A lane's scores are of the tokens of its V vectors: those of vector u are tokens at(u) .. + NV - 1 of the
+    // step, and token c of unit(4 kd + v) is number place(v, c) of vector v * TU / NV
+    constexpr int NV = 16 / F::E;
+    auto at = [&](int u) { return (F32 ? 16 : 32) * u + NV * kd; };
+    auto place = [](int v, int c) { return (v * TU + c) % NV; };
     const int there = blocks_there(w_cur);
     const int base = tile_of(cur) * STEP;
     const bool in_head = cur.t < cur.nh;
     const bool full = there == (1 << MB) - 1 &&
                       ((base >= lo_all && base + STEP <= lim_all) ||
                        (in_head && base + STEP <= hs_all));
+    // NV tokens from token t of the step on, as bits: those of [from, to) and those below `below`
+    auto bits = [&](int t, int from, int to, int below) {
+      auto first = [](int n) { return (1u << min(max(n, 0), NV)) - 1u; };
+      t += base;
+      const uint32_t x = (first(to - t) & ~first(from - t)) | (in_head ? first(below - t) : 0u);
+      return (there >> ((t - base) >> 4)) & 1 ? x : 0u;
+    };
     if (!full) {
-      const int rel = lim - (base + tok0), from = lo - (base + tok0),
-                hrel = (in_head ? hs : 0) - (base + tok0);
 #pragma unroll
-      for (int v = 0; v < 4; ++v) {
-        const int block = F32 ? (F::UB == 8 ? v >> 1 : 0)
-                              : F::UB == 8 ? 2 * (v >> 1) + (kd >> 1) : kd >> 1;
-        const bool here = (there >> block) & 1;
+      for (int u = 0; u < NU; ++u) {
+        const uint32_t see = bits(at(u), lo, lim, hs);
 #pragma unroll
-        for (int c = 0; c < TU; ++c) {
-          const int o = token_of(v, c);
-          if (!(here && ((o >= from && o < rel) || o < hrel))) s[c][v] = -INFINITY;
-        }
+        for (int v = u * NV / TU; v < (u + 1) * NV / TU; ++v)
+#pragma unroll
+          for (int c = 0; c < TU; ++c)
+            s[c][v] = (see >> place(v, c)) & 1u ? s[c][v] : -INFINITY;
       }
     }
     // softmax, base 2
@@ -562,34 +683,29 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     bool by_row = false;
     if (!full) {
       // V of tokens that no row sees: zeros
-      const int vt = base + (F32 ? 4 : 8) * kd;  // of the lane's first vector
       uint32_t odd = 0;
 #pragma unroll
       for (int u = 0; u < NU; ++u) {
-        const int block = F32 ? u : 2 * u + (kd >> 1);
-        const bool here = (there >> block) & 1;
-        uint32_t keep[4] = {0u, 0u, 0u, 0u}, part[4] = {0u, 0u, 0u, 0u};
+        const uint32_t any = bits(at(u), lo_any, lim_any, hs_any);
+        const uint32_t some = ALIKE ? 0u : any & ~bits(at(u), lo_all, lim_all, hs_all);
+        auto words = [](uint32_t x, int w) {
+          return F32 ? ((x >> w) & 1u ? 0xffffffffu : 0u)
+                     : ((x >> (2 * w)) & 1u ? 0xffffu : 0u) | ((x >> (2 * w)) & 2u ? 0xffff0000u : 0u);
+        };
 #pragma unroll
-        for (int e = 0; e < 16 / F::E; ++e) {
-          const int tok = vt + (F32 ? 16 : 32) * u + e;
-          const bool any = here && ((tok >= lo_any && tok < lim_any) || (in_head && tok < hs_any));
-          const bool all = (tok >= lo_all && tok < lim_all) || (in_head && tok < hs_all);
-          const uint32_t bits = F32 ? 0xffffffffu : 0xffffu << (16 * (e & 1));
-          if (any) keep[e * F::E / 4] |= bits;
-          if (any && !all) part[e * F::E / 4] |= bits;
-        }
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t keep = words(any, w), part = words(some, w);
 #pragma unroll
-        for (int nb = 0; nb < NB; ++nb) {
-          uint32_t* y = &vr[u][nb].x;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) {
-            y[e] &= keep[e];
+          for (int nb = 0; nb < NB; ++nb) {
+            uint32_t& y = w == 0 ? vr[u][nb].x : w == 1 ? vr[u][nb].y : w == 2 ? vr[u][nb].z : vr[u][nb].w;
+            y &= keep;
             if constexpr (!ALIKE) {  // an exponent of all ones among what some rows do not see
-              const uint32_t z = y[e] & part[e];
-              if constexpr (F32) odd |= (z & 0x7f800000u) == 0x7f800000u;
-              else {
+              const uint32_t z = y & part;
+              if constexpr (F32) {
+                odd |= (z & 0x7f800000u) == 0x7f800000u ? 1u : 0u;
+              } else {
                 constexpr uint32_t X = DT == PIA_DTYPE_F16 ? 0x7c00u : 0x7f80u;
-                odd |= (z & X) == X || ((z >> 16) & X) == X;
+                odd |= ((z & X) == X ? 1u : 0u) | ((z & (X << 16)) == X << 16 ? 1u : 0u);
               }
             }
           }
@@ -634,7 +750,8 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
 #pragma unroll
       for (int c = 0; c < TU; ++c)
 #pragma unroll
-        for (int v = 0; v < 4; ++v) pw[n16 * (STEP + 1) + tok0 + token_of(v, c)] = s[c][v];
+        for (int v = 0; v < 4; ++v)
+          pw[n16 * (STEP + 1) + at(v * TU / NV) + place(v, c)] = s[c][v];
       __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
       __builtin_amdgcn_wave_barrier();
 #pragma unroll 1
@@ -644,15 +761,18 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
         const int id = __builtin_amdgcn_readlane(w_cur.id, block),
                   sub = __builtin_amdgcn_readlane(w_cur.sub, block);
         const bool sees = (tok >= lo && tok < lim) || (in_head && tok < hs);
+        int k4 = 4 * kd, P = a.P;  // hidden, or the rows' offsets are kept for all tokens and spilled
+        asm volatile("" : "+v"(k4), "+s"(P));
         const T* p = static_cast<const T*>(a.vp) +
-                     (int64_t(id) * a.Hkv + w_cur.h) * tile_elems + sub * 16 + (o & 15);
+                     (int64_t(id) * a.Hkv + w_cur.h) * tile_elems + sub * 16 + (o & 15) + int64_t(k4) * P;
         const float pr = pw[n16 * (STEP + 1) + o];
 #pragma unroll
         for (int nb = 0; nb < NB; ++nb) {
           if (!FULL && 16 * nb >= D) continue;
+          __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
           for (int j = 0; j < 4; ++j) {
-            const float y = Elem<DT>::load(p, int64_t(16 * nb + 4 * kd + j) * a.P);
+            const float y = Elem<DT>::load(p, int64_t(16 * nb + j) * P);
             acc[nb][j] = sees ? fmaf(pr, y, acc[nb][j]) : acc[nb][j];
           }
         }
@@ -665,7 +785,16 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     // end of the item or of the range
     if (cur.t + 1 == cur.steps || x + 1 == count) {
       const float lsum = tile32::sum_col4(l), mr = m == -INFINITY ? m : m - SHIFT<DT>;
-      if (cur.t + 1 == cur.steps && cur.t == x - begun) {
+      if constexpr (ITEM) {
+#pragma unroll
+        for (int nb = 0; nb < NB; ++nb)
+          *reinterpret_cast<float4*>(red + (wave * 16 + n16) * RS + 16 * nb + 4 * kd) =
+              make_float4(acc[nb][0], acc[nb][1], acc[nb][2], acc[nb][3]);
+        if (kd == 0) {
+          red_m[wave * 16 + n16] = mr;
+          red_l[wave * 16 + n16] = lsum;
+        }
+      } else if (cur.t + 1 == cur.steps && cur.t == x - begun) {
         if (live) finish(acc, mr, lsum, row, head);
       } else {
         float* part = a.parts + (w * 2 + (begun == 0 ? 0 : 1)) * part_floats<DP>;
@@ -686,6 +815,102 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     nxt = far;
     w_cur = w_nxt;
     w_nxt = w_far;
+  }
+  if constexpr (ITEM) {  // the waves' pieces joined in order, the splits', then the prefix's
+    __syncthreads();
+    const int rows = min(16, mine.n * a.G - 16 * cur.i), per_row = D / 4;
+    const bool prefix = a.src && reach::has_prefix(a, a.first + cur.b);
+    const int64_t R = a.rows * a.Hq;
+    float* part = a.parts + int64_t(item) * a.splits * part_floats<DP>;
+    struct Sum {
+      float m, l;
+      float4 o;
+      __device__ __forceinline__ void add(float m1, float l1, const float4& x) {
+        const float to = __builtin_elementwise_maximum(m, m1);
+        const float f0 = reach::weight(m, to), f = reach::weight(m1, to);
+        l = l * f0 + l1 * f;
+        o = make_float4(fmaf(x.x, f, o.x * f0), fmaf(x.y, f, o.y * f0), fmaf(x.z, f, o.z * f0),
+                        fmaf(x.w, f, o.w * f0));
+        m = to;
+      }
+    };
+    auto of_waves = [&](int r, int d) {
+      Sum x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      for (int p = 0; p < pieces; ++p)
+        x.add(red_m[p * 16 + r], red_l[p * 16 + r],
+              *reinterpret_cast<const float4*>(red + (p * 16 + r) * RS + d));
+      return x;
+    };
+    if (a.splits > 1) {
+      // The piece through the caches to memory, then the arrival: see arrive(). The last workgroup reads them.
+      float* p = part + split * part_floats<DP>;
+      for (int u = threadIdx.x; u < rows * per_row; u += NTH) {
+        const int r = u / per_row, d = 4 * (u - r * per_row);
+        const Sum x = of_waves(r, d);
+        float* o = p + r * DP + d;
+        put_far(o, x.o.x);
+        put_far(o + 1, x.o.y);
+        put_far(o + 2, x.o.z);
+        put_far(o + 3, x.o.w);
+        if (d == 0) {
+          put_far(p + 16 * DP + r, x.m);
+          put_far(p + 16 * DP + 16 + r, x.l);
+        }
+      }
+      __builtin_amdgcn_s_waitcnt(0);  // this wave's stores have completed
+      __syncthreads();                // and all waves'
+      if (threadIdx.x == 0) is_last = arrive(a.counters + item, a.token, a.splits) ? 1 : 0;
+      __syncthreads();
+      if (!is_last) return;
+    }
+    for (int u = threadIdx.x; u < rows * per_row; u += NTH) {
+      const int r = u / per_row, d = 4 * (u - r * per_row);
+      const int rr = 16 * cur.i + r, pos = rr / a.G;
+      const int64_t at = (mine.row0 + pos) * a.Hq + cur.h * a.G + rr - pos * a.G;
+      constexpr int N = 8;  // pieces on their way at once
+      Sum x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
+      if (a.splits > 1) {
+        for (int p0 = 0; p0 < a.splits; p0 += N) {
+          float pm[N], pl[N];
+          float4 po[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const float* p = part + min(p0 + k, a.splits - 1) * part_floats<DP>;
+            const float* o = p + r * DP + d;
+            pm[k] = get_far(p + 16 * DP + r);
+            pl[k] = get_far(p + 16 * DP + 16 + r);
+            po[k] = make_float4(get_far(o), get_far(o + 1), get_far(o + 2), get_far(o + 3));
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (p0 + k < a.splits) x.add(pm[k], pl[k], po[k]);
+        }
+      } else {
+        x = of_waves(r, d);
+      }
+      if (prefix) {
+        for (int p0 = 0; p0 < a.src_cuts; p0 += N) {
+          float2 pm[N];
+          float4 po[N];
+#pragma unroll
+          for (int k = 0; k < N; ++k) {
+            const int64_t c = min(p0 + k, a.src_cuts - 1) * R + at;
+            pm[k] = a.src_ml[c];
+            po[k] = *reinterpret_cast<const float4*>(a.src + c * D + d);
+          }
+#pragma unroll
+          for (int k = 0; k < N; ++k)
+            if (p0 + k < a.src_cuts) x.add(pm[k].x, pm[k].y, po[k]);
+        }
+      }
+      if (a.dst && !a.src) {
+        *reinterpret_cast<float4*>(a.dst + at * D + d) = x.o;
+        if (d == 0) a.dst_ml[at] = make_float2(x.m, x.l);
+      } else {
+        const float y[4] = {x.o.x, x.o.y, x.o.z, x.o.w};
+        store4<DT>(static_cast<T*>(a.out) + at * D + d, y, x.l);
+      }
+    }
   }
 }
 
@@ -832,18 +1057,40 @@ __global__ __launch_bounds__(JOIN_FEW) void reach_stream_join_kernel(Args a, int
 inline int64_t resident_waves() { return int64_t(device_cus()) * WGS_PER_CU * WG_WAVES; }
 constexpr int64_t PREF_BYTES = (MAX_SEQS + 1) * 8 + 248;  // whole 256 bytes
 
+// Into how many runs of steps, a workgroup's each, every item is cut (0: all items' steps over the resident
+// waves instead). A second step of a wave takes as long as the arrival and reading of another workgroup's piece
+// (3 us), so up to two of each wave are not cut; of more, each wave gets one where there are workgroups for it.
+inline int item_splits(int64_t items, int64_t steps) {
+  const int64_t slots = int64_t(device_cus()) * WGS_PER_CU;
+  if (items > slots) return 0;
+  if (steps <= 2 * WG_WAVES) return 1;
+  const int64_t n = std::max<int64_t>(
+      1, std::min(ceil_div(steps, WG_WAVES), std::min<int64_t>(slots / items, MAX_SPLITS)));
+  return ceil_div(steps, n * WG_WAVES) <= ITEM_STEPS ? int(n) : 0;
+}
+
 template <int DT, int DP>
 void launch_shape(const Args& a, int64_t items, bool alike, hipStream_t s) {
-  const dim3 grid{unsigned(device_cus() * WGS_PER_CU), 1u, 1u}, block{64 * WG_WAVES, 1u, 1u};
   const bool full = a.D == DP;
-#define PIA_RS(A, F) hipLaunchKernelGGL((reach_stream_kernel<DT, DP, A, F>), grid, block, 0, s, a)
-  if (alike) {
-    if (full) PIA_RS(true, true); else PIA_RS(true, false);
-  } else {
-    if (full) PIA_RS(false, true); else PIA_RS(false, false);
+#define PIA_RS(A, F, I)                                                                           \
+  hipLaunchKernelGGL(                                                                             \
+      (reach_stream_kernel<DT, DP, A, F, I>),                                                     \
+      dim3(unsigned(I ? ceil_div(items, 8) * 8 * a.splits : device_cus() * WGS_PER_CU)),          \
+      dim3(64 * WG_WAVES), 0, s, a)
+#define PIA_RS_I(I)                                              \
+  if (alike) {                                                   \
+    if (full) PIA_RS(true, true, I); else PIA_RS(true, false, I); \
+  } else {                                                       \
+    if (full) PIA_RS(false, true, I); else PIA_RS(false, false, I); \
   }
+  if (a.splits) {
+    PIA_RS_I(true)
+  } else {
+    PIA_RS_I(false)
+  }
+#undef PIA_RS_I
 #undef PIA_RS
-  if (a.whole && !a.src) return;
+  if (a.splits || (a.whole && !a.src)) return;
   // few items: many pieces each, which many threads share, on every compute unit; many: two or three
   const bool few = items * 4 <= resident_waves();
   const int rows = a.cu || a.by_group ? 16 : std::min(a.G, 16);
@@ -859,7 +1106,10 @@ template <int DT>
 int launch_dtype(Args a, int64_t tokens, hipStream_t s) {
   const int n = a.by_group ? a.groups : a.B;
   const int step = a.D > 128 ? Form<DT, 256>::STEP : Form<DT, 128>::STEP;
-  a.whole = ceil_div(tokens, step) + (a.window ? 1 : 0) <= WHOLE;
+  // a window's tiles may begin and end within one
+  const int64_t steps = std::min(ceil_div(tokens, step) + (a.window ? 2 : 0),
+                                 ceil_div((a.by_group ? a.pt_stride : a.bt_stride) * a.P, step));
+  a.whole = steps <= WHOLE;
   const bool alike = a.by_group || !a.cu || (!a.offs && !a.window);
   // more sequences than a launch's tables hold: by parts, one after the other on the stream
   for (int b0 = 0; b0 < n; b0 += MAX_SEQS) {
@@ -868,6 +1118,9 @@ int launch_dtype(Args a, int64_t tokens, hipStream_t s) {
     const int64_t items = (a.cu || a.by_group ? (a.rows * a.G >> 4) + a.count + 1
                                               : int64_t(a.count) * ((a.G + 15) / 16)) * a.Hkv;
     if (items > 0x1fffffff) return fail(PIA_EINVAL, "attention: too many rows");
+    a.splits = item_splits(items, steps);
+    a.counters = reinterpret_cast<unsigned long long*>(a.pref);
+    a.token = a.splits > 1 ? reach_token() : 0;
     if (a.D <= 64) launch_shape<DT, 64>(a, items, alike, s);
     else if (a.D <= 128) launch_shape<DT, 128>(a, items, alike, s);
     else launch_shape<DT, 256>(a, items, alike, s);

@@ -449,6 +449,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
         for (int v = 0; v < 16; ++v) acc[nb][v] *= alpha;
     }
     m = mref;
+    __builtin_amdgcn_s_setprio(1);  // a wave at its products before one that stages (1 to 7 %)
     scores(sn, buf ^ 1);
     uint4 pk[4];  // block s of the tile: the B operand of its 16 tokens, the probabilities
     float least = INFINITY;  // fp16: of the positive ones
@@ -528,6 +529,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
 #pragma unroll
     for (int i = 0; i < 4 * NB; ++i)
       acc[i % NB] = mfma32<DT>(vread(buf, i % NB, i / NB), pk[i / NB], acc[i % NB]);
+    __builtin_amdgcn_s_setprio(0);
     mx = largest(sn);
     if constexpr (!HALF) order_scores();
 #pragma unroll
