@@ -115,6 +115,12 @@ __device__ __forceinline__ float weight(float m, float joined) {
   return m == joined ? (m == -INFINITY ? 0.f : 1.f) : __builtin_amdgcn_exp2f(m - joined);
 }
 
+// How the tiled kernel takes a call: 256 rows at a time or 128, and the pieces of an item
+struct TilePlan {
+  bool wide;
+  int cuts;
+};
+
 }  // namespace reach
 
 // Any head_dim to 512, page size and group: one wave for each row and head (reach_general.hip)
@@ -129,8 +135,8 @@ int launch_reach_stream_bf16(const reach::Args& a, int64_t tokens, hipStream_t s
 // into how many pieces (at most `most`) it would cut each item of so many rows, and its launch. Pieces
 // go to dst; those of sequences are joined there, those of groups are not.
 bool reach_tiles_shape(const reach::Args& a, int dtype);
-int reach_tiles_cuts(const reach::Args& a, int64_t tokens, int64_t most);
-int launch_reach_tiles(const reach::Args& a, int dtype, int cuts, hipStream_t s);
+reach::TilePlan reach_tiles_plan(const reach::Args& a, int64_t tokens, int64_t most);
+int launch_reach_tiles(const reach::Args& a, int dtype, reach::TilePlan plan, hipStream_t s);
 // a number that no other launch has, in the upper 48 bits
 unsigned long long reach_token();
 // bytes of the streaming kernel's pieces by wave, and of the numbers before them

@@ -101,10 +101,11 @@ bool tiled(const reach::Args& a, int dtype, int64_t n) {
 }
 // Tiles for the sequences of a call, with pieces in `bytes` from dst on
 int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t bytes, hipStream_t s) {
-  const int cuts = reach_tiles_cuts(a, tokens, bytes / piece_bytes(a.rows, a.Hq, a.D));
-  a.dst = cuts > 1 ? dst : nullptr;
-  a.dst_ml = reinterpret_cast<float2*>(dst + cuts * a.rows * a.Hq * a.D);
-  return launch_reach_tiles(a, dtype, cuts, s);
+  const reach::TilePlan plan =
+      reach_tiles_plan(a, tokens, bytes / piece_bytes(a.rows, a.Hq, a.D));
+  a.dst = plan.cuts > 1 ? dst : nullptr;
+  a.dst_ml = reinterpret_cast<float2*>(dst + plan.cuts * a.rows * a.Hq * a.D);
+  return launch_reach_tiles(a, dtype, plan, s);
 }
 
 }  // namespace
@@ -207,12 +208,12 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
     g.by_group = 1;
     const bool tiles = tiled(a, dtype, num_groups);
     const int64_t R = total_q_rows * num_heads;
-    const int cuts =
-        !tiles ? 1 : reach_tiles_cuts(g, prefix_tokens,
-                                      shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
+    const reach::TilePlan plan = reach_tiles_plan(
+        g, prefix_tokens, shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
+    const int cuts = tiles ? plan.cuts : 1;
     g.dst = a.parts + parts / int64_t(sizeof(float));
     g.dst_ml = reinterpret_cast<float2*>(g.dst + (cuts + 1) * R * head_dim);
-    rc = tiles ? launch_reach_tiles(g, dtype, cuts, s) : stream_call(g, dtype, prefix_tokens, s);
+    rc = tiles ? launch_reach_tiles(g, dtype, plan, s) : stream_call(g, dtype, prefix_tokens, s);
     if (rc) return rc;
     a.src = g.dst;
     a.src_ml = g.dst_ml;

@@ -154,12 +154,29 @@ __device__ __forceinline__ Unit<UB> load_unit(const void* p) {
   return __builtin_bit_cast(Unit<UB>, v);
 }
 
-// Stores and loads of what workgroups on other XCDs read or wrote in this launch
-__device__ __forceinline__ void put_far(float* p, float v) {
-  __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+// Stores and loads of what workgroups on other XCDs read or wrote in this launch: through the XCD's L2 (SC1, what
+// relaxed atomics of agent scope are), 16 bytes at a time. at: bytes from the descriptor's base.
+constexpr int FAR_AUX = 16;
+__device__ __forceinline__ auto far_memory(float* p, int64_t floats) {
+  return __builtin_amdgcn_make_buffer_rsrc(p, 0, int(floats * 4), 0x00020000);
 }
-__device__ __forceinline__ float get_far(const float* p) {
-  return __hip_atomic_load(p, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+template <class R>
+__device__ __forceinline__ void put_far(R r, int at, const float4& v) {
+  __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4_t, v), r, at, 0, FAR_AUX);
+}
+template <class R>
+__device__ __forceinline__ void put_far(R r, int at, const float2& v) {
+  __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2_t, v), r, at, 0, FAR_AUX);
+}
+template <class R>
+__device__ __forceinline__ float4 get_far4(R r, int at) {
+  return __builtin_bit_cast(float4, __builtin_amdgcn_raw_buffer_load_b128(r, at, 0, FAR_AUX));
+}
+template <class R>
+__device__ __forceinline__ float2 get_far2(R r, int at) {
+  return __builtin_bit_cast(float2, __builtin_amdgcn_raw_buffer_load_b64(r, at, 0, FAR_AUX));
 }
 // Counts a workgroup in at its item's counter, which holds (token of the launch, arrivals); true for the last
 // of n. What it held before (another launch's, or anything) is replaced by whoever comes first. The last one
@@ -821,7 +838,8 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     const int rows = min(16, mine.n * a.G - 16 * cur.i), per_row = D / 4;
     const bool prefix = a.src && reach::has_prefix(a, a.first + cur.b);
     const int64_t R = a.rows * a.Hq;
-    float* part = a.parts + int64_t(item) * a.splits * part_floats<DP>;
+    const auto far = far_memory(a.parts + int64_t(item) * a.splits * part_floats<DP>,
+                                a.splits * part_floats<DP>);
     struct Sum {
       float m, l;
       float4 o;
@@ -842,20 +860,13 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       return x;
     };
     if (a.splits > 1) {
-      // The piece through the caches to memory, then the arrival: see arrive(). The last workgroup reads them.
-      float* p = part + split * part_floats<DP>;
+      // The piece to memory, then the arrival: see arrive(). The last workgroup reads them.
       for (int u = threadIdx.x; u < rows * per_row; u += NTH) {
         const int r = u / per_row, d = 4 * (u - r * per_row);
         const Sum x = of_waves(r, d);
-        float* o = p + r * DP + d;
-        put_far(o, x.o.x);
-        put_far(o + 1, x.o.y);
-        put_far(o + 2, x.o.z);
-        put_far(o + 3, x.o.w);
-        if (d == 0) {
-          put_far(p + 16 * DP + r, x.m);
-          put_far(p + 16 * DP + 16 + r, x.l);
-        }
+        const int p = split * int(part_floats<DP>);
+        put_far(far, 4 * (p + r * DP + d), x.o);
+        if (d == 0) put_far(far, 4 * (p + 16 * DP + 2 * r), make_float2(x.m, x.l));
       }
       __builtin_amdgcn_s_waitcnt(0);  // this wave's stores have completed
       __syncthreads();                // and all waves'
@@ -870,20 +881,18 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
       constexpr int N = 8;  // pieces on their way at once
       Sum x{-INFINITY, 0.f, make_float4(0.f, 0.f, 0.f, 0.f)};
       if (a.splits > 1) {
-        for (int p0 = 0; p0 < a.splits; p0 += N) {
-          float pm[N], pl[N];
-          float4 po[N];
+        for (int p0 = 0; p0 < a.splits; p0 += 2 * N) {
+          float2 pm[2 * N];
+          float4 po[2 * N];
 #pragma unroll
-          for (int k = 0; k < N; ++k) {
-            const float* p = part + min(p0 + k, a.splits - 1) * part_floats<DP>;
-            const float* o = p + r * DP + d;
-            pm[k] = get_far(p + 16 * DP + r);
-            pl[k] = get_far(p + 16 * DP + 16 + r);
-            po[k] = make_float4(get_far(o), get_far(o + 1), get_far(o + 2), get_far(o + 3));
+          for (int k = 0; k < 2 * N; ++k) {
+            const int p = min(p0 + k, a.splits - 1) * int(part_floats<DP>);
+            pm[k] = get_far2(far, 4 * (p + 16 * DP + 2 * r));
+            po[k] = get_far4(far, 4 * (p + r * DP + d));
           }
 #pragma unroll
-          for (int k = 0; k < N; ++k)
-            if (p0 + k < a.splits) x.add(pm[k], pl[k], po[k]);
+          for (int k = 0; k < 2 * N; ++k)
+            if (p0 + k < a.splits) x.add(pm[k].x, pm[k].y, po[k]);
         }
       } else {
         x = of_waves(r, d);

@@ -24,7 +24,7 @@
 // it is: [d][64 tokens], unit u (tokens 8 u .. + 7) at u ^ d / 2 % 8; a wave's lanes take the rows of 1 KB in the
 // order that stores without conflicts. K is turned on its way: a lane loads TL tokens of eight rows and
 // stores, for each token, a unit of eight elements. Those are the elements u, u + NU, u + 2 NU, ... (NU = DP / 8
-// units to a row), for that makes a wave's loads whole lines, and q's operands come through LDS in the same
+// units to a row), for that makes a wave's loads whole lines, and q's operands are taken in the same
 // order once an item. K [token][d]: unit u of row r at u ^ r % 16 (DP 64: 8 units, u ^ r / 2 % 8).
 #include <algorithm>
 
@@ -95,55 +95,72 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
   constexpr bool HALF = DT == PIA_DTYPE_F16;
   constexpr uint32_t K_BUF = RT_KT * UK * 16, V_BUF = DP * 128;  // bytes
-  static_assert(32 * NW * UK * 16 <= 2 * (K_BUF + V_BUF), "q passes through the tiles' LDS");
   __shared__ __align__(16) unsigned char lds[2 * (K_BUF + V_BUF)];
   __shared__ int item_pref[RT_MAX_SEQS + 1];
   __shared__ int wsum[NW];
   __shared__ int odd_seen;
+  __shared__ int4 sees[32 * NW];  // of each row: lowest, limit, and how much of the head
   const int lane = threadIdx.x & 63;
   const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   auto seq_at = [&](int b) {
     return a.by_group ? reach::group(a, a.first + b) : reach::sequence(a, a.first + b);
   };
 
-  // work items per sequence and their prefix
-  if (threadIdx.x == 0) item_pref[0] = 0;
+  // work items per sequence, those before each, and this workgroup's: item `j` of sequence `b`
   if (threadIdx.x == 0) odd_seen = 0;
-  int carry = 0;
-  for (int c0 = 0; c0 < a.count; c0 += NT) {
-    const int i = c0 + threadIdx.x;
-    int incl = 0;
-    if (i < a.count) {
-      const int n = seq_at(i).n;
-      incl = n > 0 ? (n + a.ppt - 1) / a.ppt : 0;
-    }
+  int h, j, b, piece;
+  auto mine = [&](int items) {  // of all sequences' items
+    if (!xcd_item(blockIdx.x, items * a.cuts, a.Hkv, h, j)) return false;
+    piece = a.cuts == 1 ? 0 : uint32_t(j) % uint32_t(a.cuts);  // of the item's tiles
+    if (a.cuts > 1) j = uint32_t(j) / uint32_t(a.cuts);
+    return true;
+  };
+  auto items_at = [&](int i) {
+    const int n = i < a.count ? seq_at(i).n : 0;
+    return n > 0 ? (n + a.ppt - 1) / a.ppt : 0;
+  };
+  auto scan = [&](int x) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) {
-      const int y = __shfl_up(incl, o, 64);
-      if (lane >= o) incl += y;
+      const int y = __shfl_up(x, o, 64);
+      if (lane >= o) x += y;
     }
-    if (lane == 63) wsum[wave] = incl;
-    __syncthreads();
-    int base = carry;
-    for (int x = 0; x < wave; ++x) base += wsum[x];
-    if (i < a.count) item_pref[i + 1] = base + incl;
+    return x;
+  };
+  if (a.count <= 64) {  // each wave for itself
+    const int own = items_at(lane), incl = scan(own);
+    if (!mine(__builtin_amdgcn_readlane(incl, 63))) return;
+    b = __builtin_ctzll(__ballot(incl > j));  // the first with more items up to it
+    j = __builtin_amdgcn_readlane(incl, b) - 1 - j;
+  } else {
+    if (threadIdx.x == 0) item_pref[0] = 0;
+    int carry = 0;
+    for (int c0 = 0; c0 < a.count; c0 += NT) {
+      const int i = c0 + threadIdx.x;
+      const int incl = scan(items_at(i));
+      if (lane == 63) wsum[wave] = incl;
+      __syncthreads();
+      int base = carry;
+      for (int x = 0; x < wave; ++x) base += wsum[x];
+      if (i < a.count) item_pref[i + 1] = base + incl;
 #pragma unroll
-    for (int x = 0; x < NW; ++x) carry += wsum[x];
-    __syncthreads();
+      for (int x = 0; x < NW; ++x) carry += wsum[x];
+      __syncthreads();
+    }
+    if (!mine(carry)) return;
+    int lo_b = 0, hi_b = a.count - 1;  // the last with item_pref[b] <= j
+    while (lo_b < hi_b) {
+      const int mid = (lo_b + hi_b + 1) >> 1;
+      if (item_pref[mid] <= j) lo_b = mid; else hi_b = mid - 1;
+    }
+    b = lo_b;
+    j = item_pref[b + 1] - 1 - j;
   }
-  int h, j;
-  if (!xcd_item(blockIdx.x, carry * a.cuts, a.Hkv, h, j)) return;
-  const int piece = a.cuts == 1 ? 0 : uint32_t(j) % uint32_t(a.cuts);  // of the item's tiles
-  if (a.cuts > 1) j = uint32_t(j) / uint32_t(a.cuts);
-  int lo_b = 0, hi_b = a.count - 1;  // the sequence holding the item: the last with item_pref[b] <= j
-  while (lo_b < hi_b) {
-    const int mid = (lo_b + hi_b + 1) >> 1;
-    if (item_pref[mid] <= j) lo_b = mid; else hi_b = mid - 1;
-  }
-  const int b = __builtin_amdgcn_readfirstlane(lo_b);
+  b = __builtin_amdgcn_readfirstlane(b);
+  piece = __builtin_amdgcn_readfirstlane(piece);
   h = __builtin_amdgcn_readfirstlane(h);
   // the last positions of a sequence, which see the most keys, first
-  const int s0 = __builtin_amdgcn_readfirstlane((item_pref[b + 1] - 1 - j) * a.ppt);
+  const int s0 = __builtin_amdgcn_readfirstlane(j * a.ppt);
   const Seq s = seq_at(b);
   const int64_t row0 = s.row0;
   const int s_last = min(s0 + a.ppt, s.n) - 1;
@@ -179,7 +196,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   kt0 = __builtin_amdgcn_readfirstlane(kt0);
   nkt = __builtin_amdgcn_readfirstlane(nkt);
 
-  // this lane's row; what it sees is made where it is used, on the tiles that not all rows see whole
+  // rows, and what they see: in LDS, for the tiles that not all rows see whole
   const int D = a.D;
   const int hh = lane >> 5, n32 = lane & 31, G = a.G;
   struct Row {
@@ -193,33 +210,45 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     return Row{r, pos, r < a.ppt * G && pos < s.n};
   };
 
-  // q through LDS: element NU e + u of a row to unit u, place e
+  if (threadIdx.x < 32 * NW) {
+    const int r = threadIdx.x, pos = s0 + r / G, lim = reach::limit(s, pos);
+    const bool live = r < a.ppt * G && pos < s.n;
+    sees[r] = live ? make_int4(reach::lowest(a, s, pos), lim, a.window ? min(head, lim) : head, 0)
+                   : make_int4(0, 0, 0, 0);
+  }
+
+  // q: unit u of a row is its elements u, NU + u, ..., and a lane's units 2 k + hh are the elements hh of all its
+  // words. So a lane loads its whole row and takes half of each word.
   uint4 qr[KS];
   {
-    const uint16_t* q = static_cast<const uint16_t*>(a.q);
-    auto q_at = [&](int row, int u) {
-      return uint32_t(row * UK * 16 + 16 * (u ^ (DP > 64 ? row & 15 : (row >> 1) & 7)));
+    const Row x = row_now();
+    const uint16_t* q = static_cast<const uint16_t*>(a.q) +
+                        (row0 + (x.live ? x.pos : 0)) * a.q_stride +
+                        int64_t(h * G + (x.live ? x.r % G : 0)) * D;
+    uint4 z[DP / 8];
+#pragma unroll
+    for (int i = 0; i < DP / 8; ++i) {  // rows that are none take the first one's, and are not written
+      const bool ok = 8 * i < D;
+      z[i] = *reinterpret_cast<const uint4*>(q + (ok ? 8 * i : 0));
+      z[i].x = ok ? z[i].x : 0u;
+      z[i].y = ok ? z[i].y : 0u;
+      z[i].z = ok ? z[i].z : 0u;
+      z[i].w = ok ? z[i].w : 0u;
+    }
+    const uint32_t half = hh ? 0x07060302u : 0x05040100u;
+    auto of = [&](int d) {  // the word of element d
+      const uint4& y = z[d / 8];
+      const int i = d % 8 / 2;
+      return i == 0 ? y.x : i == 1 ? y.y : i == 2 ? y.z : y.w;
     };
 #pragma unroll
-    for (int y = 0; y < KS; ++y) {  // 32 NW rows of DP / 8 vectors by 64 NW threads
-      const int v = y * NT + threadIdx.x, rr = v / (DP / 8), d = v % (DP / 8) * 8, rp = s0 + rr / G;
-      const bool ok = rr < a.ppt * G && rp < s.n && d < D;
-      const uint4 z = ok ? *reinterpret_cast<const uint4*>(
-                               q + (row0 + rp) * a.q_stride + int64_t(h * G + rr % G) * D + d)
-                         : make_uint4(0u, 0u, 0u, 0u);
-      const uint32_t w[4] = {z.x, z.y, z.z, z.w};
+    for (int k = 0; k < KS; ++k) {
+      uint32_t w[4];
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int e = (d + i) / NU, u = (d + i) - e * NU;
-        *reinterpret_cast<uint16_t*>(lds + q_at(rr, u) + 2 * e) =
-            uint16_t(w[i >> 1] >> (16 * (i & 1)));
-      }
+      for (int f = 0; f < 4; ++f)
+        w[f] = __builtin_amdgcn_perm(of(NU * (2 * f + 1) + 2 * k), of(NU * 2 * f + 2 * k), half);
+      qr[k] = make_uint4(w[0], w[1], w[2], w[3]);
     }
-    __syncthreads();
-#pragma unroll
-    for (int k = 0; k < KS; ++k)
-      qr[k] = *reinterpret_cast<const uint4*>(lds + q_at(32 * wave + n32, 2 * k + hh));
-    __syncthreads();
   }
 
   // tile `it` of the item's list: its first token, and whether it is of the head
@@ -241,10 +270,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     return (first(x.to - t) & ~first(x.from - t)) | first(x.below - t);
   };
   auto reach_of_row = [&](int it) {
-    const Row x = row_now();
-    const int lim = reach::limit(s, x.pos);
-    const Reach y = reach_of(it, reach::lowest(a, s, x.pos), lim, a.window ? min(head, lim) : head);
-    return x.live ? y : Reach{0, 0, 0};
+    const int4 x = sees[32 * wave + n32];
+    return reach_of(it, x.x, x.y, x.z);
   };
   // whether every row sees all of a tile (of the blocks that are there)
   auto seen_whole = [&](int it) {
@@ -350,7 +377,16 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   // NaN, infinite, minus infinite
   constexpr uint32_t EXP = HALF ? 0x7c00u : 0x7f80u, ONE = HALF ? 0x3c00u : 0x3f80u;
   auto stage_v = [&](Part& p, int buf, int it, int kind) {
-    if (kind || !seen_whole(it)) {
+    bool look = kind != 0;
+    if (!kind && !seen_whole(it)) {
+      // a half that is not finite carries into its top bit: |x| + 2^(mantissa bits) >= 2^15
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < 4 * VL; ++i)
+        top |= (word(p, i) & 0x7fff7fffu) + (HALF ? 0x04000400u : 0x00800080u);
+      look = __ballot((top & 0x80008000u) != 0) != 0;
+    }
+    if (look) {
       const uint32_t any = bits8(reach_of(it, lo_any, lim_any, head), 16 * blk + 8 * vh);
       uint32_t odd = 0;
 #pragma unroll
@@ -424,8 +460,11 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
         const int s4 = 2 * tb + (v >> 3);
         const uint32_t see = (there >> s4) & 1 ? bits8(x, 16 * s4 + 8 * hh) : 0u;
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          sc[tb][v + e] = (see >> e) & 1u ? sc[tb][v + e] : -INFINITY;
+        for (int e = 0; e < 8; ++e) {  // all bits of `keep`, or none: v_bfe_i32, v_bfi_b32
+          const uint32_t keep = uint32_t(int32_t(see << (31 - e)) >> 31);
+          sc[tb][v + e] = __uint_as_float((keep & __float_as_uint(sc[tb][v + e])) |
+                                          (~keep & 0xff800000u));
+        }
       }
   };
   // One tile. sc: its scores, mx: the largest of them (of the lane's) where none is hidden; sn, mx:
@@ -564,11 +603,13 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       stage_v(pb, buf_v, it_v, 0);
     }
   };
-  fetch(w1, w0, kt0 + 1);
-  stage(1, 0, kt0);
-  if (!SPLIT || first4) {  // K of the first tile; the other waves have nothing of it
-    fetch_k(pa, w0, kt0);
-    stage_k(pa, 0);
+  {  // the first tile's K and V and the second's K, all on their way at once
+    Part pc;
+    fetch(w1, w0, kt0 + 1);
+    if (!SPLIT || first4) fetch_k(pc, w0, kt0);
+    __syncthreads();  // odd_seen is cleared
+    stage(1, 0, kt0);
+    if (!SPLIT || first4) stage_k(pc, 0);
   }
   fetch(w2, w1, kt0 + 2);
   __syncthreads();
@@ -716,23 +757,28 @@ bool reach_tiles_shape(const Args& a, int dtype) {
   return dtype != PIA_DTYPE_F32 && a.D <= 128 && a.scale_log2 > 0.f && a.G <= 128;
 }
 
-int reach_tiles_cuts(const Args& a, int64_t tokens, int64_t most) {
+reach::TilePlan reach_tiles_plan(const Args& a, int64_t tokens, int64_t most) {
   const int64_t cus = device_cus(), tiles = ceil_div(tokens, RT_KT), n = a.by_group ? a.groups : a.B;
-  const int64_t items = std::max<int64_t>(1, (ceil_div(a.rows, 128 / a.G) + n / 2) * a.Hkv);
-  // Fewer items than CUs: their keys are cut into pieces, to two on every CU of 16 tiles each, or one of 4
+  auto items_of = [&](int rows) {
+    return std::max<int64_t>(1, (ceil_div(a.rows, rows / a.G) + n / 2) * a.Hkv);
+  };
+  // Items of 256 rows, one on a CU, halve what is staged for a row, where there is work for 16 tiles on
+  // every CU; else of 128 rows, two on a CU.
+  const int64_t items8 = items_of(256), items4 = items_of(128);
+  const bool wide = a.D == 128 && a.G <= 128 && a.rows * a.G >= 192 * n && items8 * tiles >= 16 * cus;
+  // Fewer items than CUs: their keys are cut into pieces, of 16 tiles at least, or of 4 to one on every CU
   const int64_t cuts =
-      std::max(std::min(2 * cus / items, tiles / 16), std::min(cus / items, tiles / 4));
-  return int(std::max<int64_t>(1, std::min(std::min<int64_t>(cuts, RT_MAX_CUTS), most)));
+      wide ? std::min(cus / items8, tiles / 16)
+           : std::max(std::min(2 * cus / items4, tiles / 16), std::min(cus / items4, tiles / 4));
+  return {wide, int(std::max<int64_t>(1, std::min(std::min<int64_t>(cuts, RT_MAX_CUTS), most)))};
 }
 
-int launch_reach_tiles(const Args& args, int dtype, int cuts, hipStream_t s) {
+int launch_reach_tiles(const Args& args, int dtype, reach::TilePlan plan, hipStream_t s) {
   TileArgs a;
   static_cast<Args&>(a) = args;
-  a.cuts = cuts;
-  const int64_t cus = device_cus();
+  const int cuts = a.cuts = plan.cuts;
+  const bool wide = plan.wide;
   const int n = a.by_group ? a.groups : a.B;
-  const int64_t items4 = std::max<int64_t>(1, (ceil_div(a.rows, 128 / a.G) + n / 2) * a.Hkv) * cuts;
-  const bool wide = a.D == 128 && a.rows * a.G >= 128 * int64_t(n) && items4 >= 2 * cus;
   a.ppt = (wide ? 256 : 128) / a.G;
   const bool joined = cuts > 1 && !a.by_group;
   for (int b0 = 0; b0 < n; b0 += RT_MAX_SEQS) {
