@@ -75,6 +75,28 @@ def test_decode(dev, case, dtype):
     O.check(got, *O.prefixed(q, k, v, pt, plens, bt, lens, cu_seqs), dtype, rows=True)
 
 
+MANY = [  # prefixes, own lengths, cu_seqs, Hq, Hkv, D, P: both parts side by side over 16-bit pools
+    ([700, 130], [i % 70 for i in range(60)], [3, 30, 58], 6, 2, 96, 16),     # loners at both ends
+    ([300], [500] * 24, None, 8, 2, 80, 32),
+    ([1500, 0, 64], [i * 7 % 300 for i in range(90)], [0, 40, 50, 90], 4, 1, 64, 16),
+    ([400, 90], [20 + i for i in range(48)], [0, 24, 48], 12, 3, 48, 48),
+    ([5000], [33] * 70, None, 32, 8, 128, 16),
+    ([200], [2500] * 20, None, 4, 1, 128, 16),        # own tokens beyond what goes side by side
+]
+
+
+@pytest.mark.parametrize("dtype", list(O.STEP))
+@pytest.mark.parametrize("ragged", [False, True])
+@pytest.mark.parametrize("case", MANY, ids=lambda c: f"{c[0]}+{len(c[1])}x{max(c[1])}h{c[3]}/{c[4]}d{c[5]}p{c[6]}")
+def test_many_sequences(dev, case, dtype, ragged):
+    plens, lens, cu_seqs, hq, hkv, dim, page = case
+    rows = [1 + i % 3 for i in range(len(lens))] if ragged else None
+    cu = _cu(rows) if ragged else None
+    q, k, v, pt, bt = _case(plens, lens, hq, hkv, dim, page, dtype, rows, seed=len(lens))
+    got = _run(dev, q, k, v, pt, plens, bt, lens, cu_seqs, cu)
+    O.check(got, *O.prefixed(q, k, v, pt, plens, bt, lens, cu_seqs, cu), dtype, rows=True)
+
+
 ROWS = [  # prefixes, rows, contexts, offsets, cu_seqs, Hq, Hkv, D, P
     ([100], [1, 3, 0, 6], [40, 30, 20, 6], [39, 27, 20, 0], None, 8, 2, 128, 16),
     ([60], [5, 2], [10, 9], [-8, 20], None, 4, 1, 64, 16),     # rows that see no own key yet
