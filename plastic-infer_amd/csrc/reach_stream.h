@@ -21,6 +21,9 @@
 // Precision: products of 16-bit values are exact in fp32, in which scores, sums and outputs are held. The
 // probabilities over 16-bit pools are two terms of the pool's type (2^-17 of each), the first rounded toward zero
 // and neither ever 0 for a positive value: an infinite V then gives that infinity and not infinity - infinity.
+// fp16's numbers end at 2^-38 of the reference, so a step with smaller ones than 2^-24 of it multiplies what
+// the two terms leave, too (the rest): without that, thousands of them before V much larger than the likely
+// tokens' were off by the least number each.
 // Over fp32 pools all products are fp32's, a step's summed on their own first.
 //
 // A row's result may depend on what it sees only. Scores of other tokens are -inf. V of tokens that no row
@@ -45,14 +48,17 @@ constexpr int MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
 constexpr int WG_WAVES = 4;
 constexpr int WGS_PER_CU = 2;   // two waves per SIMD
 constexpr int WHOLE = 3;        // steps of items that are not cut
-constexpr float RESCALE = 8.0f;  // log2: how far a row's maximum may run ahead of its reference
 constexpr int MAX_SPLITS = 64;  // workgroups of an item
 constexpr int ITEM_STEPS = 8;   // steps of a wave above which even ranges for all waves are better
 constexpr int JOIN_MANY = 128, JOIN_FEW = 512;  // threads of the joining workgroups
 
-// log2 of what probabilities are scaled by: fp16's terms then go down to 2^-32 of the largest
+// log2: how far a row's maximum may run ahead of its reference, and what probabilities are scaled by. fp16's
+// numbers, to 2^15, then go down to 2^-38 of the reference (7 and 8 in place of 1 and 14: a window of 1024 before
+// one sequence with wide scores 14.7 us for 13.7, its steps nearly all with a rest).
 template <int DT>
-constexpr float SHIFT = DT == PIA_DTYPE_F16 ? 7.0f : 0.0f;
+constexpr float RESCALE = DT == PIA_DTYPE_F16 ? 1.0f : 8.0f;
+template <int DT>
+constexpr float SHIFT = DT == PIA_DTYPE_F16 ? 14.0f : 0.0f;
 
 template <int DT, int DP>
 struct Form {
@@ -106,38 +112,75 @@ __device__ __forceinline__ int steps_of(const Args& a, const Seq& s, int step) {
   return int(min(int64_t(total), nh + (span + step - 2) / step + 1));
 }
 
-// eight probabilities as two 16-bit operands
+// Eight probabilities as two 16-bit operands. fill ~0: neither is 0 for a positive one, but the least number;
+// 0: they may be.
 template <int DT>
-__device__ __forceinline__ void split2(const float (&p)[8], uint4 (&t)[2]) {
+__device__ __forceinline__ void split2(const float (&p)[8], uint4 (&t)[2], uint32_t fill) {
   typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
   uint32_t w[2][4];
 #pragma unroll
   for (int f = 0; f < 4; ++f) {
     float a = p[2 * f], b = p[2 * f + 1];
     const uint32_t low =
-        min(__float_as_uint(a), 1u) | (min(__float_as_uint(b), 1u) << 16);  // 1 where positive
-    uint32_t hi;
+        fill & (min(__float_as_uint(a), 1u) | (min(__float_as_uint(b), 1u) << 16));  // 1 where positive
+    auto filled = [&](uint32_t x) {
+      return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, x),
+                                                                    __builtin_bit_cast(u16x2_t, low)));
+    };
     if constexpr (DT == PIA_DTYPE_F16) {
       const auto h = __builtin_amdgcn_cvt_pkrtz(a, b);
-      hi = __builtin_bit_cast(uint32_t, h);
       a -= float(h[0]);
       b -= float(h[1]);
-      hi = __builtin_bit_cast(uint32_t,
-                              __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, hi),
-                                                        __builtin_bit_cast(u16x2_t, low)));
-    } else {
-      hi = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
+      w[0][f] = filled(__builtin_bit_cast(uint32_t, h));
+    } else {  // truncated to 0 below 2^-126 alone
+      w[0][f] = __builtin_amdgcn_perm(__float_as_uint(b), __float_as_uint(a), 0x07060302u);
       a -= bf16_hi(__float_as_uint(a));
       b -= bf16_hi(__float_as_uint(b));
     }
-    w[0][f] = hi;
-    w[1][f] = __builtin_bit_cast(
-        uint32_t,
-        __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, tile::pack16x2<DT>(a, b)),
-                                  __builtin_bit_cast(u16x2_t, low)));
+    w[1][f] = filled(tile::pack16x2<DT>(a, b));
   }
 #pragma unroll
   for (int k = 0; k < 2; ++k) t[k] = make_uint4(w[k][0], w[k][1], w[k][2], w[k][3]);
+}
+
+// fp16, of probabilities below 2^-10, in 2^38ths (2^-25 at most, so 2^13 of them): what rounding to two terms
+// took or, if `least`, minus the least numbers that split2 put in.
+constexpr float REST_BELOW = 0x1p-10f, REST = 0x1p38f, PUT = 0x1p14f;
+__device__ __forceinline__ uint4 rest2(const float (&p)[8], bool least) {
+  uint32_t w[4];
+#pragma unroll
+  for (int f = 0; f < 4; ++f) {
+    float y[2];
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float x = p[2 * f + e];
+      asm volatile("" : "+v"(x));  // so that nothing of this is kept for split2, which costs registers
+      const float hi = float(__builtin_amdgcn_cvt_pkrtz(x, x)[0]);
+      const float lo = float(static_cast<_Float16>(x - hi));
+      y[e] = least ? (hi == 0.f ? -PUT : 0.f) + (lo == 0.f ? -PUT : 0.f) : (x - hi - lo) * REST;
+      y[e] = x > 0.f && x < REST_BELOW ? y[e] : 0.f;
+    }
+    w[f] = tile::pack16x2<PIA_DTYPE_F16>(y[0], y[1]);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+
+// sum of eight fp16 numbers' squares onto c: finite if they all are
+__device__ __forceinline__ float squares(const uint4& x, float c) {
+  typedef _Float16 h2 __attribute__((ext_vector_type(2)));
+  const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    c = __builtin_amdgcn_fdot2(__builtin_bit_cast(h2, w[i]), __builtin_bit_cast(h2, w[i]), c, false);
+  return c;
+}
+// zeros for those that are not finite
+__device__ __forceinline__ uint4 finite_of(const uint4& x) {
+  auto of = [](uint32_t w) {
+    return w & (((w & 0x7c00u) == 0x7c00u ? 0u : 0xffffu) |
+                ((w & 0x7c000000u) == 0x7c000000u ? 0u : 0xffff0000u));
+  };
+  return make_uint4(of(x.x), of(x.y), of(x.z), of(x.w));
 }
 
 // UB bytes of a row
@@ -681,7 +724,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
 #pragma unroll
       for (int v = 0; v < 4; ++v) mx = __builtin_elementwise_maximum(mx, s[c][v]);
     mx = tile::maximum_col4(mx);
-    const float mref = mx - m > RESCALE || mx != mx ? mx : m;
+    const float mref = mx - m > RESCALE<DT> || mx != mx ? mx : m;
     if (__ballot(m != mref)) {
       const float alpha = reach::weight(m, mref);
       l *= alpha;
@@ -747,18 +790,62 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
           for (int n = 0; n < 2; ++n) acc[n0 + n] += t[n];
         }
       } else {
+        // fp16: whether there are positive ones that need more than two terms, and whether V is finite
+        bool rest = false, finite = true;
+        if constexpr (DT == PIA_DTYPE_F16) {
+          uint32_t least = ~0u;  // of the positive ones, less one
 #pragma unroll
-        for (int u = 0; u < NU; ++u) {
-          float p[8];
+          for (int c = 0; c < TU; ++c)
+#pragma unroll
+            for (int v = 0; v < 4; ++v) least = min(least, __float_as_uint(s[c][v]) - 1u);
+          rest = __ballot(least < __float_as_uint(REST_BELOW) - 1u) != 0;
+          if (__builtin_expect(rest, 0)) {
+            float z[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) z[nb & 3] = squares(vr[u][nb], z[nb & 3]);
+            finite = __ballot(!((z[0] + z[1]) + (z[2] + z[3]) < INFINITY)) == 0;
+          }
+        }
+        const uint32_t fill = rest && finite ? 0u : ~0u;
+        auto probabilities = [&](int u, float (&p)[8]) {
 #pragma unroll
           for (int e = 0; e < 8; ++e)
             p[e] = F::UB == 8 ? s[e & 3][2 * u + (e >> 2)] : s[e & 1][e >> 1];
+        };
+#pragma unroll
+        for (int u = 0; u < NU; ++u) {
+          float p[8];
+          probabilities(u, p);
           uint4 t[2];
-          split2<DT>(p, t);
+          split2<DT>(p, t, fill);
 #pragma unroll
           for (int k = 1; k >= 0; --k)
 #pragma unroll
             for (int nb = 0; nb < NB; ++nb) acc[nb] = tile::mfma16<DT>(vr[u][nb], t[k], acc[nb]);
+        }
+        if (__builtin_expect(rest, 0)) {
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) acc[nb] *= REST;
+          if (!finite) {  // infinities have entered already
+#pragma unroll
+            for (int u = 0; u < NU; ++u)
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) vr[u][nb] = finite_of(vr[u][nb]);
+          }
+#pragma unroll 1
+          for (int put = 0; put < (finite ? 1 : 2); ++put)
+#pragma unroll
+            for (int u = 0; u < NU; ++u) {
+              float p[8];
+              probabilities(u, p);
+              const uint4 z = rest2(p, put != 0);
+#pragma unroll
+              for (int nb = 0; nb < NB; ++nb) acc[nb] = tile::mfma16<DT>(vr[u][nb], z, acc[nb]);
+            }
+#pragma unroll
+          for (int nb = 0; nb < NB; ++nb) acc[nb] *= 1.f / REST;
         }
       }
     } else if constexpr (!ALIKE) {

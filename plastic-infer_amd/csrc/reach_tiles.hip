@@ -1,5 +1,5 @@
 // Windowed attention and attention behind a shared prefix for many query rows per key, on tiles in LDS:
-// bf16 or fp16 (DT), head_dim to 128 (DP: 64, 96, 128), pages in multiples of 16 tokens.
+// bf16 or fp16 (DT), head_dim to 256 (DP: 64, 96, 128, 256), pages in multiples of 16 tokens.
 //
 // Work item (one workgroup of NW waves): one kv head and 32 NW / G consecutive query positions of one
 // sequence, i.e. up to 32 NW (position, q head) rows that share the kv head's keys: row r is position
@@ -18,7 +18,7 @@
 //                  needs no exchange between lanes.
 // The probabilities are rounded to DT once, and the sum is of the rounded ones: half a step of DT each,
 // as much as the result's own rounding. fp16 numbers are scaled by up to 2^15 and normal to 2^-25 of the
-// reference; a tile with smaller ones multiplies what rounding took of them too, in 2^24ths.
+// reference; a tile with smaller ones multiplies what rounding took of them too.
 //
 // LDS tiles (16-byte units, XORed with a term of their row). The pool's rows are [d][token]. V is staged as
 // it is: [d][64 tokens], unit u (tokens 8 u .. + 7) at u ^ d / 2 % 8; a wave's lanes take the rows of 1 KB in the
@@ -30,6 +30,10 @@
 
 #include "attn_tiles.h"
 #include "reach.h"
+
+// A lambda that is not inlined keeps all that it captures in memory: the compiler left the largest of DP 256 as
+// calls (8 x 1024 rows, 16 heads, 8192 keys each: 9200 us with them, 1914 without)
+#define RT_INLINE __attribute__((always_inline))
 
 namespace pia {
 namespace {
@@ -44,6 +48,7 @@ constexpr int RT_MAX_SEQS = 1024;    // sequences per launch (item prefix in LDS
 constexpr int RT_AHEAD = 4;          // LDS operands read ahead of their product
 constexpr int RT_PV_VALU = 2;        // vector instructions after each product of the outputs
 constexpr int RT_MAX_CUTS = 64;      // pieces of an item
+constexpr int RT_MAX_BLOCKS = 1 << 22;  // items of a call (a launch of 2^32 threads is refused)
 constexpr int RT_RSRC_WORD3 = 0x00020000;
 // log2: how far a row's maximum may run ahead of its reference, and what the reference's probability is
 template <int DT>
@@ -51,7 +56,8 @@ constexpr float RT_RESCALE = DT == PIA_DTYPE_F16 ? 4.0f : 8.0f;
 template <int DT>
 constexpr float RT_SHIFT = DT == PIA_DTYPE_F16 ? 11.0f : 0.0f;
 constexpr float RT_LEAST_HALF = 6.103515625e-5f;  // 2^-14: the least normal number
-constexpr float RT_REST = 16777216.f;             // 2^24, one over the least number
+constexpr float RT_REST = 0x1p38f;  // what such numbers' rounding takes, 2^-25, is 2^13 of its units
+constexpr uint32_t RT_PUT = 0xf400u;  // minus the least number, 2^-24, in them: -2^14
 
 struct TileArgs : Args {
   int ppt, cuts;
@@ -88,10 +94,10 @@ __device__ __forceinline__ float swap_halves(float x) {  // the value of lane l 
 }
 
 template <int DP, int NW, int DT>
-__global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a) {
+__global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 8 / NW) void reach_tiles_kernel(TileArgs a) {
   constexpr int NT = 64 * NW, KS = DP / 16, NB = DP / 32, NU = DP / 8;
-  constexpr int UK = DP > 64 ? 16 : 8;  // 16-byte units of a K row in LDS
-  constexpr int TL = DP > 64 ? 4 : 2;   // tokens of a lane's K loads
+  constexpr int UK = DP > 128 ? 32 : DP > 64 ? 16 : 8;  // 16-byte units of a K row in LDS
+  constexpr int TL = DP > 128 ? 8 : DP > 64 ? 4 : 2;    // tokens of a lane's K loads
   constexpr bool SPLIT = NW == 8;  // waves 0-3 stage K, 4-7 V; with four waves each stages both
   constexpr bool HALF = DT == PIA_DTYPE_F16;
   constexpr uint32_t K_BUF = RT_KT * UK * 16, V_BUF = DP * 128;  // bytes
@@ -297,7 +303,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   const int blk = wave & 3;
   constexpr int KL = 8, VL = DP / 32;  // loads of a lane
   struct Part {
-    uint4 x[4];
+    uint32_t w[DP > 128 ? 32 : 16];
   };
   const int du = lane % NU, tg = lane / NU;  // K: unit and token group
   const bool k_lane = DP != 96 || tg < 4;
@@ -318,9 +324,14 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     const int id = __builtin_amdgcn_readlane(ids, blk), kb = (first_token(it) >> 4) + blk;
     const int sub = PB == 1 ? 0 : kb % PB;
     const bool ok = uint32_t(id) < np;
-    // elements behind head_dim lie past the descriptor's end, and are zeros
-    return __builtin_amdgcn_make_buffer_rsrc(const_cast<char*>(pool) + (ok ? id : 0) * page_bytes + sub * 32,
-                                             0, ok ? tile_bytes - sub * 32 : 0, RT_RSRC_WORD3);
+    // elements behind head_dim lie past the descriptor's end, and are zeros. In scalar registers by force: the
+    // compiler kept the descriptors of DP 256 in vector registers, with a loop around every load
+    const uint64_t at = reinterpret_cast<uint64_t>(pool) + (ok ? id : 0) * page_bytes + sub * 32;
+    const uint32_t lo = __builtin_amdgcn_readfirstlane(uint32_t(at)),
+                   hi = __builtin_amdgcn_readfirstlane(uint32_t(at >> 32));
+    return __builtin_amdgcn_make_buffer_rsrc(
+        reinterpret_cast<void*>(uint64_t(hi) << 32 | lo), 0,
+        __builtin_amdgcn_readfirstlane(ok ? tile_bytes - sub * 32 : 0), RT_RSRC_WORD3);
   };
   // a lane's term, hidden, so that what is added to it is added at its use: kept for all uses, the sums were
   // spilled, and a wait for a spilled register is one for every load before it
@@ -328,36 +339,38 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     asm volatile("" : "+v"(x));
     return x;
   };
-  // word i of a part (a constant)
-  auto word = [](Part& p, int i) -> uint32_t& {
-    uint4& x = p.x[i >> 2];
-    return (i & 3) == 0 ? x.x : (i & 3) == 1 ? x.y : (i & 3) == 2 ? x.z : x.w;
-  };
-  auto fetch_k = [&](Part& p, int ids, int it) {
+  auto fetch_k = [&](Part& p, int ids, int it) RT_INLINE {
     const auto rs = rsrc(kp, ids, it);
     const uint32_t o = now(k_off);
 #pragma unroll
     for (int e = 0; e < KL; ++e) {
       const uint32_t at = o + uint32_t(e * NU) * row_bytes;
-      if constexpr (TL == 4) {
+      if constexpr (TL == 8) {
+        const auto y = __builtin_amdgcn_raw_buffer_load_b128(rs, at, 0, 0);
+#pragma unroll
+        for (int c = 0; c < 4; ++c) p.w[4 * e + c] = y[c];
+      } else if constexpr (TL == 4) {
         const auto y = __builtin_amdgcn_raw_buffer_load_b64(rs, at, 0, 0);
-        word(p, 2 * e) = y[0];
-        word(p, 2 * e + 1) = y[1];
+        p.w[2 * e] = y[0];
+        p.w[2 * e + 1] = y[1];
       } else {
-        word(p, e) = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
+        p.w[e] = __builtin_amdgcn_raw_buffer_load_b32(rs, at, 0, 0);
       }
     }
   };
-  auto fetch_v = [&](Part& p, int ids, int it) {
+  auto fetch_v = [&](Part& p, int ids, int it) RT_INLINE {
     const auto rs = rsrc(vp, ids, it);
     const uint32_t o = now(v_off);
 #pragma unroll
-    for (int i = 0; i < VL; ++i)
-      p.x[i] = __builtin_bit_cast(
-          uint4, __builtin_amdgcn_raw_buffer_load_b128(rs, o + uint32_t(32 * i) * row_bytes, 0, 0));
+    for (int i = 0; i < VL; ++i) {
+      const auto y =
+          __builtin_amdgcn_raw_buffer_load_b128(rs, o + uint32_t(32 * i) * row_bytes, 0, 0);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) p.w[4 * i + c] = y[c];
+    }
   };
   auto put = [&](uint32_t at, const uint4& x) { *reinterpret_cast<uint4*>(lds + at) = x; };
-  auto stage_k = [&](Part& p, int buf) {
+  auto stage_k = [&](Part& p, int buf) RT_INLINE {
     if (!k_lane) return;
     const uint32_t o = now(k_st) + buf * K_BUF;
 #pragma unroll
@@ -365,25 +378,26 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       uint32_t w[4];
 #pragma unroll
       for (int f = 0; f < 4; ++f)
-        w[f] = __builtin_amdgcn_perm(word(p, (2 * f + 1) * (TL / 2) + (t >> 1)),
-                                     word(p, 2 * f * (TL / 2) + (t >> 1)),
+        w[f] = __builtin_amdgcn_perm(p.w[(2 * f + 1) * (TL / 2) + (t >> 1)],
+                                     p.w[2 * f * (TL / 2) + (t >> 1)],
                                      (t & 1) ? 0x07060302u : 0x05040100u);
-      // row t on, whose swizzle differs by t (DP 64: by none)
-      put(((o ^ (DP > 64 ? 16 * t : 0)) + t * UK * 16), make_uint4(w[0], w[1], w[2], w[3]));
+      // so many rows on, by which the swizzle differs too (DP 64: by none)
+      const int c = (t & 3) + 2 * (t & 4);
+      put(((o ^ (DP > 64 ? 16 * c : 0)) + c * UK * 16), make_uint4(w[0], w[1], w[2], w[3]));
     }
   };
   // kind 0: V itself, but zeros for what is not finite on tiles that some row does not see whole (zero
   // times it would be NaN there; the end of the item puts it where it belongs); 1, 2, 3: a one where V is
   // NaN, infinite, minus infinite
   constexpr uint32_t EXP = HALF ? 0x7c00u : 0x7f80u, ONE = HALF ? 0x3c00u : 0x3f80u;
-  auto stage_v = [&](Part& p, int buf, int it, int kind) {
+  auto stage_v = [&](Part& p, int buf, int it, int kind) RT_INLINE {
     bool look = kind != 0;
     if (!kind && !seen_whole(it)) {
       // a half that is not finite carries into its top bit: |x| + 2^(mantissa bits) >= 2^15
       uint32_t top = 0;
 #pragma unroll
       for (int i = 0; i < 4 * VL; ++i)
-        top |= (word(p, i) & 0x7fff7fffu) + (HALF ? 0x04000400u : 0x00800080u);
+        top |= (p.w[i] & 0x7fff7fffu) + (HALF ? 0x04000400u : 0x00800080u);
       look = __ballot((top & 0x80008000u) != 0) != 0;
     }
     if (look) {
@@ -391,7 +405,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       uint32_t odd = 0;
 #pragma unroll
       for (int i = 0; i < 4 * VL; ++i) {
-        uint32_t& w = word(p, i);
+        uint32_t& w = p.w[i];
         // 0xffff for each half that is not finite
         const uint32_t bad = ((w & EXP) == EXP ? 0xffffu : 0u) |
                              ((w & (EXP << 16)) == EXP << 16 ? 0xffff0000u : 0u);
@@ -411,7 +425,8 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     }
     const uint32_t o = now(v_st) + buf * V_BUF;
 #pragma unroll
-    for (int i = 0; i < VL; ++i) put(o + 4096 * i, p.x[i]);
+    for (int i = 0; i < VL; ++i)
+      put(o + 4096 * i, make_uint4(p.w[4 * i], p.w[4 * i + 1], p.w[4 * i + 2], p.w[4 * i + 3]));
   };
   // Operand addresses (bytes): the swizzle terms of rows 32 apart are the same, and the unit's upper
   // bits enter by XOR, so one base per lane and a constant give any of them
@@ -434,7 +449,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     for (int v = 0; v < 16; ++v) acc[nb][v] = 0.f;
 
   // scores of a tile from its K, on their own
-  auto scores = [&](f32x16_t (&sc)[2], int buf) {
+  auto scores = [&](f32x16_t (&sc)[2], int buf) RT_INLINE {
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
 #pragma unroll
@@ -451,7 +466,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       for (int v = 0; v < 16; ++v) mx = __builtin_elementwise_maximum(mx, sc[tb][v]);
     return mx;
   };
-  auto hide = [&](f32x16_t (&sc)[2], int it, int there) {  // what the row may not see
+  auto hide = [&](f32x16_t (&sc)[2], int it, int there) RT_INLINE {  // what the row may not see
     const Reach x = reach_of_row(it);
 #pragma unroll
     for (int tb = 0; tb < 2; ++tb)
@@ -471,7 +486,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   // the next tile's on return. A wave keeps its matrix core and its vector ALU busy at once: the
   // next tile's scores are multiplied while this one's become probabilities, and this one's
   // outputs while the tile after is staged.
-  auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int it, int buf, int there) {
+  auto turn = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], float& mx, int it, int buf, int there) RT_INLINE {
     if (!(there == 0xf && seen_whole(it))) {
       hide(sc, it, there);
       mx = largest(sc);
@@ -524,43 +539,57 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
     };
     if constexpr (HALF) {
       order_scores();
-      // what rounding took of probabilities below the normal numbers, in 2^24ths; a positive one is
-      // never 0, which an infinite V would make NaN
-      if (__ballot(least < RT_LEAST_HALF)) {
-        typedef unsigned short u16x2_t __attribute__((ext_vector_type(2)));
+      // What rounding took of probabilities below the normal numbers, in 2^38ths. Where V is not finite, a
+      // positive one may not be 0, which would make NaN of an infinity: the least number is put in for it,
+      // and taken off again where V is finite.
+      if (__builtin_expect(__ballot(least < RT_LEAST_HALF) != 0, 0)) {
 #pragma unroll
         for (int s4 = 0; s4 < 4; ++s4) {
           __builtin_amdgcn_sched_barrier(0);  // one operand at a time (registers)
           uint32_t z[4];
           uint32_t any = 0;
+          auto word = [&](int i) -> uint32_t& {
+            return i == 0 ? pk[s4].x : i == 1 ? pk[s4].y : i == 2 ? pk[s4].z : pk[s4].w;
+          };
+          auto p = [&](int i) { return sc[s4 >> 1][8 * (s4 & 1) + i]; };
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
-            uint32_t& w = i == 0 ? pk[s4].x : i == 1 ? pk[s4].y : i == 2 ? pk[s4].z : pk[s4].w;
-            const float p0 = sc[s4 >> 1][8 * (s4 & 1) + 2 * i], p1 = sc[s4 >> 1][8 * (s4 & 1) + 2 * i + 1];
-            const float x0 = (p0 - half_to_f32(uint16_t(w))) * RT_REST;
-            const float x1 = (p1 - half_to_f32(uint16_t(w >> 16))) * RT_REST;
-            z[i] = tile::pack16x2<DT>(p0 < RT_LEAST_HALF ? x0 : 0.f, p1 < RT_LEAST_HALF ? x1 : 0.f);
+            const uint32_t w = word(i);
+            auto left = [&](float x, uint32_t half) {
+              return x < RT_LEAST_HALF ? (x - half_to_f32(uint16_t(half))) * RT_REST : 0.f;
+            };
+            z[i] = tile::pack16x2<DT>(left(p(2 * i), w), left(p(2 * i + 1), w >> 16));
             any |= z[i] & 0x7fff7fffu;
-            const uint32_t low =
-                min(__float_as_uint(p0), 1u) | (min(__float_as_uint(p1), 1u) << 16);
-            w = __builtin_bit_cast(uint32_t,
-                                   __builtin_elementwise_max(__builtin_bit_cast(u16x2_t, w),
-                                                             __builtin_bit_cast(u16x2_t, low)));
           }
           if (!__ballot(any != 0)) continue;
+          bool odd = false;
+          auto add = [&]() {
 #pragma unroll
-          for (int nb = 0; nb < NB; ++nb) {
-            __builtin_amdgcn_sched_barrier(0);
-            f32x16_t t;
+            for (int nb = 0; nb < NB; ++nb) {
+              __builtin_amdgcn_sched_barrier(0);
+              f32x16_t t;
 #pragma unroll
-            for (int v = 0; v < 16; ++v) t[v] = 0.f;
-            t = mfma32<DT>(vread(buf, nb, s4), make_uint4(z[0], z[1], z[2], z[3]), t);
+              for (int v = 0; v < 16; ++v) t[v] = 0.f;
+              t = mfma32<DT>(vread(buf, nb, s4), make_uint4(z[0], z[1], z[2], z[3]), t);
 #pragma unroll
-            for (int v = 0; v < 16; ++v) {
-              // an infinite V enters by the first terms alone
-              const float y = t[v] * (1.f / RT_REST);
-              acc[nb][v] += fabsf(y) < INFINITY ? y : 0.f;
+              for (int v = 0; v < 16; ++v) {
+                const bool fine = fabsf(t[v]) < INFINITY;
+                odd |= !fine;
+                acc[nb][v] += fine ? t[v] * (1.f / RT_REST) : 0.f;
+              }
             }
+          };
+          add();
+          if (__ballot(odd)) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              uint32_t& w = word(i);
+              const uint32_t put = (p(2 * i) > 0.f && !(w & 0xffffu) ? 1u : 0u) |
+                                   (p(2 * i + 1) > 0.f && !(w >> 16) ? 0x10000u : 0u);
+              w |= put;
+              z[i] = put * RT_PUT;
+            }
+            add();
           }
         }
       }
@@ -585,7 +614,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   Part pa, pb;  // SPLIT: K or V in pa; else K in pa, V in pb
   int w0 = where(kt0), w1 = where(kt0 + 1), w2 = where(kt0 + 2), w3 = where(kt0 + 3);
   // K of tile it_k and V of the one before (with eight waves a wave has one of them)
-  auto fetch = [&](int wk, int wv, int it_k) {
+  auto fetch = [&](int wk, int wv, int it_k) RT_INLINE {
     if constexpr (SPLIT) {
       if (first4) fetch_k(pa, wk, it_k);
       else fetch_v(pa, wv, it_k - 1);
@@ -594,7 +623,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
       fetch_v(pb, wv, it_k - 1);
     }
   };
-  auto stage = [&](int buf_k, int buf_v, int it_v) {
+  auto stage = [&](int buf_k, int buf_v, int it_v) RT_INLINE {
     if constexpr (SPLIT) {
       if (first4) stage_k(pa, buf_k);
       else stage_v(pa, buf_v, it_v, 0);
@@ -616,7 +645,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void reach_tiles_kernel(TileArgs a
   f32x16_t sa[2], sb[2];
   scores(sa, 0);
   float mx = largest(sa);
-  auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int it, int buf) {
+  auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int it, int buf) RT_INLINE {
     const int there = int(__ballot(lane < 4 && uint32_t(w0) < np)) & 0xf;
     const int w4 = where(it + 4);
     turn(sc, sn, mx, it, buf, there);
@@ -754,7 +783,8 @@ void launch(const TileArgs& a, unsigned blocks, hipStream_t s) {
 
 bool reach_tiles_shape(const Args& a, int dtype) {
   // scale > 0: the kernel keeps its references in units of the products
-  return dtype != PIA_DTYPE_F32 && a.D <= 128 && a.scale_log2 > 0.f && a.G <= 128;
+  return dtype != PIA_DTYPE_F32 && a.D <= 256 && a.scale_log2 > 0.f && a.G <= 128 &&
+         (ceil_div(a.rows, 128 / a.G) + std::max(a.B, a.groups)) * a.Hkv <= RT_MAX_BLOCKS;
 }
 
 reach::TilePlan reach_tiles_plan(const Args& a, int64_t tokens, int64_t most) {
@@ -786,10 +816,10 @@ int launch_reach_tiles(const Args& args, int dtype, reach::TilePlan plan, hipStr
     a.count = std::min(n - b0, RT_MAX_SEQS);
     const int64_t blocks =
         ceil_div((ceil_div(a.rows, a.ppt) + a.count) * cuts * a.Hkv, 8) * 8;
-    if (blocks > (1 << 22)) return fail(PIA_EINVAL, "attention: too many query rows");
 #define PIA_RT(DT)                                                 \
   {                                                                \
     if (wide) launch<128, 8, DT>(a, unsigned(blocks), s);          \
+    else if (a.D > 128) launch<256, 4, DT>(a, unsigned(blocks), s); \
     else if (a.D > 96) launch<128, 4, DT>(a, unsigned(blocks), s); \
     else if (a.D > 64) launch<96, 4, DT>(a, unsigned(blocks), s);  \
     else launch<64, 4, DT>(a, unsigned(blocks), s);                \

@@ -62,3 +62,27 @@ def test_windows_are_whole_numbers(window, sinks):
     bt, n = torch.zeros(1, 1, dtype=torch.int32), torch.ones(1, dtype=torch.int32)
     with pytest.raises(ValueError, match="whole number"):
         PW.paged_window_decode_attention(q, pool, pool, bt, n, window, sinks)
+
+
+def test_workspaces_that_do_not_do():
+    need = N.query("pia_window_attention_workspace_bytes", 64)
+    for bad in (dict(ws=None, wsb=need), dict(wsb=need - 1), dict(ws=SOME + 8, wsb=need), dict(wsb=0)):
+        with pytest.raises(N.NativeError, match="window_attention: workspace"):
+            _window(**bad)
+    need = N.query("pia_prefix_attention_workspace_bytes", 2, 4, 64)
+    for bad in (dict(ws=None, wsb=need), dict(wsb=need - 1), dict(ws=SOME + 8, wsb=need), dict(wsb=0)):
+        with pytest.raises(N.NativeError, match="prefix_attention: workspace"):
+            _prefix(**bad)
+
+
+def test_workspace_bytes():
+    def window(dim):
+        return N.query("pia_window_attention_workspace_bytes", dim)
+
+    def prefix(rows, heads, dim):
+        return N.query("pia_prefix_attention_workspace_bytes", rows, heads, dim)
+
+    assert window(64) > 0 and window(256) >= window(64)
+    assert window(33) == window(512) == 0        # the general kernel's
+    assert prefix(2, 4, 64) > window(64) and prefix(10 ** 6, 4, 64) > prefix(2, 4, 64)
+    assert prefix(2, 4, 33) == prefix(0, 4, 64) == 0
