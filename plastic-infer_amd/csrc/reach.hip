@@ -19,8 +19,14 @@ bool holds_rows(uintptr_t out, int64_t bytes, uintptr_t q, int64_t n, int64_t ro
   return r < n && from < int64_t(out) + bytes && from + row > int64_t(out);
 }
 
-// rows of a kv head and sequence (group) from which tiles in LDS take the call
+// (position, head) rows of a kv head and sequence (group) from which tiles in LDS take the call: a tile's 128
+// rows cost the same however few there are, the streaming kernel reads K and V again for every 16. 8 sequences of
+// 4096 tokens, 32 / 8 heads of 128, us (tiles, streaming): 32 rows 44 and 39, 64 rows 42 and 68.
 constexpr int64_t TILE_ROWS = 64;
+// the same for windows where there are sequences' heads for half of the compute units: 64 sequences of 2048
+// tokens, 16 rows 111 and 135, 24 rows 105 and 181 (window of 64: 17 and 45; heads of 64, 16 rows, 60 and 56)
+constexpr int64_t TILE_ROWS_MANY = 24;
+// (position, head) rows whose pieces a workspace has room for at least: 128 pieces of 128 rows and 4 heads
 constexpr int64_t PREFIX_ROWS = 65536;
 
 int elem_bytes(int dtype) { return dtype == PIA_DTYPE_F32 ? 4 : 2; }
@@ -97,7 +103,9 @@ int64_t prefix_bytes(int64_t rows, int Hq, int D) {
 
 // Whether n sequences (groups) have rows enough for tiles in LDS
 bool tiled(const reach::Args& a, int dtype, int64_t n) {
-  return reach_tiles_shape(a, dtype) && a.rows * a.G >= TILE_ROWS * n;
+  // not behind prefixes: there few rows of many sequences share the prefix's tiles as a group
+  const bool many = a.window && 2 * n * a.Hkv >= device_cus();
+  return reach_tiles_shape(a, dtype) && a.rows * a.G >= (many ? TILE_ROWS_MANY : TILE_ROWS) * n;
 }
 // Tiles for the sequences of a call, with pieces in `bytes` from dst on
 int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t bytes, hipStream_t s) {

@@ -47,9 +47,15 @@ using tile::f32x4_t;
 constexpr int MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
 constexpr int WG_WAVES = 4;
 constexpr int WGS_PER_CU = 2;   // two waves per SIMD
-constexpr int WHOLE = 3;        // steps of items that are not cut
+// Steps of items that are not cut where items outnumber the resident workgroups (32 / 8 heads of 128, us; not cut
+// for cut): 512 sequences, window of 128 (5 steps) 67.5 for 72, 128 sequences 27.7 for 31.5; a window of 192 (6) 87
+// for 90 and 39.8 for 34.6.
+constexpr int WHOLE = 5;
 constexpr int MAX_SPLITS = 64;  // workgroups of an item
-constexpr int ITEM_STEPS = 8;   // steps of a wave above which even ranges for all waves are better
+// Steps of a wave above which even ranges for all waves are better than items of workgroups' own. A window's
+// items are alike (64 sequences, 2048: 84 us for 102 in ranges; 16 sequences, 8192: 89 for 99); contexts need not
+// be, and the longest would be waited for.
+constexpr int ITEM_STEPS = 8, ITEM_STEPS_WINDOW = 16;
 constexpr int JOIN_MANY = 128, JOIN_FEW = 512;  // threads of the joining workgroups
 
 // log2: how far a row's maximum may run ahead of its reference, and what probabilities are scaled by. fp16's
@@ -1155,14 +1161,15 @@ constexpr int64_t PREF_BYTES = (MAX_SEQS + 1) * 8 + 248;  // whole 256 bytes
 
 // Into how many runs of steps, a workgroup's each, every item is cut (0: all items' steps over the resident
 // waves instead). A second step of a wave takes as long as the arrival and reading of another workgroup's piece
-// (3 us), so up to two of each wave are not cut; of more, each wave gets one where there are workgroups for it.
-inline int item_splits(int64_t items, int64_t steps) {
+// (3 us), so up to two of each wave are not cut (one sequence, window of 128: 9.2 us, cut 11.3); of more, each wave
+// gets one where there are workgroups for it.
+inline int item_splits(int64_t items, int64_t steps, bool window) {
   const int64_t slots = int64_t(device_cus()) * WGS_PER_CU;
   if (items > slots) return 0;
   if (steps <= 2 * WG_WAVES) return 1;
   const int64_t n = std::max<int64_t>(
       1, std::min(ceil_div(steps, WG_WAVES), std::min<int64_t>(slots / items, MAX_SPLITS)));
-  return ceil_div(steps, n * WG_WAVES) <= ITEM_STEPS ? int(n) : 0;
+  return ceil_div(steps, n * WG_WAVES) <= (window ? ITEM_STEPS_WINDOW : ITEM_STEPS) ? int(n) : 0;
 }
 
 template <int DT, int DP>
@@ -1214,7 +1221,7 @@ int launch_dtype(Args a, int64_t tokens, hipStream_t s) {
     const int64_t items = (a.cu || a.by_group ? (a.rows * a.G >> 4) + a.count + 1
                                               : int64_t(a.count) * ((a.G + 15) / 16)) * a.Hkv;
     if (items > 0x1fffffff) return fail(PIA_EINVAL, "attention: too many rows");
-    a.splits = item_splits(items, steps);
+    a.splits = item_splits(items, steps, a.window != 0);
     a.counters = reinterpret_cast<unsigned long long*>(a.pref);
     a.token = a.splits > 1 ? reach_token() : 0;
     if (a.D <= 64) launch_shape<DT, 64>(a, items, alike, s);
