@@ -2,8 +2,10 @@
 // head, which walks the keys that the row sees, 64 at a time, and no others. All products and sums in fp32.
 //
 // QK: a lane has a key (tokens are innermost in the pool, so lanes read neighbours), q is in LDS. PV: a
-// lane has elements lane + 64 i, the probabilities come from LDS. Nothing is shared between rows or heads;
-// the faster kernels take the common shapes, this one what is left.
+// lane has elements lane + 64 i, the probabilities come from LDS. Nothing is shared between rows or heads, so it
+// is bound by its loads of single elements, which every head of a group repeats. It takes what the faster kernels
+// do not: head_dim over 256 or not in multiples of 16, pages not in multiples of 16, addresses that are not
+// aligned to 16 bytes.
 #include <algorithm>
 
 #include "reach.h"

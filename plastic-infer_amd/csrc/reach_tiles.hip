@@ -8,6 +8,13 @@
 // those of the sinks or of the prefix, then the sequence's own that some row of the item sees. Where there are
 // few items, each is cut along its tiles into pieces (workgroups of their own) that are joined in order.
 //
+// Bound by the matrix cores, the exponentials and the LDS reads of both products, which a wave runs against each
+// other: 2.0 us for a tile of 256 rows on a CU, 1.07 PFLOP/s (a large product of the library: 1.22), and 13 us
+// around a workgroup's tiles: its search for its item, the first ids, rows and tiles one after the other, the
+// results. No LDS bank conflicts. 8 x 1024 rows, 32 / 8 heads, 8192 keys each: head_dim 128 1111 us in bf16 (0.99
+// PFLOP/s) and 1210 in fp16, 96 970 and 1083, 64 754 and 835 (half the products for the same exponentials); 16 / 4
+// heads of 256 1914 and 2120 (one wave to a SIMD). A window of 2048 of the chunks' own and earlier tokens: 360.
+//
 // Per tile each wave runs (v_mfma_f32_32x32x16: A rows and B columns are lane l % 32, k slots
 // 8 (l / 32) + e; of C, lane l has column l % 32 and rows 8 i + 4 (l / 32) + j, i, j < 4; hh = l / 32)
 //   S^T = K . q^T  K rows lie in LDS with bits 2 and 3 of the token exchanged, so that a lane has the
@@ -793,7 +800,8 @@ reach::TilePlan reach_tiles_plan(const Args& a, int64_t tokens, int64_t most) {
     return std::max<int64_t>(1, (ceil_div(a.rows, rows / a.G) + n / 2) * a.Hkv);
   };
   // Items of 256 rows, one on a CU, halve what is staged for a row, where there is work for 16 tiles on
-  // every CU; else of 128 rows, two on a CU.
+  // every CU (8 x 1024 rows, window of 2048: 362 us, by 128 rows 398; 256 rows on a prefix of 32768: 213
+  // for 235); else of 128 rows, two on a CU, of which one stages while the other starts.
   const int64_t items8 = items_of(256), items4 = items_of(128);
   const bool wide = a.D == 128 && a.G <= 128 && a.rows * a.G >= 192 * n && items8 * tiles >= 16 * cus;
   // Fewer items than CUs: their keys are cut into pieces, of 16 tiles at least, or of 4 to one on every CU
