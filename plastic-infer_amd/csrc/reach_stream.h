@@ -1170,16 +1170,25 @@ inline int64_t resident_waves() { return int64_t(device_cus()) * WGS_PER_CU * WG
 constexpr int64_t PREF_BYTES = (MAX_SEQS + 1) * 8 + 248;  // whole 256 bytes
 
 // Into how many runs of steps, a workgroup's each, every item is cut (0: all items' steps over the resident
-// waves instead). A second step of a wave takes as long as the arrival and reading of another workgroup's piece
-// (3 us), so up to two of each wave are not cut (one sequence, window of 128: 9.2 us, cut 11.3); of more, each wave
-// gets one where there are workgroups for it.
-inline int item_splits(int64_t items, int64_t steps, bool window) {
-  const int64_t slots = int64_t(device_cus()) * WGS_PER_CU;
+// waves instead). items: at most so many; likely: about so many. A second step of a wave takes as long as the
+// arrival and reading of another workgroup's piece (3 us), so up to two of each wave are not cut (one sequence,
+// window of 128: 9.2 us, cut 11.3). Of more, each wave gets one where a workgroup for each compute unit is enough
+// for that, else as many as that leaves it (4 sequences, window of 4096: 22 us, with two workgroups on each 32; 24
+// fp32 sequences, 500: 24 and 28): further ones share a unit's bandwidth and leave more pieces. One more where
+// that would leave a third of the units idle (16 sequences of 1 .. 6 rows: 19 us, without 22); two on each where a
+// wave's run would be too long.
+inline int item_splits(int64_t items, int64_t likely, int64_t steps, bool window) {
+  const int64_t cus = device_cus(), slots = cus * WGS_PER_CU;
   if (items > slots) return 0;
   if (steps <= 2 * WG_WAVES) return 1;
-  const int64_t n = std::max<int64_t>(
-      1, std::min(ceil_div(steps, WG_WAVES), std::min<int64_t>(slots / items, MAX_SPLITS)));
-  return ceil_div(steps, n * WG_WAVES) <= (window ? ITEM_STEPS_WINDOW : ITEM_STEPS) ? int(n) : 0;
+  const int64_t one = cus / likely;
+  for (const int64_t cut : {3 * one * likely < 2 * cus ? one + 1 : one, slots / items}) {
+    const int64_t n =
+        std::max<int64_t>(1, std::min({ceil_div(steps, WG_WAVES), cut, int64_t(MAX_SPLITS),
+                                       2 * WG_WAVES * slots / items}));  // the workspace's pieces
+    if (ceil_div(steps, n * WG_WAVES) <= (window ? ITEM_STEPS_WINDOW : ITEM_STEPS)) return int(n);
+  }
+  return 0;
 }
 
 template <int DT, int DP>
@@ -1231,7 +1240,10 @@ int launch_dtype(Args a, int64_t tokens, hipStream_t s) {
     const int64_t items = (a.cu || a.by_group ? (a.rows * a.G >> 4) + a.count + 1
                                               : int64_t(a.count) * ((a.G + 15) / 16)) * a.Hkv;
     if (items > 0x1fffffff) return fail(PIA_EINVAL, "attention: too many rows");
-    a.splits = item_splits(items, steps, a.window != 0);
+    // of the bound above, half an item of each sequence is not there
+    const int64_t likely =
+        std::max<int64_t>(1, items - (a.cu || a.by_group ? (a.count / 2 + 1) * int64_t(a.Hkv) : 0));
+    a.splits = item_splits(items, likely, steps, a.window != 0);
     a.counters = reinterpret_cast<unsigned long long*>(a.pref);
     a.token = a.splits > 1 ? reach_token() : 0;
     if (a.D <= 64) launch_shape<DT, 64>(a, items, alike, s);
