@@ -69,7 +69,7 @@ constexpr int ITEM_STEPS = 8, ITEM_STEPS_WINDOW = 16;
 constexpr int JOIN_MANY = 128, JOIN_FEW = 512;  // threads of the joining workgroups
 
 // log2: how far a row's maximum may run ahead of its reference, and what probabilities are scaled by. fp16's
-// numbers, to 2^15, then go down to 2^-38 of the reference (7 and 8 in place of 1 and 14: a window of 1024 before
+// numbers, to 2^15, then go down to 2^-38 of the reference (8 and 7 in place of 1 and 14: a window of 1024 before
 // one sequence with wide scores 14.7 us for 13.7, its steps nearly all with a rest).
 template <int DT>
 constexpr float RESCALE = DT == PIA_DTYPE_F16 ? 1.0f : 8.0f;
