@@ -652,6 +652,7 @@ __global__ __launch_bounds__(64 * NW, DP > 128 ? 1 : 8 / NW) void reach_tiles_ke
   f32x16_t sa[2], sb[2];
   scores(sa, 0);
   float mx = largest(sa);
+  __syncthreads();  // the first step stages K where these scores were read
   auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int it, int buf) RT_INLINE {
     const int there = int(__ballot(lane < 4 && uint32_t(w0) < np)) & 0xf;
     const int w4 = where(it + 4);
