@@ -529,6 +529,7 @@ __global__ __launch_bounds__(64 * NW, 8 / NW) void kv8_prefill_kernel(PrefillArg
   scores(sa, 0);
   unit_of(kt0);
   float mx = largest(sa);
+  __syncthreads();  // the first step stages K where these scores were read
   auto step = [&](f32x16_t (&sc)[2], f32x16_t (&sn)[2], int kt, int buf) {
     const int there = int(__ballot(lane < 4 && uint32_t(w0.id) < np)) & 0xf;
     const Where w4 = where(kt + 4);

@@ -105,7 +105,7 @@ def _conflicts(events):
     return bad
 
 
-@pytest.mark.parametrize("kernel", ["reach_tiles.hip"])
+@pytest.mark.parametrize("kernel", ["reach_tiles.hip", "kv8_prefill.hip"])
 def test_no_buffer_is_read_and_written_between_two_barriers(kernel):
     events = _pipeline((CSRC / kernel).read_text())
     # the test follows what it should: both buffers of K and V are written and read
