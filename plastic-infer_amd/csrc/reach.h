@@ -132,7 +132,7 @@ int launch_reach_stream_f32(const reach::Args& a, int64_t tokens, hipStream_t s)
 int launch_reach_stream_f16(const reach::Args& a, int64_t tokens, hipStream_t s);
 int launch_reach_stream_bf16(const reach::Args& a, int64_t tokens, hipStream_t s);
 // Tiles in LDS for 128 or 256 rows at a time (reach_tiles.hip), 16-bit pools: whether a call's shape is taken,
-// into how many pieces (at most `most`) it would cut each item of so many rows, and its launch. Pieces
+// into how many pieces (at most `most`) it would cut each item of such a call, and its launch. Pieces
 // go to dst; those of sequences are joined there, those of groups are not.
 bool reach_tiles_shape(const reach::Args& a, int dtype);
 reach::TilePlan reach_tiles_plan(const reach::Args& a, int64_t tokens, int64_t most);

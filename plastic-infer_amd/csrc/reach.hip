@@ -216,9 +216,11 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
     g.by_group = 1;
     const bool tiles = tiled(a, dtype, num_groups);
     const int64_t R = total_q_rows * num_heads;
-    const reach::TilePlan plan = reach_tiles_plan(
-        g, prefix_tokens, shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
-    const int cuts = tiles ? plan.cuts : 1;
+    reach::TilePlan plan{false, 1};  // a plan is of shapes that tiles take
+    if (tiles)
+      plan = reach_tiles_plan(g, prefix_tokens,
+                              shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
+    const int cuts = plan.cuts;
     g.dst = a.parts + parts / int64_t(sizeof(float));
     g.dst_ml = reinterpret_cast<float2*>(g.dst + (cuts + 1) * R * head_dim);
     rc = tiles ? launch_reach_tiles(g, dtype, plan, s) : stream_call(g, dtype, prefix_tokens, s);
