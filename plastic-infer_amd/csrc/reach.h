@@ -105,6 +105,34 @@ __device__ __forceinline__ int lowest(const Args& a, const Seq& s, int pos) {
   return int(max(int64_t(0), min(int64_t(FAR), int64_t(s.off) + pos + 1 - a.window)));
 }
 
+// Items of 16 (position, head) rows, whose tokens go by steps: a tile of `step` tokens each.
+__device__ __forceinline__ int items_of(int n, int G) { return int((int64_t(n) * G + 15) >> 4); }
+// Tiles of the sinks that some row sees
+__device__ __forceinline__ int head_tiles(const Args& a, const Seq& s, int step) {
+  if (!a.window) return 0;
+  return (min(a.sinks, limit(s, s.n - 1)) + step - 1) / step;
+}
+// Steps of each item of a sequence: as many as any of them needs
+__device__ __forceinline__ int steps_of(const Args& a, const Seq& s, int step) {
+  const int total = (limit(s, s.n - 1) + step - 1) / step;
+  if (!a.window) return total;
+  const int nh = head_tiles(a, s, step);
+  if (s.n == 1) return nh + max(0, total - max(nh, lowest(a, s, 0) / step));
+  // an item's rows are of 15 / G + 2 positions at most; that many tokens and the window's lie in so many tiles
+  const int64_t span = int64_t(a.window) + min(s.n, 15 / a.G + 2) - 1;
+  return int(min(int64_t(total), nh + (span + step - 2) / step + 1));
+}
+// The tile of an item's step t: nh tiles of the sinks, then those from t0 on. Items have steps past their own
+// tokens, and where positions come near 2^31 past all that 32 bits count: those are the tile at FAR, where no
+// token is.
+__device__ __forceinline__ int tile_of(int nh, int t0, int t, int step) {
+  return t < nh ? t : min(t0 + t - nh, FAR / step);
+}
+// Whether some row of an item sees a token of block kb (16 tokens), where they see the sinks' and lo .. end - 1
+__device__ __forceinline__ bool block_seen(const Args& a, int lo, int end, int kb) {
+  return kb * 16 < end && (!a.window || kb * 16 < a.sinks || kb * 16 + 16 > lo);
+}
+
 // The prefix's pieces of a row of sequence b, if it has any
 __device__ __forceinline__ bool has_prefix(const Args& a, int b) {
   const int g = group_of(a, b);

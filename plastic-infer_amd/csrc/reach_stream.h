@@ -52,6 +52,9 @@ namespace reach_stream {
 
 using reach::Args;
 using reach::Seq;
+using reach::head_tiles;
+using reach::items_of;
+using reach::steps_of;
 using tile::f32x4_t;
 
 constexpr int MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
@@ -111,23 +114,6 @@ constexpr int64_t part_floats = 16 * (DP + 2);  // 16 rows' outputs, references 
 __device__ __forceinline__ Seq seq_at(const Args& a, int b) {
   return a.by_group ? reach::group(a, a.first + b) : reach::sequence(a, a.first + b);
 }
-__device__ __forceinline__ int items_of(int n, int G) { return int((int64_t(n) * G + 15) >> 4); }
-// Tiles of the sinks that some row sees
-__device__ __forceinline__ int head_tiles(const Args& a, const Seq& s, int step) {
-  if (!a.window) return 0;
-  return (min(a.sinks, reach::limit(s, s.n - 1)) + step - 1) / step;
-}
-// Steps of each item of a sequence: as many as any of them needs
-__device__ __forceinline__ int steps_of(const Args& a, const Seq& s, int step) {
-  const int total = (reach::limit(s, s.n - 1) + step - 1) / step;
-  if (!a.window) return total;
-  const int nh = head_tiles(a, s, step);
-  if (s.n == 1) return nh + max(0, total - max(nh, reach::lowest(a, s, 0) / step));
-  // an item's rows are of 15 / G + 2 positions at most; that many tokens and the window's lie in so many tiles
-  const int64_t span = int64_t(a.window) + min(s.n, 15 / a.G + 2) - 1;
-  return int(min(int64_t(total), nh + (span + step - 2) / step + 1));
-}
-
 // Eight probabilities as two 16-bit operands. fill ~0: neither is 0 for a positive one, but the least number;
 // 0: they may be.
 template <int DT>
@@ -481,7 +467,7 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
     }
     open(c);
   };
-  auto tile_of = [&](const Cursor& c) { return c.t < c.nh ? c.t : c.t0 + c.t - c.nh; };
+  auto tile_of = [&](const Cursor& c) { return reach::tile_of(c.nh, c.t0, c.t, STEP); };
   int pieces = 0;  // ITEM: waves that have steps
   if constexpr (ITEM) {
     cur.nh = head_tiles(a, mine, STEP);
@@ -517,12 +503,8 @@ __global__ __launch_bounds__(64 * WG_WAVES, WGS_PER_CU) void reach_stream_kernel
   auto where = [&](const Cursor& c, bool real) {
     const int kb = tile_of(c) * MB + lane, slot = PB == 1 ? kb : kb / PB;
     Where r{-1, kb - slot * PB, c.h};
-    bool in = real && lane < MB && kb * 16 < c.end;
-    if (a.window && in) {
-      const Seq s = get(c.b);
-      in = kb * 16 < a.sinks || kb * 16 + 16 > reach::lowest(a, s, 16 * c.i / a.G);
-    }
-    if (in) r.id = table[int64_t(a.first + c.b) * stride + slot];
+    if (real && lane < MB && reach::block_seen(a, reach::lowest(a, get(c.b), 16 * c.i / a.G), c.end, kb))
+      r.id = table[int64_t(a.first + c.b) * stride + slot];
     return r;
   };
   // The element that a lane's block begins at, in the pool. Lanes of a block that is not there read another
