@@ -62,10 +62,10 @@ def rope_params(head_dim: int, base: float = 10000.0, rotary_dim: int | None = N
     if not 0 < base < math.inf:
         raise ValueError("base must be positive and finite")
     if sections is not None:
-        sections = [int(x) for x in sections]
+        given = tuple(sections)
+        sections = [int(x) if x == x // 1 else -1 for x in given]   # no parts of a pair
         if not sections or min(sections) < 0 or sum(sections) != rd // 2:
-            raise ValueError(f"sections must be counts that add up to the {rd // 2} pairs, got "
-                             f"{tuple(sections)}")
+            raise ValueError(f"sections must be counts that add up to the {rd // 2} pairs, got {given}")
     i = torch.arange(0, rd, 2, dtype=torch.float64)
     factor = 1.0
     kind = None if scaling is None else scaling.get("type")
