@@ -638,8 +638,16 @@ int pia_window_attention(void* out, const void* q, int64_t q_stride, const void*
  * is the first prefix_lens[g] tokens of prefix_tables[g] (pt_stride entries a row). Row s of sequence b
  * attends the whole prefix of b's group (none: no prefix) and the sequence's own keys j < kv_lens[b] of
  * block_tables[b], with q_pos_offsets j <= q_pos_offsets[b] + s. All else as pia_window_attention.
- * workspace: 16-byte aligned, of pia_prefix_attention_workspace_bytes for so many rows or more. */
+ * workspace: 16-byte aligned, of pia_prefix_attention_workspace_bytes for so many rows or more, which is
+ * enough for any call of them (its pieces of all rows are twice their outputs in fp32), or of what the call
+ * itself takes: pia_prefix_attention_call_workspace_bytes, with ragged for a call with cu_q. Many rows of each
+ * sequence over 16-bit pools take little or none. */
 int64_t pia_prefix_attention_workspace_bytes(int64_t total_q_rows, int num_heads, int head_dim);
+int64_t pia_prefix_attention_call_workspace_bytes(int num_groups, int64_t pt_stride,
+                                                  int64_t bt_stride, int ragged, int num_seqs,
+                                                  int64_t total_q_rows, int num_heads,
+                                                  int num_kv_heads, int head_dim, int page_size,
+                                                  float scale, int dtype);
 int pia_prefix_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
                          const void* v_pages, const int32_t* prefix_tables, int64_t pt_stride,
                          const int32_t* prefix_lens, const int32_t* cu_seqs, int num_groups,

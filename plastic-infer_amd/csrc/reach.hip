@@ -107,13 +107,42 @@ bool tiled(const reach::Args& a, int dtype, int64_t n) {
   const bool many = a.window && 2 * n * a.Hkv >= device_cus();
   return reach_tiles_shape(a, dtype) && a.rows * a.G >= (many ? TILE_ROWS_MANY : TILE_ROWS) * n;
 }
-// Tiles for the sequences of a call, with pieces in `bytes` from dst on
-int tile_call(reach::Args a, int dtype, int64_t tokens, float* dst, int64_t bytes, hipStream_t s) {
-  const reach::TilePlan plan =
-      reach_tiles_plan(a, tokens, bytes / piece_bytes(a.rows, a.Hq, a.D));
-  a.dst = plan.cuts > 1 ? dst : nullptr;
-  a.dst_ml = reinterpret_cast<float2*>(dst + plan.cuts * a.rows * a.Hq * a.D);
+// Tiles for the sequences of a call, with the plan's pieces from dst on
+int tile_call(reach::Args a, int dtype, reach::TilePlan plan, float* dst, hipStream_t s) {
+  if (plan.cuts > 1) {
+    a.dst = dst;
+    a.dst_ml = reinterpret_cast<float2*>(dst + plan.cuts * a.rows * a.Hq * a.D);
+  }
   return launch_reach_tiles(a, dtype, plan, s);
+}
+
+// How a prefix call runs, and the workspace that it takes. general: no workspace. tiles: for the sequences, the
+// prefix and their own keys as one list; a workspace for items that are cut, of which there are few rows.
+// Else the prefix's part of all rows as pieces of rows (by tiles or streaming), then the rest.
+struct PrefixRoute {
+  bool general, tiles, group_tiles;
+  reach::TilePlan plan;
+  int64_t bytes;
+};
+PrefixRoute prefix_route(reach::Args a, int dtype, bool ragged) {
+  PrefixRoute r{!streams(a, dtype), false, false, {false, 1}, 0};
+  if (r.general) return r;
+  const int64_t piece = piece_bytes(a.rows, a.Hq, a.D), parts = reach_stream_parts_bytes(a.D),
+                shared = prefix_bytes(a.rows, a.Hq, a.D);
+  const int64_t prefix_tokens = a.pt_stride * a.P;
+  r.tiles = ragged && tiled(a, dtype, a.B);
+  if (r.tiles) {  // they share their own keys' tiles too
+    r.plan = reach_tiles_plan(a, prefix_tokens + a.bt_stride * a.P, (parts + shared) / piece);
+    r.bytes = r.plan.cuts > 1 ? reach_stream_pref_bytes() + r.plan.cuts * piece : 0;
+    return r;
+  }
+  r.bytes = reach_stream_pref_bytes() + parts;
+  if (!a.groups) return r;
+  r.bytes += shared;
+  r.group_tiles = tiled(a, dtype, a.groups);
+  a.by_group = 1;
+  if (r.group_tiles) r.plan = reach_tiles_plan(a, prefix_tokens, shared / piece - 1);
+  return r;
 }
 
 }  // namespace
@@ -159,9 +188,11 @@ extern "C" int pia_window_attention(void* out, const void* q, int64_t q_stride, 
   // tokens that an item walks: the sinks' and the window's, of the table's
   const int64_t tokens = std::min(bt_stride * page_size,
                                   int64_t(window) + sinks + std::min<int64_t>(total_q_rows, 16));
-  if (cu_q && tiled(a, dtype, num_seqs))
-    return tile_call(a, dtype, tokens, a.parts, reach_stream_parts_bytes(head_dim),
-                     as_stream(stream));
+  if (cu_q && tiled(a, dtype, num_seqs)) {
+    const reach::TilePlan plan = reach_tiles_plan(
+        a, tokens, reach_stream_parts_bytes(head_dim) / piece_bytes(a.rows, a.Hq, a.D));
+    return tile_call(a, dtype, plan, a.parts, as_stream(stream));
+  }
   return stream_call(a, dtype, tokens, as_stream(stream));
 }
 
@@ -171,6 +202,28 @@ extern "C" int64_t pia_prefix_attention_workspace_bytes(int64_t total_q_rows, in
     return 0;
   return reach_stream_pref_bytes() + reach_stream_parts_bytes(head_dim) +
          prefix_bytes(total_q_rows, num_heads, head_dim);
+}
+
+extern "C" int64_t pia_prefix_attention_call_workspace_bytes(
+    int num_groups, int64_t pt_stride, int64_t bt_stride, int ragged, int num_seqs,
+    int64_t total_q_rows, int num_heads, int num_kv_heads, int head_dim, int page_size, float scale,
+    int dtype) {
+  if (num_seqs <= 0 || total_q_rows <= 0 || num_heads <= 0 || num_kv_heads <= 0 ||
+      num_heads % num_kv_heads || head_dim <= 0 || page_size <= 0 || pt_stride < 0 || bt_stride < 0)
+    return 0;
+  reach::Args a{};
+  a.rows = total_q_rows;
+  a.B = num_seqs;
+  a.Hq = num_heads;
+  a.Hkv = num_kv_heads;
+  a.G = num_heads / num_kv_heads;
+  a.D = head_dim;
+  a.P = page_size;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.pt_stride = pt_stride;
+  a.bt_stride = bt_stride;
+  a.groups = num_groups > 0 && pt_stride > 0 ? num_groups : 0;
+  return prefix_route(a, dtype, ragged != 0).bytes;
 }
 
 extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, const void* k_pages,
@@ -197,33 +250,23 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
                 head_dim, page_size, 0, 0, some ? prefix_tables : nullptr, pt_stride, prefix_lens,
                 cu_seqs, some ? num_groups : 0};
   int rc = check(a, dtype, "prefix_attention");
-  if (!rc)
-    rc = check_workspace(
-        workspace, workspace_bytes,
-        pia_prefix_attention_workspace_bytes(total_q_rows, num_heads, head_dim), "prefix_attention");
   if (rc) return rc < 0 ? rc : 0;
+  const PrefixRoute r = prefix_route(a, dtype, cu_q != nullptr);
+  rc = check_workspace(workspace, workspace_bytes, r.bytes, "prefix_attention");
+  if (rc) return rc;
   hipStream_t s = as_stream(stream);
-  if (!streams(a, dtype)) return launch_reach_general(a, dtype, s);
-  place(a, workspace);
-  const int64_t prefix_tokens = pt_stride * page_size, tokens = bt_stride * page_size;
-  const int64_t parts = reach_stream_parts_bytes(head_dim),
-                shared = prefix_bytes(total_q_rows, num_heads, head_dim);
-  // many rows of a sequence: they share their own keys' tiles too, and need no pieces
-  if (cu_q && tiled(a, dtype, num_seqs))
-    return tile_call(a, dtype, prefix_tokens + tokens, a.parts, parts + shared, s);
-  if (some) {  // the prefix's part of all rows, then the rest
+  if (r.general) return launch_reach_general(a, dtype, s);
+  if (r.bytes) place(a, workspace);
+  if (r.tiles) return tile_call(a, dtype, r.plan, a.parts, s);
+  if (some) {
     reach::Args g = a;
     g.by_group = 1;
-    const bool tiles = tiled(a, dtype, num_groups);
     const int64_t R = total_q_rows * num_heads;
-    reach::TilePlan plan{false, 1};  // a plan is of shapes that tiles take
-    if (tiles)
-      plan = reach_tiles_plan(g, prefix_tokens,
-                              shared / piece_bytes(total_q_rows, num_heads, head_dim) - 1);
-    const int cuts = plan.cuts;
-    g.dst = a.parts + parts / int64_t(sizeof(float));
+    const int cuts = r.plan.cuts;
+    g.dst = a.parts + reach_stream_parts_bytes(head_dim) / int64_t(sizeof(float));
     g.dst_ml = reinterpret_cast<float2*>(g.dst + (cuts + 1) * R * head_dim);
-    rc = tiles ? launch_reach_tiles(g, dtype, plan, s) : stream_call(g, dtype, prefix_tokens, s);
+    rc = r.group_tiles ? launch_reach_tiles(g, dtype, r.plan, s)
+                       : stream_call(g, dtype, pt_stride * page_size, s);
     if (rc) return rc;
     a.src = g.dst;
     a.src_ml = g.dst_ml;
@@ -231,5 +274,5 @@ extern "C" int pia_prefix_attention(void* out, const void* q, int64_t q_stride, 
     a.dst = g.dst + cuts * R * head_dim;
     a.dst_ml = g.dst_ml + cuts * R;
   }
-  return stream_call(a, dtype, tokens, s);
+  return stream_call(a, dtype, bt_stride * page_size, s);
 }

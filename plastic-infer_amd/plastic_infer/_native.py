@@ -91,13 +91,15 @@ _SIGNATURES: dict[str, tuple[object, list[object]]] = {
     "pia_window_attention": (_I, [_P, _P, _L, _P, _P, _P, _L, _P, _P, _P, _I, _I, _I, _L, _I, _I, _I,
                                   _I, _L, _F, _I, _P, _L, _P]),
     "pia_prefix_attention_workspace_bytes": (_L, [_L, _I, _I]),
+    "pia_prefix_attention_call_workspace_bytes": (_L, [_I, _L, _L, _I, _I, _L, _I, _I, _I, _I, _F,
+                                                       _I]),
     "pia_prefix_attention": (_I, [_P, _P, _L, _P, _P, _P, _L, _P, _P, _I, _P, _L, _P, _P, _P, _I, _L,
                                   _I, _I, _I, _I, _L, _F, _I, _P, _L, _P]),
     "pia_hbm_read_probe": (_I, [_P, _L, _P, _L, _P, _P]),
     "pia_hbm_read_rows_probe": (_I, [_P, _L, _I, _I, _P, _P]),
 }
 
-EXPECTED_ABI = 11
+EXPECTED_ABI = 12
 
 _HIP = torch.version.hip is not None
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)

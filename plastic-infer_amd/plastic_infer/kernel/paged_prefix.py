@@ -22,11 +22,17 @@ def _workspace_bytes(rows: int, num_heads: int, head_dim: int, device: int) -> i
         return N.query("pia_prefix_attention_workspace_bytes", rows, num_heads, head_dim)
 
 
+@functools.lru_cache(maxsize=1024)
+def _call_bytes(device: int, *call: int | float) -> int:
+    with torch.cuda.device(device):
+        return N.query("pia_prefix_attention_call_workspace_bytes", *call)
+
+
 def prefix_attention_workspace_bytes(rows: int, num_heads: int, head_dim: int,
                                      device: torch.device | None = None) -> int:
-    """Bytes of the workspace of both calls for so many query rows or fewer. Calls that share a
-    workspace must be ordered on one stream (a captured graph keeps using the one it was captured
-    with)."""
+    """Bytes of a workspace that does for every call of so many query rows or fewer: room for two pieces
+    of all rows in fp32. Calls that share a workspace must be ordered on one stream (a captured graph
+    keeps using the one it was captured with)."""
     index = torch.cuda.current_device() if device is None or device.index is None else device.index
     return _workspace_bytes(rows, num_heads, head_dim, index)
 
@@ -48,7 +54,8 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     outside the pool holds no keys. Rows behind the last sequence are left as they were in `out`, which
     may be q itself and must not overlap it otherwise.
     workspace: device memory of prefix_attention_workspace_bytes, kept between calls that are ordered
-    on one stream; allocated for the call where none (or too little) is given."""
+    on one stream; where none (or too little) is given, what the call takes is allocated for it: little
+    or nothing for many rows of each sequence over 16-bit pools."""
     dev, q, stride, out = checked_call(
         q, k_pages, v_pages, block_tables, kv_lens, cu_q, q_pos_offsets, out, workspace,
         {"prefix_tables": prefix_tables, "prefix_lens": prefix_lens, "cu_seqs": cu_seqs})
@@ -67,9 +74,13 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
         raise ValueError("cu_seqs must be int32 [groups + 1]")
     if rows == 0 or B == 0:
         return out
-    need = _workspace_bytes(rows, Hq, D, dev.index)
-    ws = scratch(workspace, need, dev)
     scale = (1.0 / math.sqrt(D)) if scale is None else float(scale)
+    need = _workspace_bytes(rows, Hq, D, dev.index)
+    if workspace is None or workspace.numel() * workspace.element_size() < need:
+        need = _call_bytes(dev.index, groups, prefix_tables.shape[1], block_tables.shape[1],
+                           int(cu_q is not None), B, rows, Hq, Hkv, D, P, scale,
+                           N.dtype_code(q.dtype))
+    ws = scratch(workspace, need, dev)
     pt, plens = prefix_tables.contiguous(), prefix_lens.contiguous()
     bt, lens = block_tables.contiguous(), kv_lens.contiguous()
     gs = None if cu_seqs is None else cu_seqs.contiguous()
