@@ -24,7 +24,8 @@ bool holds_rows(uintptr_t out, int64_t bytes, uintptr_t q, int64_t n, int64_t ro
 // 4096 tokens, 32 / 8 heads of 128, us (tiles, streaming): 32 rows 44 and 39, 64 rows 42 and 68.
 constexpr int64_t TILE_ROWS = 64;
 // the same for windows where there are sequences' heads for half of the compute units: 64 sequences of 2048
-// tokens, 16 rows 111 and 135, 24 rows 105 and 181 (window of 64: 17 and 45; heads of 64, 16 rows, 60 and 56)
+// tokens, 24 rows 105 and 181 (window of 64: 17 and 45). One number for every head_dim: with heads of 64 streaming
+// is ahead at 16 rows (60 and 56), with heads of 128 it is not (111 and 135, which such calls pay).
 constexpr int64_t TILE_ROWS_MANY = 24;
 // (position, head) rows whose pieces a workspace has room for at least: 128 pieces of 128 rows and 4 heads
 constexpr int64_t PREFIX_ROWS = 65536;
@@ -101,7 +102,9 @@ int64_t prefix_bytes(int64_t rows, int Hq, int D) {
   return std::max(2 * piece_bytes(rows, Hq, D), piece_bytes(PREFIX_ROWS, 1, D));
 }
 
-// Whether n sequences (groups) have rows enough for tiles in LDS
+// Whether n sequences (groups) have rows enough for tiles in LDS: on average, for the lengths are known on the
+// device alone. A call of 128 single rows and one chunk of 512 (window of 1024, 2048 tokens, 32 / 8 heads of 128)
+// streams them all, 178 us; apart the two take 139 and 39, the single rows without cu_q 108.
 bool tiled(const reach::Args& a, int dtype, int64_t n) {
   // not behind prefixes: there few rows of many sequences share the prefix's tiles as a group
   const bool many = a.window && 2 * n * a.Hkv >= device_cus();

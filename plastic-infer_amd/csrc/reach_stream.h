@@ -4,7 +4,8 @@
 // Bound by HBM where there is enough to read: K and V of the keys that some row sees, once (128 sequences, window
 // of 4096 on 512 .. 8192 tokens, 32 / 8 heads of 128, bf16: 283 us with the joining, 6.0 TB/s, 1.01 times the bytes);
 // small calls by their chain of dependent loads (lengths, page ids, K, V) and the launch: one sequence in a window
-// of 1024 13.3 us, of 64 8.7. An item is 16 (position, head) rows of a sequence (or of a group, over its
+// of 1024 13.3 us, of 64 8.7. Their waves wait for memory for half of their cycles (24 fp32 sequences in a window of
+// 500: 45 %, with 17 % in products; 16 sequences of 1 .. 6 rows: 57 % and 2 %). An item is 16 (position, head) rows of a sequence (or of a group, over its
 // prefix) and kv head; it walks the tiles that some of its rows see by steps of STEP tokens. The next step's K and
 // V are on their way while a step is computed. Two forms:
 //
@@ -59,7 +60,9 @@ using tile::f32x4_t;
 
 constexpr int MAX_SEQS = 1024;  // sequences per launch (their tables in LDS)
 constexpr int WG_WAVES = 4;
-constexpr int WGS_PER_CU = 2;   // two waves per SIMD
+// Two waves per SIMD. Ranges and runs are made for as many, also where LDS holds one workgroup on a CU: fp32 at
+// head_dim over 128 (89 to 99 KB) and items of rows that see different tokens there (89 KB) take them in two rounds.
+constexpr int WGS_PER_CU = 2;
 // Steps of items that are not cut where items outnumber the resident workgroups (32 / 8 heads of 128, us; not cut
 // for cut): 512 sequences, window of 128 (5 steps) 67.5 for 72, 128 sequences 27.7 for 31.5; a window of 192 (6) 87
 // for 90 and 39.8 for 34.6.
@@ -1210,7 +1213,9 @@ template <int DT>
 int launch_dtype(Args a, int64_t tokens, hipStream_t s) {
   const int n = a.by_group ? a.groups : a.B;
   const int step = a.D > 128 ? Form<DT, 256>::STEP : Form<DT, 128>::STEP;
-  // a window's tiles may begin and end within one
+  // As many as the tables have room for (lengths are on the device): short contexts under wide tables are cut as
+  // long ones (64 sequences of 300 tokens behind a prefix of 8192: 52 us, with tables of 4096 tokens 63, of
+  // 32768 69). A window's tiles may begin and end within one.
   const int64_t steps = std::min(ceil_div(tokens, step) + (a.window ? 2 : 0),
                                  ceil_div((a.by_group ? a.pt_stride : a.bt_stride) * a.P, step));
   a.whole = steps <= WHOLE;

@@ -52,7 +52,8 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     and, when q_pos_offsets is given, j <= q_pos_offsets[b] + s. q: [rows, Hq, D], rows of sequence b =
     cu_q[b]..cu_q[b+1] (cu_q None: one row per sequence). A row without a key is zeros; a page id
     outside the pool holds no keys. Rows behind the last sequence are left as they were in `out`, which
-    may be q itself and must not overlap it otherwise.
+    may be q itself and must not overlap it otherwise. Probabilities as in paged_window_attention;
+    here many rows of a group are enough.
     workspace: device memory of prefix_attention_workspace_bytes, kept between calls that are ordered
     on one stream; where none (or too little) is given, what the call takes is allocated for it: little
     or nothing for many rows of each sequence over 16-bit pools."""

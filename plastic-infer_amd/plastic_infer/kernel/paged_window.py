@@ -115,7 +115,8 @@ def paged_window_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     are the context's last) and attends the keys j < kv_lens[b], j <= p with p - j < window or
     j < sinks. A row without a key is zeros; a page id outside the pool holds no keys. Rows behind the
     last sequence are left as they were in `out`, which may be q itself and must not overlap it
-    otherwise.
+    otherwise. Probabilities are held to 2^-16 of each or better; calls of many rows for each sequence, on
+    average, over 16-bit pools round them once to the pool's type.
     workspace: device memory of window_attention_workspace_bytes, kept between calls that are ordered
     on one stream; allocated for the call where none (or too little) is given."""
     window, sinks = _whole("window", window, 1), _whole("sinks", sinks, 0)
