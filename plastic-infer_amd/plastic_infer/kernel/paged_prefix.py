@@ -76,11 +76,8 @@ def paged_prefix_attention(q: torch.Tensor, k_pages: torch.Tensor, v_pages: torc
     if rows == 0 or B == 0:
         return out
     scale = (1.0 / math.sqrt(D)) if scale is None else float(scale)
-    need = _workspace_bytes(rows, Hq, D, dev.index)
-    if workspace is None or workspace.numel() * workspace.element_size() < need:
-        need = _call_bytes(dev.index, groups, prefix_tables.shape[1], block_tables.shape[1],
-                           int(cu_q is not None), B, rows, Hq, Hkv, D, P, scale,
-                           N.dtype_code(q.dtype))
+    need = _call_bytes(dev.index, groups, prefix_tables.shape[1], block_tables.shape[1],
+                       int(cu_q is not None), B, rows, Hq, Hkv, D, P, scale, N.dtype_code(q.dtype))
     ws = scratch(workspace, need, dev)
     pt, plens = prefix_tables.contiguous(), prefix_lens.contiguous()
     bt, lens = block_tables.contiguous(), kv_lens.contiguous()

@@ -50,6 +50,18 @@ def test_many_rows_allocate_their_output(dev, dtype):
     assert torch.equal(got, want)
 
 
+def test_a_workspace_that_is_not_one_is_replaced_by_what_the_call_takes(dev):
+    rows = [2, 1]
+    args, cu, ref = _case(dev, 300, [40] * 2, rows, 8, 2, 128, torch.bfloat16)
+    need = _call_bytes(dev, args, 2, 3)
+    for ws in (torch.empty(need + 16, dtype=torch.uint8, device=dev)[8:],       # between vectors
+               torch.empty(2 * need, dtype=torch.uint8, device=dev)[::2],       # with holes
+               torch.empty(need - 1, dtype=torch.uint8, device=dev)):           # too little
+        ws.fill_(0x7f)
+        O.check(PP.paged_prefix_attention(*args, cu_q=cu, workspace=ws), *ref(), torch.bfloat16, rows=True)
+        assert (ws == 0x7f).all()
+
+
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
 @pytest.mark.parametrize("rows,prefix,dim", [([100], 3000, 128), ([70, 33], 2000, 64), ([65], 4000, 256),
                                              ([2, 1, 3], 500, 128)])
